@@ -436,6 +436,68 @@ int biops_moe_sparse_noalloc(int dtype, int64_t tokens, int64_t experts, int64_t
                              const void* weights, int w_dtype, const int64_t* sel,
                              void* out, int32_t* bad_index, void* stream);
 
+/* -------------------------------------------------------------------- served decoder ---- */
+
+/* Operators that the reference has no counterpart of.  Device-side indices (slots, page tables, lengths, packed
+ * offsets) never make a kernel read or write out of range; `flag` (one int32 on the device, never cleared by the
+ * library) is set to 1 when one lies outside its tensor. */
+
+/* Rotary positions: pair i < pairs of a head turns by positions[axis[i]][token] * 2 pi turns[i] (inverse: by its
+ * negative), (x0, x1) -> (x0 cos - x1 sin, x1 cos + x0 sin), elements (i, i + pairs) or, with neighbours, (2i, 2i + 1);
+ * elements behind 2 * pairs are copied.  q [batch, tokens, hq, d] -> oq and k [batch, tokens, hk, d] -> ok in one
+ * launch, unit stride in d; hq or hk may be 0.  positions [axes, batch, tokens] of pos_type 0 int64, 1 int32,
+ * 2 float32.  turns and axis are host arrays of `pairs` (at most 128) values, copied by the call; axis values must
+ * lie inside positions.  Angles in 64 bits, the rotation in 32, one rounding. */
+int biops_rotary(int dtype, int64_t batch, int64_t tokens, int64_t hq, int64_t hk, int64_t d,
+                 const void* q, int64_t sqB, int64_t sqT, int64_t sqH, void* oq, int64_t soqB, int64_t soqT, int64_t soqH,
+                 const void* k, int64_t skB, int64_t skT, int64_t skH, void* ok, int64_t sokB, int64_t sokT, int64_t sokH,
+                 const void* positions, int pos_type, int64_t spA, int64_t spB, int64_t spT,
+                 int64_t pairs, const double* turns, const uint8_t* axis, int neighbours, int inverse, void* stream);
+
+/* Rows k [rows, heads, d] and v [rows, heads, dv] into the slots (int32 or int64, `slots64`) of a cache in pages: slot
+ * s is page s / page_size, place s % page_size of kc [pages, page_size, heads, d] and vc [..., dv].  Unit stride in d
+ * and dv.  Negative slots are left out; slots past the cache too, with the flag.  Of rows that name one slot the
+ * last stays.  At most 2^31 - 1 slots. */
+int biops_paged_write(int dtype, int64_t rows, int64_t heads, int64_t d, int64_t dv,
+                      const void* k, int64_t skT, int64_t skH, const void* v, int64_t svT, int64_t svH,
+                      void* kc, int64_t skcP, int64_t skcS, int64_t skcH, void* vc, int64_t svcP, int64_t svcS,
+                      int64_t svcH, int64_t pages, int64_t page_size, const void* slots, int slots64,
+                      int64_t slot_stride, int* flag, void* stream);
+
+/* Workspace bytes of biops_paged_attention (0: none needed), -1 for bad sizes. */
+int64_t biops_paged_attention_workspace_size(int64_t batch, int64_t hq, int64_t dv, int64_t width, int64_t page_size,
+                                             int64_t max_length, int64_t window, int64_t sinks);
+
+/* Attention of one new token per sequence over a cache in pages: q [batch, hq, d] -> out [batch, hq, dv] (contiguous),
+ * key j of sequence b at place j % page_size of page table[b][j / page_size] of kc / vc (as biops_paged_write),
+ * lengths[b] keys, the query at the last.  Visible: j >= length - window (window 0: all) or j < sinks.  Lengths
+ * outside [0, min(width * page_size, max_length)] (max_length < 0: no bound) and visible pages outside the cache give
+ * rows of zeros and set the flag.  d and dv: multiples of 16 bytes, up to 256 elements; unit stride in d.
+ * The chunks that a sequence is split into depend on its own visible keys only.  Workspace 16-byte aligned. */
+int biops_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t dv,
+                          const void* q, int64_t sqB, int64_t sqH, const void* kc, int64_t skP, int64_t skS, int64_t skH,
+                          const void* vc, int64_t svP, int64_t svS, int64_t svH, int64_t pages, int64_t page_size,
+                          const void* table, int table64, int64_t stB, int64_t stW, int64_t width,
+                          const void* lengths, int lengths64, int64_t slB, int64_t max_length, int64_t window,
+                          int64_t sinks, float scale, void* out, int* flag, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/* Largest head size of biops_window_attention: 256 (16-bit types), 128 (float32), 0 otherwise. */
+int biops_window_attention_max_head(int dtype);
+
+/* Causal attention under a sliding window with sinks.  Query r of a sequence is at p = lk - lq + r and sees keys j <= p
+ * with p - j < window or j < sinks; rows that see none are zeros.  Dense (cu_q null): nseq sequences of lq queries and
+ * lk keys, q / k / v / out [batch, tokens, heads, dim] by strides.  Packed: sequence s is rows cu_q[s] .. cu_q[s + 1]
+ * of lq query rows and cu_k[s] .. cu_k[s + 1] of lk key rows (device offsets, int32 or int64, by strides; batch strides
+ * unused); rows outside of all sequences become zeros; bad offsets set the flag.  d and dv: multiples of 16 bytes up
+ * to biops_window_attention_max_head; unit stride in dim; the scale is finite. */
+int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64_t hkv, int64_t lq, int64_t lk, int64_t d, int64_t dv,
+                           const void* q, int64_t sqB, int64_t sqT, int64_t sqH, const void* k, int64_t skB, int64_t skT,
+                           int64_t skH, const void* v, int64_t svB, int64_t svT, int64_t svH, void* out, int64_t soB,
+                           int64_t soT, int64_t soH, const void* cu_q, int cu_q64, int64_t cu_q_stride, const void* cu_k,
+                           int cu_k64, int64_t cu_k_stride, int64_t window, int64_t sinks, float scale, int* flag,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

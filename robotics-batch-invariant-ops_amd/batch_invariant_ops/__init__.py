@@ -26,6 +26,16 @@ from .batch_invariant_ops import (
 )
 from .moe import deterministic_token_choice_moe
 
+# Operators of a served decoder, which the reference's package does not have: ``__all__`` stays its surface.
+from .decoder import (  # noqa: F401
+    multi_axis_rotary,
+    paged_cache_write,
+    paged_attention_batch_invariant,
+    sliding_window_attention_batch_invariant,
+    varlen_sliding_window_attention_batch_invariant,
+    check_cache_indices,
+)
+
 __version__ = "0.2.0"
 
 __all__ = [

@@ -102,6 +102,25 @@ _SIGNATURES = {
         _i,
         [_i, _l, _l, _l, _l] + [_p, _l, _l] * 4 + [_p, _p, _i, _f, _p, _l, _p],
     ),
+    "biops_rotary": (
+        _i,
+        [_i, _l, _l, _l, _l, _l] + [_p, _l, _l, _l] * 4 + [_p, _i, _l, _l, _l, _l, _p, _p, _i, _i, _p],
+    ),
+    "biops_paged_write": (
+        _i,
+        [_i, _l, _l, _l, _l] + [_p, _l, _l] * 2 + [_p, _l, _l, _l] * 2 + [_l, _l, _p, _i, _l, _p, _p],
+    ),
+    "biops_paged_attention_workspace_size": (_l, [_l, _l, _l, _l, _l, _l, _l, _l]),
+    "biops_paged_attention": (
+        _i,
+        [_i, _l, _l, _l, _l, _l] + [_p, _l, _l] + [_p, _l, _l, _l] * 2 + [_l, _l]
+        + [_p, _i, _l, _l, _l] + [_p, _i, _l] + [_l, _l, _l, _f, _p, _p, _p, _l, _p],
+    ),
+    "biops_window_attention_max_head": (_i, [_i]),
+    "biops_window_attention": (
+        _i,
+        [_i, _l, _l, _l, _l, _l, _l, _l] + [_p, _l, _l, _l] * 4 + [_p, _i, _l] * 2 + [_l, _l, _f, _p, _p],
+    ),
     "biops_moe_workspace_size": (_l, [_i, _l, _l, _l, _l]),
     "biops_moe": (
         _i,
@@ -205,7 +224,10 @@ _FAST = {"biops_gemm": "gemm", "biops_gemm_padded": "gemm_padded", "biops_reduce
          "biops_sdpa_split_workspace_size": "sdpa_split_workspace_size", "biops_sdpa_f32": "sdpa_f32",
          "biops_varlen_plan": "varlen_plan", "biops_varlen_fused_order": "varlen_fused_order",
          "biops_varlen_sdpa_fused": "varlen_sdpa_fused",
-         "biops_varlen_sdpa_fused_planned": "varlen_sdpa_fused_planned"}
+         "biops_varlen_sdpa_fused_planned": "varlen_sdpa_fused_planned",
+         "biops_rotary": "rotary", "biops_paged_write": "paged_write",
+         "biops_paged_attention_workspace_size": "paged_attention_workspace_size",
+         "biops_paged_attention": "paged_attention", "biops_window_attention": "window_attention"}
 
 
 def fast_function(name: str):

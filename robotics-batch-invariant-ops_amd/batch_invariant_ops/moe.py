@@ -9,8 +9,6 @@ import torch
 
 from . import _native as nat
 
-_INDEX_ERROR = "selected_experts contains an expert index outside [0, num_experts)"
-
 
 class _IndexWatch:
     """Deferred report of out-of-range expert indices on one device, without a host wait.
@@ -22,6 +20,7 @@ class _IndexWatch:
     during stream capture).  The next call, or ``check_moe_indices``, reads a landed copy and
     raises ``RuntimeError`` if the flag was set, after clearing it."""
 
+    MESSAGE = "selected_experts contains an expert index outside [0, num_experts)"
     PERIOD = 1e-3
     _by_device: dict = {}
     _lock = threading.Lock()
@@ -46,11 +45,12 @@ class _IndexWatch:
         if value != 0:
             self.host[0] = 0
             self.flag.zero_()
-            raise RuntimeError(f"{_INDEX_ERROR} in a call since the last report")
+            raise RuntimeError(f"{self.MESSAGE} in a call since the last report")
 
     def poll(self) -> None:
-        """Raise for a flag copy that has landed with the flag set."""
-        if self.pending and self.event.query():
+        """Raise for a flag copy that has landed with the flag set (not during stream capture, which
+        an event query would end)."""
+        if self.pending and not torch.cuda.is_current_stream_capturing() and self.event.query():
             self.pending = False
             self._raise_if_set(int(self.host[0]))
 

@@ -1,6 +1,6 @@
 /* Fast-call CPython binding of the library's most frequent entry points (GEMM, padded GEMM, row
- * reductions, softmax, fused attention, the varlen planner and fused varlen attention), of
- * the host-to-device copy of the varlen work list and of the device-to-host copy of the MoE
+ * reductions, softmax, fused attention, the varlen planner and fused varlen attention, rotary
+ * positions, paged cache writes, paged and windowed attention), of the host-to-device copy of the varlen work list and of the device-to-host copy of the MoE
  * index flag: the same C ABI as the ctypes binding,
  * without the per-argument ctypes conversions.  Python integers are taken as
  * int64 values or addresses (None is a null pointer), Python floats as float; each function
@@ -226,6 +226,77 @@ static PyObject* fast_sdpa_split_workspace_size(PyObject* self, PyObject* const*
                                                              iv[7], (int)iv[8]));
 }
 
+/* rotary(dtype, batch, tokens, hq, hk, d, {q, sB, sT, sH, oq, sB, sT, sH}, {k, ..., ok, ...}, positions, type, sA, sB, sT,
+ *        pairs, turns, axis, neighbours, inverse, stream) */
+static PyObject* fast_rotary(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  int64_t iv[33];
+  void* pv[33];
+  (void)self;
+  if (!parse(args, nargs, "llllllplllplllplllplllplllllppllp", iv, pv, NULL)) return NULL;
+  int rc;
+  WITHOUT_GIL(rc, biops_rotary((int)iv[0], iv[1], iv[2], iv[3], iv[4], iv[5], pv[6], iv[7], iv[8], iv[9], pv[10], iv[11],
+                               iv[12], iv[13], pv[14], iv[15], iv[16], iv[17], pv[18], iv[19], iv[20], iv[21], pv[22],
+                               (int)iv[23], iv[24], iv[25], iv[26], iv[27], (const double*)pv[28],
+                               (const uint8_t*)pv[29], (int)iv[30], (int)iv[31], pv[32]));
+  return PyLong_FromLong(rc);
+}
+
+/* paged_write(dtype, rows, heads, d, dv, k, sT, sH, v, sT, sH, kc, sP, sS, sH, vc, sP, sS, sH, pages, page_size, slots,
+ *             slots64, slot_stride, flag, stream) */
+static PyObject* fast_paged_write(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  int64_t iv[26];
+  void* pv[26];
+  (void)self;
+  if (!parse(args, nargs, "lllllpllpllplllplllllpllpp", iv, pv, NULL)) return NULL;
+  int rc;
+  WITHOUT_GIL(rc, biops_paged_write((int)iv[0], iv[1], iv[2], iv[3], iv[4], pv[5], iv[6], iv[7], pv[8], iv[9], iv[10],
+                                    pv[11], iv[12], iv[13], iv[14], pv[15], iv[16], iv[17], iv[18], iv[19], iv[20],
+                                    pv[21], (int)iv[22], iv[23], (int*)pv[24], pv[25]));
+  return PyLong_FromLong(rc);
+}
+
+/* paged_attention_workspace_size(batch, hq, dv, width, page_size, max_length, window, sinks) -> bytes or -1 */
+static PyObject* fast_paged_attention_workspace_size(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  int64_t iv[8];
+  (void)self;
+  if (!parse(args, nargs, "llllllll", iv, NULL, NULL)) return NULL;
+  return PyLong_FromLongLong(
+      biops_paged_attention_workspace_size(iv[0], iv[1], iv[2], iv[3], iv[4], iv[5], iv[6], iv[7]));
+}
+
+/* paged_attention(dtype, batch, hq, hkv, d, dv, q, sB, sH, kc, sP, sS, sH, vc, sP, sS, sH, pages, page_size, table,
+ *                 table64, sB, sW, width, lengths, lengths64, sB, max_length, window, sinks, scale, out, flag,
+ *                 workspace, bytes, stream) */
+static PyObject* fast_paged_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  int64_t iv[36];
+  void* pv[36];
+  float fv[36];
+  (void)self;
+  if (!parse(args, nargs, "llllllpllplllplllllpllllplllllfppplp", iv, pv, fv)) return NULL;
+  int rc;
+  WITHOUT_GIL(rc, biops_paged_attention((int)iv[0], iv[1], iv[2], iv[3], iv[4], iv[5], pv[6], iv[7], iv[8], pv[9], iv[10],
+                                        iv[11], iv[12], pv[13], iv[14], iv[15], iv[16], iv[17], iv[18], pv[19],
+                                        (int)iv[20], iv[21], iv[22], iv[23], pv[24], (int)iv[25], iv[26], iv[27], iv[28],
+                                        iv[29], fv[30], pv[31], (int*)pv[32], pv[33], iv[34], pv[35]));
+  return PyLong_FromLong(rc);
+}
+
+/* window_attention(dtype, nseq, hq, hkv, lq, lk, d, dv, {q, k, v, out: pointer, sB, sT, sH}, cu_q, cu_q64, stride, cu_k,
+ *                  cu_k64, stride, window, sinks, scale, flag, stream) */
+static PyObject* fast_window_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  int64_t iv[35];
+  void* pv[35];
+  float fv[35];
+  (void)self;
+  if (!parse(args, nargs, "llllllllplllplllplllplllpllpllllfpp", iv, pv, fv)) return NULL;
+  int rc;
+  WITHOUT_GIL(rc, biops_window_attention((int)iv[0], iv[1], iv[2], iv[3], iv[4], iv[5], iv[6], iv[7], pv[8], iv[9],
+                                         iv[10], iv[11], pv[12], iv[13], iv[14], iv[15], pv[16], iv[17], iv[18], iv[19],
+                                         pv[20], iv[21], iv[22], iv[23], pv[24], (int)iv[25], iv[26], pv[27],
+                                         (int)iv[28], iv[29], iv[30], iv[31], fv[32], (int*)pv[33], pv[34]));
+  return PyLong_FromLong(rc);
+}
+
 /* copy_h2d(dst, src, bytes, stream) -> hipError_t: hipMemcpyAsync host -> device on `stream` */
 static PyObject* fast_copy_h2d(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   int64_t iv[4];
@@ -274,6 +345,12 @@ static PyMethodDef kMethods[] = {
      "biops_varlen_sdpa_fused"},
     {"varlen_sdpa_fused_planned", (PyCFunction)(void (*)(void))fast_varlen_sdpa_fused_planned, METH_FASTCALL,
      "biops_varlen_sdpa_fused_planned"},
+    {"rotary", (PyCFunction)(void (*)(void))fast_rotary, METH_FASTCALL, "biops_rotary"},
+    {"paged_write", (PyCFunction)(void (*)(void))fast_paged_write, METH_FASTCALL, "biops_paged_write"},
+    {"paged_attention_workspace_size", (PyCFunction)(void (*)(void))fast_paged_attention_workspace_size, METH_FASTCALL,
+     "biops_paged_attention_workspace_size"},
+    {"paged_attention", (PyCFunction)(void (*)(void))fast_paged_attention, METH_FASTCALL, "biops_paged_attention"},
+    {"window_attention", (PyCFunction)(void (*)(void))fast_window_attention, METH_FASTCALL, "biops_window_attention"},
     {"copy_h2d", (PyCFunction)(void (*)(void))fast_copy_h2d, METH_FASTCALL, "hipMemcpyAsync host to device"},
     {"copy_d2h", (PyCFunction)(void (*)(void))fast_copy_d2h, METH_FASTCALL, "hipMemcpyAsync device to host"},
     {NULL, NULL, 0, NULL},
