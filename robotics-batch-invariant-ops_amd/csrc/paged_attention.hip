@@ -45,37 +45,44 @@ struct PagedArgs {
   int* flag;
   int64_t qB, qH, kP, kS, kH, vP, vS, vH;  // byte strides
   int64_t tB, tW, lB;                      // element strides of the page table and the lengths
-  int64_t batch, hkv, group, zs;           // zs: workgroups per key/value head (16 query heads each)
-  int64_t pages, page_size, limit;         // limit: longest length that the table (and the caller) allow
-  int64_t total;
+  uint32_t batch, hkv, group, zs;          // zs: workgroups per key/value head (16 query heads each)
+  uint32_t page_size;
+  int64_t pages;
+  int limit;                               // longest length that the table (and the caller) allow
+  uint32_t first, rows;                    // first workgroup of a launch; batch * hkv * zs
   int d, dv, chunks;                       // chunks: most chunks of a sequence
-  int64_t window, sinks;                   // window 0: all
+  int window, sinks;                       // window 0: all
   int table64, lengths64;
   int negate;                              // the scale is negative: queries enter with their sign flipped
   float scale;                             // |scale| log2 e, > 0
 };
 
 struct PagedSpan {
-  int64_t n;             // visible keys
-  int64_t ns, shift;     // key of v: v < ns ? v : v + shift
-  int64_t chunk;         // keys per chunk
+  int n;          // visible keys
+  int ns, shift;  // key of v: v < ns ? v : v + shift
+  int chunk;      // keys per chunk
   int chunks;
   bool bad;
 };
+
+// Keys per chunk, by the number of visible keys alone.
+__host__ __device__ __forceinline__ int paged_chunk(int n) {
+  constexpr int most = kPagedKeys * kPagedChunks;
+  return n <= most ? kPagedKeys : kPagedKeys * ((n - 1) / most + 1);
+}
 
 __device__ __forceinline__ PagedSpan paged_span(const PagedArgs& a, int64_t b) {
   PagedSpan s;
   const int64_t len = a.lengths64 ? reinterpret_cast<const int64_t*>(a.lengths)[b * a.lB]
                                   : (int64_t) reinterpret_cast<const int32_t*>(a.lengths)[b * a.lB];
   s.bad = len < 0 || len > a.limit;
-  const int64_t l = s.bad ? 0 : len;
-  const int64_t start = a.window > 0 && l > a.window ? l - a.window : 0;
+  const int l = s.bad ? 0 : (int)len;
+  const int start = a.window > 0 && l > a.window ? l - a.window : 0;
   s.ns = a.sinks < start ? a.sinks : start;
   s.shift = start - s.ns;
   s.n = s.ns + l - start;
-  const int64_t most = (int64_t)kPagedKeys * kPagedChunks;
-  s.chunk = s.n <= most ? kPagedKeys : kPagedKeys * cdiv(s.n, most);
-  s.chunks = (int)cdiv(s.n, s.chunk);
+  s.chunk = paged_chunk(s.n);
+  s.chunks = s.n > 0 ? (s.n - 1) / s.chunk + 1 : 0;
   return s;
 }
 
@@ -96,8 +103,16 @@ __device__ __forceinline__ uint32_t pack_pair(float x, float y) {
   else return (uint32_t)Num<T>::to_bits(x) | ((uint32_t)Num<T>::to_bits(y) << 16);
 }
 
+// Wavefronts per SIMD that registers are given out for.
 template <typename T, int DP, int DVP>
-__global__ __launch_bounds__(256) void paged_chunk_kernel(PagedArgs a) {
+constexpr int paged_waves() {
+  constexpr int wide = (DP > DVP ? DP : DVP) * (sizeof(T) / 2);
+  return wide <= 64 ? 4 : (wide <= 128 ? 3 : (wide <= 256 ? 2 : 1));
+}
+
+template <typename T, int DP, int DVP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_waves<T, DP, DVP>(), paged_waves<T, DP, DVP>())))
+void paged_chunk_kernel(PagedArgs a) {
   constexpr int E = sizeof(T), VEC = 16 / E;
   constexpr int KW = 4 * VEC, KS = DP / KW;             // elements and number of the score steps
   constexpr int W = E == 2 && DVP <= 64 ? 4 : VEC;      // elements of a value load
@@ -109,234 +124,231 @@ __global__ __launch_bounds__(256) void paged_chunk_kernel(PagedArgs a) {
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int m16 = lane & 15, q4 = lane >> 4;
   const u32x4_t zero4 = {0u, 0u, 0u, 0u};
-  const int64_t heads = a.hkv * a.group;
+  const int64_t heads = (int64_t)a.hkv * a.group;
 
-  for (int64_t u = blockIdx.x; u < a.total; u += gridDim.x) {
-    // chunk slowest: the first chunks of all sequences, which exist, go first
-    const int64_t rows = a.batch * a.hkv * a.zs;
-    const int c = (int)(u / rows);
-    int64_t r = u - c * rows;
-    const int64_t z = r % a.zs;
-    r /= a.zs;
-    const int64_t hk = r % a.hkv, b = r / a.hkv;
-    const PagedSpan span = paged_span(a, b);
-    const int cols = a.group - z * kPagedCols < kPagedCols ? (int)(a.group - z * kPagedCols) : kPagedCols;
-    const int64_t h0 = hk * a.group + z * kPagedCols;
-    if (c >= span.chunks) {
-      if (c == 0 && a.chunks == 1) {  // no join: rows that see nothing are written here
-        if (span.bad) *a.flag = 1;
-        for (int i = tid; i < cols * a.dv; i += 256)
-          Num<T>::store(reinterpret_cast<T*>(a.out) + (b * heads + h0) * a.dv + i, 0.f);
-      }
-      continue;
+  // chunk slowest: the first chunks of all sequences, which exist, go first
+  const uint32_t u = a.first + blockIdx.x;
+  const int c = (int)(u / a.rows);
+  uint32_t r = u - c * a.rows;
+  const uint32_t z = r % a.zs;
+  r /= a.zs;
+  const uint32_t hk = r % a.hkv, b = r / a.hkv;
+  const PagedSpan span = paged_span(a, b);
+  const int cols = a.group - z * kPagedCols < kPagedCols ? (int)(a.group - z * kPagedCols) : kPagedCols;
+  const int64_t h0 = hk * a.group + z * kPagedCols;
+  if (c >= span.chunks) {
+    if (c == 0 && a.chunks == 1) {  // no join: rows that see nothing are written here
+      if (span.bad) *a.flag = 1;
+      for (int i = tid; i < cols * a.dv; i += 256)
+        Num<T>::store(reinterpret_cast<T*>(a.out) + (b * heads + h0) * a.dv + i, 0.f);
     }
-    if (tid == 0) bad_page = 0;
-    const int64_t v0 = c * span.chunk;
-    const int nkeys = (int)(span.n - v0 < span.chunk ? span.n - v0 : span.chunk);
-    const int tiles = (nkeys + 31) >> 5;
+    return;
+  }
+  if (tid == 0) bad_page = 0;
+  const int v0 = c * span.chunk;
+  const int nkeys = span.n - v0 < span.chunk ? span.n - v0 : span.chunk;
+  const int tiles = (nkeys + 31) >> 5;
 
-    // queries (B operand): lane holds query column m16, elements KW s + VEC q4 ..
-    u32x4_t qf[KS];
-    {
-      const char* qr = a.q + b * a.qB + (h0 + (m16 < cols ? m16 : 0)) * a.qH;
+  // queries (B operand): lane holds query column m16, elements KW s + VEC q4 ..
+  u32x4_t qf[KS];
+  {
+    const char* qr = a.q + b * a.qB + (h0 + (m16 < cols ? m16 : 0)) * a.qH;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = KW * s + VEC * q4;
+      qf[s] = m16 < cols && d0 < a.d ? load_16(qr + E * d0) : zero4;
+      if (a.negate) qf[s] ^= E == 2 ? 0x80008000u : 0x80000000u;
+    }
+  }
+  __syncthreads();  // bad_page is clear
+
+  // byte offset of key `lane % 32` of a tile in the key cache (lanes 0-31) or the value cache
+  bool bad = false;
+  auto lookup = [&](int tile) -> int64_t {
+    int i = 32 * tile + (lane & 31);
+    if (i >= nkeys) i = nkeys - 1;
+    const int v = v0 + i;
+    const uint32_t key = (uint32_t)(v < span.ns ? v : v + span.shift);
+    const uint32_t page = key / a.page_size, at = key - page * a.page_size;
+    const int64_t e = b * a.tB + page * a.tW;
+    int64_t id = a.table64 ? reinterpret_cast<const int64_t*>(a.table)[e]
+                           : (int64_t) reinterpret_cast<const int32_t*>(a.table)[e];
+    if (id < 0 || id >= a.pages) {
+      bad = true;
+      id = 0;
+    }
+    return lane < 32 ? id * a.kP + at * a.kS : id * a.vP + at * a.vS;
+  };
+
+  // of query m16: largest product so far, m * scale, sum (of this lane's keys)
+  float m = -INFINITY, sh = 0.f, l = 0.f;
+  f32x4_t acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const char* const kb = a.kc + hk * a.kH;
+  const char* const vb = a.vc + hk * a.vH;
+
+  int64_t off = w < tiles ? lookup(w) : 0;
+  for (int tile = w; tile < tiles; tile += 4) {
+    offs[w][lane >> 5][lane & 31] = off;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    u32x4_t kf[2][KS];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char* p = kb + offs[w][0][8 * (m16 >> 2) + 4 * i + (m16 & 3)];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int d0 = KW * s + VEC * q4;
-        qf[s] = m16 < cols && d0 < a.d ? load_16(qr + E * d0) : zero4;
-        if (a.negate) qf[s] ^= E == 2 ? 0x80008000u : 0x80000000u;
+        kf[i][s] = d0 < a.d ? load_16(p + E * d0) : zero4;
       }
     }
-    __syncthreads();  // bad_page is clear; also the last round's merge has been read
-
-    // byte offset of key `lane % 32` of a tile in the key cache (lanes 0-31) or the value cache
-    bool bad = false;
-    auto lookup = [&](int tile) -> int64_t {
-      int i = 32 * tile + (lane & 31);
-      if (i >= nkeys) i = nkeys - 1;
-      const int64_t v = v0 + i;
-      const int64_t key = v < span.ns ? v : v + span.shift;
-      const uint32_t page = (uint32_t)key / (uint32_t)a.page_size, at = (uint32_t)key - page * (uint32_t)a.page_size;
-      const int64_t e = b * a.tB + page * a.tW;
-      int64_t id = a.table64 ? reinterpret_cast<const int64_t*>(a.table)[e]
-                             : (int64_t) reinterpret_cast<const int32_t*>(a.table)[e];
-      if (id < 0 || id >= a.pages) {
-        bad = true;
-        id = 0;
-      }
-      return lane < 32 ? id * a.kP + at * a.kS : id * a.vP + at * a.vS;
-    };
-
-    // of query m16: largest product so far, m * scale, sum (of this lane's keys)
-    float m = -INFINITY, sh = 0.f, l = 0.f;
-    f32x4_t acc[NT];
+    uint32_t vf[NB][8][VD];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const char* const kb = a.kc + hk * a.kH;
-    const char* const vb = a.vc + hk * a.vH;
-
-    int64_t off = w < tiles ? lookup(w) : 0;
-    for (int tile = w; tile < tiles; tile += 4) {
-      offs[w][lane >> 5][lane & 31] = off;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      u32x4_t kf[2][KS];
+    for (int j = 0; j < 8; ++j) {
+      const char* p = vb + offs[w][1][8 * q4 + j];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const char* p = kb + offs[w][0][8 * (m16 >> 2) + 4 * i + (m16 & 3)];
+      for (int n = 0; n < NB; ++n) {
+        const int e0 = 16 * W * n + W * m16;
+        if constexpr (VD == 4) {
+          const u32x4_t x = e0 < a.dv ? load_16(p + E * e0) : zero4;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int d0 = KW * s + VEC * q4;
-          kf[i][s] = d0 < a.d ? load_16(p + E * d0) : zero4;
+          for (int i = 0; i < 4; ++i) vf[n][j][i] = x[i];
+        } else {
+          const u32x2_t x = e0 < a.dv ? *reinterpret_cast<const u32x2_any_t*>(p + E * e0) : u32x2_t{0u, 0u};
+          vf[n][j][0] = x[0];
+          vf[n][j][1] = x[1];
         }
       }
-      uint32_t vf[NB][8][VD];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (tile + 4 < tiles) off = lookup(tile + 4);
+
+    f32x4_t sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) mfma16<T>(sc[i], kf[i][s], qf[s]);
+    }
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = sc[j >> 2][j & 3];
+    const int left = nkeys - 32 * tile;
+    if (left < 32) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const char* p = vb + offs[w][1][8 * q4 + j];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int e0 = 16 * W * n + W * m16;
-          if constexpr (VD == 4) {
-            const u32x4_t x = e0 < a.dv ? load_16(p + E * e0) : zero4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vf[n][j][i] = x[i];
-          } else {
-            const u32x2_t x = e0 < a.dv ? *reinterpret_cast<const u32x2_any_t*>(p + E * e0) : u32x2_t{0u, 0u};
-            vf[n][j][0] = x[0];
-            vf[n][j][1] = x[1];
-          }
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (tile + 4 < tiles) off = lookup(tile + 4);
-
-      f32x4_t sc[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) mfma16<T>(sc[i], kf[i][s], qf[s]);
-      }
-      float p[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = sc[j >> 2][j & 3];
-      const int left = nkeys - 32 * tile;
-      if (left < 32) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = 8 * q4 + j < left;
-          p[j] = in ? p[j] : -INFINITY;
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < VD; ++i) vf[n][j][i] = in ? vf[n][j][i] : 0u;
-        }
-      }
-      float mx = p[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, p[j]);
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      if (__any(mx > m)) {
-        const float mn = fmaxf(m, mx);
-        const float to = mn == -INFINITY ? 0.f : mn * a.scale;
-        const float corr = mx > m ? (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - to)) : 1.f;
-        l *= corr;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t] *= corr;
-        m = mn;
-        sh = to;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], a.scale, -sh));
-        l += p[j];
-      }
-      if constexpr (E == 4) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int t = 0; t < W; ++t)
-              acc[W * n + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[n][j][t]), p[j], acc[W * n + t], 0, 0, 0);
-      } else {
-        u32x4_t hi, lo;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          hi[i] = pack_pair<T>(p[2 * i], p[2 * i + 1]);
-          lo[i] = pack_pair<T>(p[2 * i] - Num<T>::from_bits(hi[i] & 0xffffu), p[2 * i + 1] - Num<T>::from_bits(hi[i] >> 16));
-        }
+        const bool in = 8 * q4 + j < left;
+        p[j] = in ? p[j] : -INFINITY;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int t = 0; t < W; ++t) {
-            u32x4_t va;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              va[i] = __builtin_amdgcn_perm(vf[n][2 * i + 1][t >> 1], vf[n][2 * i][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-            mfma16<T>(acc[W * n + t], va, hi);
-            mfma16<T>(acc[W * n + t], va, lo);
-          }
+          for (int i = 0; i < VD; ++i) vf[n][j][i] = in ? vf[n][j][i] : 0u;
       }
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (bad) bad_page = 1;
-
-    // the four wavefronts' results, joined in order
-    float* const os = reinterpret_cast<float*>(smem);
-    float* const mls = os + 4 * cols * DVP;
-    if (m16 < cols) {
-      if (q4 == 0) {
-        mls[2 * (w * cols + m16)] = m == -INFINITY ? m : sh;
-        mls[2 * (w * cols + m16) + 1] = l;
+    float mx = p[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, p[j]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    if (__any(mx > m)) {
+      const float mn = fmaxf(m, mx);
+      const float to = mn == -INFINITY ? 0.f : mn * a.scale;
+      const float corr = mx > m ? (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - to)) : 1.f;
+      l *= corr;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] *= corr;
+      m = mn;
+      sh = to;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], a.scale, -sh));
+      l += p[j];
+    }
+    if constexpr (E == 4) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int t = 0; t < W; ++t)
+            acc[W * n + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[n][j][t]), p[j], acc[W * n + t], 0, 0, 0);
+    } else {
+      u32x4_t hi, lo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        hi[i] = pack_pair<T>(p[2 * i], p[2 * i + 1]);
+        lo[i] = pack_pair<T>(p[2 * i] - Num<T>::from_bits(hi[i] & 0xffffu), p[2 * i + 1] - Num<T>::from_bits(hi[i] >> 16));
       }
-      float* o = os + (w * cols + m16) * DVP;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int t = 0; t < W; ++t) {
+          u32x4_t va;
 #pragma unroll
-          for (int t = 0; t < W; t += 4)
-            *reinterpret_cast<f32x4_t*>(o + 16 * W * n + W * (4 * q4 + i) + t) =
-                f32x4_t{acc[W * n + t][i], acc[W * n + t + 1][i], acc[W * n + t + 2][i], acc[W * n + t + 3][i]};
-    }
-    __syncthreads();
-    const bool void_ = bad_page != 0;
-    if (void_ && tid == 0) *a.flag = 1;
-    const int pieces = a.dv >> 2;
-    for (int i = tid; i < cols * pieces; i += 256) {
-      const int col = i / pieces, e = 4 * (i - col * pieces);
-      float M = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) M = fmaxf(M, mls[2 * (x * cols + col)]);
-      const float base = M == -INFINITY ? 0.f : M;
-      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-      float sum = 0.f;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float f = __builtin_amdgcn_exp2f(mls[2 * (x * cols + col)] - base);
-        sum = __builtin_fmaf(mls[2 * (x * cols + col) + 1], f, sum);
-        o += *reinterpret_cast<const f32x4_t*>(os + (x * cols + col) * DVP + e) * f;
-      }
-      const int64_t row = b * heads + h0 + col;
-      if (a.chunks == 1) {
-        const float inv = void_ || sum == 0.f ? 0.f : 1.f / sum;
-        T* dst = reinterpret_cast<T*>(a.out) + row * a.dv + e;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) Num<T>::store(dst + x, inv == 0.f ? 0.f : o[x] * inv);
-      } else {
-        const int64_t at = row * a.chunks + c;
-        *reinterpret_cast<f32x4_t*>(a.part + at * a.dv + e) = o;
-        if (e == 0) {
-          a.ml[2 * at] = M;
-          a.ml[2 * at + 1] = void_ ? -1.f : sum;
+          for (int i = 0; i < 4; ++i)
+            va[i] = __builtin_amdgcn_perm(vf[n][2 * i + 1][t >> 1], vf[n][2 * i][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+          mfma16<T>(acc[W * n + t], va, hi);
+          mfma16<T>(acc[W * n + t], va, lo);
         }
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (bad) bad_page = 1;
+
+  // the four wavefronts' results, joined in order
+  float* const os = reinterpret_cast<float*>(smem);
+  float* const mls = os + 4 * cols * DVP;
+  if (m16 < cols) {
+    if (q4 == 0) {
+      mls[2 * (w * cols + m16)] = m == -INFINITY ? m : sh;
+      mls[2 * (w * cols + m16) + 1] = l;
+    }
+    float* o = os + (w * cols + m16) * DVP;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < W; t += 4)
+          *reinterpret_cast<f32x4_t*>(o + 16 * W * n + W * (4 * q4 + i) + t) =
+              f32x4_t{acc[W * n + t][i], acc[W * n + t + 1][i], acc[W * n + t + 2][i], acc[W * n + t + 3][i]};
+  }
+  __syncthreads();
+  const bool void_ = bad_page != 0;
+  if (void_ && tid == 0) *a.flag = 1;
+  const int pieces = a.dv >> 2;
+  for (int i = tid; i < cols * pieces; i += 256) {
+    const int col = i / pieces, e = 4 * (i - col * pieces);
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) M = fmaxf(M, mls[2 * (x * cols + col)]);
+    const float base = M == -INFINITY ? 0.f : M;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = __builtin_amdgcn_exp2f(mls[2 * (x * cols + col)] - base);
+      sum = __builtin_fmaf(mls[2 * (x * cols + col) + 1], f, sum);
+      o += *reinterpret_cast<const f32x4_t*>(os + (x * cols + col) * DVP + e) * f;
+    }
+    const int64_t row = b * heads + h0 + col;
+    if (a.chunks == 1) {
+      const float inv = void_ || sum == 0.f ? 0.f : 1.f / sum;
+      T* dst = reinterpret_cast<T*>(a.out) + row * a.dv + e;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) Num<T>::store(dst + x, inv == 0.f ? 0.f : o[x] * inv);
+    } else {
+      const int64_t at = row * a.chunks + c;
+      *reinterpret_cast<f32x4_t*>(a.part + at * a.dv + e) = o;
+      if (e == 0) {
+        a.ml[2 * at] = M;
+        a.ml[2 * at + 1] = void_ ? -1.f : sum;
       }
     }
-    __syncthreads();
   }
 }
 
@@ -349,64 +361,67 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) f32x4_t so[256];
   __shared__ float sl[256];
   const int tid = threadIdx.x;
-  const int64_t rows = a.batch * a.hkv * a.group;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const PagedSpan span = paged_span(a, row / (a.hkv * a.group));
-    T* dst = reinterpret_cast<T*>(a.out) + row * a.dv;
-    if (span.bad && tid == 0) *a.flag = 1;
-    if (tid == 0) void_row = 0;
-    __syncthreads();
-    const float* ml = a.ml + 2 * row * a.chunks;
-    const float* part = a.part + row * a.chunks * a.dv;
-    float mx = -INFINITY;
-    for (int c = tid; c < span.chunks; c += 256) {
-      mx = fmaxf(mx, ml[2 * c]);
-      if (ml[2 * c + 1] == -1.f) void_row = 1;
+  const int64_t row = a.first + blockIdx.x;
+  const PagedSpan span = paged_span(a, (uint32_t)row / (a.hkv * a.group));
+  T* dst = reinterpret_cast<T*>(a.out) + row * a.dv;
+  if (span.bad && tid == 0) *a.flag = 1;
+  if (tid == 0) void_row = 0;
+  __syncthreads();
+  const float* ml = a.ml + 2 * row * a.chunks;
+  const float* part = a.part + row * a.chunks * a.dv;
+  float mx = -INFINITY;
+  for (int c = tid; c < span.chunks; c += 256) {
+    mx = fmaxf(mx, ml[2 * c]);
+    if (ml[2 * c + 1] == -1.f) void_row = 1;
+  }
+  mx = wave_max(mx);
+  if ((tid & 63) == 0) red[tid >> 6] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float base = mx == -INFINITY ? 0.f : mx;
+  const int pieces = a.dv >> 2, splits = 256 / pieces;
+  const int piece = tid % pieces, split = tid / pieces;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  if (split < splits)
+    for (int c = split; c < span.chunks; c += splits) {
+      const float f = __builtin_amdgcn_exp2f(ml[2 * c] - base);
+      sum = __builtin_fmaf(ml[2 * c + 1], f, sum);
+      o += *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * a.dv + 4 * piece) * f;
     }
-    mx = wave_max(mx);
-    if ((tid & 63) == 0) red[tid >> 6] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float base = mx == -INFINITY ? 0.f : mx;
-    const int pieces = a.dv >> 2, splits = 256 / pieces;
-    const int piece = tid % pieces, split = tid / pieces;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    if (split < splits)
-      for (int c = split; c < span.chunks; c += splits) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * c] - base);
-        sum = __builtin_fmaf(ml[2 * c + 1], f, sum);
-        o += *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * a.dv + 4 * piece) * f;
-      }
-    so[tid] = o;
-    sl[tid] = sum;
-    __syncthreads();
-    if (split == 0) {
-      for (int s = 1; s < splits; ++s) {
-        o += so[s * pieces + piece];
-        sum += sl[s * pieces + piece];
-      }
-      const float inv = void_row || sum == 0.f ? 0.f : 1.f / sum;
+  so[tid] = o;
+  sl[tid] = sum;
+  __syncthreads();
+  if (split == 0) {
+    for (int s = 1; s < splits; ++s) {
+      o += so[s * pieces + piece];
+      sum += sl[s * pieces + piece];
+    }
+    const float inv = void_row || sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) Num<T>::store(dst + 4 * piece + x, inv == 0.f ? 0.f : o[x] * inv);
-    }
-    __syncthreads();
+    for (int x = 0; x < 4; ++x) Num<T>::store(dst + 4 * piece + x, inv == 0.f ? 0.f : o[x] * inv);
   }
 }
 
 template <typename T, int DP, int DVP>
-static int paged_launch(const PagedArgs& a, hipStream_t s) {
-  const int cols = a.group < kPagedCols ? (int)a.group : kPagedCols;
+static int paged_launch(PagedArgs a, hipStream_t s) {
+  const unsigned cols = a.group < kPagedCols ? a.group : kPagedCols;
   const unsigned lds = (unsigned)(4 * cols * (DVP + 2) * sizeof(float));
-  const int64_t most = 1 << 22;
-  hipLaunchKernelGGL((paged_chunk_kernel<T, DP, DVP>), dim3((unsigned)(a.total < most ? a.total : most)), dim3(256), lds, s, a);
-  int rc = check_launch("paged_chunk_kernel");
-  if (rc == BIOPS_OK && a.chunks > 1) {
-    const int64_t rows = a.batch * a.hkv * a.group;
-    hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)(rows < most ? rows : most)), dim3(256), 0, s, a);
-    rc = check_launch("paged_join_kernel");
+  constexpr uint32_t most = 1 << 22;  // a launch has less than 2^32 threads
+  const uint32_t total = a.rows * a.chunks, joins = a.batch * a.hkv * a.group;
+  for (a.first = 0; a.first < total; a.first += most) {
+    const uint32_t n = total - a.first < most ? total - a.first : most;
+    hipLaunchKernelGGL((paged_chunk_kernel<T, DP, DVP>), dim3(n), dim3(256), lds, s, a);
+    const int rc = check_launch("paged_chunk_kernel");
+    if (rc != BIOPS_OK) return rc;
   }
-  return rc;
+  for (a.first = 0; a.chunks > 1 && a.first < joins; a.first += most) {
+    const uint32_t n = joins - a.first < most ? joins - a.first : most;
+    hipLaunchKernelGGL((paged_join_kernel<T>), dim3(n), dim3(256), 0, s, a);
+    const int rc = check_launch("paged_join_kernel");
+    if (rc != BIOPS_OK) return rc;
+  }
+  return BIOPS_OK;
 }
 template <typename T, int DP>
 static int paged_launch_dv(const PagedArgs& a, hipStream_t s) {
@@ -428,6 +443,7 @@ static int64_t paged_limit(int64_t width, int64_t page_size, int64_t max_length)
   if (max_length >= 0 && max_length < limit) limit = max_length;
   return limit;
 }
+// Most chunks of a sequence (the count grows with the visible keys up to kPagedChunks).
 static int paged_chunks(int64_t limit, int64_t window, int64_t sinks) {
   int64_t n = limit;
   if (window > 0 && window < limit && sinks < limit - window) n = window + sinks;
@@ -446,7 +462,7 @@ extern "C" int64_t biops_paged_attention_workspace_size(int64_t batch, int64_t h
   if (batch < 0 || hq < 0 || dv < 0 || dv > 256 || width < 0 || page_size < 0 || window < 0 || sinks < 0) return -1;
   const int chunks = paged_chunks(paged_limit(width, page_size, max_length), window, sinks);
   if (chunks == 1 || batch == 0 || hq == 0) return 0;
-  if (hq > (INT64_C(1) << 40) / batch) return -1;
+  if (hq > (INT64_C(1) << 30) / kPagedChunks / batch) return -1;
   return batch * hq * chunks * (dv + 2) * (int64_t)sizeof(float);
 }
 
@@ -470,11 +486,15 @@ extern "C" int biops_paged_attention(int dtype, int64_t batch, int64_t hq, int64
   if (batch == 0 || hq == 0) return BIOPS_OK;
   if (!q || !kc || !vc || !lengths || !out || !flag || (width > 0 && !table))
     return fail(BIOPS_ERR_ARG, "biops_paged_attention: null pointer");
-  if (hq > (INT64_C(1) << 40) / batch) return fail(BIOPS_ERR_ARG, "biops_paged_attention: too many rows");
+  // counted in 32 bits: workgroups and output rows
+  if (hq > (INT64_C(1) << 30) / kPagedChunks / batch) return fail(BIOPS_ERR_ARG, "biops_paged_attention: more than 2^24 rows");
   PagedArgs a;
-  a.limit = paged_limit(width, page_size, max_length);
-  a.chunks = paged_chunks(a.limit, window, sinks);
-  a.batch = batch, a.hkv = hkv, a.group = hq / hkv, a.zs = cdiv(a.group, kPagedCols);
+  const int64_t limit = paged_limit(width, page_size, max_length), all = INT64_C(0x7fffffff);
+  a.limit = (int)limit;
+  a.chunks = paged_chunks(limit, window, sinks);
+  a.batch = (uint32_t)batch, a.hkv = (uint32_t)hkv, a.group = (uint32_t)(hq / hkv);
+  a.zs = (a.group + kPagedCols - 1) / kPagedCols;
+  a.rows = a.batch * a.hkv * a.zs;
   const int64_t rows = batch * hq * a.chunks;
   if (a.chunks > 1) {
     const int64_t need = rows * (dv + 2) * (int64_t)sizeof(float);
@@ -491,10 +511,9 @@ extern "C" int biops_paged_attention(int dtype, int64_t batch, int64_t hq, int64
   a.kP = elt * skP, a.kS = elt * skS, a.kH = elt * skH;
   a.vP = elt * svP, a.vS = elt * svS, a.vH = elt * svH;
   a.tB = stB, a.tW = stW, a.lB = slB;
-  a.pages = pages, a.page_size = page_size;
-  a.total = a.chunks * batch * hkv * a.zs;
+  a.pages = pages, a.page_size = (uint32_t)page_size;
   a.d = (int)d, a.dv = (int)dv;
-  a.window = window, a.sinks = sinks;
+  a.window = (int)(window < all ? window : all), a.sinks = (int)(sinks < all ? sinks : all);
   a.table64 = table64 != 0, a.lengths64 = lengths64 != 0;
   a.negate = scale < 0.f;
   // a scale of zero: every weight 1, and 0 * -inf stays out of the masked scores

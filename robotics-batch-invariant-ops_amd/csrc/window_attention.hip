@@ -30,7 +30,7 @@
 
 namespace biops {
 
-constexpr int kWindowRows = 128;   // query rows of a workgroup
+constexpr int kWindowShort = 512;  // visible keys up to which tiles of 64 rows are taken
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
 struct WindowArgs {
@@ -41,10 +41,12 @@ struct WindowArgs {
   int cu_q64, cu_k64;
   int64_t cu_q_stride, cu_k_stride;
   int* flag;
-  int64_t nseq, total;      // sequences (batch); workgroups' tiles
+  int64_t nseq;             // sequences (batch)
+  uint32_t first, total;    // first tile of a launch; tiles of the call
   int lq, lk;               // dense lengths; packed: all query and key rows
-  int tiles;                // dense: tiles of a sequence; packed: most tiles of a head
-  int hkv, group, d, dv;
+  uint32_t tiles;           // dense: tiles of a sequence; packed: most tiles of a head
+  uint32_t hkv, group;
+  int d, dv;
   int window, sinks;        // window >= 1 (2^31 - 1: all)
   int negate;               // the scale is negative: queries enter with their sign flipped
   float scale;              // |scale| log2 e, > 0
@@ -63,12 +65,20 @@ __device__ __forceinline__ int64_t window_offset(const void* cu, int is64, int64
 // Tile `tl` of the packed rows.  Segment 0 are rows in front of the first offset, segment i sequence i - 1,
 // the last one the rows behind the last offset; the outer two have no keys and become zeros.  Offsets are
 // taken into [0, rows] and as their running maximum, so every row is in one segment whatever they hold.
+template <int ROWS>
 __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lane, WindowTile& t) {
   const int n = (int)a.nseq, segments = n + 2;
   int before = 0, done = 0;  // end of the last segment, tiles so far
   for (int base = 0; base < segments; base += 64) {
     const int i = base + lane;
     const int64_t raw = i <= n ? window_offset(a.cu_q, a.cu_q64, a.cu_q_stride, i) : (int64_t)a.lq;
+    // keys of the lane's segment, fetched along
+    int64_t ks = 0, ke = -1;
+    if (i >= 1 && i <= n) {
+      ks = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, i - 1);
+      ke = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, i);
+    }
+    const bool keys_ok = ks >= 0 && ke >= ks && ke <= a.lk;
     int end = raw < 0 ? 0 : (raw > a.lq ? a.lq : (int)raw);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -79,7 +89,7 @@ __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lan
     if ((end != raw || (i == 0 && raw != 0))) *a.flag = 1;
     int begin = __shfl_up(end, 1, 64);
     if (lane == 0) begin = before;
-    const int mine = (end - begin + kWindowRows - 1) / kWindowRows;
+    const int mine = (end - begin + ROWS - 1) / ROWS;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -93,19 +103,10 @@ __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lan
       const int b = __shfl(begin, f, 64), e = __shfl(end, f, 64), u = __shfl(upto, f, 64), m = __shfl(mine, f, 64);
       t.qrow = b;
       t.ql = e - b;
-      t.i0 = (tl - (u - m)) * kWindowRows;
-      t.krow = 0;
-      t.kl = 0;
-      const int seq = base + f - 1;
-      if (seq >= 0 && seq < n) {
-        const int64_t ks = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, seq), ke = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, seq + 1);
-        if (ks >= 0 && ke >= ks && ke <= a.lk) {
-          t.krow = ks;
-          t.kl = (int)(ke - ks);
-        } else {
-          *a.flag = 1;
-        }
-      }
+      t.i0 = (tl - (u - m)) * ROWS;
+      t.krow = __shfl(keys_ok ? (int)ks : 0, f, 64);
+      t.kl = __shfl(keys_ok ? (int)(ke - ks) : 0, f, 64);
+      if (base + f >= 1 && base + f <= n && !__shfl((int)keys_ok, f, 64)) *a.flag = 1;
       return true;
     }
     before = __shfl(end, 63, 64);
@@ -114,25 +115,37 @@ __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lan
   return false;
 }
 
-template <typename T, int DP, int DVP>
+// DP, DVP: head and value size rounded up to whole fragments; RW row groups of 32 by KW wavefronts that share a
+// row group and take turns at the keys.
+template <typename T, int DP, int DVP, int RW>
 struct WindowShape {
   static constexpr int E = sizeof(T), VEC = 16 / E;
-  static constexpr int BN = E == 2 ? 64 : 32;          // keys of a block
+  static constexpr int KW = 4 / RW;
+  static constexpr int ROWS = 32 * RW;
+  static constexpr int BN = 64;                        // keys of a block
+  static constexpr int NH = BN / 32 / KW;              // 32-key parts of a block that a wavefront takes
+  static constexpr int STAGES = E == 2 ? 2 : 1;        // blocks in LDS
   static constexpr int KCH = DP / VEC, VCH = DVP / VEC;  // 16-byte chunks of a K / V row
-  static constexpr int K_BYTES = BN * DP * E, V_BYTES = BN * DVP * E;
-  static constexpr int KL = BN * KCH / 256, VL = BN * VCH / 256;  // loads per thread and block
+  static constexpr int slots(int chunks) { return chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32); }
+  static constexpr int KS = slots(KCH), VS = slots(VCH);  // ... and their places in LDS
+  static constexpr int K_BYTES = BN * KS * 16, V_BYTES = BN * VS * 16;
+  // A thread loads chunk tid % KS of every (256 / KS)th row (nothing where that is behind the head size).
+  static constexpr int KR = 256 / KS, VR = 256 / VS;
+  static constexpr int KL = BN / KR, VL = BN / VR;
   static constexpr int QF = DP / (2 * VEC);            // fragment steps of a 32x32 score block
-  static constexpr int OF = DVP / 32;
-  static constexpr int NH = BN / 32;
-  static_assert(BN * KCH % 256 == 0 && BN * VCH % 256 == 0, "whole loads");
+  static constexpr int OF = (DVP + 31) / 32;
+  static constexpr int JOIN_BYTES = KW > 1 ? (KW - 1) * RW * 64 * (16 * OF + 2) * 4 : 0;
+  static constexpr int BLOCK_BYTES = STAGES * (K_BYTES + V_BYTES);
+  static constexpr int LDS_BYTES = BLOCK_BYTES > JOIN_BYTES ? BLOCK_BYTES : JOIN_BYTES;
+  static_assert(32 * OF <= VS * VEC, "V fragments stay inside a row");
   // chunk c of K row r: sixteen consecutive rows of one chunk in sixteen different 16-byte slots
   __device__ static __forceinline__ int k_off(int r, int c) {
-    if constexpr (KCH >= 16) return r * (DP * E) + ((c ^ (r & 15)) << 4);
-    else return r * (DP * E) + ((c ^ ((r >> 1) & 7)) << 4);
+    if constexpr (KS >= 16) return (r * KS + (c ^ (r & 15))) << 4;
+    else return (r * KS + (c ^ ((r >> 1) & 7))) << 4;
   }
   __device__ static __forceinline__ int v_off(int r, int col) {
-    if constexpr (E == 2) return lds_off_n<VCH>(r, col);
-    else return lds_off_n32<VCH>(r, col);
+    if constexpr (E == 2) return lds_off_n<VS>(r, col);
+    else return lds_off_n32<VS>(r, col);
   }
 };
 
@@ -179,234 +192,283 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const char* q, c
     if (lane + 64 * i < a.dv) Num<T>::store(reinterpret_cast<T*>(out) + lane + 64 * i, o[i]);
 }
 
-template <int DP, int DVP>
-constexpr int window_waves() { return DP > 128 || DVP > 128 ? 1 : 2; }
-
+// Wavefronts per SIMD that registers are given out for.
 template <typename T, int DP, int DVP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(window_waves<DP, DVP>(), window_waves<DP, DVP>())))
+constexpr int window_waves() { return DP > 128 || DVP > 128 ? 1 : (sizeof(T) == 2 && DP <= 64 && DVP <= 64 ? 3 : 2); }
+
+template <typename T, int DP, int DVP, int RW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP>(), window_waves<T, DP, DVP>())))
 void window_attn_kernel(WindowArgs a) {
-  using F = WindowShape<T, DP, DVP>;
+  using F = WindowShape<T, DP, DVP, RW>;
   constexpr int E = F::E, BN = F::BN, NH = F::NH;
-  __shared__ __attribute__((aligned(16))) char smem[2 * (F::K_BYTES + F::V_BYTES)];
+  __shared__ __attribute__((aligned(16))) char smem[F::LDS_BYTES];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, hf = lane >> 5, l32 = lane & 31;
+  const int rw = w % RW, part = w / RW;  // row group, turn at the keys
   const u32x4_t zero4 = {0u, 0u, 0u, 0u};
 
-  for (int64_t turn = blockIdx.x; turn < a.total; turn += gridDim.x) {
-    // Workgroups are dealt to the 8 XCDs in turn: every XCD takes a run of each kWindowOrder tiles, so that
-    // the heads of a group and neighbouring tiles, which read the same keys, share one L2.
-    int64_t t = turn;
-    {
-      const int64_t first = t / kWindowOrder * kWindowOrder;
-      const int64_t n = a.total - first < kWindowOrder ? a.total - first : kWindowOrder;
-      const int64_t j = t - first;
-      if ((n & 7) == 0) t = first + (j & 7) * (n >> 3) + (j >> 3);
-    }
-    const int g = (int)(t % a.group);
-    t /= a.group;
-    WindowTile tile;
-    int64_t b = 0;
-    int hk;
-    if (a.cu_q) {
-      hk = (int)(t % a.hkv);
-      if (!window_find(a, (int)(t / a.hkv), lane, tile)) continue;
-    } else {
-      tile.i0 = (a.tiles - 1 - (int)(t % a.tiles)) * kWindowRows;  // longest ranges first
-      t /= a.tiles;
-      hk = (int)(t % a.hkv);
-      b = t / a.hkv;
-      tile.qrow = tile.krow = 0;
-      tile.ql = a.lq;
-      tile.kl = a.lk;
-    }
-    const int h = hk * a.group + g;
-    const int kl = tile.kl, qrows = tile.ql - tile.i0 < kWindowRows ? tile.ql - tile.i0 : kWindowRows;
-    const char* const qb = a.q + b * a.qB + (tile.qrow + tile.i0) * a.qT + h * a.qH;
-    const char* const kb = a.k + b * a.kB + tile.krow * a.kT + hk * a.kH;
-    const char* const vb = a.v + b * a.vB + tile.krow * a.vT + hk * a.vH;
-    char* const ob = a.out + b * a.oB + (tile.qrow + tile.i0) * a.oT + h * a.oH;
+  // Workgroups are dealt to the 8 XCDs in turn: every XCD takes a run of each kWindowOrder tiles, so that the
+  // heads of a group and neighbouring tiles, which read the same keys, share one L2.
+  uint32_t t = a.first + blockIdx.x;
+  {
+    const uint32_t first = t / kWindowOrder * kWindowOrder;
+    const uint32_t n = a.total - first < kWindowOrder ? a.total - first : kWindowOrder;
+    const uint32_t j = t - first;
+    if ((n & 7) == 0) t = first + (j & 7) * (n >> 3) + (j >> 3);
+  }
+  const uint32_t g = t % a.group;
+  t /= a.group;
+  WindowTile tile;
+  int64_t b = 0;
+  int hk;
+  if (a.cu_q) {
+    hk = (int)(t % a.hkv);
+    if (!window_find<F::ROWS>(a, (int)(t / a.hkv), lane, tile)) return;
+  } else {
+    tile.i0 = (int)(a.tiles - 1 - t % a.tiles) * F::ROWS;  // longest ranges first
+    t /= a.tiles;
+    hk = (int)(t % a.hkv);
+    b = t / a.hkv;
+    tile.qrow = tile.krow = 0;
+    tile.ql = a.lq;
+    tile.kl = a.lk;
+  }
+  const int h = hk * (int)a.group + (int)g;
+  const int kl = tile.kl, qrows = tile.ql - tile.i0 < F::ROWS ? tile.ql - tile.i0 : F::ROWS;
+  const char* const qb = a.q + b * a.qB + (tile.qrow + tile.i0) * a.qT + h * a.qH;
+  const char* const kb = a.k + b * a.kB + tile.krow * a.kT + hk * a.kH;
+  const char* const vb = a.v + b * a.vB + tile.krow * a.vT + hk * a.vH;
+  char* const ob = a.out + b * a.oB + (tile.qrow + tile.i0) * a.oT + h * a.oH;
 
-    // positions of the tile's first and last row; keys of v: v < ns ? v : v + shift
-    const int p0 = kl - tile.ql + tile.i0, p1 = p0 + qrows - 1;
-    const int64_t begin = (int64_t)p0 - a.window + 1;
-    const int start = begin > 0 ? (int)begin : 0;
-    const int ns = kl > 0 ? (a.sinks < start ? a.sinks : start) : 0;
-    const int shift = start - ns;
-    const int nv = kl > 0 && p1 >= 0 ? p1 + 1 - shift : 0;
-    const int nblk = (nv + BN - 1) / BN;
+  // positions of the tile's first and last row; keys of v: v < ns ? v : v + shift
+  const int p0 = kl - tile.ql + tile.i0, p1 = p0 + qrows - 1;
+  const int64_t begin = (int64_t)p0 - a.window + 1;
+  const int start = begin > 0 ? (int)begin : 0;
+  const int ns = kl > 0 ? (a.sinks < start ? a.sinks : start) : 0;
+  const int shift = start - ns;
+  const int nv = kl > 0 && p1 >= 0 ? p1 + 1 - shift : 0;
+  const int nblk = (nv + BN - 1) / BN;
+  // What a row sees of the counted keys: lo .. hi (its window), and v < sv (sinks; all of those in front of the
+  // first row's window are before every row, the others are among the window's keys and cut off at hi).
+  const int sv = shift > 0 ? ns : a.sinks;
+  auto row_lo = [&](int p) -> int {
+    const int64_t x = (int64_t)p - a.window + 1 - shift;
+    return x > 0 ? (int)x : 0;
+  };
 
-    const int rloc = 32 * w + l32;
-    const bool row_ok = rloc < qrows;
-    const int p = p0 + rloc;                 // this lane's row
-    const int wp0 = p0 + 32 * w;             // first and last position of the wavefront's rows
-    const int wp1 = wp0 + 31 < p1 ? wp0 + 31 : p1;
+  const int rloc = 32 * rw + l32;
+  const bool row_ok = rloc < qrows;
+  const int hi = row_ok ? p0 + rloc - shift : -1;  // negative: nothing
+  const int lo = row_lo(p0 + rloc);
+  const int wlast = 32 * rw + 31 < qrows ? 32 * rw + 31 : qrows - 1;  // last row of the wavefront
+  const bool wany = 32 * rw < qrows;
+  const int wlo0 = row_lo(p0 + 32 * rw), wlo1 = row_lo(p0 + wlast);
+  const int whi0 = p0 + 32 * rw - shift, whi1 = p0 + wlast - shift;
 
-    u32x4_t qf[F::QF];
+  u32x4_t qf[F::QF];
 #pragma unroll
-    for (int c = 0; c < F::QF; ++c) {
-      const int d0 = F::VEC * (2 * c + hf);
-      qf[c] = row_ok && d0 < a.d ? load_16(qb + rloc * a.qT + E * d0) : zero4;
-      if (a.negate) qf[c] ^= E == 2 ? 0x80008000u : 0x80000000u;
-    }
+  for (int c = 0; c < F::QF; ++c) {
+    const int d0 = F::VEC * (2 * c + hf);
+    qf[c] = row_ok && d0 < a.d ? load_16(qb + rloc * a.qT + E * d0) : zero4;
+    if (a.negate) qf[c] ^= E == 2 ? 0x80008000u : 0x80000000u;
+  }
 
-    u32x4_t kr[F::KL], vr[F::VL];
-    auto load = [&](int blk) {
-      const int v0 = blk * BN;
-      const bool whole = v0 >= ns && v0 + BN <= nv && a.d == DP && a.dv == DVP;
-      if (whole) {
-        const char* kp = kb + (int64_t)(v0 + shift) * a.kT;
-        const char* vp = vb + (int64_t)(v0 + shift) * a.vT;
-#pragma unroll
-        for (int i = 0; i < F::KL; ++i) {
-          const int s = tid + 256 * i;
-          kr[i] = load_16(kp + (s / F::KCH) * a.kT + 16 * (s % F::KCH));
-        }
-#pragma unroll
-        for (int i = 0; i < F::VL; ++i) {
-          const int s = tid + 256 * i;
-          vr[i] = load_16(vp + (s / F::VCH) * a.vT + 16 * (s % F::VCH));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < F::KL; ++i) {
-          const int s = tid + 256 * i, v = v0 + s / F::KCH, c = s % F::KCH;
-          kr[i] = v < nv && F::VEC * c < a.d ? load_16(kb + (int64_t)(v < ns ? v : v + shift) * a.kT + 16 * c) : zero4;
-        }
-#pragma unroll
-        for (int i = 0; i < F::VL; ++i) {
-          const int s = tid + 256 * i, v = v0 + s / F::VCH, c = s % F::VCH;
-          vr[i] = v < nv && F::VEC * c < a.dv ? load_16(vb + (int64_t)(v < ns ? v : v + shift) * a.vT + 16 * c) : zero4;
-        }
-      }
-    };
-    auto store = [&](int blk) {
-      char* ks = smem + (blk & 1) * (F::K_BYTES + F::V_BYTES);
+  u32x4_t kr[F::KL], vr[F::VL];
+  const int krow = tid / F::KS, kc = tid % F::KS, vrow0 = tid / F::VS, vc = tid % F::VS;
+  const bool kin = F::VEC * kc < a.d, vin = F::VEC * vc < a.dv;
+  const uint32_t koff = (uint32_t)(krow * (int)a.kT + 16 * kc), voff = (uint32_t)(vrow0 * (int)a.vT + 16 * vc);
+  auto load = [&](int blk) {
+    const int v0 = blk * BN;
+    if (v0 >= ns && v0 + BN <= nv) {
+      const char* kp = kb + (int64_t)(v0 + shift) * a.kT;
+      const char* vp = vb + (int64_t)(v0 + shift) * a.vT;
 #pragma unroll
       for (int i = 0; i < F::KL; ++i) {
-        const int s = tid + 256 * i;
-        *reinterpret_cast<u32x4_t*>(ks + F::k_off(s / F::KCH, s % F::KCH)) = kr[i];
+        kr[i] = zero4;
+        if (kin) kr[i] = load_16(kp + koff);
+        kp += F::KR * a.kT;
       }
 #pragma unroll
       for (int i = 0; i < F::VL; ++i) {
-        const int s = tid + 256 * i;
-        *reinterpret_cast<u32x4_t*>(ks + F::K_BYTES + F::v_off(s / F::VCH, F::VEC * (s % F::VCH))) = vr[i];
+        vr[i] = zero4;
+        if (vin) vr[i] = load_16(vp + voff);
+        vp += F::VR * a.vT;
       }
-    };
-
-    // m: largest score so far (raw), sh = m * scale, l: this lane's part of the row's sum
-    float m = -INFINITY, sh = 0.f, l = 0.f;
-    f32x16_t oacc[F::OF];  // O^T: register r of block e is column 32e + 8(r/4) + 4hf + r%4 of row l32
+    } else {
 #pragma unroll
-    for (int e = 0; e < F::OF; ++e)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[e][r] = 0.f;
-
-    auto block = [&](int blk, auto open) {
-      const char* ks = smem + (blk & 1) * (F::K_BYTES + F::V_BYTES);
-      const char* vs = ks + F::K_BYTES;
-      f32x16_t sc[NH];
-#pragma unroll
-      for (int hb = 0; hb < NH; ++hb) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[hb][r] = 0.f;
-#pragma unroll
-        for (int c = 0; c < F::QF; ++c)
-          Mfma<T>::step(sc[hb], *reinterpret_cast<const u32x4_t*>(ks + F::k_off(32 * hb + l32, 2 * c + hf)), qf[c]);
+      for (int i = 0; i < F::KL; ++i) {
+        const int v = v0 + krow + F::KR * i;
+        kr[i] = v < nv && kin ? load_16(kb + (int64_t)(v < ns ? v : v + shift) * a.kT + 16 * kc) : zero4;
       }
-      if constexpr (!decltype(open)::value) {
 #pragma unroll
-        for (int hb = 0; hb < NH; ++hb)
+      for (int i = 0; i < F::VL; ++i) {
+        const int v = v0 + vrow0 + F::VR * i;
+        vr[i] = v < nv && vin ? load_16(vb + (int64_t)(v < ns ? v : v + shift) * a.vT + 16 * vc) : zero4;
+      }
+    }
+  };
+  auto store = [&](int blk) {
+    char* ks = smem + (F::STAGES > 1 ? blk & 1 : 0) * (F::K_BYTES + F::V_BYTES);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int v = blk * BN + 32 * hb + 8 * (r >> 2) + 4 * hf + (r & 3);
-            const int key = v < ns ? v : v + shift;
-            const bool seen = row_ok && v < nv && key <= p && (p - key < a.window || key < a.sinks);
-            sc[hb][r] = seen ? sc[hb][r] : -INFINITY;
+    for (int i = 0; i < F::KL; ++i) *reinterpret_cast<u32x4_t*>(ks + F::k_off(krow + F::KR * i, kc)) = kr[i];
+#pragma unroll
+    for (int i = 0; i < F::VL; ++i)
+      *reinterpret_cast<u32x4_t*>(ks + F::K_BYTES + F::v_off(vrow0 + F::VR * i, F::VEC * vc)) = vr[i];
+  };
+
+  // m: largest score so far (raw), sh = m * scale, l: this lane's part of the row's sum
+  float m = -INFINITY, sh = 0.f, l = 0.f;
+  f32x16_t oacc[F::OF];  // O^T: register r of block e is column 32e + 8(r/4) + 4hf + r%4 of row l32
+#pragma unroll
+  for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) oacc[e][r] = 0.f;
+
+  // 32-key parts hb0 .. hb0 + NH - 1 of a block
+  auto block = [&](int blk, int hb0, bool open) {
+    const char* ks = smem + (F::STAGES > 1 ? blk & 1 : 0) * (F::K_BYTES + F::V_BYTES);
+    const char* vs = ks + F::K_BYTES;
+    f32x16_t sc[NH];
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      const int hb = hb0 + x;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[x][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < F::QF; ++c)
+        Mfma<T>::step(sc[x], *reinterpret_cast<const u32x4_t*>(ks + F::k_off(32 * hb + l32, 2 * c + hf)), qf[c]);
+    }
+    if (!open) {
+      const int vb0 = blk * BN + 32 * hb0 + 4 * hf;  // register r of part x: key vb0 + 32 x + 8(r/4) + r%4
+      const int from = lo - vb0, to = hi - vb0, sink = sv - vb0;
+#pragma unroll
+      for (int x = 0; x < NH; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int o = 32 * x + 8 * (r >> 2) + (r & 3);
+          sc[x][r] = o <= to && (o >= from || o < sink) ? sc[x][r] : -INFINITY;
+        }
+    }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int x = 0; x < NH; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[x][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    if (__any(mx > m)) {
+      const float mn = fmaxf(m, mx);
+      const float to = mn == -INFINITY ? 0.f : mn * a.scale;
+      const float corr = mx > m ? (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - to)) : 1.f;
+      l *= corr;
+#pragma unroll
+      for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[e][r] *= corr;
+      m = mn;
+      sh = to;
+    }
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      const int hb = hb0 + x;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        sc[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][r], a.scale, -sh));
+        l += sc[x][r];
+      }
+      if constexpr (E == 4) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int e = 0; e < F::OF; ++e)
+            oacc[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                *reinterpret_cast<const float*>(vs + F::v_off(32 * hb + 8 * (r >> 2) + 4 * hf + (r & 3), 32 * e + l32)),
+                sc[x][r], oacc[e], 0, 0, 0);
+      } else {
+        // transposing reads: lane s of a 16-lane group points at row k0 + s/4, column n0 + 4(s%4), and
+        // receives rows k0 .. k0+3 of column n0 + s
+        const int vrow = 4 * hf + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) {
+          u32x4_t pb;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x0 = sc[x][8 * c2 + 2 * i], x1 = sc[x][8 * c2 + 2 * i + 1];
+            if constexpr (std::is_same<T, bf16_t>::value) pb[i] = f32x2_to_bf16x2_bits(x0, x1);
+            else pb[i] = (uint32_t)f32_to_f16_bits(x0) | ((uint32_t)f32_to_f16_bits(x1) << 16);
           }
+          const int row = 32 * hb + 16 * c2 + vrow;
+#pragma unroll
+          for (int e = 0; e < F::OF; ++e) {
+            const u32x2_t x0 = lds_read_tr16(vs + F::v_off(row, 32 * e + vcol));
+            const u32x2_t x1 = lds_read_tr16(vs + F::v_off(row + 8, 32 * e + vcol));
+            Mfma<T>::step(oacc[e], u32x4_t{x0[0], x0[1], x1[0], x1[1]}, pb);
+          }
+        }
       }
-      float mx = sc[0][0];
+    }
+  };
+
+  if (nblk > 0) {
+    load(0);
+    store(0);
+  }
+  __syncthreads();
+  for (int blk = 0; blk < nblk; ++blk) {
+    if (blk + 1 < nblk) load(blk + 1);
+    // this wavefront's keys of the block: seen by any of its rows, by all of them
+    const int v0 = blk * BN + 32 * NH * part, v1 = v0 + 32 * NH - 1;
+    const bool some = wany && v0 <= whi1 && (v1 >= wlo0 || v0 < sv);
+    const bool all = wlast == 32 * rw + 31 && v0 >= wlo1 && v1 <= whi0;
+    if (some) block(blk, NH * part, all);
+    if constexpr (F::STAGES == 1) __syncthreads();
+    if (blk + 1 < nblk) store(blk + 1);
+    __syncthreads();
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (F::KW > 1) {  // join the wavefronts of a row group, in order
+    float* const js = reinterpret_cast<float*>(smem);
+    if (part > 0) {
+      float* o = js + ((part - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane;
 #pragma unroll
-      for (int hb = 0; hb < NH; ++hb)
+      for (int e = 0; e < F::OF; ++e)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[hb][r]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      if (__any(mx > m)) {
-        const float mn = fmaxf(m, mx);
-        const float to = mn == -INFINITY ? 0.f : mn * a.scale;
-        const float corr = mx > m ? (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - to)) : 1.f;
-        l *= corr;
+        for (int r = 0; r < 16; ++r) o[64 * (16 * e + r)] = oacc[e][r];
+      o[64 * 16 * F::OF] = m == -INFINITY ? m : sh;
+      o[64 * (16 * F::OF + 1)] = l;
+    }
+    __syncthreads();
+    if (part == 0) {
+      float top = m == -INFINITY ? m : sh;
+#pragma unroll
+      for (int x = 1; x < F::KW; ++x) top = fmaxf(top, js[((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane + 64 * 16 * F::OF]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float own = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - base);
+      l *= own;
+#pragma unroll
+      for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[e][r] *= own;
+#pragma unroll
+      for (int x = 1; x < F::KW; ++x) {
+        const float* o = js + ((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane;
+        const float f = __builtin_amdgcn_exp2f(o[64 * 16 * F::OF] - base);
+        l = __builtin_fmaf(o[64 * (16 * F::OF + 1)], f, l);
 #pragma unroll
         for (int e = 0; e < F::OF; ++e)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) oacc[e][r] *= corr;
-        m = mn;
-        sh = to;
+          for (int r = 0; r < 16; ++r) oacc[e][r] = __builtin_fmaf(o[64 * (16 * e + r)], f, oacc[e][r]);
       }
-#pragma unroll
-      for (int hb = 0; hb < NH; ++hb) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          sc[hb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[hb][r], a.scale, -sh));
-          l += sc[hb][r];
-        }
-        if constexpr (E == 4) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int e = 0; e < F::OF; ++e)
-              oacc[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                  *reinterpret_cast<const float*>(vs + F::v_off(32 * hb + 8 * (r >> 2) + 4 * hf + (r & 3), 32 * e + l32)),
-                  sc[hb][r], oacc[e], 0, 0, 0);
-        } else {
-          // transposing reads: lane s of a 16-lane group points at row k0 + s/4, column n0 + 4(s%4), and
-          // receives rows k0 .. k0+3 of column n0 + s
-          const int vrow = 4 * hf + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-#pragma unroll
-          for (int c2 = 0; c2 < 2; ++c2) {
-            u32x4_t pb;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x = sc[hb][8 * c2 + 2 * i], y = sc[hb][8 * c2 + 2 * i + 1];
-              if constexpr (std::is_same<T, bf16_t>::value) pb[i] = f32x2_to_bf16x2_bits(x, y);
-              else pb[i] = (uint32_t)f32_to_f16_bits(x) | ((uint32_t)f32_to_f16_bits(y) << 16);
-            }
-            const int row = 32 * hb + 16 * c2 + vrow;
-#pragma unroll
-            for (int e = 0; e < F::OF; ++e) {
-              const u32x2_t lo = lds_read_tr16(vs + F::v_off(row, 32 * e + vcol));
-              const u32x2_t hi = lds_read_tr16(vs + F::v_off(row + 8, 32 * e + vcol));
-              Mfma<T>::step(oacc[e], u32x4_t{lo[0], lo[1], hi[0], hi[1]}, pb);
-            }
-          }
-        }
-      }
-    };
-
-    if (nblk > 0) {
-      load(0);
-      store(0);
     }
-    __syncthreads();
-    for (int blk = 0; blk < nblk; ++blk) {
-      if (blk + 1 < nblk) load(blk + 1);
-      const int v0 = blk * BN, v1 = v0 + BN - 1;
-      const int k0 = v0 < ns ? v0 : v0 + shift, k1 = v1 < ns ? v1 : v1 + shift;  // first and last key
-      // any row of the wavefront sees a key / all rows see all of them
-      const bool some = 32 * w < qrows && k0 <= wp1 && (v0 < ns || k0 < a.sinks || (int64_t)k1 > (int64_t)wp0 - a.window);
-      const bool all = 32 * w + 31 < qrows && v1 < nv && k1 <= wp0 && v0 >= ns && (int64_t)wp1 - k0 < a.window;
-      if (all) block(blk, std::true_type{});
-      else if (some) block(blk, std::false_type{});
-      if (blk + 1 < nblk) store(blk + 1);
-      __syncthreads();
-    }
-
-    l += __shfl_xor(l, 32, 64);
+  }
+  if (part == 0) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bool lost = false;  // an output that is not finite over a finite sum
     if (l > 0.f && l < INFINITY) {
 #pragma unroll
       for (int e = 0; e < F::OF; ++e)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) lost |= !(fabsf(oacc[e][r]) < INFINITY);
+        for (int r = 0; r < 16; ++r)  // (columns behind the value size hold anything)
+          lost |= 32 * e + 8 * (r >> 2) + 4 * hf < a.dv && !(fabsf(oacc[e][r]) < INFINITY);
     }
     const uint64_t again = __ballot(lost && row_ok);
     const bool mine_again = (again >> l32 | again >> (l32 + 32)) & 1;
@@ -434,25 +496,55 @@ void window_attn_kernel(WindowArgs a) {
         }
     }
     for (uint64_t rest = (again | again >> 32) & 0xffffffffull; rest != 0; rest &= rest - 1) {
-      const int r = 32 * w + __builtin_ctzll(rest);
+      const int r = 32 * rw + __builtin_ctzll(rest);
       window_row<T>(a, qb + r * a.qT, kb, vb, ob + r * a.oT, p0 + r, kl, lane);
     }
   }
 }
 
-template <typename T, int DP, int DVP>
-static int window_launch(const WindowArgs& a, hipStream_t s) {
-  const int64_t most = 1 << 22;  // a multiple of kWindowOrder; further tiles by the kernel's own loop
-  hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP>), dim3((unsigned)(a.total < most ? a.total : most)), dim3(256), 0, s, a);
-  return check_launch("window_attn_kernel");
+template <typename T, int DP, int DVP, int RW>
+static int window_launch(WindowArgs a, hipStream_t s) {
+  constexpr int rows = 32 * RW;
+  // packed: every sequence and the two ends may end in a part of a tile
+  const int64_t tiles = a.cu_q ? a.lq / rows + a.nseq + 2 : cdiv(a.lq, rows);
+  const int64_t heads = (int64_t)a.hkv * a.group * (a.cu_q ? 1 : a.nseq);
+  if (tiles > INT64_C(0x7fffffff) / heads) return fail(BIOPS_ERR_ARG, "biops_window_attention: more than 2^31 tiles");
+  a.tiles = (uint32_t)tiles;
+  a.total = (uint32_t)(tiles * heads);
+  constexpr uint32_t most = 1 << 22;  // a launch has less than 2^32 threads
+  for (a.first = 0; a.first < a.total; a.first += most) {
+    const uint32_t n = a.total - a.first < most ? a.total - a.first : most;
+    hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW>), dim3(n), dim3(256), 0, s, a);
+    const int rc = check_launch("window_attn_kernel");
+    if (rc != BIOPS_OK) return rc;
+  }
+  return BIOPS_OK;
+}
+// Rows per workgroup.  Only sizes that all sequences of a call share may enter: the rows of a tile decide where
+// its blocks of keys begin, and so the bits.
+template <typename T, int DP>
+static int window_launch_rows(const WindowArgs& a, hipStream_t s) {
+  if constexpr (sizeof(T) == 4) {
+    return window_launch<T, DP, DP, 2>(a, s);
+  } else if constexpr (DP > 128) {
+    return window_launch<T, DP, DP, 4>(a, s);
+  } else {
+    if ((int64_t)a.window + a.sinks <= kWindowShort) return window_launch<T, DP, DP, 2>(a, s);
+    return window_launch<T, DP, DP, 4>(a, s);
+  }
 }
 template <typename T>
 static int window_launch_d(const WindowArgs& a, hipStream_t s) {
+  const int d = a.d > a.dv ? a.d : a.dv;
   if constexpr (sizeof(T) == 2) {
-    if (a.d > 128 || a.dv > 128) return window_launch<T, 256, 256>(a, s);
+    if (d > 128) return window_launch_rows<T, 256>(a, s);
   }
-  if (a.d <= 64 && a.dv <= 64) return window_launch<T, 64, 64>(a, s);
-  return window_launch<T, 128, 128>(a, s);
+  if (d <= 64) return window_launch_rows<T, 64>(a, s);
+  if constexpr (sizeof(T) == 4) {
+    if (d <= 80) return window_launch_rows<T, 80>(a, s);
+  }
+  if (d <= 96) return window_launch_rows<T, 96>(a, s);
+  return window_launch_rows<T, 128>(a, s);
 }
 
 }  // namespace biops
@@ -480,6 +572,9 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   if (!(scale - scale == 0.f)) return fail(BIOPS_ERR_ARG, "biops_window_attention: scale is not finite");
   const int64_t longest = INT64_C(0x7fffffff) - 1024;  // tiles and blocks may round positions up
   if (lq > longest || lk > longest || nseq > longest) return fail(BIOPS_ERR_ARG, "biops_window_attention: more than 2^31 rows");
+  // a block's rows are addressed by 32-bit offsets
+  if (skT < 0 || svT < 0 || skT > (1 << 23) || svT > (1 << 23))
+    return fail(BIOPS_ERR_LAYOUT, "biops_window_attention: key and value rows more than 2^23 elements apart");
   if (hq == 0 || lq == 0 || (!cu_q && nseq == 0)) return BIOPS_OK;
   if (!q || !out || (lk > 0 && (!k || !v)) || (cu_q && (!cu_k || !flag)))
     return fail(BIOPS_ERR_ARG, "biops_window_attention: null pointer");
@@ -495,7 +590,7 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   a.flag = flag;
   a.nseq = nseq;
   a.lq = (int)lq, a.lk = (int)lk;
-  a.hkv = (int)hkv, a.group = (int)(hq / hkv);
+  a.hkv = (uint32_t)hkv, a.group = (uint32_t)(hq / hkv);
   a.d = (int)d, a.dv = (int)dv;
   const int64_t all = INT64_C(0x7fffffff);
   a.window = (int)(window < all ? window : all), a.sinks = (int)(sinks < all ? sinks : all);
@@ -503,11 +598,6 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   // a scale of zero: every weight 1, and 0 * -inf stays out of the masked scores
   const float s = (scale < 0.f ? -scale : scale) * kLog2e;
   a.scale = s > 1e-30f ? s : 1e-30f;
-  // packed: every sequence and the two ends may end in a part of a tile
-  const int64_t tiles = cu_q ? lq / kWindowRows + nseq + 2 : cdiv(lq, kWindowRows);
-  if (tiles > all) return fail(BIOPS_ERR_ARG, "biops_window_attention: too many sequences");
-  a.tiles = (int)tiles;
-  a.total = tiles * hq * (cu_q ? 1 : nseq);
   BIOPS_DISPATCH_FLOAT(dtype, return window_launch_d<T>(a, static_cast<hipStream_t>(stream)));
   return BIOPS_OK;
 }
