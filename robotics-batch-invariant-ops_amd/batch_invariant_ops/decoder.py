@@ -21,6 +21,7 @@ from __future__ import annotations
 import functools
 import math
 import threading
+import time
 from collections.abc import Sequence
 
 import numpy as np
@@ -49,6 +50,20 @@ class _CacheWatch(_IndexWatch):
     _by_device: dict = {}
     _lock = threading.Lock()
 
+    def __init__(self, device: torch.device):
+        super().__init__(device)
+        self.flag_at = self.flag.data_ptr()
+
+    def poll(self) -> None:
+        """As the base class, but a copy in flight is asked after once per PERIOD (an event query costs as
+        much as the rest of a small call's host time)."""
+        if self.pending and time.monotonic() - self.last >= self.PERIOD:
+            super().poll()
+
+    def after_call(self, stream: int | None = None) -> None:
+        if not self.pending and time.monotonic() - self.last >= self.PERIOD:
+            super().after_call(nat.stream_of(self.flag) if stream is None else stream)
+
 
 def check_cache_indices(device: torch.device | int | None = None) -> None:
     """Raise ``RuntimeError`` if a call of this module on ``device`` (default: the current device) met an
@@ -60,6 +75,37 @@ def check_cache_indices(device: torch.device | int | None = None) -> None:
         device = torch.device("cuda", device)
     with torch.cuda.device(device):
         _CacheWatch.of(device).check()
+
+
+_tensor_module = None  # csrc/tensorfast.cpp: False without it or without a GPU
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def _direct():
+    """The module that takes tensors as they are, or False."""
+    global _tensor_module
+    if _tensor_module is None:
+        if _current_device is None or not torch.cuda.is_available():
+            return False
+        nat.load()
+        torch.cuda.current_device()  # torch's own initialisation
+        try:
+            from . import _biops_tensor
+        except ImportError:
+            _biops_tensor = False
+        _tensor_module = _biops_tensor
+    return _tensor_module
+
+
+def _direct_watch():
+    """(module, watch of the current device): a pair of None until a call has set both up."""
+    module = _tensor_module or _direct()
+    if module:
+        watch = _CacheWatch._by_device.get(_current_device())
+        if watch is not None:
+            watch.poll()
+            return module, watch
+    return None, None
 
 
 def _watch(device: torch.device) -> _CacheWatch:
@@ -79,6 +125,8 @@ def _check_tensors(what: str, *tensors) -> torch.device:
     for t in tensors:
         if t.device != device:
             raise ValueError(f"{what}: tensors on {device} and {t.device}")
+        if t.is_neg():
+            raise ValueError(f"{what}: a lazily negated tensor (call resolve_neg)")
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
@@ -194,7 +242,8 @@ class _Rotary(torch.autograd.Function):
         grad_q = grad_q if ctx.needs_input_grad[0] else None
         grad_k = grad_k if ctx.needs_input_grad[1] else None
         if grad_q is not None or grad_k is not None:
-            grad_q, grad_k = _Rotary.apply(grad_q, grad_k, positions, ctx.plan, not ctx.inverse)
+            turn = _Rotary.apply if torch.is_grad_enabled() else _rotate  # (with create_graph, or without)
+            grad_q, grad_k = turn(grad_q, grad_k, positions, ctx.plan, not ctx.inverse)
         return grad_q, grad_k, None, None, None
 
 
@@ -226,6 +275,13 @@ def multi_axis_rotary(
     tensors ``(query, key)``, or the rotated query alone when ``key`` is None.  Differentiable with respect
     to ``query`` and ``key``.
     """
+    plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(inv_freq),
+                        bool(interleaved_axes), bool(interleaved_pairs))
+    module = _tensor_module or _direct()
+    if module:
+        out = module.rotary(query, key, positions, len(sections), plan.pairs, plan.turns_at, plan.axis_at, plan.neighbours)
+        if out is not None:
+            return out
     tensors = (query,) if key is None else (query, key)
     for x in tensors:
         if x.dim() < 2:
@@ -235,8 +291,6 @@ def multi_axis_rotary(
     if key is not None and (key.dtype != query.dtype or key.shape[:-2] != query.shape[:-2]
                             or key.shape[-1] != query.shape[-1]):
         raise ValueError("query and key must share dtype, leading dimensions and head dimension")
-    plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(inv_freq),
-                        bool(interleaved_axes), bool(interleaved_pairs))
     if 2 * plan.pairs > query.shape[-1]:
         raise ValueError(f"{plan.pairs} pairs do not fit a head of {query.shape[-1]}")
     if positions.dtype not in _POSITION_CODE:
@@ -246,6 +300,8 @@ def multi_axis_rotary(
     nat.require_gpu_tensors(*tensors, positions)
     if any(x.device != query.device for x in (*tensors, positions)):
         raise ValueError("query, key and positions must be on one device")
+    if any(x.is_neg() for x in (*tensors, positions)):
+        raise ValueError("multi_axis_rotary: a lazily negated tensor (call resolve_neg)")
     if query.device.index != torch.cuda.current_device():
         with torch.cuda.device(query.device):
             return multi_axis_rotary(query, key, positions, sections, base=base, inv_freq=inv_freq,
@@ -309,6 +365,10 @@ def paged_cache_write(
     place``.  A negative slot leaves its row out (padding).  A slot past the cache is left out too and reported
     as an error later (see the module).  Of several rows that name one slot the last one stays.
     """
+    module, watch = _direct_watch()
+    if module and module.paged_write(key, value, key_cache, value_cache, slots, watch.flag_at):
+        watch.after_call()
+        return
     _check_caches(key_cache, value_cache)
     if key.dim() < 2 or value.dim() != key.dim() or key.shape[:-1] != value.shape[:-1]:
         raise ValueError("key and value must have shapes [..., kv_heads, dim] with the same leading dimensions")
@@ -390,6 +450,14 @@ def paged_attention_batch_invariant(
     Scores, softmax and sums are in 32 bits, with one rounding to the output's type; 16-bit products take
     the weights as two 16-bit parts.  Returns ``[batch, heads, value_dim]``.
     """
+    module, watch = _direct_watch()
+    if module and window != 0 and (max_length is None or max_length >= 0):
+        out = module.paged_attention(query, key_cache, value_cache, block_table, lengths, scale,
+                                     0 if window is None else window, sinks, -1 if max_length is None else max_length,
+                                     watch.flag_at)
+        if out is not None:
+            watch.after_call()
+            return out
     _check_caches(key_cache, value_cache)
     if query.dim() != 3:
         raise ValueError(f"query must have shape [batch, heads, head_dim], got {tuple(query.shape)}")
@@ -441,8 +509,12 @@ def paged_attention_batch_invariant(
 
 
 # ---------------------------------------------------------------------- windowed attention ----
+_MOST_ROW_STRIDE = 1 << 23  # elements between key rows that the kernel's 32-bit offsets inside a block take
+
+
 def _windowed(q, k, v, out, nseq, lengths, window_size, sinks, scale, offsets, watch):
     """biops_window_attention on tensors of [batch, tokens, heads, dim] strides."""
+    k, v = (t if t.stride(1) <= _MOST_ROW_STRIDE else t.contiguous() for t in (k, v))
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
     d = q.shape[-1]
     if offsets is None:
@@ -479,6 +551,11 @@ def sliding_window_attention_batch_invariant(
     in 32 bits; 16-bit products take weights rounded to the type.  Output rows depend on their own sequence
     only.
     """
+    module = _tensor_module or _direct()
+    if module:
+        out = module.window_attention(query, key, value, 0x7FFFFFFF if window is None else window, sinks, scale, enable_gqa)
+        if out is not None:
+            return out
     if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
         raise ValueError("sliding-window attention expects rank-4 query, key, and value")
     if query.dtype != key.dtype or query.dtype != value.dtype:
@@ -533,6 +610,13 @@ def varlen_sliding_window_attention_batch_invariant(
     start at zero or exceed their tensor are reported as an error later (see the module); the rows they
     concern are unspecified, and nothing outside of the tensors is read or written.
     """
+    module, watch = _direct_watch()
+    if module:
+        out = module.window_packed(query, key, value, cumulative_seqlen_q, cumulative_seqlen_kv,
+                                   0x7FFFFFFF if window is None else window, sinks, scale, watch.flag_at)
+        if out is not None:
+            watch.after_call()
+            return out
     if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
         raise ValueError("varlen attention expects rank-4 query, key, and value")
     if query.shape[0] != 1 or key.shape[0] != 1 or value.shape[0] != 1:

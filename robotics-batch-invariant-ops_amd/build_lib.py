@@ -5,7 +5,8 @@
 Each csrc/*.hip file is compiled to an object with hipcc for gfx950, then linked into
 batch_invariant_ops/libbiops.so next to the Python package that loads it.  csrc/pyfast.c, a
 CPython fast-call binding of the most frequent entry points, is compiled with the host C
-compiler into batch_invariant_ops/_biops_fast (linked against libbiops.so beside it).
+compiler into batch_invariant_ops/_biops_fast (linked against libbiops.so beside it), and
+csrc/tensorfast.cpp, the decoder operators on torch tensors, against torch into _biops_tensor.
 """
 
 from __future__ import annotations
@@ -78,6 +79,8 @@ def build(jobs: int | None = None, verbose: bool = True, incremental: bool = Fal
         raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, OUT)
     _build_fast()
+    if not incremental or _stale_tensor():
+        _build_tensor()
     if verbose:
         print(f"built {OUT} from {len(sources)} sources", file=sys.stderr)
     return OUT
@@ -97,6 +100,43 @@ def _build_fast() -> pathlib.Path:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"fast-call module build failed:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
+def _tensor_path() -> pathlib.Path:
+    import sysconfig
+
+    return OUT.parent / ("_biops_tensor" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _stale_tensor() -> bool:
+    out, deps = _tensor_path(), [CSRC / "tensorfast.cpp", *(ROOT.parent / "include").glob("*.h")]
+    return not out.exists() or out.stat().st_mtime < max(d.stat().st_mtime for d in deps)
+
+
+def _build_tensor() -> pathlib.Path:
+    """The decoder operators on torch tensors, next to libbiops.so (rpath $ORIGIN)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    out = _tensor_path()
+    tmp = out.with_suffix(".tmp")
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no host C++ compiler for the tensor module")
+    libs = pathlib.Path(torch.__file__).resolve().parent / "lib"
+    rocm = pathlib.Path(hipcc()).resolve().parent.parent
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in [*include_paths(), str(rocm / "include"), sysconfig.get_paths()["include"]]),
+           str(CSRC / "tensorfast.cpp"), f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip",
+           f"-L{OUT.parent}", "-l:libbiops.so", "-Wl,-rpath,$ORIGIN", "-o", str(tmp)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"tensor module build failed:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, out)
     return out
 

@@ -1,0 +1,277 @@
+// The decoder operators on torch tensors without Python's per-attribute costs (about 0.1 us each, and
+// some sixty of them in a call): a call whose tensors are as the kernels take them is checked, given its
+// output and workspace, and launched here.  Every function returns None where it does not take the call
+// as it is -- other layouts, empty tensors, what needs a gradient, and everything that is refused: the
+// Python functions then do what is left, and raise the errors.  Optional: without this module they do all.
+#define PY_SSIZE_T_CLEAN
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+
+#include "../../include/biops.h"
+
+namespace {
+
+int type_code(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return BIOPS_F32;
+    case at::kHalf: return BIOPS_F16;
+    case at::kBFloat16: return BIOPS_BF16;
+    default: return -1;
+  }
+}
+bool is_index(const at::Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+int is_long(const at::Tensor& t) { return t.scalar_type() == at::kLong ? 1 : 0; }
+bool unit_last(const at::Tensor& t) { return t.stride(-1) == 1; }
+
+// A plain tensor with elements on the current device that needs no gradient here.
+const at::Tensor* take(PyObject* o, c10::DeviceIndex device) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.get_device() != device || t.numel() == 0 || t.is_neg()) return nullptr;
+  if (c10::GradMode::is_enabled() && t.requires_grad()) return nullptr;
+  return &t;
+}
+bool number(PyObject* o, int64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int over = 0;
+  *v = PyLong_AsLongLongAndOverflow(o, &over);
+  return over == 0;
+}
+// A float, or None for 1 / sqrt(d).
+bool scale_of(PyObject* o, int64_t d, float* v) {
+  if (o == Py_None) {
+    *v = (float)(1.0 / std::sqrt((double)d));
+    return true;
+  }
+  if (!PyFloat_CheckExact(o)) return false;
+  *v = (float)PyFloat_AS_DOUBLE(o);
+  return std::isfinite(*v);
+}
+void* stream_on(c10::DeviceIndex device) { return (void*)c10::hip::getCurrentHIPStream(device).stream(); }
+char* ptr(const at::Tensor& t) { return static_cast<char*>(t.data_ptr()); }
+
+#define TAKE(name, object)                              \
+  const at::Tensor* name##_ = take(object, device);     \
+  if (!name##_) Py_RETURN_NONE;                         \
+  const at::Tensor& name = *name##_
+
+#define LAUNCH(rc, call)   \
+  int rc;                  \
+  Py_BEGIN_ALLOW_THREADS   \
+  rc = (call);             \
+  Py_END_ALLOW_THREADS
+
+// rotary(query, key or None, positions, axes, pairs, turns, axis, neighbours) -> query or (query, key)
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 8) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(q, args[0]);
+  const bool both = args[1] != Py_None;
+  const at::Tensor* k = both ? take(args[1], device) : nullptr;
+  if (both && !k) Py_RETURN_NONE;
+  TAKE(p, args[2]);
+  int64_t axes, pairs, turns, axis, neighbours;
+  if (!number(args[3], &axes) || !number(args[4], &pairs) || !number(args[5], &turns) || !number(args[6], &axis) ||
+      !number(args[7], &neighbours))
+    Py_RETURN_NONE;
+  const int64_t nd = q.dim();
+  const int code = type_code(q.scalar_type());
+  if ((nd != 3 && nd != 4) || code < 0 || !unit_last(q) || 2 * pairs > q.size(-1)) Py_RETURN_NONE;
+  const int lead = (int)nd - 2;
+  const int pos = p.scalar_type() == at::kLong ? 0 : p.scalar_type() == at::kInt ? 1 : p.scalar_type() == at::kFloat ? 2 : -1;
+  if (pos < 0 || p.dim() != lead + 1 || p.size(0) != axes) Py_RETURN_NONE;
+  for (int i = 0; i < lead; ++i)
+    if (p.size(i + 1) != q.size(i)) Py_RETURN_NONE;
+  if (both) {
+    if (k->dim() != nd || k->scalar_type() != q.scalar_type() || !unit_last(*k) || k->size(-1) != q.size(-1)) Py_RETURN_NONE;
+    for (int i = 0; i < lead; ++i)
+      if (k->size(i) != q.size(i)) Py_RETURN_NONE;
+  }
+  at::Tensor oq = at::empty_like(q);
+  at::Tensor ok = both ? at::empty_like(*k) : at::Tensor();
+  if (!unit_last(oq) || (both && !unit_last(ok))) Py_RETURN_NONE;
+  const bool four = nd == 4;
+  auto batch = [four](const at::Tensor& t) { return four ? t.stride(0) : (int64_t)0; };
+  LAUNCH(rc, biops_rotary(code, four ? q.size(0) : 1, q.size(-3), q.size(-2), both ? k->size(-2) : 0, q.size(-1),
+                          ptr(q), batch(q), q.stride(-3), q.stride(-2), ptr(oq), batch(oq), oq.stride(-3), oq.stride(-2),
+                          both ? ptr(*k) : nullptr, both ? batch(*k) : 0, both ? k->stride(-3) : 0,
+                          both ? k->stride(-2) : 0, both ? ptr(ok) : nullptr, both ? batch(ok) : 0,
+                          both ? ok.stride(-3) : 0, both ? ok.stride(-2) : 0, ptr(p), pos, p.stride(0),
+                          four ? p.stride(1) : 0, p.stride(-1), pairs, reinterpret_cast<const double*>(turns),
+                          reinterpret_cast<const uint8_t*>(axis), (int)neighbours, 0, stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  if (!both) return THPVariable_Wrap(std::move(oq));
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(oq)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(ok)));
+  return pair;
+}
+
+bool caches(const at::Tensor& kc, const at::Tensor& vc) {
+  if (kc.dim() != 4 || vc.dim() != 4 || kc.scalar_type() != vc.scalar_type() || !unit_last(kc) || !unit_last(vc)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (kc.size(i) != vc.size(i)) return false;
+  return true;
+}
+
+// paged_write(key, value, key_cache, value_cache, slots, flag) -> True
+PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(k, args[0]);
+  TAKE(v, args[1]);
+  TAKE(kc, args[2]);
+  TAKE(vc, args[3]);
+  TAKE(slots, args[4]);
+  int64_t flag;
+  const int code = type_code(k.scalar_type());
+  if (!number(args[5], &flag) || code < 0 || !caches(kc, vc) || k.scalar_type() != kc.scalar_type() ||
+      v.scalar_type() != kc.scalar_type())
+    Py_RETURN_NONE;
+  // (an overlapping cache is refused in Python)
+  if (!kc.is_non_overlapping_and_dense() || !vc.is_non_overlapping_and_dense()) Py_RETURN_NONE;
+  if (k.dim() != 3 || v.dim() != 3 || !unit_last(k) || !unit_last(v) || k.size(0) != v.size(0) || k.size(1) != kc.size(2) ||
+      v.size(1) != kc.size(2) || k.size(2) != kc.size(3) || v.size(2) != vc.size(3))
+    Py_RETURN_NONE;
+  if (slots.dim() != 1 || !is_index(slots) || slots.size(0) != k.size(0)) Py_RETURN_NONE;
+  LAUNCH(rc, biops_paged_write(code, k.size(0), k.size(1), k.size(2), v.size(2), ptr(k), k.stride(0), k.stride(1), ptr(v),
+                               v.stride(0), v.stride(1), ptr(kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr(vc),
+                               vc.stride(0), vc.stride(1), vc.stride(2), kc.size(0), kc.size(1), ptr(slots),
+                               is_long(slots), slots.stride(0), reinterpret_cast<int*>(flag), stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+}
+
+// paged_attention(query, key_cache, value_cache, table, lengths, scale or None, window or 0, sinks, max_length or -1,
+//                 flag) -> output
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 10) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(q, args[0]);
+  TAKE(kc, args[1]);
+  TAKE(vc, args[2]);
+  TAKE(table, args[3]);
+  TAKE(lengths, args[4]);
+  int64_t window, sinks, bound, flag;
+  float scale;
+  const int code = type_code(q.scalar_type());
+  if (code < 0 || q.dim() != 3 || !unit_last(q) || !caches(kc, vc) || q.scalar_type() != kc.scalar_type()) Py_RETURN_NONE;
+  const int64_t batch = q.size(0), hq = q.size(1), hkv = kc.size(2), d = q.size(2), dv = vc.size(3);
+  if (!scale_of(args[5], d, &scale) || !number(args[6], &window) || !number(args[7], &sinks) || !number(args[8], &bound) ||
+      !number(args[9], &flag) || window < 0 || sinks < 0)
+    Py_RETURN_NONE;
+  if (d != kc.size(3) || hq % hkv != 0 || table.dim() != 2 || table.size(0) != batch || !is_index(table) ||
+      lengths.dim() != 1 || lengths.size(0) != batch || !is_index(lengths))
+    Py_RETURN_NONE;
+  const int64_t page = kc.size(1), width = table.size(1);
+  const int64_t need = biops_paged_attention_workspace_size(batch, hq, dv, width, page, bound, window, sinks);
+  if (need < 0) Py_RETURN_NONE;
+  at::Tensor out = at::empty({batch, hq, dv}, q.options());
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, q.options().dtype(at::kByte));
+  LAUNCH(rc, biops_paged_attention(code, batch, hq, hkv, d, dv, ptr(q), q.stride(0), q.stride(1), ptr(kc), kc.stride(0),
+                                   kc.stride(1), kc.stride(2), ptr(vc), vc.stride(0), vc.stride(1), vc.stride(2),
+                                   kc.size(0), page, ptr(table), is_long(table), table.stride(0), table.stride(1), width,
+                                   ptr(lengths), is_long(lengths), lengths.stride(0), bound, window, sinks, scale, ptr(out),
+                                   reinterpret_cast<int*>(flag), need > 0 ? ptr(ws) : nullptr, need, stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// window_attention(query, key, value, window, sinks, scale or None, enable_gqa) -> output   [batch, heads, tokens, dim]
+PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(q, args[0]);
+  TAKE(k, args[1]);
+  TAKE(v, args[2]);
+  int64_t window, sinks;
+  float scale;
+  const int code = type_code(q.scalar_type());
+  if (code < 0 || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || k.scalar_type() != q.scalar_type() ||
+      v.scalar_type() != q.scalar_type() || !unit_last(q) || !unit_last(k) || !unit_last(v))
+    Py_RETURN_NONE;
+  const int64_t batch = q.size(0), hq = q.size(1), lq = q.size(2), d = q.size(3), hkv = k.size(1), lk = k.size(2);
+  const int64_t dv = v.size(3);
+  if (!number(args[3], &window) || !number(args[4], &sinks) || !scale_of(args[5], d, &scale) || window < 1 || sinks < 0)
+    Py_RETURN_NONE;
+  if (k.size(0) != batch || v.size(0) != batch || v.size(1) != hkv || v.size(2) != lk || k.size(3) != d || hq % hkv != 0 ||
+      (hq != hkv && args[6] != Py_True))
+    Py_RETURN_NONE;
+  // tokens before heads in memory where the queries have them so
+  at::Tensor out = q.stride(1) < q.stride(2) ? at::empty({batch, lq, hq, dv}, q.options()).transpose(1, 2)
+                                             : at::empty({batch, hq, lq, dv}, q.options());
+  LAUNCH(rc, biops_window_attention(code, batch, hq, hkv, lq, lk, d, dv, ptr(q), q.stride(0), q.stride(2), q.stride(1),
+                                    ptr(k), k.stride(0), k.stride(2), k.stride(1), ptr(v), v.stride(0), v.stride(2),
+                                    v.stride(1), ptr(out), out.stride(0), out.stride(2), out.stride(1), nullptr, 0, 0,
+                                    nullptr, 0, 0, window, sinks, scale, nullptr, stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// window_packed(query, key, value, cu_q, cu_kv, window, sinks, scale or None, flag) -> output   [1, tokens, heads, dim]
+PyObject* window_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(q, args[0]);
+  TAKE(k, args[1]);
+  TAKE(v, args[2]);
+  TAKE(cu_q, args[3]);
+  TAKE(cu_k, args[4]);
+  int64_t window, sinks, flag;
+  float scale;
+  const int code = type_code(q.scalar_type());
+  if (code < 0 || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || k.scalar_type() != q.scalar_type() ||
+      v.scalar_type() != q.scalar_type() || !unit_last(q) || !unit_last(k) || !unit_last(v))
+    Py_RETURN_NONE;
+  const int64_t lq = q.size(1), hq = q.size(2), d = q.size(3), lk = k.size(1), hkv = k.size(2), dv = v.size(3);
+  if (!number(args[5], &window) || !number(args[6], &sinks) || !scale_of(args[7], d, &scale) || !number(args[8], &flag) ||
+      window < 1 || sinks < 0)
+    Py_RETURN_NONE;
+  if (q.size(0) != 1 || k.size(0) != 1 || v.size(0) != 1 || v.size(1) != lk || v.size(2) != hkv || k.size(3) != d ||
+      hq % hkv != 0 || cu_q.dim() != 1 || cu_k.dim() != 1 || cu_q.size(0) != cu_k.size(0) || !is_index(cu_q) || !is_index(cu_k))
+    Py_RETURN_NONE;
+  at::Tensor out = at::empty({1, lq, hq, dv}, q.options());
+  LAUNCH(rc, biops_window_attention(code, cu_q.size(0) - 1, hq, hkv, lq, lk, d, dv, ptr(q), 0, q.stride(1), q.stride(2),
+                                    ptr(k), 0, k.stride(1), k.stride(2), ptr(v), 0, v.stride(1), v.stride(2), ptr(out), 0,
+                                    out.stride(1), out.stride(2), ptr(cu_q), is_long(cu_q), cu_q.stride(0), ptr(cu_k),
+                                    is_long(cu_k), cu_k.stride(0), window, sinks, scale, reinterpret_cast<int*>(flag),
+                                    stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// C++ exceptions (out of memory) end here: the Python function then meets the same condition and raises it.
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  try {
+    return F(self, args, n);
+  } catch (...) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyCFunction fast() {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<F>));
+}
+
+PyMethodDef methods[] = {
+    {"rotary", fast<rotary>(), METH_FASTCALL, "biops_rotary on tensors, or None"},
+    {"paged_write", fast<paged_write>(), METH_FASTCALL, "biops_paged_write on tensors, or None"},
+    {"paged_attention", fast<paged_attention>(), METH_FASTCALL, "biops_paged_attention on tensors, or None"},
+    {"window_attention", fast<window_attention>(), METH_FASTCALL, "biops_window_attention on dense tensors, or None"},
+    {"window_packed", fast<window_packed>(), METH_FASTCALL, "biops_window_attention on packed tensors, or None"},
+    {nullptr, nullptr, 0, nullptr},
+};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_biops_tensor", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__biops_tensor(void) { return PyModule_Create(&module); }
