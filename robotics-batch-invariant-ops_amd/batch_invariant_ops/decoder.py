@@ -273,7 +273,7 @@ def multi_axis_rotary(
 
     Angles are computed in 64 bits, the rotation in 32, with one rounding to the tensors' type.  Returns new
     tensors ``(query, key)``, or the rotated query alone when ``key`` is None.  Differentiable with respect
-    to ``query`` and ``key``.
+    to ``query`` and ``key`` (not to ``positions``).
     """
     plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(inv_freq),
                         bool(interleaved_axes), bool(interleaved_pairs))
@@ -300,6 +300,8 @@ def multi_axis_rotary(
     nat.require_gpu_tensors(*tensors, positions)
     if any(x.device != query.device for x in (*tensors, positions)):
         raise ValueError("query, key and positions must be on one device")
+    if positions.requires_grad and torch.is_grad_enabled():
+        raise ValueError("multi_axis_rotary has no gradient for positions: detach them")
     if any(x.is_neg() for x in (*tensors, positions)):
         raise ValueError("multi_axis_rotary: a lazily negated tensor (call resolve_neg)")
     if query.device.index != torch.cuda.current_device():

@@ -8,9 +8,13 @@
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
+#include <optional>
+#include <utility>
 
 #include "../../include/biops.h"
 
@@ -28,13 +32,13 @@ bool is_index(const at::Tensor& t) { return t.scalar_type() == at::kInt || t.sca
 int is_long(const at::Tensor& t) { return t.scalar_type() == at::kLong ? 1 : 0; }
 bool unit_last(const at::Tensor& t) { return t.stride(-1) == 1; }
 
-// A plain tensor with elements on the current device that needs no gradient here.
-const at::Tensor* take(PyObject* o, c10::DeviceIndex device) {
+bool needs_grad(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// A plain tensor with elements on the current device that needs no gradient here (`grad`: or does).
+const at::Tensor* take(PyObject* o, c10::DeviceIndex device, bool grad = false) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.layout() != at::kStrided || t.get_device() != device || t.numel() == 0 || t.is_neg()) return nullptr;
-  if (c10::GradMode::is_enabled() && t.requires_grad()) return nullptr;
-  return &t;
+  return !grad && needs_grad(t) ? nullptr : &t;
 }
 bool number(PyObject* o, int64_t* v) {
   if (!PyLong_CheckExact(o)) return false;
@@ -60,56 +64,142 @@ char* ptr(const at::Tensor& t) { return static_cast<char*>(t.data_ptr()); }
   if (!name##_) Py_RETURN_NONE;                         \
   const at::Tensor& name = *name##_
 
-#define LAUNCH(rc, call)   \
-  int rc;                  \
-  Py_BEGIN_ALLOW_THREADS   \
-  rc = (call);             \
-  Py_END_ALLOW_THREADS
+// The GIL is released around the library's calls (a gradient's runs without it from the start).
+struct WithoutGil {
+  PyThreadState* held = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
+  ~WithoutGil() {
+    if (held) PyEval_RestoreThread(held);
+  }
+};
+#define LAUNCH(rc, call) \
+  int rc;                \
+  {                      \
+    WithoutGil without;  \
+    rc = (call);         \
+  }
+
+struct Rotation {
+  const double* turns;
+  const uint8_t* axis;
+  int64_t pairs;
+  int neighbours;
+};
+
+// Rotated copies of [tokens, heads, dim] or [batch, tokens, heads, dim] tensors (either may be undefined); any strides.
+std::pair<at::Tensor, at::Tensor> rotated(const at::Tensor& query, const at::Tensor& key, const at::Tensor& p, const Rotation& r, bool inverse) {
+  auto unit = [](const at::Tensor& t) { return !t.defined() || unit_last(t) ? t : t.contiguous(); };
+  auto like = [](const at::Tensor& t) {
+    if (!t.defined()) return t;
+    at::Tensor y = at::empty_like(t);
+    return unit_last(y) ? y : at::empty(t.sizes(), t.options());
+  };
+  const at::Tensor q = unit(query), k = unit(key);
+  at::Tensor oq = like(q), ok = like(k);
+  const at::Tensor& some = q.defined() ? q : k;
+  const bool four = some.dim() == 4;
+  auto at_ = [](const at::Tensor& t) { return t.defined() ? ptr(t) : nullptr; };
+  auto st = [](const at::Tensor& t, int i) { return t.defined() ? t.stride(i) : (int64_t)0; };
+  auto sb = [four, st](const at::Tensor& t) { return four ? st(t, 0) : (int64_t)0; };
+  const int pos = p.scalar_type() == at::kLong ? 0 : p.scalar_type() == at::kInt ? 1 : 2;
+  LAUNCH(rc, biops_rotary(type_code(some.scalar_type()), four ? some.size(0) : 1, some.size(-3), q.defined() ? q.size(-2) : 0,
+                          k.defined() ? k.size(-2) : 0, some.size(-1), at_(q), sb(q), st(q, -3), st(q, -2), at_(oq), sb(oq),
+                          st(oq, -3), st(oq, -2), at_(k), sb(k), st(k, -3), st(k, -2), at_(ok), sb(ok), st(ok, -3),
+                          st(ok, -2), ptr(p), pos, p.stride(0), four ? p.stride(1) : 0, p.stride(-1), r.pairs, r.turns,
+                          r.axis, r.neighbours, inverse ? 1 : 0, stream_on(some.get_device())))
+  TORCH_CHECK(rc == BIOPS_OK, "biops_rotary failed (", rc, "): ", biops_last_error());
+  return {oq, ok};
+}
+
+// The rotation with its gradient, the inverse rotation (and so on).  The frequencies are copied: the graph may
+// outlive the table that they came from.  A call without keys has no `key` (not an undefined one).
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                                                const std::optional<at::Tensor>& key, const at::Tensor& p,
+                                                const at::Tensor& turns, const at::Tensor& axis, bool neighbours,
+                                                bool inverse) {
+    const at::Tensor k = key.value_or(at::Tensor());
+    ctx->save_for_backward({p});
+    ctx->saved_data["turns"] = turns;
+    ctx->saved_data["axis"] = axis;
+    ctx->saved_data["neighbours"] = neighbours;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["both"] = k.defined();
+    ctx->set_materialize_grads(false);
+    const Rotation r{turns.const_data_ptr<double>(), axis.const_data_ptr<uint8_t>(), turns.numel(), neighbours ? 1 : 0};
+    auto y = rotated(q, k, p, r, inverse);
+    torch::autograd::variable_list out{y.first};
+    if (k.defined()) out.push_back(y.second);
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const at::Tensor p = ctx->get_saved_variables()[0], turns = ctx->saved_data["turns"].toTensor(),
+                     axis = ctx->saved_data["axis"].toTensor();
+    const bool neighbours = ctx->saved_data["neighbours"].toBool(), inverse = ctx->saved_data["inverse"].toBool();
+    torch::autograd::variable_list out(7);  // one for each argument of forward
+    const at::Tensor first = ctx->needs_input_grad(0) ? g[0] : at::Tensor();
+    const at::Tensor second = ctx->saved_data["both"].toBool() && ctx->needs_input_grad(1) ? g[1] : at::Tensor();
+    if (!first.defined() && !second.defined()) return out;
+    if (c10::GradMode::is_enabled()) {  // create_graph
+      const bool alone = !first.defined();  // (the first tensor of a call is a defined one)
+      const std::optional<at::Tensor> other = alone || !second.defined() ? std::nullopt : std::optional<at::Tensor>(second);
+      auto y = RotaryFunction::apply(alone ? second : first, other, p, turns, axis, neighbours, !inverse);
+      out[alone ? 1 : 0] = y[0];
+      if (y.size() > 1) out[1] = y[1];
+    } else {
+      const Rotation r{turns.const_data_ptr<double>(), axis.const_data_ptr<uint8_t>(), turns.numel(), neighbours ? 1 : 0};
+      auto y = rotated(first, second, p, r, !inverse);
+      out[0] = y.first;
+      out[1] = y.second;
+    }
+    return out;
+  }
+};
 
 // rotary(query, key or None, positions, axes, pairs, turns, axis, neighbours) -> query or (query, key)
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 8) Py_RETURN_NONE;
   const auto device = c10::hip::current_device();
-  TAKE(q, args[0]);
   const bool both = args[1] != Py_None;
-  const at::Tensor* k = both ? take(args[1], device) : nullptr;
-  if (both && !k) Py_RETURN_NONE;
+  const at::Tensor* q_ = take(args[0], device, true);
+  const at::Tensor* k_ = both ? take(args[1], device, true) : nullptr;
+  if (!q_ || (both && !k_)) Py_RETURN_NONE;
   TAKE(p, args[2]);
+  const at::Tensor& q = *q_;
+  const at::Tensor k = both ? *k_ : at::Tensor();
   int64_t axes, pairs, turns, axis, neighbours;
   if (!number(args[3], &axes) || !number(args[4], &pairs) || !number(args[5], &turns) || !number(args[6], &axis) ||
       !number(args[7], &neighbours))
     Py_RETURN_NONE;
   const int64_t nd = q.dim();
-  const int code = type_code(q.scalar_type());
-  if ((nd != 3 && nd != 4) || code < 0 || !unit_last(q) || 2 * pairs > q.size(-1)) Py_RETURN_NONE;
+  if ((nd != 3 && nd != 4) || type_code(q.scalar_type()) < 0 || 2 * pairs > q.size(-1)) Py_RETURN_NONE;
   const int lead = (int)nd - 2;
-  const int pos = p.scalar_type() == at::kLong ? 0 : p.scalar_type() == at::kInt ? 1 : p.scalar_type() == at::kFloat ? 2 : -1;
-  if (pos < 0 || p.dim() != lead + 1 || p.size(0) != axes) Py_RETURN_NONE;
+  const bool known = p.scalar_type() == at::kLong || p.scalar_type() == at::kInt || p.scalar_type() == at::kFloat;
+  if (!known || p.dim() != lead + 1 || p.size(0) != axes) Py_RETURN_NONE;
   for (int i = 0; i < lead; ++i)
     if (p.size(i + 1) != q.size(i)) Py_RETURN_NONE;
   if (both) {
-    if (k->dim() != nd || k->scalar_type() != q.scalar_type() || !unit_last(*k) || k->size(-1) != q.size(-1)) Py_RETURN_NONE;
+    if (k.dim() != nd || k.scalar_type() != q.scalar_type() || k.size(-1) != q.size(-1)) Py_RETURN_NONE;
     for (int i = 0; i < lead; ++i)
-      if (k->size(i) != q.size(i)) Py_RETURN_NONE;
+      if (k.size(i) != q.size(i)) Py_RETURN_NONE;
   }
-  at::Tensor oq = at::empty_like(q);
-  at::Tensor ok = both ? at::empty_like(*k) : at::Tensor();
-  if (!unit_last(oq) || (both && !unit_last(ok))) Py_RETURN_NONE;
-  const bool four = nd == 4;
-  auto batch = [four](const at::Tensor& t) { return four ? t.stride(0) : (int64_t)0; };
-  LAUNCH(rc, biops_rotary(code, four ? q.size(0) : 1, q.size(-3), q.size(-2), both ? k->size(-2) : 0, q.size(-1),
-                          ptr(q), batch(q), q.stride(-3), q.stride(-2), ptr(oq), batch(oq), oq.stride(-3), oq.stride(-2),
-                          both ? ptr(*k) : nullptr, both ? batch(*k) : 0, both ? k->stride(-3) : 0,
-                          both ? k->stride(-2) : 0, both ? ptr(ok) : nullptr, both ? batch(ok) : 0,
-                          both ? ok.stride(-3) : 0, both ? ok.stride(-2) : 0, ptr(p), pos, p.stride(0),
-                          four ? p.stride(1) : 0, p.stride(-1), pairs, reinterpret_cast<const double*>(turns),
-                          reinterpret_cast<const uint8_t*>(axis), (int)neighbours, 0, stream_on(device)))
-  if (rc != BIOPS_OK) Py_RETURN_NONE;
-  if (!both) return THPVariable_Wrap(std::move(oq));
+  const Rotation r{reinterpret_cast<const double*>(turns), reinterpret_cast<const uint8_t*>(axis), pairs, (int)neighbours};
+  std::pair<at::Tensor, at::Tensor> out;
+  if (needs_grad(q) || (both && needs_grad(k))) {
+    at::Tensor t = at::empty({pairs}, at::kDouble), a = at::empty({pairs}, at::kByte);
+    std::copy_n(r.turns, pairs, t.data_ptr<double>());
+    std::copy_n(r.axis, pairs, a.data_ptr<uint8_t>());
+    const std::optional<at::Tensor> key = both ? std::optional<at::Tensor>(k) : std::nullopt;
+    auto y = RotaryFunction::apply(q, key, p, t, a, neighbours != 0, false);
+    out.first = y[0];
+    if (both) out.second = y[1];
+  } else {
+    out = rotated(q, k, p, r, false);
+  }
+  if (!both) return THPVariable_Wrap(std::move(out.first));
   PyObject* pair = PyTuple_New(2);
   if (!pair) return nullptr;
-  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(oq)));
-  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(ok)));
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out.first)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(out.second)));
   return pair;
 }
 

@@ -69,6 +69,32 @@ def test_both_paths(name, monkeypatch):
         assert_bitwise(a, b)
 
 
+def test_gradients_of_both_paths(monkeypatch):
+    q, k = randn(2, 5, 4, 64, seed=9).requires_grad_(), randn(2, 5, 2, 64, seed=10).requires_grad_()
+    p = torch.arange(20, device="cuda").view(2, 2, 5)
+    g = [randn(2, 5, 4, 64, seed=11), randn(2, 5, 2, 64, seed=12)]
+
+    def both():
+        return torch.autograd.grad(bio.multi_axis_rotary(q, k, p, (20, 12)), (q, k), g)
+
+    def alone():
+        return torch.autograd.grad(bio.multi_axis_rotary(q, None, p, (20, 12)), q, g[0].transpose(-1, -2).contiguous().transpose(-1, -2))
+
+    def broadcast():
+        return torch.autograd.grad(bio.multi_axis_rotary(q, k, p, (20, 12))[1].sum(), k)
+
+    for call in (both, alone, broadcast):
+        with monkeypatch.context() as m:
+            m.setattr(decoder._Rotary, "forward", None)  # the Python path's
+            fast = call()
+        with monkeypatch.context() as m:
+            m.setattr(decoder, "_tensor_module", False)
+            m.setattr(decoder, "_direct", lambda: False)
+            slow = call()
+        for a, b in zip(fast, slow):
+            assert_bitwise(a, b)
+
+
 def test_errors_are_the_python_ones():
     q = randn(1, 4, 5, 64, seed=6)
     with pytest.raises(ValueError, match="window"):

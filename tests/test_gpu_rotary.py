@@ -142,6 +142,40 @@ def test_gradients_of_one_tensor_and_of_gradients():
     assert (gx.cpu().double() - want.sum((0, 1), keepdim=True)).abs().max() <= 8 * (bound.max() + 8 * 2.0**-24 * 8)
 
 
+def test_second_gradient_of_the_keys_alone():
+    """Only the keys' output gets a gradient, and that gradient one of its own."""
+    q, k = randn(4, 2, 16, seed=60, dtype=torch.float32), randn(4, 1, 16, seed=61, dtype=torch.float32).requires_grad_()
+    p = places(1, 4, seed=62)
+    for queries in (q, q.clone().requires_grad_()):
+        out_k = multi_axis_rotary(queries, k, p, (8,))[1]
+        g = torch.ones_like(k).requires_grad_()
+        (gk,) = torch.autograd.grad(out_k, k, g, create_graph=True)
+        check_rotated(gk, g, p, (8,), inverse=True)
+        (gg,) = torch.autograd.grad(gk, g, k.detach())
+        check_rotated(gg, k, p, (8,))
+
+
+def test_graphs_outlive_the_frequency_table():
+    """The host's table of a call may be gone (64 are kept) when its gradient runs."""
+    q = randn(3, 2, 16, seed=63, dtype=torch.float32).requires_grad_()
+    p = places(1, 3, seed=64)
+    out = multi_axis_rotary(q, None, p, (8,), base=77.0)
+    for i in range(100):
+        multi_axis_rotary(q.detach(), None, p, (8,), base=100.0 + i)
+    g = randn(3, 2, 16, seed=65, dtype=torch.float32)
+    (gq,) = torch.autograd.grad(out, q, g)
+    check_rotated(gq, g, p, (8,), base=77.0, inverse=True)
+
+
+def test_no_gradient_for_positions():
+    q = randn(3, 2, 16, seed=66, dtype=torch.float32)
+    p = torch.rand(1, 3, device="cuda").requires_grad_()
+    with pytest.raises(ValueError, match="positions"):
+        multi_axis_rotary(q, None, p, (8,))
+    with torch.no_grad():
+        check_rotated(multi_axis_rotary(q, None, p, (8,)), q, p, (8,))
+
+
 def test_graph_replays_forward_and_gradient():
     q = randn(5, 4, 64, seed=23, dtype=torch.bfloat16).requires_grad_()
     p = places(2, 5, seed=24)
