@@ -514,9 +514,18 @@ def paged_attention_batch_invariant(
 _MOST_ROW_STRIDE = 1 << 23  # elements between key rows that the kernel's 32-bit offsets inside a block take
 
 
+def _fetchable(t: torch.Tensor) -> bool:
+    """Whether keys or values ``[batch, tokens, heads, dim]`` go straight to LDS: rows at multiples of 16 bytes."""
+    vec = 16 // t.element_size()
+    return (t.stride(1) <= _MOST_ROW_STRIDE and t.data_ptr() % 16 == 0
+            and all(t.stride(i) % vec == 0 or t.shape[i] == 1 for i in range(3)))
+
+
 def _windowed(q, k, v, out, nseq, lengths, window_size, sinks, scale, offsets, watch):
     """biops_window_attention on tensors of [batch, tokens, heads, dim] strides."""
-    k, v = (t if t.stride(1) <= _MOST_ROW_STRIDE else t.contiguous() for t in (k, v))
+    k, v = (t if _fetchable(t) else t.contiguous() for t in (k, v))
+    if not (_fetchable(k) and _fetchable(v)):  # contiguous, and off the 16 bytes: a slice of a flat buffer
+        k, v = k.clone(), v.clone()
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
     d = q.shape[-1]
     if offsets is None:

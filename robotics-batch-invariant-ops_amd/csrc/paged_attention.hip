@@ -100,7 +100,7 @@ __device__ __forceinline__ void mfma16(f32x4_t& acc, const u32x4_t& a, const u32
 template <typename T>
 __device__ __forceinline__ uint32_t pack_pair(float x, float y) {
   if constexpr (std::is_same<T, bf16_t>::value) return f32x2_to_bf16x2_bits(x, y);
-  else return (uint32_t)Num<T>::to_bits(x) | ((uint32_t)Num<T>::to_bits(y) << 16);
+  else return f32x2_to_f16x2_bits(x, y);
 }
 
 // Wavefronts per SIMD that registers are given out for.

@@ -61,8 +61,7 @@ __device__ __forceinline__ u32x4_t pack(const float (&x)[16 / sizeof(T)]) {
     for (int i = 0; i < 4; ++i) v[i] = f32x2_to_bf16x2_bits(x[2 * i], x[2 * i + 1]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = (uint32_t)Num<T>::to_bits(x[2 * i]) | ((uint32_t)Num<T>::to_bits(x[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) v[i] = f32x2_to_f16x2_bits(x[2 * i], x[2 * i + 1]);
   }
   return v;
 }

@@ -30,7 +30,12 @@
 
 namespace biops {
 
-constexpr int kWindowShort = 512;  // visible keys up to which tiles of 64 rows are taken
+// Visible keys up to which 16-bit tiles have 64 rows and two wavefronts for each 32 of them, by head size; 128 rows
+// and one wavefront each otherwise.  bf16, us (64 rows / 128 rows), batch 8 x 16/4 heads x 2048: 64-wide, window 64
+// 38 / 41, 256 57 / 59, 512 80 / 79, 2048 147 / 137; 128-wide, 256 116 / 98, 1024 218 / 182.  With one sequence the
+// small tile fills more of the chip (128-wide, 1 x 2048, window 256: 18 / 21), and a 128-wide head's shortest windows
+// take it for that.
+constexpr int kWindowShort64 = 512, kWindowShort128 = 128;
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
 struct WindowArgs {
@@ -53,7 +58,7 @@ struct WindowArgs {
 };
 
 struct WindowTile {
-  int64_t qrow, krow;  // first row of the sequence in the packed tensors (0 in dense)
+  int qrow, krow;      // first row of the sequence in the packed tensors (0 in dense)
   int ql, kl;          // lengths
   int i0;              // first row of the tile in its sequence
 };
@@ -65,6 +70,20 @@ __device__ __forceinline__ int64_t window_offset(const void* cu, int is64, int64
 // Tile `tl` of the packed rows.  Segment 0 are rows in front of the first offset, segment i sequence i - 1,
 // the last one the rows behind the last offset; the outer two have no keys and become zeros.  Offsets are
 // taken into [0, rows] and as their running maximum, so every row is in one segment whatever they hold.
+template <typename T>
+__device__ __forceinline__ uint32_t window_pack(float x, float y) {
+  if constexpr (std::is_same<T, bf16_t>::value) return f32x2_to_bf16x2_bits(x, y);
+  else return f32x2_to_f16x2_bits(x, y);
+}
+// l + x + y of a packed pair: the sum is of the rounded weights, which the product takes, at one instruction for two.
+template <typename T>
+__device__ __forceinline__ float window_add_pair(uint32_t xy, float l) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, xy), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, xy), __builtin_bit_cast(f16x2_t, 0x3c003c00u), l, false);
+}
+
 template <int ROWS>
 __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lane, WindowTile& t) {
   const int n = (int)a.nseq, segments = n + 2;
@@ -117,35 +136,36 @@ __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lan
 
 // DP, DVP: head and value size rounded up to whole fragments; RW row groups of 32 by KW wavefronts that share a
 // row group and take turns at the keys.
-template <typename T, int DP, int DVP, int RW>
+template <typename T, int DP, int DVP, int RW, int KW_, int NH_>
 struct WindowShape {
   static constexpr int E = sizeof(T), VEC = 16 / E;
-  static constexpr int KW = 4 / RW;
-  static constexpr int ROWS = 32 * RW;
-  static constexpr int BN = 64;                        // keys of a block
-  static constexpr int NH = BN / 32 / KW;              // 32-key parts of a block that a wavefront takes
-  static constexpr int STAGES = E == 2 ? 2 : 1;        // blocks in LDS
+  static constexpr int KW = KW_, NH = NH_;             // NH: 32-key parts of a block that a wavefront takes
+  static constexpr int ROWS = 32 * RW, THREADS = 64 * RW * KW;
+  static constexpr int BN = 32 * NH * KW;              // keys of a block
   static constexpr int KCH = DP / VEC, VCH = DVP / VEC;  // 16-byte chunks of a K / V row
   static constexpr int slots(int chunks) { return chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32); }
   static constexpr int KS = slots(KCH), VS = slots(VCH);  // ... and their places in LDS
   static constexpr int K_BYTES = BN * KS * 16, V_BYTES = BN * VS * 16;
-  // A thread loads chunk tid % KS of every (256 / KS)th row (nothing where that is behind the head size).
-  static constexpr int KR = 256 / KS, VR = 256 / VS;
+  // A thread loads chunk slot tid % KS of every KRth row.
+  static constexpr int KR = THREADS / KS, VR = THREADS / VS;
   static constexpr int KL = BN / KR, VL = BN / VR;
   static constexpr int QF = DP / (2 * VEC);            // fragment steps of a 32x32 score block
+  static constexpr int QSTEP = 4 / NH;                 // score steps whose fragments are read at a time
   static constexpr int OF = (DVP + 31) / 32;
   static constexpr int JOIN_BYTES = KW > 1 ? (KW - 1) * RW * 64 * (16 * OF + 2) * 4 : 0;
-  static constexpr int BLOCK_BYTES = STAGES * (K_BYTES + V_BYTES);
+  static constexpr int BLOCK_BYTES = 2 * (K_BYTES + V_BYTES);
   static constexpr int LDS_BYTES = BLOCK_BYTES > JOIN_BYTES ? BLOCK_BYTES : JOIN_BYTES;
+  static_assert(BN % KR == 0 && BN % VR == 0, "whole loads");
   static_assert(32 * OF <= VS * VEC, "V fragments stay inside a row");
-  // chunk c of K row r: sixteen consecutive rows of one chunk in sixteen different 16-byte slots
-  __device__ static __forceinline__ int k_off(int r, int c) {
-    if constexpr (KS >= 16) return (r * KS + (c ^ (r & 15))) << 4;
-    else return (r * KS + (c ^ ((r >> 1) & 7))) << 4;
+  // Place of chunk c in row r: K so that sixteen consecutive rows of one chunk lie in sixteen different 16-byte
+  // slots, V as the transposing reads want it (float32: rows r and r + 4 in opposite halves of the banks).
+  __device__ static __forceinline__ int k_slot(int r, int c) { return KS >= 16 ? c ^ (r & 15) : c ^ ((r >> 1) & 7); }
+  __device__ static __forceinline__ int v_slot(int r, int c) {
+    return E == 2 ? c ^ nmajor_swz<VS>(r) : c ^ nmajor32_swz<VS>(r);
   }
+  __device__ static __forceinline__ int k_off(int r, int c) { return (r * KS + k_slot(r, c)) << 4; }
   __device__ static __forceinline__ int v_off(int r, int col) {
-    if constexpr (E == 2) return lds_off_n<VS>(r, col);
-    else return lds_off_n32<VS>(r, col);
+    return ((r * VS + v_slot(r, col / VEC)) << 4) + (col % VEC) * E;
   }
 };
 
@@ -193,16 +213,18 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const char* q, c
 }
 
 // Wavefronts per SIMD that registers are given out for.
-template <typename T, int DP, int DVP>
-constexpr int window_waves() { return DP > 128 || DVP > 128 ? 1 : (sizeof(T) == 2 && DP <= 64 && DVP <= 64 ? 3 : 2); }
+template <typename T, int DP, int DVP, int RW, int KW, int NH>
+constexpr int window_waves() { return DP > 128 || DVP > 128 ? 1 : (sizeof(T) == 2 && DP <= 64 && DVP <= 64 ? (RW < 4 ? 4 : 3) : 2); }
 
-template <typename T, int DP, int DVP, int RW>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP>(), window_waves<T, DP, DVP>())))
+template <typename T, int DP, int DVP, int RW, int KW, int NH>
+__global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP, RW, KW, NH>(), window_waves<T, DP, DVP, RW, KW, NH>())))
 void window_attn_kernel(WindowArgs a) {
-  using F = WindowShape<T, DP, DVP, RW>;
-  constexpr int E = F::E, BN = F::BN, NH = F::NH;
+  using F = WindowShape<T, DP, DVP, RW, KW, NH>;
+  constexpr int E = F::E, BN = F::BN;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS_BYTES];
-  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, hf = lane >> 5, l32 = lane & 31;
+  // What is the same for a wavefront is told to the compiler, and then computed once for it.
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63, hf = lane >> 5, l32 = lane & 31;
   const int rw = w % RW, part = w / RW;  // row group, turn at the keys
   const u32x4_t zero4 = {0u, 0u, 0u, 0u};
 
@@ -215,29 +237,29 @@ void window_attn_kernel(WindowArgs a) {
     const uint32_t j = t - first;
     if ((n & 7) == 0) t = first + (j & 7) * (n >> 3) + (j >> 3);
   }
-  const uint32_t g = t % a.group;
-  t /= a.group;
   WindowTile tile;
-  int64_t b = 0;
-  int hk;
+  const uint32_t tl = t % a.tiles;
+  t /= a.tiles;
+  const int h = (int)(t % (a.hkv * a.group)), hk = h / (int)a.group;
+  const int64_t b = t / (a.hkv * a.group);
   if (a.cu_q) {
-    hk = (int)(t % a.hkv);
-    if (!window_find<F::ROWS>(a, (int)(t / a.hkv), lane, tile)) return;
+    if (!window_find<F::ROWS>(a, (int)tl, lane, tile)) return;
+    tile.i0 = uniform(tile.i0);
+    tile.ql = uniform(tile.ql);
+    tile.kl = uniform(tile.kl);
+    tile.qrow = uniform(tile.qrow);
+    tile.krow = uniform(tile.krow);
   } else {
-    tile.i0 = (int)(a.tiles - 1 - t % a.tiles) * F::ROWS;  // longest ranges first
-    t /= a.tiles;
-    hk = (int)(t % a.hkv);
-    b = t / a.hkv;
+    tile.i0 = (int)(a.tiles - 1 - tl) * F::ROWS;  // longest ranges first
     tile.qrow = tile.krow = 0;
     tile.ql = a.lq;
     tile.kl = a.lk;
   }
-  const int h = hk * (int)a.group + (int)g;
   const int kl = tile.kl, qrows = tile.ql - tile.i0 < F::ROWS ? tile.ql - tile.i0 : F::ROWS;
-  const char* const qb = a.q + b * a.qB + (tile.qrow + tile.i0) * a.qT + h * a.qH;
+  const char* const qb = a.q + b * a.qB + (int64_t)(tile.qrow + tile.i0) * a.qT + h * a.qH;
   const char* const kb = a.k + b * a.kB + tile.krow * a.kT + hk * a.kH;
   const char* const vb = a.v + b * a.vB + tile.krow * a.vT + hk * a.vH;
-  char* const ob = a.out + b * a.oB + (tile.qrow + tile.i0) * a.oT + h * a.oH;
+  char* const ob = a.out + b * a.oB + (int64_t)(tile.qrow + tile.i0) * a.oT + h * a.oH;
 
   // positions of the tile's first and last row; keys of v: v < ns ? v : v + shift
   const int p0 = kl - tile.ql + tile.i0, p1 = p0 + qrows - 1;
@@ -264,56 +286,98 @@ void window_attn_kernel(WindowArgs a) {
   const int wlo0 = row_lo(p0 + 32 * rw), wlo1 = row_lo(p0 + wlast);
   const int whi0 = p0 + 32 * rw - shift, whi1 = p0 + wlast - shift;
 
+  // Rows behind the last one take its queries; they see nothing.
   u32x4_t qf[F::QF];
+  {
+    const char* qr = qb + (row_ok ? rloc : qrows - 1) * a.qT;
+    if (a.d == DP) {
 #pragma unroll
-  for (int c = 0; c < F::QF; ++c) {
-    const int d0 = F::VEC * (2 * c + hf);
-    qf[c] = row_ok && d0 < a.d ? load_16(qb + rloc * a.qT + E * d0) : zero4;
-    if (a.negate) qf[c] ^= E == 2 ? 0x80008000u : 0x80000000u;
-  }
-
-  u32x4_t kr[F::KL], vr[F::VL];
-  const int krow = tid / F::KS, kc = tid % F::KS, vrow0 = tid / F::VS, vc = tid % F::VS;
-  const bool kin = F::VEC * kc < a.d, vin = F::VEC * vc < a.dv;
-  const uint32_t koff = (uint32_t)(krow * (int)a.kT + 16 * kc), voff = (uint32_t)(vrow0 * (int)a.vT + 16 * vc);
-  auto load = [&](int blk) {
-    const int v0 = blk * BN;
-    if (v0 >= ns && v0 + BN <= nv) {
-      const char* kp = kb + (int64_t)(v0 + shift) * a.kT;
-      const char* vp = vb + (int64_t)(v0 + shift) * a.vT;
-#pragma unroll
-      for (int i = 0; i < F::KL; ++i) {
-        kr[i] = zero4;
-        if (kin) kr[i] = load_16(kp + koff);
-        kp += F::KR * a.kT;
-      }
-#pragma unroll
-      for (int i = 0; i < F::VL; ++i) {
-        vr[i] = zero4;
-        if (vin) vr[i] = load_16(vp + voff);
-        vp += F::VR * a.vT;
-      }
+      for (int c = 0; c < F::QF; ++c) qf[c] = load_16(qr + 16 * (2 * c + hf));
     } else {
 #pragma unroll
-      for (int i = 0; i < F::KL; ++i) {
-        const int v = v0 + krow + F::KR * i;
-        kr[i] = v < nv && kin ? load_16(kb + (int64_t)(v < ns ? v : v + shift) * a.kT + 16 * kc) : zero4;
-      }
+      for (int c = 0; c < F::QF; ++c) qf[c] = F::VEC * (2 * c + hf) < a.d ? load_16(qr + 16 * (2 * c + hf)) : zero4;
+    }
+    if (a.negate) {
 #pragma unroll
-      for (int i = 0; i < F::VL; ++i) {
-        const int v = v0 + vrow0 + F::VR * i;
-        vr[i] = v < nv && vin ? load_16(vb + (int64_t)(v < ns ? v : v + shift) * a.vT + 16 * vc) : zero4;
+      for (int c = 0; c < F::QF; ++c) qf[c] ^= E == 2 ? 0x80008000u : 0x80000000u;
+    }
+  }
+
+  // Blocks go from memory straight to LDS (16 bytes a lane, at consecutive places: the lane that fills slot x of a
+  // row fetches the chunk whose place that is).  Chunks behind the head size are zeroed once and stay.
+  // (Rows of 32 slots: a thread's rows alternate between two K chunks.)
+  constexpr int KV = F::KS >= 16 && F::KR < 16 ? 2 : 1;
+  const int krow = tid / F::KS, vrow0 = tid / F::VS, vc = F::v_slot(vrow0, tid % F::VS);
+  int kc[KV];
+  bool kin[KV];
+  uint32_t koff[KV];
+#pragma unroll
+  for (int j = 0; j < KV; ++j) {
+    kc[j] = F::k_slot(krow + F::KR * j, tid % F::KS);
+    kin[j] = F::VEC * kc[j] < a.d;
+    koff[j] = (uint32_t)(krow * (int)a.kT + 16 * kc[j]);
+  }
+  const bool vin = F::VEC * vc < a.dv;
+  const uint32_t voff = (uint32_t)(vrow0 * (int)a.vT + 16 * vc);
+  auto kbuf = [&](int blk) { return smem + (blk & 1) * F::K_BYTES; };
+  auto vbuf = [&](int blk) { return smem + 2 * F::K_BYTES + (blk & 1) * F::V_BYTES; };
+  // Row v of the counted keys; behind the last one, that one (no row sees it there).
+  auto key_of = [&](int v) -> int64_t {
+    v = v < nv ? v : nv - 1;
+    return v < ns ? v : v + shift;
+  };
+  auto fetch = [&](const char* from, char* to) {
+    __builtin_amdgcn_global_load_lds((global_cvoid_t*)from, (lds_void_t*)to, 16, 0, 0);
+  };
+  auto load_k = [&](int blk) {
+    const int v0 = blk * BN;
+    char* to = kbuf(blk) + w * 1024;
+    const bool whole = v0 >= ns && v0 + BN <= nv;
+    const char* kp = kb + (int64_t)(v0 + shift) * a.kT;
+#pragma unroll
+    for (int j = 0; j < KV; ++j) {
+      if (!kin[j]) continue;
+      if (whole) {
+#pragma unroll
+        for (int i = j; i < F::KL; i += KV) fetch(kp + i * (F::KR * a.kT) + koff[j], to + 16 * F::THREADS * i);
+      } else {
+#pragma unroll
+        for (int i = j; i < F::KL; i += KV) fetch(kb + key_of(v0 + krow + F::KR * i) * a.kT + 16 * kc[j], to + 16 * F::THREADS * i);
       }
     }
   };
-  auto store = [&](int blk) {
-    char* ks = smem + (F::STAGES > 1 ? blk & 1 : 0) * (F::K_BYTES + F::V_BYTES);
+  auto load_v = [&](int blk) {
+    if (!vin) return;
+    const int v0 = blk * BN;
+    char* to = vbuf(blk) + w * 1024;
+    if (v0 >= ns && v0 + BN <= nv) {
+      const char* vp = vb + (int64_t)(v0 + shift) * a.vT;
 #pragma unroll
-    for (int i = 0; i < F::KL; ++i) *reinterpret_cast<u32x4_t*>(ks + F::k_off(krow + F::KR * i, kc)) = kr[i];
+      for (int i = 0; i < F::VL; ++i) fetch(vp + i * (F::VR * a.vT) + voff, to + 16 * F::THREADS * i);
+    } else {
 #pragma unroll
-    for (int i = 0; i < F::VL; ++i)
-      *reinterpret_cast<u32x4_t*>(ks + F::K_BYTES + F::v_off(vrow0 + F::VR * i, F::VEC * vc)) = vr[i];
+      for (int i = 0; i < F::VL; ++i) fetch(vb + key_of(v0 + vrow0 + F::VR * i) * a.vT + 16 * vc, to + 16 * F::THREADS * i);
+    }
   };
+  // Everything fetched and every LDS read has landed, in all wavefronts.
+  auto meet = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  if (a.d < F::KS * F::VEC || a.dv < F::VS * F::VEC) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+      for (int i = 0; i < F::KL; ++i)
+        if (!kin[i % KV]) *reinterpret_cast<u32x4_t*>(kbuf(x) + 16 * tid + 16 * F::THREADS * i) = zero4;
+      if (!vin) {
+#pragma unroll
+        for (int i = 0; i < F::VL; ++i) *reinterpret_cast<u32x4_t*>(vbuf(x) + 16 * tid + 16 * F::THREADS * i) = zero4;
+      }
+    }
+  }
 
   // m: largest score so far (raw), sh = m * scale, l: this lane's part of the row's sum
   float m = -INFINITY, sh = 0.f, l = 0.f;
@@ -323,29 +387,53 @@ void window_attn_kernel(WindowArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) oacc[e][r] = 0.f;
 
-  // 32-key parts hb0 .. hb0 + NH - 1 of a block
-  auto block = [&](int blk, int hb0, bool open) {
-    const char* ks = smem + (F::STAGES > 1 ? blk & 1 : 0) * (F::K_BYTES + F::V_BYTES);
-    const char* vs = ks + F::K_BYTES;
-    f32x16_t sc[NH];
+  const int hb0 = NH * part;  // this wavefront's 32-key parts of a block: hb0 .. hb0 + NH - 1
+  f32x16_t sc[NH];
+  auto scores = [&](int blk) {
+    const char* ks = kbuf(blk);
 #pragma unroll
-    for (int x = 0; x < NH; ++x) {
-      const int hb = hb0 + x;
+    for (int x = 0; x < NH; ++x)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[x][r] = 0.f;
+    // The fragments of a group of steps are read before the MFMAs of the group before it (the barriers keep the
+    // compiler from sinking each read next to its MFMA, where it would show its latency).
+    u32x4_t kf[2][F::QSTEP][NH];
+    auto read = [&](int c0, int to) {
 #pragma unroll
-      for (int c = 0; c < F::QF; ++c)
-        Mfma<T>::step(sc[x], *reinterpret_cast<const u32x4_t*>(ks + F::k_off(32 * hb + l32, 2 * c + hf)), qf[c]);
+      for (int c = 0; c < F::QSTEP; ++c)
+#pragma unroll
+        for (int x = 0; x < NH; ++x)
+          if (c0 + c < F::QF)
+            kf[to][c][x] = *reinterpret_cast<const u32x4_t*>(ks + F::k_off(32 * (hb0 + x) + l32, 2 * (c0 + c) + hf));
+    };
+    read(0, 0);
+#pragma unroll
+    for (int g = 0; g * F::QSTEP < F::QF; ++g) {
+      if ((g + 1) * F::QSTEP < F::QF) read((g + 1) * F::QSTEP, (g + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < F::QSTEP; ++c)
+#pragma unroll
+        for (int x = 0; x < NH; ++x)
+          if (g * F::QSTEP + c < F::QF) Mfma<T>::step(sc[x], kf[g & 1][c][x], qf[g * F::QSTEP + c]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (!open) {
-      const int vb0 = blk * BN + 32 * hb0 + 4 * hf;  // register r of part x: key vb0 + 32 x + 8(r/4) + r%4
-      const int from = lo - vb0, to = hi - vb0, sink = sv - vb0;
+  };
+  // Masks the scores of a block, rescales what is summed where a row's maximum grows, and turns scores into weights.
+  u32x4_t pw[E == 2 ? NH : 1][2];  // 16-bit weights, packed; float32 ones stay in sc
+  auto weigh = [&](int blk) {
+    const int v0 = blk * BN + 32 * hb0, v1 = v0 + 32 * NH - 1;
+    if (!(wlast == 32 * rw + 31 && v0 >= wlo1 && v1 <= whi0)) {  // not all rows see all keys
+      const int vb0 = v0 + 4 * hf;  // register r of part x: key vb0 + 32 x + 8(r/4) + r%4
+      // lo <= v <= hi by one unsigned comparison; rows that see nothing have a bound that none passes
+      const uint32_t span = hi < lo ? 0u : (uint32_t)(hi - lo);
+      const int from = hi < lo ? 0x7fffffff : lo - vb0, sink = (sv <= hi ? sv : hi + 1) - vb0;
 #pragma unroll
       for (int x = 0; x < NH; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int o = 32 * x + 8 * (r >> 2) + (r & 3);
-          sc[x][r] = o <= to && (o >= from || o < sink) ? sc[x][r] : -INFINITY;
+          sc[x][r] = (uint32_t)(o - from) <= span || o < sink ? sc[x][r] : -INFINITY;
         }
     }
     float mx = sc[0][0];
@@ -357,75 +445,118 @@ void window_attn_kernel(WindowArgs a) {
     if (__any(mx > m)) {
       const float mn = fmaxf(m, mx);
       const float to = mn == -INFINITY ? 0.f : mn * a.scale;
-      const float corr = mx > m ? (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - to)) : 1.f;
-      l *= corr;
+      if (__any(m > -INFINITY)) {  // (nothing is summed before a row's first keys)
+        const float corr = mx > m && m > -INFINITY ? __builtin_amdgcn_exp2f(sh - to) : 1.f;
+        l *= corr;
 #pragma unroll
-      for (int e = 0; e < F::OF; ++e)
+        for (int e = 0; e < F::OF; ++e)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) oacc[e][r] *= corr;
+          for (int r = 0; r < 16; ++r) oacc[e][r] *= corr;
+      }
       m = mn;
       sh = to;
     }
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
-      const int hb = hb0 + x;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         sc[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][r], a.scale, -sh));
-        l += sc[x][r];
+        if constexpr (E == 4) l += sc[x][r];
       }
-      if constexpr (E == 4) {
+      if constexpr (E == 2) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-          for (int e = 0; e < F::OF; ++e)
-            oacc[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                *reinterpret_cast<const float*>(vs + F::v_off(32 * hb + 8 * (r >> 2) + 4 * hf + (r & 3), 32 * e + l32)),
-                sc[x][r], oacc[e], 0, 0, 0);
-      } else {
-        // transposing reads: lane s of a 16-lane group points at row k0 + s/4, column n0 + 4(s%4), and
-        // receives rows k0 .. k0+3 of column n0 + s
-        const int vrow = 4 * hf + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-#pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2) {
-          u32x4_t pb;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x0 = sc[x][8 * c2 + 2 * i], x1 = sc[x][8 * c2 + 2 * i + 1];
-            if constexpr (std::is_same<T, bf16_t>::value) pb[i] = f32x2_to_bf16x2_bits(x0, x1);
-            else pb[i] = (uint32_t)f32_to_f16_bits(x0) | ((uint32_t)f32_to_f16_bits(x1) << 16);
-          }
-          const int row = 32 * hb + 16 * c2 + vrow;
-#pragma unroll
-          for (int e = 0; e < F::OF; ++e) {
-            const u32x2_t x0 = lds_read_tr16(vs + F::v_off(row, 32 * e + vcol));
-            const u32x2_t x1 = lds_read_tr16(vs + F::v_off(row + 8, 32 * e + vcol));
-            Mfma<T>::step(oacc[e], u32x4_t{x0[0], x0[1], x1[0], x1[1]}, pb);
-          }
+        for (int i = 0; i < 8; ++i) {
+          pw[x][i >> 2][i & 3] = window_pack<T>(sc[x][2 * i], sc[x][2 * i + 1]);
+          l = window_add_pair<T>(pw[x][i >> 2][i & 3], l);
         }
       }
     }
   };
+  // What the weights add to the output.
+  auto gather = [&](int blk) {
+    const char* vs = vbuf(blk);
+    if constexpr (E == 4) {
+      // the values of a group of four steps are read before the MFMAs of the group before it
+      float xv[2][4][F::OF];
+      auto read = [&](int g, int to) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < F::OF; ++e)
+            xv[to][r][e] = *reinterpret_cast<const float*>(vs + F::v_off(32 * hb0 + 8 * g + 4 * hf + r, 32 * e + l32));
+      };
+      read(0, 0);
+#pragma unroll
+      for (int g = 0; g < 4 * NH; ++g) {
+        if (g + 1 < 4 * NH) read(g + 1, (g + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < F::OF; ++e)
+            oacc[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[g & 1][r][e], sc[g >> 2][4 * (g & 3) + r], oacc[e], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      // Transposing reads: lane s of a 16-lane group points at row k0 + s/4, column n0 + 4(s%4), and receives rows
+      // k0 .. k0+3 of column n0 + s.  In assembly, since the compiler would wait for all fetches before each; the
+      // fragments of a 16-key step are read before the MFMAs of the step before it.
+      const int vrow = 4 * hf + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      u32x2_t vl[2][F::OF], vh[2][F::OF];
+      auto read = [&](int step, int to) {
+        const int row = 32 * hb0 + 16 * step + vrow;
+#pragma unroll
+        for (int e = 0; e < F::OF; ++e) {
+          vl[to][e] = lds_read_tr16_asm(vs + F::v_off(row, 32 * e + vcol));
+          vh[to][e] = lds_read_tr16_asm(vs + F::v_off(row + 8, 32 * e + vcol));
+        }
+      };
+      read(0, 0);
+#pragma unroll
+      for (int step = 0; step < 2 * NH; ++step) {
+        const int at = step & 1;
+#pragma unroll
+        for (int e = 0; e < F::OF; ++e) lds_wait_anchor(vl[at][e], vh[at][e]);
+        if (step + 1 < 2 * NH) read(step + 1, at ^ 1);
+#pragma unroll
+        for (int e = 0; e < F::OF; ++e)
+          Mfma<T>::step(oacc[e], u32x4_t{vl[at][e][0], vl[at][e][1], vh[at][e][0], vh[at][e][1]}, pw[step >> 1][step & 1]);
+      }
+    }
+  };
+  // Whether any row of the wavefront sees a key of its part of a block.
+  auto sees = [&](int blk) {
+    const int v0 = blk * BN + 32 * hb0, v1 = v0 + 32 * NH - 1;
+    return wany && blk < nblk && v0 <= whi1 && (v1 >= wlo0 || v0 < sv);
+  };
 
+  // A turn: weights of a block (vector work), then its product and the next block's scores (matrix work, at a
+  // higher priority: of two wavefronts of a SIMD one multiplies while the other takes exponentials).  K is a block
+  // ahead of V in LDS; what the next turn needs is fetched during this one.
   if (nblk > 0) {
-    load(0);
-    store(0);
+    load_k(0);
+    load_v(0);
   }
-  __syncthreads();
+  if (nblk > 1) load_k(1);
+  meet();
+  bool here = sees(0);
+  if (here) scores(0);
   for (int blk = 0; blk < nblk; ++blk) {
-    if (blk + 1 < nblk) load(blk + 1);
-    // this wavefront's keys of the block: seen by any of its rows, by all of them
-    const int v0 = blk * BN + 32 * NH * part, v1 = v0 + 32 * NH - 1;
-    const bool some = wany && v0 <= whi1 && (v1 >= wlo0 || v0 < sv);
-    const bool all = wlast == 32 * rw + 31 && v0 >= wlo1 && v1 <= whi0;
-    if (some) block(blk, NH * part, all);
-    if constexpr (F::STAGES == 1) __syncthreads();
-    if (blk + 1 < nblk) store(blk + 1);
-    __syncthreads();
+    meet();
+    if (blk + 2 < nblk) load_k(blk + 2);
+    if (blk + 1 < nblk) load_v(blk + 1);
+    if (here) weigh(blk);
+    const bool then = sees(blk + 1);
+    __builtin_amdgcn_s_setprio(1);
+    if (here) gather(blk);
+    if (then) scores(blk + 1);
+    __builtin_amdgcn_s_setprio(0);
+    here = then;
   }
+  meet();
 
   l += __shfl_xor(l, 32, 64);
-  if constexpr (F::KW > 1) {  // join the wavefronts of a row group, in order
+  if constexpr (KW > 1) {  // join the wavefronts of a row group, in order
     float* const js = reinterpret_cast<float*>(smem);
     if (part > 0) {
       float* o = js + ((part - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane;
@@ -440,7 +571,7 @@ void window_attn_kernel(WindowArgs a) {
     if (part == 0) {
       float top = m == -INFINITY ? m : sh;
 #pragma unroll
-      for (int x = 1; x < F::KW; ++x) top = fmaxf(top, js[((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane + 64 * 16 * F::OF]);
+      for (int x = 1; x < KW; ++x) top = fmaxf(top, js[((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane + 64 * 16 * F::OF]);
       const float base = top == -INFINITY ? 0.f : top;
       const float own = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - base);
       l *= own;
@@ -449,7 +580,7 @@ void window_attn_kernel(WindowArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) oacc[e][r] *= own;
 #pragma unroll
-      for (int x = 1; x < F::KW; ++x) {
+      for (int x = 1; x < KW; ++x) {
         const float* o = js + ((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane;
         const float f = __builtin_amdgcn_exp2f(o[64 * 16 * F::OF] - base);
         l = __builtin_fmaf(o[64 * (16 * F::OF + 1)], f, l);
@@ -461,39 +592,47 @@ void window_attn_kernel(WindowArgs a) {
     }
   }
   if (part == 0) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    bool lost = false;  // an output that is not finite over a finite sum
-    if (l > 0.f && l < INFINITY) {
+    if (__any(l == 0.f)) {  // rows that see nothing, or only scores of -inf
 #pragma unroll
       for (int e = 0; e < F::OF; ++e)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)  // (columns behind the value size hold anything)
-          lost |= 32 * e + 8 * (r >> 2) + 4 * hf < a.dv && !(fabsf(oacc[e][r]) < INFINITY);
+        for (int r = 0; r < 16; ++r) oacc[e][r] = l == 0.f ? 0.f : oacc[e][r];
     }
-    const uint64_t again = __ballot(lost && row_ok);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // An output that is not finite over a finite sum: o * 0 is NaN.
+    float odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(oacc[e][r], 0.f, odd);
+    const uint64_t again = __ballot(row_ok && l > 0.f && l < INFINITY && odd != 0.f);
     const bool mine_again = (again >> l32 | again >> (l32 + 32)) & 1;
     if (row_ok && !mine_again) {
       char* orow = ob + rloc * a.oT;
+      auto put = [&](int e, int j) {
+        const int col = 32 * e + 8 * j + 4 * hf;
+        float x[4];
 #pragma unroll
-      for (int e = 0; e < F::OF; ++e)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = 32 * e + 8 * j + 4 * hf;
-          if (col >= a.dv) continue;
-          float x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = l == 0.f ? 0.f : oacc[e][4 * j + i] * inv;
-          if constexpr (E == 4) {
-            *reinterpret_cast<u32x4_any_t*>(orow + E * col) =
-                u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
-          } else if constexpr (std::is_same<T, bf16_t>::value) {
-            *reinterpret_cast<u32x2_any_t*>(orow + E * col) = u32x2_t{f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3])};
-          } else {
-            *reinterpret_cast<u32x2_any_t*>(orow + E * col) =
-                u32x2_t{(uint32_t)f32_to_f16_bits(x[0]) | ((uint32_t)f32_to_f16_bits(x[1]) << 16),
-                        (uint32_t)f32_to_f16_bits(x[2]) | ((uint32_t)f32_to_f16_bits(x[3]) << 16)};
-          }
+        for (int i = 0; i < 4; ++i) x[i] = oacc[e][4 * j + i] * inv;
+        if constexpr (E == 4) {
+          *reinterpret_cast<u32x4_any_t*>(orow + E * col) =
+              u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+        } else {
+          *reinterpret_cast<u32x2_any_t*>(orow + E * col) = u32x2_t{window_pack<T>(x[0], x[1]), window_pack<T>(x[2], x[3])};
         }
+      };
+      if (a.dv == 32 * F::OF) {
+#pragma unroll
+        for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) put(e, j);
+      } else {
+#pragma unroll
+        for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (32 * e + 8 * j + 4 * hf < a.dv) put(e, j);
+      }
     }
     for (uint64_t rest = (again | again >> 32) & 0xffffffffull; rest != 0; rest &= rest - 1) {
       const int r = 32 * rw + __builtin_ctzll(rest);
@@ -502,7 +641,7 @@ void window_attn_kernel(WindowArgs a) {
   }
 }
 
-template <typename T, int DP, int DVP, int RW>
+template <typename T, int DP, int DVP, int RW, int KW, int NH>
 static int window_launch(WindowArgs a, hipStream_t s) {
   constexpr int rows = 32 * RW;
   // packed: every sequence and the two ends may end in a part of a tile
@@ -514,7 +653,7 @@ static int window_launch(WindowArgs a, hipStream_t s) {
   constexpr uint32_t most = 1 << 22;  // a launch has less than 2^32 threads
   for (a.first = 0; a.first < a.total; a.first += most) {
     const uint32_t n = a.total - a.first < most ? a.total - a.first : most;
-    hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW>), dim3(n), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW, KW, NH>), dim3(n), dim3(64 * RW * KW), 0, s, a);
     const int rc = check_launch("window_attn_kernel");
     if (rc != BIOPS_OK) return rc;
   }
@@ -525,12 +664,15 @@ static int window_launch(WindowArgs a, hipStream_t s) {
 template <typename T, int DP>
 static int window_launch_rows(const WindowArgs& a, hipStream_t s) {
   if constexpr (sizeof(T) == 4) {
-    return window_launch<T, DP, DP, 2>(a, s);
+    return window_launch<T, DP, DP, 2, 2, 1>(a, s);
   } else if constexpr (DP > 128) {
-    return window_launch<T, DP, DP, 4>(a, s);
+    return window_launch<T, DP, DP, 4, 1, 2>(a, s);
+  } else if constexpr (DP > 64) {
+    if ((int64_t)a.window + a.sinks <= kWindowShort128) return window_launch<T, DP, DP, 2, 2, 1>(a, s);
+    return window_launch<T, DP, DP, 4, 1, 2>(a, s);
   } else {
-    if ((int64_t)a.window + a.sinks <= kWindowShort) return window_launch<T, DP, DP, 2>(a, s);
-    return window_launch<T, DP, DP, 4>(a, s);
+    if ((int64_t)a.window + a.sinks <= kWindowShort64) return window_launch<T, DP, DP, 2, 2, 1>(a, s);
+    return window_launch<T, DP, DP, 4, 1, 2>(a, s);
   }
 }
 template <typename T>
@@ -575,6 +717,12 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   // a block's rows are addressed by 32-bit offsets
   if (skT < 0 || svT < 0 || skT > (1 << 23) || svT > (1 << 23))
     return fail(BIOPS_ERR_LAYOUT, "biops_window_attention: key and value rows more than 2^23 elements apart");
+  // ... and goes straight to LDS in 16-byte pieces
+  if (lk > 0) {
+    const int64_t all_k = (int64_t)reinterpret_cast<uintptr_t>(k) | elt * skB | elt * skT | elt * skH;
+    const int64_t all_v = (int64_t)reinterpret_cast<uintptr_t>(v) | elt * svB | elt * svT | elt * svH;
+    if ((all_k | all_v) & 15) return fail(BIOPS_ERR_LAYOUT, "biops_window_attention: keys or values not aligned to 16 bytes");
+  }
   if (hq == 0 || lq == 0 || (!cu_q && nseq == 0)) return BIOPS_OK;
   if (!q || !out || (lk > 0 && (!k || !v)) || (cu_q && (!cu_k || !flag)))
     return fail(BIOPS_ERR_ARG, "biops_window_attention: null pointer");
