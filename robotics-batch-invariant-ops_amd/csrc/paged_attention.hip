@@ -33,8 +33,8 @@
 
 namespace biops {
 
-constexpr int kPagedKeys = 128;    // keys of a chunk: a tile of 32 for each of four wavefronts ...
-constexpr int kPagedChunks = 64;   // ... or a multiple of it where there were more chunks than this
+constexpr int kPagedKeys = 128;    // keys of the shortest chunk: a tile of 32 for each of four wavefronts
+constexpr int kPagedChunks = 64;   // most chunks of a sequence
 constexpr int kPagedCols = 16;     // query heads of a workgroup
 
 struct PagedArgs {
@@ -65,18 +65,29 @@ struct PagedSpan {
   bool bad;
 };
 
-// Keys per chunk, by the number of visible keys alone.
+// Keys per chunk, by the number of visible keys alone.  Short sequences need their chunks for units to run on, long
+// ones have enough of them, and every chunk starts with three reads that wait for one another and ends with a result
+// to be joined.  us by chunk size (128 / 256 / 512): 16/4 heads of 128, one sequence of 2047 keys 10.4 / 12.5 / 13,
+// 64 of 3920 keys 130 / 120 / 111; 32/8 heads, 128 sequences of 1024 keys 138 / 123 / 117 (what one sequence of that
+// length gains weighs more: in a batch of one every layer of every token pays it).
 __host__ __device__ __forceinline__ int paged_chunk(int n) {
-  constexpr int most = kPagedKeys * kPagedChunks;
-  return n <= most ? kPagedKeys : kPagedKeys * ((n - 1) / most + 1);
+  if (n <= 2048) return kPagedKeys;
+  if (n <= 4096) return 2 * kPagedKeys;
+  constexpr int most = 4 * kPagedKeys * kPagedChunks;
+  return 4 * kPagedKeys * (n <= most ? 1 : (n - 1) / most + 1);
 }
 
-__device__ __forceinline__ PagedSpan paged_span(const PagedArgs& a, int64_t b) {
-  PagedSpan s;
+// Length of sequence b, -1 where it is outside of what the table allows.
+__device__ __forceinline__ int paged_length(const PagedArgs& a, int64_t b) {
   const int64_t len = a.lengths64 ? reinterpret_cast<const int64_t*>(a.lengths)[b * a.lB]
                                   : (int64_t) reinterpret_cast<const int32_t*>(a.lengths)[b * a.lB];
-  s.bad = len < 0 || len > a.limit;
-  const int l = s.bad ? 0 : (int)len;
+  return len < 0 || len > a.limit ? -1 : (int)len;
+}
+
+__device__ __forceinline__ PagedSpan paged_span(const PagedArgs& a, int len) {
+  PagedSpan s;
+  s.bad = len < 0;
+  const int l = s.bad ? 0 : len;
   const int start = a.window > 0 && l > a.window ? l - a.window : 0;
   s.ns = a.sinks < start ? a.sinks : start;
   s.shift = start - s.ns;
@@ -84,6 +95,35 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedArgs& a, int64_t b) {
   s.chunk = paged_chunk(s.n);
   s.chunks = s.n > 0 ? (s.n - 1) / s.chunk + 1 : 0;
   return s;
+}
+
+// Work item `it` of the batch: chunk c of sequence b, all chunks of the first sequence, then of the next.  Counting
+// them here leaves no idle workgroups between those with work (64 sequences of 250 to 16384 keys: 142 us with a
+// workgroup for every chunk that the longest sequence could have).
+__device__ __forceinline__ bool paged_find(const PagedArgs& a, int it, int lane, uint32_t& b, int& c, int& length) {
+  int done = 0;
+  for (uint32_t base = 0; base < a.batch; base += 64) {
+    const uint32_t i = base + lane;
+    const int len = i < a.batch ? paged_length(a, i) : 0;
+    const int mine = paged_span(a, len).chunks;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += x;
+    }
+    upto += done;
+    const uint64_t hit = __ballot(upto > it);
+    if (hit != 0) {
+      const int f = __builtin_ctzll(hit);
+      b = base + f;
+      c = it - (__builtin_amdgcn_readlane(upto, f) - __builtin_amdgcn_readlane(mine, f));
+      length = __builtin_amdgcn_readlane(len, f);
+      return true;
+    }
+    done = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
 }
 
 template <typename T>
@@ -126,22 +166,21 @@ void paged_chunk_kernel(PagedArgs a) {
   const u32x4_t zero4 = {0u, 0u, 0u, 0u};
   const int64_t heads = (int64_t)a.hkv * a.group;
 
-  // chunk slowest: the first chunks of all sequences, which exist, go first
-  const uint32_t u = a.first + blockIdx.x;
-  const int c = (int)(u / a.rows);
-  uint32_t r = u - c * a.rows;
+  uint32_t r = a.first + blockIdx.x;
   const uint32_t z = r % a.zs;
   r /= a.zs;
-  const uint32_t hk = r % a.hkv, b = r / a.hkv;
-  const PagedSpan span = paged_span(a, b);
+  const uint32_t hk = r % a.hkv;
+  uint32_t b = r / a.hkv;
+  int c = 0, length;
+  if (a.chunks == 1) length = paged_length(a, b);
+  else if (!paged_find(a, (int)b, lane, b, c, length)) return;
+  const PagedSpan span = paged_span(a, length);
   const int cols = a.group - z * kPagedCols < kPagedCols ? (int)(a.group - z * kPagedCols) : kPagedCols;
   const int64_t h0 = hk * a.group + z * kPagedCols;
-  if (c >= span.chunks) {
-    if (c == 0 && a.chunks == 1) {  // no join: rows that see nothing are written here
-      if (span.bad) *a.flag = 1;
-      for (int i = tid; i < cols * a.dv; i += 256)
-        Num<T>::store(reinterpret_cast<T*>(a.out) + (b * heads + h0) * a.dv + i, 0.f);
-    }
+  if (span.chunks == 0) {  // (one chunk at most, and no join) a row that sees nothing
+    if (span.bad) *a.flag = 1;
+    for (int i = tid; i < cols * a.dv; i += 256)
+      Num<T>::store(reinterpret_cast<T*>(a.out) + (b * heads + h0) * a.dv + i, 0.f);
     return;
   }
   if (tid == 0) bad_page = 0;
@@ -356,44 +395,63 @@ void paged_chunk_kernel(PagedArgs a) {
 // ... for four columns; the splits are then added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-  __shared__ float red[4];
+  __shared__ float top;
   __shared__ int void_row;
   __shared__ __attribute__((aligned(16))) f32x4_t so[256];
   __shared__ float sl[256];
   const int tid = threadIdx.x;
   const int64_t row = a.first + blockIdx.x;
-  const PagedSpan span = paged_span(a, (uint32_t)row / (a.hkv * a.group));
-  T* dst = reinterpret_cast<T*>(a.out) + row * a.dv;
-  if (span.bad && tid == 0) *a.flag = 1;
-  if (tid == 0) void_row = 0;
-  __syncthreads();
   const float* ml = a.ml + 2 * row * a.chunks;
   const float* part = a.part + row * a.chunks * a.dv;
-  float mx = -INFINITY;
-  for (int c = tid; c < span.chunks; c += 256) {
-    mx = fmaxf(mx, ml[2 * c]);
-    if (ml[2 * c + 1] == -1.f) void_row = 1;
-  }
-  mx = wave_max(mx);
-  if ((tid & 63) == 0) red[tid >> 6] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float base = mx == -INFINITY ? 0.f : mx;
   const int pieces = a.dv >> 2, splits = 256 / pieces;
   const int piece = tid % pieces, split = tid / pieces;
+  // The first reads do not wait for the length: their places exist, whether a chunk is there or not.
+  float m0 = -INFINITY, l0 = 0.f, ms = 0.f, ls = 0.f;
+  f32x4_t os = {0.f, 0.f, 0.f, 0.f};
+  if (tid < a.chunks) {
+    m0 = ml[2 * tid];
+    l0 = ml[2 * tid + 1];
+  }
+  if (split < splits && split < a.chunks) {
+    ms = ml[2 * split];
+    ls = ml[2 * split + 1];
+    os = *reinterpret_cast<const f32x4_t*>(part + (int64_t)split * a.dv + 4 * piece);
+  }
+  const PagedSpan span = paged_span(a, paged_length(a, (uint32_t)row / (a.hkv * a.group)));
+  T* dst = reinterpret_cast<T*>(a.out) + row * a.dv;
+  if (span.bad && tid == 0) *a.flag = 1;
+  // (a sequence has at most 64 chunks: the first wavefront sees them all)
+  static_assert(kPagedChunks <= 64, "one wavefront holds all chunks' maxima");
+  if (tid < 64) {
+    const bool there = tid < span.chunks;
+    const float mx = wave_max(there ? m0 : -INFINITY);
+    const bool bad = __any(there && l0 == -1.f);
+    if (tid == 0) {
+      top = mx;
+      void_row = bad;
+    }
+  }
+  __syncthreads();
+  const float base = top == -INFINITY ? 0.f : top;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
   if (split < splits)
     for (int c = split; c < span.chunks; c += splits) {
-      const float f = __builtin_amdgcn_exp2f(ml[2 * c] - base);
-      sum = __builtin_fmaf(ml[2 * c + 1], f, sum);
-      o += *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * a.dv + 4 * piece) * f;
+      if (c != split) {
+        ms = ml[2 * c];
+        ls = ml[2 * c + 1];
+        os = *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * a.dv + 4 * piece);
+      }
+      const float f = __builtin_amdgcn_exp2f(ms - base);
+      sum = __builtin_fmaf(ls, f, sum);
+      o += os * f;
     }
   so[tid] = o;
   sl[tid] = sum;
   __syncthreads();
   if (split == 0) {
-    for (int s = 1; s < splits; ++s) {
+    const int filled = span.chunks < splits ? span.chunks : splits;
+    for (int s = 1; s < filled; ++s) {
       o += so[s * pieces + piece];
       sum += sl[s * pieces + piece];
     }
@@ -443,13 +501,19 @@ static int64_t paged_limit(int64_t width, int64_t page_size, int64_t max_length)
   if (max_length >= 0 && max_length < limit) limit = max_length;
   return limit;
 }
-// Most chunks of a sequence (the count grows with the visible keys up to kPagedChunks).
+// Most chunks that a sequence of up to `limit` keys can have: the count grows with the visible keys between the sizes
+// at which chunks grow.
 static int paged_chunks(int64_t limit, int64_t window, int64_t sinks) {
   int64_t n = limit;
   if (window > 0 && window < limit && sinks < limit - window) n = window + sinks;
-  if (n > (int64_t)kPagedKeys * kPagedChunks) return kPagedChunks;
-  const int64_t c = cdiv(n, kPagedKeys);
-  return c > 1 ? (int)c : 1;
+  int most = 1;
+  for (const int64_t x : {INT64_C(2048), INT64_C(4096), n}) {
+    const int64_t m = x < n ? x : n;
+    const int64_t c = m > 0 ? (m - 1) / paged_chunk((int)m) + 1 : 1;
+    if (c > most) most = (int)c;
+  }
+  // past the last size the count saw-tooths below its bound
+  return n > (int64_t)4 * kPagedKeys * kPagedChunks ? kPagedChunks : most;
 }
 
 }  // namespace biops

@@ -216,7 +216,8 @@ def test_host_checks_of_the_entry_points():
     assert size(3, 4, 64, 8, 16, -1, 0, 0) == 0  # 128 keys: one chunk
     assert size(3, 4, 64, 9, 16, -1, 0, 0) == 3 * 4 * 2 * 66 * 4
     assert size(3, 4, 64, 9, 16, 128, 0, 0) == 0 and size(3, 4, 64, 1 << 20, 16, -1, 100, 28) == 0
-    assert size(3, 4, 64, 1 << 20, 16, -1, 0, 0) == size(3, 4, 64, 512, 16, -1, 0, 0) == 3 * 4 * 64 * 66 * 4
+    assert size(3, 4, 64, 1 << 20, 16, -1, 0, 0) == size(3, 4, 64, 2048, 16, -1, 0, 0) == 3 * 4 * 64 * 66 * 4
+    assert size(3, 4, 64, 256, 16, -1, 0, 0) == size(3, 4, 64, 260, 16, -1, 0, 0) == 3 * 4 * 16 * 66 * 4  # the most up to there
     assert size(-1, 4, 64, 8, 16, -1, 0, 0) == -1 and size(3, 4, 264, 8, 16, -1, 0, 0) == -1
 
     def win(dtype=2, nseq=1, hq=4, hkv=2, lq=5, lk=5, d=64, window=4, sinks=0, scale=1.0, q=p, cu_q=N, flag=p):

@@ -160,8 +160,20 @@ def test_token_attention_with_a_window(dtype, window, sinks):
 
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 def test_long_sequences(index):
-    """More keys than fixed chunks hold: both sides of the border, and far beyond it."""
-    check([8191, 8192, 8193, 20000, 3], 4, 1, 64, 64, 16, 300, index=index)
+    """Both sides of the lengths at which chunks grow, and of the most chunks."""
+    check([1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8192, 20000, 32767, 32768, 32769, 70001, 3], 4, 1, 64, 64, 16, 300, index=index)
+
+
+def test_tables_of_every_width():
+    """The most chunks that a table allows, at the widths where it changes; the lengths are the same."""
+    lengths = [128, 1, 77]
+    kc, vc, table, lens = batch(lengths, 2, 64, 64, 16, 350)
+    q = randn(3, 4, 64, seed=351)
+    want = paged_attention_batch_invariant(q, kc, vc, table, lens)
+    for width in (8, 9, 64, 65, 256, 257, 512, 2048, 2049, 5000):
+        wide = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+        wide[:, :8] = table[:, :8]
+        assert_bitwise(paged_attention_batch_invariant(q, kc, vc, wide, lens), want, f"{width} pages")
 
 
 def test_pages_behind_the_window_are_not_read():
