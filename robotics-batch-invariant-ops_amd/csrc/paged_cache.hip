@@ -2,17 +2,26 @@
 //
 // Row r goes to slot s = slots[r]: page s / page_size, place s % page_size, all heads.  A negative slot
 // leaves the row out (padding); a slot past the cache is left out too and reported through the flag.
-// Pure data movement: each row is read and written once.
+// Pure data movement: each row is read and written once, and the copy's rate is the bound.
 //
 // Of rows that name one slot the last stays, whatever order workgroups run in: a workgroup looks
-// through the slots behind its rows and leaves a row out whose slot comes again.  That is quadratic, so
-// rows go in launches of kWriteRows, whose order on the stream does the rest.
+// through the slots behind its rows and leaves a row out whose slot comes again.  It does so while its own
+// rows are on their way into registers, and compares with the smallest and largest of its slots first,
+// which two instructions settle where a prompt's slots lie together.  The search is quadratic, so rows go in
+// launches of kWriteRows, whose order on the stream does the rest.
+//
+// us for rows of 8 + 8 heads of 128 fp16 (4 KB, read and written): 16383 rows 29.4 (4.6 TB/s; a plain copy
+// 27), with every slot somewhere else 38; 48 rows of half that 3.2, of which a launch is 2.6.
 #include "biops_common.h"
 
 namespace biops {
 
-constexpr int kWriteRows = 8192;   // rows of a launch
-constexpr int kWriteGroup = 8;     // rows of a workgroup
+constexpr int kWriteRows = 8192;  // rows of a launch; 16384: 32.3 us for the 29.4 above
+
+// Rows of a workgroup: one as long as that does not fill the card, then eight, which share a search.
+// us (one / eight) at 2 KB a row: 48 rows 3.2 / 5.0, 1024 4.1 / 5.3, 2048 5.7 / 5.4; the 16383 rows above 55 / 29
+// (four: 38, sixteen: 35).
+constexpr int kWriteGroup = 8, kWriteFew = 1024;
 
 struct WriteArgs {
   const char *k, *v;
@@ -32,75 +41,111 @@ __device__ __forceinline__ void copy_tail(const char* src, char* dst, int from, 
   for (int e = from; e < to; e += sizeof(U)) *reinterpret_cast<U*>(dst + e) = *reinterpret_cast<const U*>(src + e);
 }
 
-template <int E>
+// E: bytes of an element; G: rows of a workgroup.
+template <int E, int G>
 __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
-  __shared__ int64_t place[kWriteGroup];
-  __shared__ int again[kWriteGroup];
+  __shared__ int64_t place[G];
+  __shared__ int again[G];
   const int tid = threadIdx.x;
-  const int r0 = blockIdx.x * kWriteGroup;
-  const int n = a.rows - r0 < kWriteGroup ? a.rows - r0 : kWriteGroup;
+  const int r0 = blockIdx.x * G;
+  const int n = a.rows - r0 < G ? a.rows - r0 : G;
   auto slot = [&](int r) -> int64_t {
     return a.slots64 ? reinterpret_cast<const int64_t*>(a.slots)[r * a.slot_stride]
                      : (int64_t) reinterpret_cast<const int32_t*>(a.slots)[r * a.slot_stride];
   };
-  if (tid < kWriteGroup) {
-    int64_t s = tid < n ? slot(r0 + tid) : -1;
-    if (s >= (int64_t)a.total) {
-      *a.flag = 1;
-      s = -1;
-    }
-    place[tid] = s;
-    again[tid] = 0;
-  }
-  __syncthreads();
-  int64_t mine[kWriteGroup];
-#pragma unroll
-  for (int i = 0; i < kWriteGroup; ++i) mine[i] = place[i];
-  int hit = 0;
-  for (int r = r0 + 1 + tid; r < a.rows; r += 256) {
-    const int64_t s = slot(r);
-#pragma unroll
-    for (int i = 0; i < kWriteGroup; ++i)
-      if (s == mine[i] && r > r0 + i) hit |= 1 << i;
-  }
-#pragma unroll
-  for (int i = 0; i < kWriteGroup; ++i)
-    if (hit >> i & 1) again[i] = 1;
-  __syncthreads();
+  int64_t first = -1;
+  if (tid < n) first = slot(r0 + tid);
+
+  // 16-byte pieces of a row: the keys of all heads, then their values.  A thread keeps one piece of every
+  // `step`-th row, and another 256 pieces further on where rows are longer than that.
   const int kn = (a.kbytes + 15) >> 4, vn = (a.vbytes + 15) >> 4;
   const int per_row = a.heads * (kn + vn);
-  for (int u = tid; u < n * per_row; u += 256) {
-    const int i = u / per_row;
-    int c = u - i * per_row;
-    const int64_t s = place[i];
-    if (s < 0 || again[i]) continue;
-    const uint32_t page = (uint32_t)s / a.page, at = (uint32_t)s - page * a.page;
-    const int64_t r = r0 + i;
-    const char* src;
-    char* dst;
-    int bytes;
-    if (c < a.heads * kn) {
-      const int h = c / kn;
-      c -= h * kn;
-      src = a.k + r * a.kT + h * a.kH;
-      dst = a.kc + page * a.kcP + at * a.kcS + h * a.kcH;
-      bytes = a.kbytes;
-    } else {
-      c -= a.heads * kn;
-      const int h = c / vn;
-      c -= h * vn;
-      src = a.v + r * a.vT + h * a.vH;
-      dst = a.vc + page * a.vcP + at * a.vcS + h * a.vcH;
-      bytes = a.vbytes;
+  const int step = per_row < 256 ? 256 / per_row : 1;
+  const int i0 = per_row < 256 ? tid / per_row : 0;
+  for (int base = 0; base < per_row; base += 256) {
+    const int c = base + (per_row < 256 ? tid - i0 * per_row : tid);
+    const bool active = c < per_row && i0 < step;
+    const bool value = c >= a.heads * kn;
+    const int x = value ? c - a.heads * kn : c;
+    const int h = active ? x / (value ? vn : kn) : 0;
+    const int e = 16 * (x - h * (value ? vn : kn));
+    const bool whole = e + 16 <= (value ? a.vbytes : a.kbytes);
+    const int64_t sT = value ? a.vT : a.kT;
+    const char* const src = (value ? a.v + h * a.vH : a.k + h * a.kH) + e;
+    char* const dst = (value ? a.vc + h * a.vcH : a.kc + h * a.kcH) + e;
+    const int64_t dP = value ? a.vcP : a.kcP, dS = value ? a.vcS : a.kcS;
+    u32x4_t piece[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int i = i0 + j * step;
+      if (active && whole && i < n) piece[j] = load_16(src + (r0 + i) * sT);
     }
-    const int e = 16 * c;
-    if (e + 16 <= bytes) {
-      *reinterpret_cast<u32x4_any_t*>(dst + e) = load_16(src + e);
-    } else {
-      if constexpr (E == 4) copy_tail<uint32_t>(src, dst, e, bytes);
-      else copy_tail<uint16_t>(src, dst, e, bytes);
+    if (base == 0) {  // the rows are on their way: which of them stay?
+      if (tid < G) {
+        if (first >= (int64_t)a.total) {
+          *a.flag = 1;
+          first = -1;
+        }
+        place[tid] = first;
+        again[tid] = 0;
+      }
+      __syncthreads();
+      int64_t lo = -1, hi = -1;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int64_t s = place[i];
+        if (s < 0) continue;
+        lo = lo < 0 || s < lo ? s : lo;
+        hi = s > hi ? s : hi;
+      }
+      if (hi >= 0) {
+        constexpr int kAhead = 4;
+        for (int r = r0 + 1; r < a.rows; r += 256 * kAhead) {
+          int64_t s[kAhead];
+          int at[kAhead];
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            at[j] = r + tid + 256 * j < a.rows ? r + tid + 256 * j : a.rows - 1;
+            s[j] = slot(at[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            if (s[j] < lo || s[j] > hi) continue;
+            for (int i = 0; i < G; ++i)
+              if (s[j] == place[i] && at[j] > r0 + i) again[i] = 1;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (!active) continue;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int i = i0 + j * step;
+      if (i >= n) break;
+      const int64_t s = place[i];
+      if (s < 0 || again[i]) continue;
+      const uint32_t page = (uint32_t)s / a.page, at = (uint32_t)s - page * a.page;
+      char* const to = dst + page * dP + at * dS;
+      if (whole) {
+        *reinterpret_cast<u32x4_any_t*>(to) = piece[j];
+      } else {
+        const char* from = src + (r0 + i) * sT;
+        const int left = (value ? a.vbytes : a.kbytes) - e;
+        if constexpr (E == 4) copy_tail<uint32_t>(from, to, 0, left);
+        else copy_tail<uint16_t>(from, to, 0, left);
+      }
     }
   }
+}
+
+template <int E>
+static int write_launch(const WriteArgs& a, hipStream_t s) {
+  const int group = a.rows <= kWriteFew ? 1 : kWriteGroup;
+  const dim3 grid((unsigned)cdiv(a.rows, group));
+  if (group == 1) hipLaunchKernelGGL((paged_write_kernel<E, 1>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((paged_write_kernel<E, kWriteGroup>), grid, dim3(256), 0, s, a);
+  return check_launch("paged_write_kernel");
 }
 
 }  // namespace biops
@@ -137,10 +182,8 @@ extern "C" int biops_paged_write(int dtype, int64_t rows, int64_t heads, int64_t
     a.k = static_cast<const char*>(k) + r * a.kT;
     a.v = static_cast<const char*>(v) + r * a.vT;
     a.slots = static_cast<const char*>(slots) + r * slot_stride * (slots64 ? 8 : 4);
-    const dim3 grid((unsigned)cdiv(a.rows, kWriteGroup));
-    if (elt == 4) hipLaunchKernelGGL((paged_write_kernel<4>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
-    else hipLaunchKernelGGL((paged_write_kernel<2>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
-    const int rc = check_launch("paged_write_kernel");
+    const int rc = elt == 4 ? write_launch<4>(a, static_cast<hipStream_t>(stream))
+                            : write_launch<2>(a, static_cast<hipStream_t>(stream));
     if (rc != BIOPS_OK) return rc;
   }
   return BIOPS_OK;

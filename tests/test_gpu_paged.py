@@ -53,6 +53,28 @@ def test_write(dtype, d, dv, page, heads, tokens):
     assert_bitwise(vc.cpu(), want_v)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d, dv, page, heads", [(128, 128, 16, 4), (72, 80, 100, 3), (70, 6, 7, 5), (1, 3, 3, 2), (256, 300, 64, 9),
+                                                (8, 0, 4, 1), (512, 512, 8, 3)])
+@pytest.mark.parametrize("tokens", [1024, 1031])
+def test_write_of_many_rows(dtype, d, dv, page, heads, tokens):
+    """Several rows of a workgroup, rows shorter and longer than its threads, slots that repeat, scattered and padding."""
+    pages = -(-2 * tokens // page)
+    k, v = randn(tokens, heads, d, seed=21, dtype=dtype), randn(tokens, heads, dv, seed=22, dtype=dtype)
+    kc, vc = randn(pages, page, heads, d, seed=23, dtype=dtype), randn(pages, page, heads, dv, seed=24, dtype=dtype)
+    g = torch.Generator().manual_seed(25)
+    slots = torch.randperm(pages * page, generator=g)[:tokens]
+    slots[100:400] = torch.arange(300) + 11  # a prompt
+    slots[torch.randint(0, tokens, (64,), generator=g)] = -1
+    slots[::97] = slots[torch.randint(0, tokens, (len(slots[::97]),), generator=g)]
+    slots[40:44] = 5  # neighbours, and the rest of their workgroup padding
+    slots[44:48] = -1
+    want_k, want_v = written(kc, k, slots), written(vc, v, slots)
+    paged_cache_write(k, v, kc, vc, slots.cuda())
+    assert_bitwise(kc.cpu(), want_k)
+    assert_bitwise(vc.cpu(), want_v)
+
+
 def test_write_from_and_into_views():
     """Rows from one projection's output, caches as halves of one allocation, slots by strides."""
     qkv = randn(2, 5, 8 * 64, seed=6)
