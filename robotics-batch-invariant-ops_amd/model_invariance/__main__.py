@@ -1,4 +1,4 @@
-"""python -m model_invariance [--adapter synthetic_vla] [--preset small|vla] [--batch-sizes 1,2,...]
+"""python -m model_invariance [--adapter synthetic_vla|synthetic_decoder] [--preset small|vla] [--batch-sizes 1,2,...]
 [--invariant-ops] [--seed 0] [--output report.json]: run the investigation and print its
 summary (one line per composition and batch size)."""
 
@@ -13,7 +13,7 @@ from .harness import DEFAULT_BATCH_SIZES, run_investigation
 def main(argv=None) -> int:
     p = argparse.ArgumentParser(prog="python -m model_invariance")
     p.add_argument("--adapter", choices=sorted(ADAPTERS), default="synthetic_vla")
-    p.add_argument("--preset", default="small", help="synthetic_vla sizes: small or vla")
+    p.add_argument("--preset", default="small", help="sizes: small or vla")
     p.add_argument("--batch-sizes", default=",".join(map(str, DEFAULT_BATCH_SIZES)))
     p.add_argument("--invariant-ops", action="store_true", help="run under set_batch_invariant_mode()")
     p.add_argument("--seed", type=int, default=0)
