@@ -4,11 +4,12 @@
 // Query r of a sequence (lq queries, lk keys) is the token at p = lk - lq + r and sees the keys j <= p
 // with p - j < window or j < sinks:  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q.k_j.
 //
-// One workgroup (four wavefronts of 32 rows) owns 128 query rows of one head and passes once over the
-// keys that any of them sees, counted through from 0: the sinks in front of the first row's window, then
-// everything up to the last row.  So the sinks share the first block with the window's first keys, and work
-// grows with the window, not with the sequence.  Blocks of 64 keys (32 in float32) go through LDS, double
-// buffered; running maximum m and sum l per row, O rescaled when a maximum grows.
+// A workgroup's wavefronts own 32 query rows each, of one head or of several that share a key/value head
+// (window_launch_rows has the variants and what they measured), and pass once over the keys that any of
+// them sees, counted through from 0: the sinks in front of the first row's window, then everything up to the last
+// row.  So the sinks share the first block with the window's first keys, and work grows with the window, not with the
+// sequence.  Blocks of 64 keys (float32 with one turn: 32) go straight from memory to LDS, double buffered, keys a
+// block ahead of values; running maximum m and sum l per row, O rescaled when a maximum grows.
 //
 // Register layout: S^T = K Q^T (K as the A operand of 32x32 MFMAs) leaves lane L with query row L % 32 and
 // keys 8j + 4(L/32) + i of a 32-key block, which is the B operand of O^T = V^T P^T with the same key order
@@ -22,7 +23,15 @@
 // another does not (0 * inf): a row whose sum is finite and whose output is not is computed again, key by
 // key over what it sees (window_row).
 //
-// Batch invariance: a tile's keys, blocks and order follow from its own sequence's lengths alone.
+// Batch invariance: a tile's keys, blocks and order follow from its own sequence's lengths, and the variant from
+// sizes that a call's sequences share.
+//
+// What bounds it: the vector units and the matrix cores in turn.  A score costs about seven vector slots
+// (maximum, fused multiply-add, exponential at a quarter of the rate, conversion, sum) and 4 D / 1024 matrix cycles of
+// a 16-bit type; two or three wavefronts of a SIMD overlap the two in part.  bf16, 16/4 heads of 128, 2 x 8192 tokens
+// under a window of 2048: 332 us, 770 TF/s of visible pairs (without any exponential 270, without any product 191,
+// fetches alone 100); fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 32 us.  float32 products
+// run at 1/16 of the 16-bit rate and bound it alone: 3 x 257 rows of 1281 keys, 16 heads of 72, window 500: 42 us.
 #include <type_traits>
 
 #include "gemm_core.h"
@@ -30,12 +39,7 @@
 
 namespace biops {
 
-// Visible keys up to which 16-bit tiles have 64 rows and two wavefronts for each 32 of them, by head size; 128 rows
-// and one wavefront each otherwise.  bf16, us (64 rows / 128 rows), batch 8 x 16/4 heads x 2048: 64-wide, window 64
-// 38 / 41, 256 57 / 59, 512 80 / 79, 2048 147 / 137; 128-wide, 256 116 / 98, 1024 218 / 182.  With one sequence the
-// small tile fills more of the chip (128-wide, 1 x 2048, window 256: 18 / 21), and a 128-wide head's shortest windows
-// take it for that.
-constexpr int kWindowShort64 = 512, kWindowShort128 = 128;
+constexpr int kWindowFew = 64, kWindowMany = 2048, kWindowShort = 512;  // see window_launch_rows
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
 struct WindowArgs {
@@ -67,9 +71,6 @@ __device__ __forceinline__ int64_t window_offset(const void* cu, int is64, int64
   return is64 ? reinterpret_cast<const int64_t*>(cu)[i * stride] : (int64_t) reinterpret_cast<const int32_t*>(cu)[i * stride];
 }
 
-// Tile `tl` of the packed rows.  Segment 0 are rows in front of the first offset, segment i sequence i - 1,
-// the last one the rows behind the last offset; the outer two have no keys and become zeros.  Offsets are
-// taken into [0, rows] and as their running maximum, so every row is in one segment whatever they hold.
 template <typename T>
 __device__ __forceinline__ uint32_t window_pack(float x, float y) {
   if constexpr (std::is_same<T, bf16_t>::value) return f32x2_to_bf16x2_bits(x, y);
@@ -84,6 +85,9 @@ __device__ __forceinline__ float window_add_pair(uint32_t xy, float l) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, xy), __builtin_bit_cast(f16x2_t, 0x3c003c00u), l, false);
 }
 
+// Tile `tl` of the packed rows.  Segment 0 are rows in front of the first offset, segment i sequence i - 1,
+// the last one the rows behind the last offset; the outer two have no keys and become zeros.  Offsets are
+// taken into [0, rows] and as their running maximum, so every row is in one segment whatever they hold.
 template <int ROWS>
 __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lane, WindowTile& t) {
   const int n = (int)a.nseq, segments = n + 2;
@@ -136,11 +140,11 @@ __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lan
 
 // DP, DVP: head and value size rounded up to whole fragments; RW row groups of 32 by KW wavefronts that share a
 // row group and take turns at the keys.
-template <typename T, int DP, int DVP, int RW, int KW_, int NH_>
+template <typename T, int DP, int DVP, int RW, int KW_, int NH_, int HG>
 struct WindowShape {
   static constexpr int E = sizeof(T), VEC = 16 / E;
   static constexpr int KW = KW_, NH = NH_;             // NH: 32-key parts of a block that a wavefront takes
-  static constexpr int ROWS = 32 * RW, THREADS = 64 * RW * KW;
+  static constexpr int ROWS = 32 * RW / HG, THREADS = 64 * RW * KW;
   static constexpr int BN = 32 * NH * KW;              // keys of a block
   static constexpr int KCH = DP / VEC, VCH = DVP / VEC;  // 16-byte chunks of a K / V row
   static constexpr int slots(int chunks) { return chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32); }
@@ -213,19 +217,20 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const char* q, c
 }
 
 // Wavefronts per SIMD that registers are given out for.
-template <typename T, int DP, int DVP, int RW, int KW, int NH>
-constexpr int window_waves() { return DP > 128 || DVP > 128 ? 1 : (sizeof(T) == 2 && DP <= 64 && DVP <= 64 ? (RW < 4 ? 4 : 3) : 2); }
+template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
+constexpr int window_waves() { return DP > 128 || DVP > 128 || (sizeof(T) == 4 && DP > 64 && KW > 1) ? 1 : (sizeof(T) == 2 && DP <= 64 && DVP <= 64 ? (NH == 1 ? 4 : 3) : 2); }
 
-template <typename T, int DP, int DVP, int RW, int KW, int NH>
-__global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP, RW, KW, NH>(), window_waves<T, DP, DVP, RW, KW, NH>())))
+template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
+__global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP, RW, KW, NH, HG>(), window_waves<T, DP, DVP, RW, KW, NH, HG>())))
 void window_attn_kernel(WindowArgs a) {
-  using F = WindowShape<T, DP, DVP, RW, KW, NH>;
+  using F = WindowShape<T, DP, DVP, RW, KW, NH, HG>;
   constexpr int E = F::E, BN = F::BN;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS_BYTES];
   // What is the same for a wavefront is told to the compiler, and then computed once for it.
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63, hf = lane >> 5, l32 = lane & 31;
   const int rw = w % RW, part = w / RW;  // row group, turn at the keys
+  const int r0 = 32 * (rw / HG);         // its first row
   const u32x4_t zero4 = {0u, 0u, 0u, 0u};
 
   // Workgroups are dealt to the 8 XCDs in turn: every XCD takes a run of each kWindowOrder tiles, so that the
@@ -240,8 +245,9 @@ void window_attn_kernel(WindowArgs a) {
   WindowTile tile;
   const uint32_t tl = t % a.tiles;
   t /= a.tiles;
-  const int h = (int)(t % (a.hkv * a.group)), hk = h / (int)a.group;
-  const int64_t b = t / (a.hkv * a.group);
+  const uint32_t htiles = a.hkv * a.group / HG;
+  const int h = (int)(t % htiles) * HG + rw % HG, hk = h / (int)a.group;
+  const int64_t b = t / htiles;
   if (a.cu_q) {
     if (!window_find<F::ROWS>(a, (int)tl, lane, tile)) return;
     tile.i0 = uniform(tile.i0);
@@ -277,14 +283,14 @@ void window_attn_kernel(WindowArgs a) {
     return x > 0 ? (int)x : 0;
   };
 
-  const int rloc = 32 * rw + l32;
+  const int rloc = r0 + l32;
   const bool row_ok = rloc < qrows;
   const int hi = row_ok ? p0 + rloc - shift : -1;  // negative: nothing
   const int lo = row_lo(p0 + rloc);
-  const int wlast = 32 * rw + 31 < qrows ? 32 * rw + 31 : qrows - 1;  // last row of the wavefront
-  const bool wany = 32 * rw < qrows;
-  const int wlo0 = row_lo(p0 + 32 * rw), wlo1 = row_lo(p0 + wlast);
-  const int whi0 = p0 + 32 * rw - shift, whi1 = p0 + wlast - shift;
+  const int wlast = r0 + 31 < qrows ? r0 + 31 : qrows - 1;  // last row of the wavefront
+  const bool wany = r0 < qrows;
+  const int wlo0 = row_lo(p0 + r0), wlo1 = row_lo(p0 + wlast);
+  const int whi0 = p0 + r0 - shift, whi1 = p0 + wlast - shift;
 
   // Rows behind the last one take its queries; they see nothing.
   u32x4_t qf[F::QF];
@@ -415,7 +421,7 @@ void window_attn_kernel(WindowArgs a) {
       for (int c = 0; c < F::QSTEP; ++c)
 #pragma unroll
         for (int x = 0; x < NH; ++x)
-          if (g * F::QSTEP + c < F::QF) Mfma<T>::step(sc[x], kf[g & 1][c][x], qf[g * F::QSTEP + c]);
+          if (g * F::QSTEP + c < F::QF && (E == 2 || 2 * F::VEC * (g * F::QSTEP + c) < a.d)) Mfma<T>::step(sc[x], kf[g & 1][c][x], qf[g * F::QSTEP + c]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -423,18 +429,20 @@ void window_attn_kernel(WindowArgs a) {
   u32x4_t pw[E == 2 ? NH : 1][2];  // 16-bit weights, packed; float32 ones stay in sc
   auto weigh = [&](int blk) {
     const int v0 = blk * BN + 32 * hb0, v1 = v0 + 32 * NH - 1;
-    if (!(wlast == 32 * rw + 31 && v0 >= wlo1 && v1 <= whi0)) {  // not all rows see all keys
-      const int vb0 = v0 + 4 * hf;  // register r of part x: key vb0 + 32 x + 8(r/4) + r%4
-      // lo <= v <= hi by one unsigned comparison; rows that see nothing have a bound that none passes
-      const uint32_t span = hi < lo ? 0u : (uint32_t)(hi - lo);
-      const int from = hi < lo ? 0x7fffffff : lo - vb0, sink = (sv <= hi ? sv : hi + 1) - vb0;
+    if (!(wlast == r0 + 31 && v0 >= wlo1 && v1 <= whi0)) {  // not all rows see all keys
+      // A row's keys of a part as bits, so that a score costs one bit's extension and one selection.
+      auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : ~0u >> (n < 32 ? 32 - n : 0); };  // the n lowest bits
 #pragma unroll
-      for (int x = 0; x < NH; ++x)
+      for (int x = 0; x < NH; ++x) {
+        const int v = v0 + 32 * x;
+        // register r: key 8(r/4) + 4hf + r%4
+        const uint32_t seen = ((below(hi + 1 - v) & ~below(lo - v)) | below((sv <= hi ? sv : hi + 1) - v)) >> (4 * hf);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int o = 32 * x + 8 * (r >> 2) + (r & 3);
-          sc[x][r] = (uint32_t)(o - from) <= span || o < sink ? sc[x][r] : -INFINITY;
+          const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - (8 * (r >> 2) + (r & 3)))) >> 31);
+          sc[x][r] = __uint_as_float((__float_as_uint(sc[x][r]) & keep) | (0xff800000u & ~keep));
         }
+      }
     }
     float mx = sc[0][0];
 #pragma unroll
@@ -635,44 +643,70 @@ void window_attn_kernel(WindowArgs a) {
       }
     }
     for (uint64_t rest = (again | again >> 32) & 0xffffffffull; rest != 0; rest &= rest - 1) {
-      const int r = 32 * rw + __builtin_ctzll(rest);
+      const int r = r0 + __builtin_ctzll(rest);
       window_row<T>(a, qb + r * a.qT, kb, vb, ob + r * a.oT, p0 + r, kl, lane);
     }
   }
 }
 
-template <typename T, int DP, int DVP, int RW, int KW, int NH>
+template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
 static int window_launch(WindowArgs a, hipStream_t s) {
-  constexpr int rows = 32 * RW;
+  constexpr int rows = 32 * RW / HG;
   // packed: every sequence and the two ends may end in a part of a tile
   const int64_t tiles = a.cu_q ? a.lq / rows + a.nseq + 2 : cdiv(a.lq, rows);
-  const int64_t heads = (int64_t)a.hkv * a.group * (a.cu_q ? 1 : a.nseq);
+  const int64_t heads = (int64_t)a.hkv * a.group / HG * (a.cu_q ? 1 : a.nseq);
   if (tiles > INT64_C(0x7fffffff) / heads) return fail(BIOPS_ERR_ARG, "biops_window_attention: more than 2^31 tiles");
   a.tiles = (uint32_t)tiles;
   a.total = (uint32_t)(tiles * heads);
   constexpr uint32_t most = 1 << 22;  // a launch has less than 2^32 threads
   for (a.first = 0; a.first < a.total; a.first += most) {
     const uint32_t n = a.total - a.first < most ? a.total - a.first : most;
-    hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW, KW, NH>), dim3(n), dim3(64 * RW * KW), 0, s, a);
+    hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW, KW, NH, HG>), dim3(n), dim3(64 * RW * KW), 0, s, a);
     const int rc = check_launch("window_attn_kernel");
     if (rc != BIOPS_OK) return rc;
   }
   return BIOPS_OK;
 }
-// Rows per workgroup.  Only sizes that all sequences of a call share may enter: the rows of a tile decide where
+// What a workgroup takes.  Only sizes that all sequences of a call share may enter: the rows of a tile decide where
 // its blocks of keys begin, and so the bits.
+//
+// Heads of a group in one workgroup share its fetches, and their tile of fewer rows has fewer keys that only some of its
+// rows see.  Two wavefronts for the same rows, with the keys in turns, halve a tile's time where there are too few
+// tiles to fill the chip, and cost their join.  us, variants as <wavefronts for rows and heads, turns, 32-key parts,
+// heads>, 16/4 heads unless said otherwise:
+//   16-bit                        <4,1,2,4> <4,1,2,2> <4,1,2,1> <2,2,1,2> <2,2,1,1>
+//   64-wide, 4 x 2048, window 512    38.7      46.6      50.8      38.9      43.3
+//   128-wide, the same               55.0      60.7      67.0      74.8      82.1
+//   256-wide, the same              163       172       192       229       247
+//   128-wide, 8/8 heads                                  37.7                45.1
+//   64-wide, 8/8 heads, w. 512 / all                   25 / 50             25 / 58
+//   64-wide, 8/4 heads, w. 512 / all         23 / 49   25 / 50   22 / 47   24 / 57
+//   64-wide, 50 rows of 700 keys     18.7      19.0      18.7      14.2      14.3  (one sequence)
+//   128-wide, the same, 1 / 64 seq. 24 / 33   24 / 35   23 / 53   18 / 43   18 / 44
+//   float32                       <4,1,1,4> <4,1,1,2> <4,1,1,1> <2,2,1,2> <2,2,1,1>
+//   64-wide, 1 x 700 / 4 x 2048    52 / 167  55 / 180  57 / 198  30 / 170  32 / 192
+//   72-wide, the same              67 / 224  71 / 244  74 / 267  43 / 300  46 / 335
 template <typename T, int DP>
 static int window_launch_rows(const WindowArgs& a, hipStream_t s) {
+  const bool pairs = a.group % 2 == 0, fours = a.group % 4 == 0;
   if constexpr (sizeof(T) == 4) {
-    return window_launch<T, DP, DP, 2, 2, 1>(a, s);
-  } else if constexpr (DP > 128) {
-    return window_launch<T, DP, DP, 4, 1, 2>(a, s);
-  } else if constexpr (DP > 64) {
-    if ((int64_t)a.window + a.sinks <= kWindowShort128) return window_launch<T, DP, DP, 2, 2, 1>(a, s);
-    return window_launch<T, DP, DP, 4, 1, 2>(a, s);
+    if constexpr (DP > 64) {
+      if (!a.cu_q && a.lq >= kWindowMany) {
+        if (fours) return window_launch<T, DP, DP, 4, 1, 1, 4>(a, s);
+        return pairs ? window_launch<T, DP, DP, 4, 1, 1, 2>(a, s) : window_launch<T, DP, DP, 4, 1, 1, 1>(a, s);
+      }
+    }
+    return pairs ? window_launch<T, DP, DP, 2, 2, 1, 2>(a, s) : window_launch<T, DP, DP, 2, 2, 1, 1>(a, s);
   } else {
-    if ((int64_t)a.window + a.sinks <= kWindowShort64) return window_launch<T, DP, DP, 2, 2, 1>(a, s);
-    return window_launch<T, DP, DP, 4, 1, 2>(a, s);
+    const bool few = !a.cu_q && a.lq <= kWindowFew;
+    if (pairs && (few || (DP <= 64 && !fours))) return window_launch<T, DP, DP, 2, 2, 1, 2>(a, s);
+    if (few || (DP <= 64 && !pairs && (int64_t)a.window + a.sinks <= kWindowShort))
+      return window_launch<T, DP, DP, 2, 2, 1, 1>(a, s);
+    if (fours) return window_launch<T, DP, DP, 4, 1, 2, 4>(a, s);
+    if constexpr (DP > 64) {
+      if (pairs) return window_launch<T, DP, DP, 4, 1, 2, 2>(a, s);
+    }
+    return window_launch<T, DP, DP, 4, 1, 2, 1>(a, s);
   }
 }
 template <typename T>

@@ -8,7 +8,7 @@ import torch
 from batch_invariant_ops import (check_cache_indices, sliding_window_attention_batch_invariant as window_attention,
                                  varlen_sliding_window_attention_batch_invariant as packed_attention)
 
-from _decoder import check_window
+from _decoder import assert_within, attend64, attention_bound, check_window, prompt_rounding, window_visible
 from _tol import assert_bitwise
 
 pytestmark = pytest.mark.gpu
@@ -57,6 +57,54 @@ def test_windows_and_sinks(dtype, window, sinks):
 @pytest.mark.parametrize("d, dv", [(256, 256), (192, 128), (64, 136)])
 def test_wide_heads(dtype, d, dv):
     check(1, 2, 1, 150, 170, d, dv, 60, 3, 20, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 6, 8])
+@pytest.mark.parametrize("d", [64, 88, 128, 256])
+@pytest.mark.parametrize("lq", [50, 64, 65, 130])
+def test_heads_of_a_group(dtype, group, d, lq):
+    """Query heads that share a workgroup, with few rows and many."""
+    if dtype == torch.float32 and d > 128:
+        pytest.skip("float32 heads go up to 128")
+    check(1, 2 * group, 2, lq, 170, d, d, 60, 3, 25, dtype)
+    if d == 64 and group < 4:
+        check(1, 2 * group, 2, lq, 170, d, d, None, 0, 26, dtype)  # a longer window takes another tile
+
+
+@pytest.mark.parametrize("group", [1, 2, 4])
+@pytest.mark.parametrize("d", [72, 128])
+def test_long_float32_prompts(group, d):
+    q, k, v = (randn(1, h, 2050, d, seed=27 + h, dtype=torch.float32) for h in (group, 1, 1))
+    out = window_attention(q, k, v, 100, 4, enable_gqa=True)
+    for a in (0, 1000, 1900):  # a part of the rows, with the keys up to its last
+        rows = slice(a, a + 150)
+        check = out[0, :, rows], q[0, :, rows], k[0, :, :a + 150], v[0, :, :a + 150]
+        check_window(*check, 100, 4, what=f"rows from {a}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group, lq", [(4, 200), (4, 40), (2, 200), (1, 200)])
+def test_masked_values_with_heads_of_a_group(dtype, group, lq):
+    q, k, v = (randn(1, h, n, 64, seed=28 + h, dtype=dtype) for h, n in ((2 * group, lq), (2, 200), (2, 200)))
+    for at, bad in ((170, float("nan")), (190, float("inf")), (20, float("nan"))):
+        k[:, :, at] = bad
+        v[:, :, at + 1] = bad
+    out = window_attention(q, k, v, 7, 2, enable_gqa=True)
+    seen = torch.isnan(out[0]).any(-1)
+    assert bool(seen.any()) and not bool(seen.all())
+    first = 200 - lq
+    for r in range(lq):  # a row is touched if and only if it sees one of the six
+        p = first + r
+        touched = any(0 <= p - x < 7 for at in (170, 190, 20) for x in (at, at + 1))
+        if not touched:
+            assert not bool(torch.isnan(out[0, :, r]).any()) and not bool(torch.isinf(out[0, :, r]).any()), f"row {r}"
+    fine = torch.tensor([not any(0 <= first + r - x < 7 for at in (170, 190, 20) for x in (at, at + 1)) for r in range(lq)])
+    clean = [torch.nan_to_num(t, 0.0, 0.0, 0.0) for t in (k, v)]
+    for h in range(2 * group):
+        parts = attend64(q[0, h], clean[0][0, h // group], clean[1][0, h // group], window_visible(lq, 200, 7, 2), 0.125)
+        bound = attention_bound(dtype, *parts, 9, *prompt_rounding(dtype))
+        assert_within(out[0, h][fine.cuda()], parts[0][fine], bound[fine], f"head {h}")
 
 
 def test_longer_than_the_window_many_times():
