@@ -21,6 +21,8 @@
 //     elements (16 bytes; 8 with 64-wide heads) of value rows 8q .. 8q + 7 at column W m -- whole
 //     rows, contiguous over the lanes -- and turns its own 8 x W block with byte permutes: row m of output
 //     block t is column W m + t.
+// Weights are kept 2^-31 times their size where the type has float's range, so that sums of values near its end
+// stay finite (of fewer than 2^31 keys none can pass the largest value); fp16's cannot get there.
 // 16-bit weights go in as a rounded part and the rounded rest (two MFMAs), which leaves an error of
 // 2^-16 (bf16) instead of 2^-8 where the matrix cores have the time.
 //
@@ -158,6 +160,7 @@ void paged_chunk_kernel(PagedArgs a) {
   constexpr int W = E == 2 && DVP <= 64 ? 4 : VEC;      // elements of a value load
   constexpr int NB = DVP / (16 * W), NT = NB * W;       // value blocks of a row; 16-column output blocks
   constexpr int VD = W * E / 4;                         // dwords of a value load
+  constexpr float kDown = std::is_same<T, f16_t>::value ? 1.f : 0x1p-31f;
   extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][cols][DVP] O, then [4][cols][2] m, l
   __shared__ __attribute__((aligned(16))) int64_t offs[4][2][32];
   __shared__ int bad_page;
@@ -303,7 +306,7 @@ void paged_chunk_kernel(PagedArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], a.scale, -sh));
+      p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], a.scale, -sh)) * kDown;
       l += p[j];
     }
     if constexpr (E == 4) {

@@ -313,6 +313,19 @@ def test_bad_lengths_and_pages_give_zeros_and_are_reported():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_values_at_the_end_of_the_range(dtype):
+    """Their mean is in the range where their sum is not."""
+    lengths = [2, 40, 700, 3000]
+    kc, vc, table, lens = batch(lengths, 1, 64, 64, 16, 1100, dtype)
+    vc.copy_(torch.where(torch.isnan(vc), vc, torch.where(vc > 0, 0.99, 0.9) * torch.finfo(dtype).max))
+    q = randn(4, 2, 64, seed=1101, dtype=dtype)
+    out = paged_attention_batch_invariant(q, kc, vc, table, lens)
+    assert bool(torch.isfinite(out).all())
+    for b, n in enumerate(lengths):
+        check_token(out[b], q[b], kc, vc, table[b], n, what=f"sequence of {n}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_special_values(dtype):
     """A score of -inf has weight 0; one of +inf or NaN makes its own row NaN and no other."""
     kc, vc, table, lens = batch([40, 200, 300], 1, 64, 64, 16, 1000, dtype)
