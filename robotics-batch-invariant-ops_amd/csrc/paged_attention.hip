@@ -99,33 +99,25 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedArgs& a, int len) {
   return s;
 }
 
-// Work item `it` of the batch: chunk c of sequence b, all chunks of the first sequence, then of the next.  Counting
-// them here leaves no idle workgroups between those with work (64 sequences of 250 to 16384 keys: 142 us with a
-// workgroup for every chunk that the longest sequence could have).
+// Work item `it` of a batch of up to 64 sequences: chunk c of sequence b, all chunks of the first sequence, then of the
+// next.  Counting them here leaves no idle workgroups between those with work (64 sequences of 250 to 16384 keys: 142 us
+// with a workgroup for every chunk that the longest sequence could have, 113 so).
 __device__ __forceinline__ bool paged_find(const PagedArgs& a, int it, int lane, uint32_t& b, int& c, int& length) {
-  int done = 0;
-  for (uint32_t base = 0; base < a.batch; base += 64) {
-    const uint32_t i = base + lane;
-    const int len = i < a.batch ? paged_length(a, i) : 0;
-    const int mine = paged_span(a, len).chunks;
-    int upto = mine;
+  const int len = lane < (int)a.batch ? paged_length(a, lane) : 0;
+  const int mine = paged_span(a, len).chunks;
+  int upto = mine;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += x;
-    }
-    upto += done;
-    const uint64_t hit = __ballot(upto > it);
-    if (hit != 0) {
-      const int f = __builtin_ctzll(hit);
-      b = base + f;
-      c = it - (__builtin_amdgcn_readlane(upto, f) - __builtin_amdgcn_readlane(mine, f));
-      length = __builtin_amdgcn_readlane(len, f);
-      return true;
-    }
-    done = __builtin_amdgcn_readlane(upto, 63);
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += x;
   }
-  return false;
+  const uint64_t hit = __ballot(upto > it);
+  if (hit == 0) return false;
+  const int f = __builtin_ctzll(hit);
+  b = f;
+  c = it - (__builtin_amdgcn_readlane(upto, f) - __builtin_amdgcn_readlane(mine, f));
+  length = __builtin_amdgcn_readlane(len, f);
+  return true;
 }
 
 template <typename T>
@@ -175,9 +167,17 @@ void paged_chunk_kernel(PagedArgs a) {
   const uint32_t hk = r % a.hkv;
   uint32_t b = r / a.hkv;
   int c = 0, length;
-  if (a.chunks == 1) length = paged_length(a, b);
-  else if (!paged_find(a, (int)b, lane, b, c, length)) return;
+  if (a.chunks == 1) {
+    length = paged_length(a, b);
+  } else if (a.batch <= 64) {
+    if (!paged_find(a, (int)b, lane, b, c, length)) return;
+  } else {  // first chunks of all sequences, then second ones: what is idle comes last
+    c = (int)(b / a.batch);
+    b -= c * a.batch;
+    length = paged_length(a, b);
+  }
   const PagedSpan span = paged_span(a, length);
+  if (a.chunks > 1 && c >= span.chunks) return;
   const int cols = a.group - z * kPagedCols < kPagedCols ? (int)(a.group - z * kPagedCols) : kPagedCols;
   const int64_t h0 = hk * a.group + z * kPagedCols;
   if (span.chunks == 0) {  // (one chunk at most, and no join) a row that sees nothing

@@ -85,57 +85,57 @@ __device__ __forceinline__ float window_add_pair(uint32_t xy, float l) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, xy), __builtin_bit_cast(f16x2_t, 0x3c003c00u), l, false);
 }
 
-// Tile `tl` of the packed rows.  Segment 0 are rows in front of the first offset, segment i sequence i - 1,
-// the last one the rows behind the last offset; the outer two have no keys and become zeros.  Offsets are
-// taken into [0, rows] and as their running maximum, so every row is in one segment whatever they hold.
+// Tile `tl` of the packed rows.  Segment 0 are rows in front of the first offset, segment j sequence j - 1, the last one
+// the rows behind the last offset; the outer two have no keys and become zeros.  Segment j's tiles are numbered from
+// begin / ROWS + j: that leaves room for as many as it can need, without counting those in front of it, so the
+// segment is found by a search, 64 places at a time.  Offsets are taken into [0, rows]; where they do not rise the search
+// ends somewhere, and what it finds is inside the tensors.
 template <int ROWS>
 __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lane, WindowTile& t) {
-  const int n = (int)a.nseq, segments = n + 2;
-  int before = 0, done = 0;  // end of the last segment, tiles so far
-  for (int base = 0; base < segments; base += 64) {
-    const int i = base + lane;
-    const int64_t raw = i <= n ? window_offset(a.cu_q, a.cu_q64, a.cu_q_stride, i) : (int64_t)a.lq;
-    // keys of the lane's segment, fetched along
-    int64_t ks = 0, ke = -1;
-    if (i >= 1 && i <= n) {
-      ks = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, i - 1);
-      ke = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, i);
+  const int n = (int)a.nseq;
+  int at = 0, left = n + 2;  // segments that are left to choose from
+  for (;;) {
+    const int step = (left - 1) / 64 + 1;
+    const bool in = lane < (left - 1) / step + 1;
+    const int j = at + (in ? lane * step : 0);
+    int64_t qs = 0, qe = a.lq, ks = 0, ke = -1;
+    if (j >= 1) qs = window_offset(a.cu_q, a.cu_q64, a.cu_q_stride, j - 1);
+    if (step == 1) {  // what the last round needs, fetched along
+      if (j <= n) qe = window_offset(a.cu_q, a.cu_q64, a.cu_q_stride, j);
+      if (j >= 1 && j <= n) {
+        ks = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, j - 1);
+        ke = window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, j);
+      }
     }
-    const bool keys_ok = ks >= 0 && ke >= ks && ke <= a.lk;
-    int end = raw < 0 ? 0 : (raw > a.lq ? a.lq : (int)raw);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(end, o, 64);
-      if (lane >= o && x > end) end = x;
+    auto row = [&](int64_t x) -> int { return x < 0 ? 0 : (x > a.lq ? a.lq : (int)x); };
+    const int begin = row(qs), rows = row(qe) - begin;
+    const int tile = tl - (begin / ROWS + j);
+    const uint64_t hit = __ballot(in && tile >= 0);
+    if (hit == 0) return false;
+    const int f = 63 - __builtin_clzll(hit);
+    if (step == 1) {
+      const bool keys_ok = ks >= 0 && ke >= ks && ke <= a.lk;
+      t.qrow = __builtin_amdgcn_readlane(begin, f);
+      t.ql = __builtin_amdgcn_readlane(rows, f);
+      t.krow = __builtin_amdgcn_readlane(keys_ok ? (int)ks : 0, f);
+      t.kl = __builtin_amdgcn_readlane(keys_ok ? (int)(ke - ks) : 0, f);
+      const int64_t i0 = (int64_t)__builtin_amdgcn_readlane(tile, f) * ROWS;
+      t.i0 = (int)i0;
+      return i0 < t.ql;
     }
-    if (before > end) end = before;
-    if ((end != raw || (i == 0 && raw != 0))) *a.flag = 1;
-    int begin = __shfl_up(end, 1, 64);
-    if (lane == 0) begin = before;
-    const int mine = (end - begin + ROWS - 1) / ROWS;
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += x;
-    }
-    upto += done;
-    const uint64_t hit = __ballot(i < segments && upto > tl);
-    if (hit != 0) {
-      const int f = __builtin_ctzll(hit);
-      const int b = __shfl(begin, f, 64), e = __shfl(end, f, 64), u = __shfl(upto, f, 64), m = __shfl(mine, f, 64);
-      t.qrow = b;
-      t.ql = e - b;
-      t.i0 = (tl - (u - m)) * ROWS;
-      t.krow = __shfl(keys_ok ? (int)ks : 0, f, 64);
-      t.kl = __shfl(keys_ok ? (int)(ke - ks) : 0, f, 64);
-      if (base + f >= 1 && base + f <= n && !__shfl((int)keys_ok, f, 64)) *a.flag = 1;
-      return true;
-    }
-    before = __shfl(end, 63, 64);
-    done = __shfl(upto, 63, 64);
+    at += f * step;
+    left = step < left - f * step ? step : left - f * step;
   }
-  return false;
+}
+
+// Whether sequence i's offsets rise and stay inside the tensors (i = nseq: whether the first one is zero and the last one
+// inside).
+__device__ __forceinline__ bool window_offsets_ok(const WindowArgs& a, int64_t i) {
+  auto q = [&](int64_t x) { return window_offset(a.cu_q, a.cu_q64, a.cu_q_stride, x); };
+  auto k = [&](int64_t x) { return window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, x); };
+  if (i == a.nseq) return q(0) == 0 && q(i) <= a.lq;
+  const int64_t ks = k(i), ke = k(i + 1);
+  return q(i) <= q(i + 1) && ks >= 0 && ks <= ke && ke <= a.lk;
 }
 
 // DP, DVP: head and value size rounded up to whole fragments; RW row groups of 32 by KW wavefronts that share a
@@ -249,12 +249,9 @@ void window_attn_kernel(WindowArgs a) {
   const int h = (int)(t % htiles) * HG + rw % HG, hk = h / (int)a.group;
   const int64_t b = t / htiles;
   if (a.cu_q) {
-    if (!window_find<F::ROWS>(a, (int)tl, lane, tile)) return;
-    tile.i0 = uniform(tile.i0);
-    tile.ql = uniform(tile.ql);
-    tile.kl = uniform(tile.kl);
-    tile.qrow = uniform(tile.qrow);
-    tile.krow = uniform(tile.krow);
+    const bool work = window_find<F::ROWS>(a, (int)tl, lane, tile);
+    if (h < HG && tl <= a.nseq && w == RW * KW - 1 && !window_offsets_ok(a, tl)) *a.flag = 1;
+    if (!work) return;
   } else {
     tile.i0 = (int)(a.tiles - 1 - tl) * F::ROWS;  // longest ranges first
     tile.qrow = tile.krow = 0;

@@ -151,6 +151,48 @@ def test_many_sequences():
         check_window(out[0, a:b].transpose(0, 1), *(x[0, a:b].transpose(0, 1) for x in (q, k, v)), 9, 1, what=f"sequence {s}")
 
 
+@pytest.mark.parametrize("count", [61, 62, 63, 64, 4093, 4094, 4095, 5000])
+def test_the_search_for_a_sequence(count):
+    """Both sides of the counts at which the search takes another round, with empty sequences among the others."""
+    g = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 5, (count,), generator=g)
+    lengths[count // 2] = 150
+    lengths[-1] = 40
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)])
+    total = int(cu[-1])
+    q, k, v = (randn(1, total + 37, h, 64, seed=61 + h) for h in (4, 1, 1))
+    out = packed_attention(q, k, v, cu.cuda(), cu.cuda(), 3, 1)
+    assert float(out[:, total:].abs().max()) == 0.0
+    # the same from the definition for all rows at once: three keys of the window and the first one, in 64 bits
+    place = torch.cat([torch.arange(n) for n in lengths.tolist()])
+    first = torch.arange(total) - place
+    at = torch.stack([torch.arange(total) - 2, torch.arange(total) - 1, torch.arange(total), first], 1)
+    seen = torch.stack([place >= 2, place >= 1, place >= 0, place >= 3], 1)
+    kk, vv = (t[0, :total, 0].cpu().double()[at.clamp(min=0)] for t in (k, v))
+    qq = q[0, :total].cpu().double()
+    s = torch.einsum("thd,tjd->thj", qq, kk) * 0.125
+    w = torch.softmax(s.masked_fill(~seen.unsqueeze(1), float("-inf")), -1)
+    o, mag = (torch.einsum("thj,tjd->thd", w, x) for x in (vv, vv.abs()))
+    err = 66 * 2.0**-24 * 0.125 * torch.einsum("thd,tjd->thj", qq.abs(), kk.abs()).amax(-1, keepdim=True)
+    assert_within(out[0, :total], o, attention_bound(BF16, o, mag, err, torch.zeros_like(o), 4, *prompt_rounding(BF16)))
+
+
+@pytest.mark.parametrize("at", [0, 3000, 4999])
+def test_bad_offsets_among_many_are_reported(at):
+    cu = torch.arange(5001, dtype=torch.int32)
+    q = randn(1, 5000, 2, 64, seed=65)
+    packed_attention(q, q, q, cu.cuda(), cu.cuda(), 3, 1)
+    check_cache_indices()
+    for which in range(2):
+        bad = cu.clone()
+        bad[at + (which == 0 or at == 0)] -= 2  # below the offset in front of it, or below zero
+        offsets = [cu.cuda(), cu.cuda()]
+        offsets[which] = bad.cuda()
+        packed_attention(q, q, q, *offsets, 3, 1)
+        with pytest.raises(RuntimeError, match="outside its tensor"):
+            check_cache_indices()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_bits_do_not_depend_on_the_batch(dtype):
     lengths = [300, 1, 0, 129, 700, 128]
@@ -251,7 +293,7 @@ def test_bad_offsets_are_reported_and_stay_inside():
     q, k, v, cu, _ = pack(lengths, lengths, 2, 1, 64, 64, 110)
     want = packed_attention(q, k, v, cu, cu, 30, 2)
     for bad_q, bad_k, same in (
-        ([0, 40, 30, 190], [0, 40, 170, 190], 40), ([0, 40, 170, 1000], [0, 40, 170, 190], 170),
+        ([0, 40, 30, 190], [0, 40, 170, 190], 30), ([0, 40, 170, 1000], [0, 40, 170, 190], 170),
         ([5, 40, 170, 190], [0, 40, 170, 190], 0), ([0, 40, 170, 190], [0, 40, 170, 191], 170),
         ([0, 40, 170, 190], [0, 40, -3, 190], 40), ([0, -(2**31), 170, 2**31 - 1], [0, 40, 170, 190], 0),
     ):
