@@ -275,7 +275,7 @@ def multi_axis_rotary(
     tensors ``(query, key)``, or the rotated query alone when ``key`` is None.  Differentiable with respect
     to ``query`` and ``key`` (not to ``positions``).
     """
-    plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(inv_freq),
+    plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(map(float, inv_freq)),
                         bool(interleaved_axes), bool(interleaved_pairs))
     module = _tensor_module or _direct()
     if module:
@@ -365,7 +365,9 @@ def paged_cache_write(
 
     ``slots`` (int32 or int64, the leading shape of ``key``) names the slot of each row: ``page * page_size +
     place``.  A negative slot leaves its row out (padding).  A slot past the cache is left out too and reported
-    as an error later (see the module).  Of several rows that name one slot the last one stays.
+    as an error later (see the module).  Of several rows that name one slot the last one stays.  ``key`` and
+    ``value`` may be rows of the caches themselves (a page that is copied) as long as no slot that is written is
+    among them.
     """
     module, watch = _direct_watch()
     if module and module.paged_write(key, value, key_cache, value_cache, slots, watch.flag_at):
@@ -400,6 +402,8 @@ def paged_cache_write(
           key_cache.data_ptr(), kcs[0], kcs[1], kcs[2], value_cache.data_ptr(), vcs[0], vcs[1], vcs[2],
           key_cache.shape[0], key_cache.shape[1], slots.data_ptr(), int(slots.dtype == torch.int64),
           slots.stride(0), watch.flag.data_ptr(), stream)
+    # autograd has to know of the change, as of any other in place
+    torch.autograd.graph.increment_version([c for c in (key_cache, value_cache) if not c.is_inference()])
     watch.after_call(stream)
 
 
@@ -493,7 +497,7 @@ def paged_attention_batch_invariant(
     out = torch.empty((batch, heads, dv), dtype=query.dtype, device=device)
     if batch and heads:
         width = block_table.shape[1]
-        bound = -1 if max_length is None else int(max_length)
+        bound = -1 if max_length is None else min(int(max_length), 0x7FFFFFFF)
         sinks = min(int(sinks), 0x7FFFFFFF)
         need = _fn("biops_paged_attention_workspace_size")(batch, heads, dv, width, page_size, bound, window_size, sinks)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None

@@ -180,6 +180,7 @@ extern "C" int biops_rotary(int dtype, int64_t batch, int64_t tokens, int64_t hq
   if (elt == 0) return fail(BIOPS_ERR_DTYPE, "biops_rotary: unsupported dtype %d", dtype);
   if (batch < 0 || tokens < 0 || hq < 0 || hk < 0 || hq + hk > 65536 || d < 0 || d > (1 << 20))
     return fail(BIOPS_ERR_ARG, "biops_rotary: bad sizes");
+  if ((hq + hk) * d > (INT64_C(1) << 26)) return fail(BIOPS_ERR_ARG, "biops_rotary: tokens of more than 2^26 elements");
   if (pairs < 0 || pairs > kRotaryPairs || 2 * pairs > d)
     return fail(BIOPS_ERR_ARG, "biops_rotary: %lld pairs (at most %d, and half the head size)", (long long)pairs, kRotaryPairs);
   if (pos_type < 0 || pos_type > 2) return fail(BIOPS_ERR_DTYPE, "biops_rotary: bad position type %d", pos_type);

@@ -235,6 +235,8 @@ PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                vc.stride(0), vc.stride(1), vc.stride(2), kc.size(0), kc.size(1), ptr(slots),
                                is_long(slots), slots.stride(0), reinterpret_cast<int*>(flag), stream_on(device)))
   if (rc != BIOPS_OK) Py_RETURN_NONE;
+  for (const at::Tensor* c : {&kc, &vc})  // autograd has to know of the change, as of any other in place
+    if (!c->is_inference()) c->unsafeGetTensorImpl()->bump_version();
   Py_RETURN_TRUE;
 }
 

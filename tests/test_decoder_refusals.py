@@ -193,6 +193,7 @@ def test_host_checks_of_the_entry_points():
 
     assert rot(dtype=3) == 3 and rot(pos_type=3) == 3
     assert rot(pairs=33) == 1 and rot(d=512, pairs=129) == 1 and rot(tokens=-1) == 1 and rot(turns=N) == 1 and rot(q=N) == 1
+    assert rot(hq=60000, d=2048) == 1  # more than 2^26 elements a token
     assert rot(tokens=0) == 0 and rot(batch=0) == 0 and rot(hq=0) == 0
 
     def put(dtype=2, rows=1, heads=1, d=64, pages=4, page=16, k=p, flag=p, kc=p):
@@ -251,6 +252,21 @@ def test_fast_call_bindings_match():
     if not torch.cuda.is_available():
         with pytest.raises(RuntimeError, match="ROCm GPU"):
             nat.fast_function("biops_rotary")
+
+
+def test_frequencies_may_be_a_tensor():
+    """Numbers are taken from it at the call: a change of the tensor is a change of the plan."""
+    f = torch.tensor([0.5, 0.25], dtype=torch.float64)
+    seen = []
+    from batch_invariant_ops import decoder
+
+    plan = decoder._rotary_plan
+    for value in (0.5, 0.125):
+        f[0] = value
+        with pytest.raises((RuntimeError, ValueError)):  # on the CPU
+            bio.multi_axis_rotary(zeros(1, 2, 4), None, torch.zeros(1, 1, dtype=torch.int64), (2,), inv_freq=f)
+        seen.append(plan((2,), 10000.0, tuple(map(float, f)), False, False).turns.tolist())
+    assert seen[0][0] == 4 * seen[1][0] and seen[0][1] == seen[1][1]
 
 
 def test_frequencies_and_axes():

@@ -125,6 +125,34 @@ def test_slots_past_the_cache_are_left_out_and_reported():
     assert_bitwise(kc, before)
 
 
+@pytest.mark.parametrize("heads_in_front", [False, True])
+def test_autograd_knows_of_a_write(heads_in_front):
+    """By both host paths: a cache that a graph has saved cannot change unnoticed."""
+    kc = randn(2, 4, 2, 8, seed=31)
+    vc = randn(2, 4, 2, 8, seed=32)
+    k = randn(1, 3, 2, 8, seed=33) if heads_in_front else randn(3, 2, 8, seed=33)  # (four dimensions: in Python)
+    w = torch.ones_like(kc, requires_grad=True)
+    loss = (kc * w).sum()
+    before = kc._version, vc._version
+    paged_cache_write(k, k, kc, vc, torch.arange(3).cuda().view(k.shape[:-2]))
+    assert (kc._version, vc._version) == (before[0] + 1, before[1] + 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        kc = torch.zeros(2, 4, 2, 8, dtype=BF16, device="cuda")
+        paged_cache_write(k, k, kc, kc.clone(), torch.arange(3).cuda().view(k.shape[:-2]))
+        assert_bitwise(kc[0, :3], k.view(3, 2, 8))
+
+
+def test_a_page_is_copied():
+    kc, vc = randn(4, 4, 2, 8, seed=34), randn(4, 4, 2, 16, seed=35)
+    want = kc[1].clone(), vc[1].clone()
+    paged_cache_write(kc[1], vc[1], kc, vc, torch.arange(8, 12).cuda())
+    assert_bitwise(kc[2], want[0])
+    assert_bitwise(vc[2], want[1])
+    assert_bitwise(kc[1], want[0])
+
+
 def test_a_gradient_is_refused():
     kc = randn(2, 4, 2, 8, seed=19)
     k = randn(3, 2, 8, seed=20).requires_grad_()
