@@ -273,7 +273,8 @@ def multi_axis_rotary(
 
     Angles are computed in 64 bits, the rotation in 32, with one rounding to the tensors' type.  Returns new
     tensors ``(query, key)``, or the rotated query alone when ``key`` is None.  Differentiable with respect
-    to ``query`` and ``key`` (not to ``positions``).
+    to ``query`` and ``key`` (not to ``positions``).  A capture into a graph is refused while a leaf among them has a
+    living autograd graph from another stream, whose backward pass the capture would run into.
     """
     plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(map(float, inv_freq)),
                         bool(interleaved_axes), bool(interleaved_pairs))

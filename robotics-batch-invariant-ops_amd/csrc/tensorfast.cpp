@@ -155,6 +155,21 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   }
 };
 
+// Whether a gradient that is captured into a graph here would run into one outside of it: an older graph of the leaf that
+// is still held keeps the leaf's accumulation node on another stream, and the engine would make that stream wait
+// for the capturing one in the middle of a backward pass, where no error leads back to the caller.
+bool held_elsewhere(const at::Tensor& t, c10::DeviceIndex device) {
+  if (!t.requires_grad() || !t.is_leaf()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return false;
+  const auto stream = node->stream();
+  return stream && *stream != c10::hip::getCurrentHIPStream(device).unwrap();
+}
+bool capturing(c10::DeviceIndex device) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing((hipStream_t)stream_on(device), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+}
+
 // rotary(query, key or None, positions, axes, pairs, turns, axis, neighbours) -> query or (query, key)
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 8) Py_RETURN_NONE;
@@ -166,6 +181,11 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   TAKE(p, args[2]);
   const at::Tensor& q = *q_;
   const at::Tensor k = both ? *k_ : at::Tensor();
+  if (c10::GradMode::is_enabled() && capturing(device) && (held_elsewhere(q, device) || (both && held_elsewhere(k, device)))) {
+    PyErr_SetString(PyExc_RuntimeError, "multi_axis_rotary: a graph of this leaf from outside of the capture is still alive; "
+                                        "delete its outputs (or capture on the stream that they were made on)");
+    return nullptr;
+  }
   int64_t axes, pairs, turns, axis, neighbours;
   if (!number(args[3], &axes) || !number(args[4], &pairs) || !number(args[5], &turns) || !number(args[6], &axis) ||
       !number(args[7], &neighbours))

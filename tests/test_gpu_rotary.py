@@ -192,7 +192,7 @@ def test_graph_replays_forward_and_gradient():
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        held = step()
+        held = [t.detach() for t in step()]
     for i in range(3):
         with torch.no_grad():
             q.copy_(randn(5, 4, 64, seed=30 + i, dtype=torch.bfloat16))
@@ -201,6 +201,33 @@ def test_graph_replays_forward_and_gradient():
         torch.cuda.synchronize()
         for got, want in zip(held, step()):
             assert_bitwise(got.detach(), want.detach(), f"replay {i}")
+
+
+def test_capture_beside_a_living_graph_of_the_leaf_is_refused():
+    q, k = (randn(5, h, 64, seed=26 + h, dtype=torch.bfloat16).requires_grad_() for h in (4, 2))
+    p = places(2, 5, seed=29)
+    for leaf in (q, k):
+        alive = leaf * 2.0
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                multi_axis_rotary(q, k, p, (16, 16))
+        del alive
+    five = q.detach().view(1, 1, 5, 4, 64).requires_grad_()  # (the Python path)
+    alive = five * 2.0
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            multi_axis_rotary(five, None, p.view(2, 1, 1, 5), (16, 16))
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [t.detach() for t in torch.autograd.grad(multi_axis_rotary(q, k, p, (16, 16)), (q, k), (q.detach(), k.detach()))]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.autograd.grad(multi_axis_rotary(q, k, p, (16, 16)), (q, k), (q.detach(), k.detach()))
+        for a, b in zip(got, want):
+            assert_bitwise(a, b)
 
 
 def test_without_pairs_and_with_special_values():
