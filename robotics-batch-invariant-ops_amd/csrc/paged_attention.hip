@@ -99,13 +99,16 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedArgs& a, int len) {
   return s;
 }
 
-// Work item `it` of a batch of up to 64 sequences: chunk c of sequence b, all chunks of the first sequence, then of the
-// next.  Counting them here leaves no idle workgroups between those with work (64 sequences of 250 to 16384 keys: 142 us
-// with a workgroup for every chunk that the longest sequence could have, 113 so).
+// Work item `it` of a batch of up to 128 sequences: chunk c of sequence b, all chunks of the first sequence, then of the
+// next.  Counting them here, two sequences a lane, leaves no idle workgroups between those with work (64 sequences of 250
+// to 16384 keys: 142 us with a workgroup for every chunk that the longest sequence could have, 113 so).
+constexpr uint32_t kPagedListed = 128;
 __device__ __forceinline__ bool paged_find(const PagedArgs& a, int it, int lane, uint32_t& b, int& c, int& length) {
-  const int len = lane < (int)a.batch ? paged_length(a, lane) : 0;
-  const int mine = paged_span(a, len).chunks;
-  int upto = mine;
+  const uint32_t first = 2 * lane;
+  const int len0 = first < a.batch ? paged_length(a, first) : 0;
+  const int len1 = first + 1 < a.batch ? paged_length(a, first + 1) : 0;
+  const int one = paged_span(a, len0).chunks, both = one + paged_span(a, len1).chunks;
+  int upto = both;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int x = __shfl_up(upto, o, 64);
@@ -114,9 +117,12 @@ __device__ __forceinline__ bool paged_find(const PagedArgs& a, int it, int lane,
   const uint64_t hit = __ballot(upto > it);
   if (hit == 0) return false;
   const int f = __builtin_ctzll(hit);
-  b = f;
-  c = it - (__builtin_amdgcn_readlane(upto, f) - __builtin_amdgcn_readlane(mine, f));
-  length = __builtin_amdgcn_readlane(len, f);
+  c = it - (__builtin_amdgcn_readlane(upto, f) - __builtin_amdgcn_readlane(both, f));
+  const int in_first = __builtin_amdgcn_readlane(one, f);
+  const bool second = c >= in_first;
+  b = 2 * f + second;
+  if (second) c -= in_first;
+  length = second ? __builtin_amdgcn_readlane(len1, f) : __builtin_amdgcn_readlane(len0, f);
   return true;
 }
 
@@ -169,7 +175,7 @@ void paged_chunk_kernel(PagedArgs a) {
   int c = 0, length;
   if (a.chunks == 1) {
     length = paged_length(a, b);
-  } else if (a.batch <= 64) {
+  } else if (a.batch <= kPagedListed) {
     if (!paged_find(a, (int)b, lane, b, c, length)) return;
   } else {  // first chunks of all sequences, then second ones: what is idle comes last
     c = (int)(b / a.batch);

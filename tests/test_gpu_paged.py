@@ -214,15 +214,17 @@ def test_long_sequences(index):
     check([1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8192, 20000, 32767, 32768, 32769, 70001, 3], 4, 1, 64, 64, 16, 300, index=index)
 
 
-@pytest.mark.parametrize("count", [63, 64, 65, 130])
+@pytest.mark.parametrize("count", [2, 3, 64, 65, 127, 128, 129, 150])
 def test_batches_of_many_sequences(count):
     """Both sides of the batches whose chunks are listed."""
     lengths = [(37 * i) % 300 for i in range(count)]
     lengths[count - 2] = 1500
     lengths[count // 2] = 0
     q, kc, vc, table, lens, out = check(lengths, 2, 1, 64, 64, 16, 360)
-    for b in (0, 1, count - 2, count - 1):
+    for b in {0, 1, count - 2, count - 1}:
         assert_bitwise(paged_attention_batch_invariant(q[b:b + 1], kc, vc, table[b:b + 1], lens[b:b + 1])[0], out[b])
+    if count < 10:
+        return
     bad = lens.clone()
     bad[count - 3] = -1
     again = paged_attention_batch_invariant(q, kc, vc, table, bad)
