@@ -8,8 +8,8 @@
 // (window_launch_rows has the variants and what they measured), and pass once over the keys that any of
 // them sees, counted through from 0: the sinks in front of the first row's window, then everything up to the last
 // row.  So the sinks share the first block with the window's first keys, and work grows with the window, not with the
-// sequence.  Blocks of 64 keys (float32: 32 for each turn) go straight from memory to LDS, double buffered with keys a
-// block ahead of values (one buffer each where four turns fill the LDS); running maximum m and sum l per row, O rescaled when a maximum grows.
+// sequence.  Blocks of 64 keys go straight from memory to LDS; running maximum m and sum l per row, O rescaled when a
+// maximum grows.
 //
 // Register layout: S^T = K Q^T (K as the A operand of 32x32 MFMAs) leaves lane L with query row L % 32 and
 // keys 8j + 4(L/32) + i of a 32-key block, which is the B operand of O^T = V^T P^T with the same key order
@@ -29,8 +29,7 @@
 // What bounds it: the vector units and the matrix cores in turn.  A score costs about seven vector slots
 // (maximum, fused multiply-add, exponential at a quarter of the rate, conversion, sum) and 4 D / 1024 matrix cycles of
 // a 16-bit type; two or three wavefronts of a SIMD overlap the two in part.  bf16, 16/4 heads of 128, 2 x 8192 tokens
-// under a window of 2048: 332 us, 770 TF/s of visible pairs (without any exponential 270, without any product 191,
-// fetches alone 100); fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 32 us.  float32 products
+// under a window of 2048: 295 us, 815 TF/s of visible pairs; fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 31 us.  float32 products
 // run at 1/16 of the 16-bit rate and bound it alone: 3 x 257 rows of 1281 keys, 16 heads of 72, window 500: 37 us.
 #include <type_traits>
 
@@ -39,7 +38,7 @@
 
 namespace biops {
 
-constexpr int kWindowFew = 64, kWindowMany = 2048, kWindowShort = 512;  // see window_launch_rows
+constexpr int kWindowFew = 64;      // rows up to which two wavefronts share them (window_launch_rows)
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
 struct WindowArgs {
@@ -139,8 +138,8 @@ __device__ __forceinline__ bool window_offsets_ok(const WindowArgs& a, int64_t i
 }
 
 // DP, DVP: head and value size rounded up to whole fragments; RW row groups of 32 (of HG heads) by KW wavefronts that
-// share a row group and take turns at the keys; STAGES blocks in LDS.
-template <typename T, int DP, int DVP, int RW, int KW_, int NH_, int HG, int STAGES>
+// share a row group and take turns at the keys.
+template <typename T, int DP, int DVP, int RW, int KW_, int NH_, int HG>
 struct WindowShape {
   static constexpr int E = sizeof(T), VEC = 16 / E;
   static constexpr int KW = KW_, NH = NH_;             // NH: 32-key parts of a block that a wavefront takes
@@ -157,7 +156,7 @@ struct WindowShape {
   static constexpr int QSTEP = 4 / NH;                 // score steps whose fragments are read at a time
   static constexpr int OF = (DVP + 31) / 32;
   static constexpr int JOIN_BYTES = KW > 1 ? (KW - 1) * RW * 64 * (16 * OF + 2) * 4 : 0;
-  static constexpr int BLOCK_BYTES = STAGES * (K_BYTES + V_BYTES);
+  static constexpr int BLOCK_BYTES = K_BYTES + V_BYTES;
   static constexpr int LDS_BYTES = BLOCK_BYTES > JOIN_BYTES ? BLOCK_BYTES : JOIN_BYTES;
   static_assert(BN % KR == 0 && BN % VR == 0, "whole loads");
   static_assert(32 * OF <= VS * VEC, "V fragments stay inside a row");
@@ -222,11 +221,11 @@ constexpr int window_waves() {
   return DP > 128 || DVP > 128 ? 1 : (sizeof(T) == 2 && DP <= 64 && DVP <= 64 ? (NH == 1 ? 4 : 3) : 2);
 }
 
-template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG, int STAGES>
+template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
 __global__ __launch_bounds__(64 * RW * KW)
 __attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP, NH>(), window_waves<T, DP, DVP, NH>())))
 void window_attn_kernel(WindowArgs a) {
-  using F = WindowShape<T, DP, DVP, RW, KW, NH, HG, STAGES>;
+  using F = WindowShape<T, DP, DVP, RW, KW, NH, HG>;
   constexpr int E = F::E, BN = F::BN;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS_BYTES];
   // What is the same for a wavefront is told to the compiler, and then computed once for it.
@@ -325,8 +324,8 @@ void window_attn_kernel(WindowArgs a) {
   }
   const bool vin = F::VEC * vc < a.dv;
   const uint32_t voff = (uint32_t)(vrow0 * (int)a.vT + 16 * vc);
-  auto kbuf = [&](int blk) { return smem + (blk & (STAGES - 1)) * F::K_BYTES; };
-  auto vbuf = [&](int blk) { return smem + STAGES * F::K_BYTES + (blk & (STAGES - 1)) * F::V_BYTES; };
+  char* const kbuf = smem;
+  char* const vbuf = smem + F::K_BYTES;
   // Row v of the counted keys; behind the last one, that one (no row sees it there).
   auto key_of = [&](int v) -> int64_t {
     v = v < nv ? v : nv - 1;
@@ -337,7 +336,7 @@ void window_attn_kernel(WindowArgs a) {
   };
   auto load_k = [&](int blk) {
     const int v0 = blk * BN;
-    char* to = kbuf(blk) + w * 1024;
+    char* to = kbuf + w * 1024;
     const bool whole = v0 >= ns && v0 + BN <= nv;
     const char* kp = kb + (int64_t)(v0 + shift) * a.kT;
 #pragma unroll
@@ -355,7 +354,7 @@ void window_attn_kernel(WindowArgs a) {
   auto load_v = [&](int blk) {
     if (!vin) return;
     const int v0 = blk * BN;
-    char* to = vbuf(blk) + w * 1024;
+    char* to = vbuf + w * 1024;
     if (v0 >= ns && v0 + BN <= nv) {
       const char* vp = vb + (int64_t)(v0 + shift) * a.vT;
 #pragma unroll
@@ -374,14 +373,11 @@ void window_attn_kernel(WindowArgs a) {
   };
   if (a.d < F::KS * F::VEC || a.dv < F::VS * F::VEC) {
 #pragma unroll
-    for (int x = 0; x < STAGES; ++x) {
+    for (int i = 0; i < F::KL; ++i)
+      if (!kin[i % KV]) *reinterpret_cast<u32x4_t*>(kbuf + 16 * tid + 16 * F::THREADS * i) = zero4;
+    if (!vin) {
 #pragma unroll
-      for (int i = 0; i < F::KL; ++i)
-        if (!kin[i % KV]) *reinterpret_cast<u32x4_t*>(kbuf(x) + 16 * tid + 16 * F::THREADS * i) = zero4;
-      if (!vin) {
-#pragma unroll
-        for (int i = 0; i < F::VL; ++i) *reinterpret_cast<u32x4_t*>(vbuf(x) + 16 * tid + 16 * F::THREADS * i) = zero4;
-      }
+      for (int i = 0; i < F::VL; ++i) *reinterpret_cast<u32x4_t*>(vbuf + 16 * tid + 16 * F::THREADS * i) = zero4;
     }
   }
 
@@ -395,8 +391,8 @@ void window_attn_kernel(WindowArgs a) {
 
   const int hb0 = NH * part;  // this wavefront's 32-key parts of a block: hb0 .. hb0 + NH - 1
   f32x16_t sc[NH];
-  auto scores = [&](int blk) {
-    const char* ks = kbuf(blk);
+  auto scores = [&]() {
+    const char* ks = kbuf;
 #pragma unroll
     for (int x = 0; x < NH; ++x)
 #pragma unroll
@@ -481,8 +477,8 @@ void window_attn_kernel(WindowArgs a) {
     }
   };
   // What the weights add to the output.
-  auto gather = [&](int blk) {
-    const char* vs = vbuf(blk);
+  auto gather = [&]() {
+    const char* vs = vbuf;
     if constexpr (E == 4) {
       // the values of a group of four steps are read before the MFMAs of the group before it
       float xv[2][4][F::OF];
@@ -539,32 +535,23 @@ void window_attn_kernel(WindowArgs a) {
   };
 
   // A turn: weights of a block (vector work), then its product and the next block's scores (matrix work, at a
-  // higher priority: of two wavefronts of a SIMD one multiplies while the other takes exponentials).  With two stages K
-  // is a block ahead of V in LDS, and what the next turn needs is fetched during this one; with one, a block's values
-  // and the next one's keys are fetched while the wavefronts weigh.
-  if (nblk > 0) {
-    load_k(0);
-    if constexpr (STAGES == 2) load_v(0);
-  }
-  if (STAGES == 2 && nblk > 1) load_k(1);
+  // higher priority: of two wavefronts of a SIMD one multiplies while the other takes exponentials).  The block's values
+  // and the next one's keys are fetched while the wavefronts weigh, when nothing reads the LDS.  Two buffers, filled a turn
+  // ahead, were 2 to 12 % slower: every read's address then depends on the block, and so costs an instruction.
+  if (nblk > 0) load_k(0);
   meet();
   bool here = sees(0);
-  if (here) scores(0);
+  if (here) scores();
   for (int blk = 0; blk < nblk; ++blk) {
     meet();
-    if constexpr (STAGES == 2) {
-      if (blk + 2 < nblk) load_k(blk + 2);
-      if (blk + 1 < nblk) load_v(blk + 1);
-    } else {
-      load_v(blk);
-      if (blk + 1 < nblk) load_k(blk + 1);
-    }
+    load_v(blk);
+    if (blk + 1 < nblk) load_k(blk + 1);
     if (here) weigh(blk);
     const bool then = sees(blk + 1);
-    if constexpr (STAGES == 1) meet();
+    meet();
     __builtin_amdgcn_s_setprio(1);
-    if (here) gather(blk);
-    if (then) scores(blk + 1);
+    if (here) gather();
+    if (then) scores();
     __builtin_amdgcn_s_setprio(0);
     here = then;
   }
@@ -656,7 +643,7 @@ void window_attn_kernel(WindowArgs a) {
   }
 }
 
-template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG, int STAGES = 2>
+template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
 static int window_launch(WindowArgs a, hipStream_t s) {
   constexpr int rows = 32 * RW / HG;
   // packed: every sequence and the two ends may end in a part of a tile
@@ -668,7 +655,7 @@ static int window_launch(WindowArgs a, hipStream_t s) {
   constexpr uint32_t most = 1 << 22;  // a launch has less than 2^32 threads
   for (a.first = 0; a.first < a.total; a.first += most) {
     const uint32_t n = a.total - a.first < most ? a.total - a.first : most;
-    hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW, KW, NH, HG, STAGES>), dim3(n), dim3(64 * RW * KW), 0, s, a);
+    hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW, KW, NH, HG>), dim3(n), dim3(64 * RW * KW), 0, s, a);
     const int rc = check_launch("window_attn_kernel");
     if (rc != BIOPS_OK) return rc;
   }
@@ -679,45 +666,35 @@ static int window_launch(WindowArgs a, hipStream_t s) {
 //
 // Heads of a group in one workgroup share its fetches, and their tile of fewer rows has fewer keys that only some of its
 // rows see.  Two wavefronts for the same rows, with the keys in turns, halve a tile's time where there are too few
-// tiles to fill the chip, and cost their join.  us, variants as <wavefronts for rows and heads, turns, 32-key parts,
-// heads>, 16/4 heads unless said otherwise:
-//   16-bit                        <4,1,2,4> <4,1,2,2> <4,1,2,1> <2,2,1,2> <2,2,1,1>
-//   64-wide, 4 x 2048, window 512    38.7      46.6      50.8      38.9      43.3
-//   128-wide, the same               55.0      60.7      67.0      74.8      82.1
-//   256-wide, the same              163       172       192       229       247
-//   128-wide, 8/8 heads                                  37.7                45.1
-//   64-wide, 8/8 heads, w. 512 / all                   25 / 50             25 / 58
-//   64-wide, 8/4 heads, w. 512 / all         23 / 49   25 / 50   22 / 47   24 / 57
-//   64-wide, 50 rows of 700 keys     18.7      19.0      18.7      14.2      14.3  (one sequence)
-//   128-wide, the same, 1 / 64 seq. 24 / 33   24 / 35   23 / 53   18 / 43   18 / 44
-//   float32                       <4,1,1,4> <4,1,1,2> <4,1,1,1> <2,4,1,2>* <2,4,1,1>* <2,2,1,2> <2,2,1,1>
-//   64-wide, 1 x 700 / 4 x 2048    52 / 167  55 / 180  56 / 196  28 / 196   30 / 213   30 / 172  32 / 193
-//   72-wide, the same              66 / 218  71 / 244  72 / 256  36 / 258   39 / 281   42 / 295  45 / 325
-//   (* one stage: four turns' blocks fill the LDS.  Two of their wavefronts share a SIMD, where <2,2,1,h> has one.)
+// tiles to fill the chip, and cost their join; with float32 they win throughout.  us, variants as <wavefronts for rows and
+// heads, turns, 32-key parts, heads>, 16/4 heads and a window of 512 unless said otherwise:
+//   16-bit                           <4,1,2,4> <4,1,2,2> <4,1,2,1> <2,2,1,2> <2,2,1,1>
+//   64-wide, 4 x 2048                  37.1      42.3      46.7      38.4      41.2
+//   128-wide / 256-wide, the same     52 / 154  56 / 166  61 / 184  71 / 217  77 / 234
+//   64-wide, 8/4 heads, all keys                 46.4      46.9      43.9      54.2
+//   128-wide, 8/4 heads, w. 512 / all           30 / 66   33 / 66   39 / 61   42 / 79
+//   64-wide, 8/8 heads, w. 64 / all                       13 / 47             13 / 54
+//   128-wide, 8/8 heads, w. 512 / all                     34 / 66             42 / 79
+//   64-wide, 50 rows of 700 keys, 1 / 64 sequences
+//                                     16 / 23   16 / 23   15 / 33   12 / 25   12 / 24
+//   128-wide, the same                20 / 33   20 / 32   19 / 45   16 / 41   16 / 41
+//   float32                          <4,1,1,4> <4,1,1,2> <4,1,1,1> <2,2,1,2> <2,2,1,1> <2,4,1,2> <2,4,1,1>
+//   64-wide, 1 x 700 / 4 x 2048       49 / 161  52 / 174  55 / 191  28 / 165  30 / 187  27 / 196  30 / 212
+//   72-wide, the same                 63 / 210  67 / 227  69 / 251  37 / 224  40 / 256  38 / 269  40 / 288
 template <typename T, int DP>
 static int window_launch_rows(const WindowArgs& a, hipStream_t s) {
   const bool pairs = a.group % 2 == 0, fours = a.group % 4 == 0;
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (DP > 64) {
-      if (!a.cu_q && a.lq >= kWindowMany) {
-        if (fours) return window_launch<T, DP, DP, 4, 1, 1, 4>(a, s);
-        return pairs ? window_launch<T, DP, DP, 4, 1, 1, 2>(a, s) : window_launch<T, DP, DP, 4, 1, 1, 1>(a, s);
-      }
-    }
-    if constexpr (DP > 64)
-      return pairs ? window_launch<T, DP, DP, 2, 4, 1, 2, 1>(a, s) : window_launch<T, DP, DP, 2, 4, 1, 1, 1>(a, s);
-    else
-      return pairs ? window_launch<T, DP, DP, 2, 2, 1, 2>(a, s) : window_launch<T, DP, DP, 2, 2, 1, 1>(a, s);
-  } else {
-    const bool few = !a.cu_q && a.lq <= kWindowFew;
-    if (pairs && (few || (DP <= 64 && !fours))) return window_launch<T, DP, DP, 2, 2, 1, 2>(a, s);
-    if (few || (DP <= 64 && !pairs && (int64_t)a.window + a.sinks <= kWindowShort))
-      return window_launch<T, DP, DP, 2, 2, 1, 1>(a, s);
+  const bool few = !a.cu_q && a.lq <= kWindowFew;
+  if (pairs && (sizeof(T) == 4 || few || (DP <= 64 && !fours))) return window_launch<T, DP, DP, 2, 2, 1, 2>(a, s);
+  if (sizeof(T) == 4 || few) return window_launch<T, DP, DP, 2, 2, 1, 1>(a, s);
+  if constexpr (sizeof(T) == 2) {
     if (fours) return window_launch<T, DP, DP, 4, 1, 2, 4>(a, s);
     if constexpr (DP > 64) {
       if (pairs) return window_launch<T, DP, DP, 4, 1, 2, 2>(a, s);
     }
     return window_launch<T, DP, DP, 4, 1, 2, 1>(a, s);
+  } else {
+    return BIOPS_OK;  // not reached
   }
 }
 template <typename T>
