@@ -9,7 +9,7 @@
 // them sees, counted through from 0: the sinks in front of the first row's window, then everything up to the last
 // row.  So the sinks share the first block with the window's first keys, and work grows with the window, not with the
 // sequence.  Blocks of 64 keys go straight from memory to LDS; running maximum m and sum l per row, O rescaled when a
-// maximum grows.
+// maximum has grown enough.
 //
 // Register layout: S^T = K Q^T (K as the A operand of 32x32 MFMAs) leaves lane L with query row L % 32 and
 // keys 8j + 4(L/32) + i of a 32-key block, which is the B operand of O^T = V^T P^T with the same key order
@@ -29,7 +29,7 @@
 // What bounds it: the vector units and the matrix cores in turn.  A score costs about seven vector slots
 // (maximum, fused multiply-add, exponential at a quarter of the rate, conversion, sum) and 4 D / 1024 matrix cycles of
 // a 16-bit type; two or three wavefronts of a SIMD overlap the two in part.  bf16, 16/4 heads of 128, 2 x 8192 tokens
-// under a window of 2048: 295 us, 815 TF/s of visible pairs; fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 31 us.  float32 products
+// under a window of 2048: 288 us, 837 TF/s of visible pairs; fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 31 us.  float32 products
 // run at 1/16 of the 16-bit rate and bound it alone: 3 x 257 rows of 1281 keys, 16 heads of 72, window 500: 37 us.
 #include <type_traits>
 
@@ -39,6 +39,7 @@
 namespace biops {
 
 constexpr int kWindowFew = 64;      // rows up to which two wavefronts share them (window_launch_rows)
+constexpr float kWindowSlack = 8.f;  // by how many powers of two weights may pass one (weigh)
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
 struct WindowArgs {
@@ -381,8 +382,9 @@ void window_attn_kernel(WindowArgs a) {
     }
   }
 
-  // m: largest score so far (raw), sh = m * scale, l: this lane's part of the row's sum
+  // m: the score (raw) that weights are relative to, sh = m * scale, l: this lane's part of the row's sum
   float m = -INFINITY, sh = 0.f, l = 0.f;
+  const float slack = kWindowSlack / a.scale;
   f32x16_t oacc[F::OF];  // O^T: register r of block e is column 32e + 8(r/4) + 4hf + r%4 of row l32
 #pragma unroll
   for (int e = 0; e < F::OF; ++e)
@@ -446,11 +448,15 @@ void window_attn_kernel(WindowArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[x][r]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__any(mx > m)) {
-      const float mn = fmaxf(m, mx);
+    // A row's maximum is followed when it has grown by more than 2^kWindowSlack in its weights: until then they are that
+    // much larger than one at most, and nothing is rescaled
+    // (2 to 5 % of the time; 16 % with 256-wide heads and few rows).  Each row by itself, so that no row's bits depend on another.
+    const bool grown = mx > m + slack;
+    if (__any(grown)) {
+      const float mn = grown ? mx : m;
       const float to = mn == -INFINITY ? 0.f : mn * a.scale;
       if (__any(m > -INFINITY)) {  // (nothing is summed before a row's first keys)
-        const float corr = mx > m && m > -INFINITY ? __builtin_amdgcn_exp2f(sh - to) : 1.f;
+        const float corr = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(sh - to) : 1.f;
         l *= corr;
 #pragma unroll
         for (int e = 0; e < F::OF; ++e)

@@ -151,6 +151,22 @@ def test_many_sequences():
         check_window(out[0, a:b].transpose(0, 1), *(x[0, a:b].transpose(0, 1) for x in (q, k, v)), 9, 1, what=f"sequence {s}")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group, lq", [(1, 150), (2, 150), (4, 150), (4, 50)])
+def test_a_row_keeps_its_bits_whatever_follows(dtype, group, lq):
+    """Other queries, keys and values behind a row, far larger ones among them, in its tile and in its blocks."""
+    q, k, v = (randn(1, h, n, 64, seed=66 + h, dtype=dtype) for h, n in ((2 * group, lq), (2, 200), (2, 200)))
+    want = window_attention(q, k, v, 90, 3, enable_gqa=True)
+    for last in (3, 31, 32, lq // 2, lq - 2):
+        p = 200 - lq + last  # the row's position
+        other = [t.clone() for t in (q, k, v)]
+        other[0][:, :, last + 1:] = 7.0 * randn(1, 2 * group, lq - last - 1, 64, seed=70, dtype=dtype)
+        for t in other[1:]:
+            t[:, :, p + 1:] = 5.0 * randn(1, 2, 199 - p, 64, seed=71, dtype=dtype)
+        out = window_attention(*other, 90, 3, enable_gqa=True)
+        assert_bitwise(out[:, :, :last + 1], want[:, :, :last + 1], f"rows up to {last}")
+
+
 @pytest.mark.parametrize("count", [61, 62, 63, 64, 4093, 4094, 4095, 5000])
 def test_the_search_for_a_sequence(count):
     """Both sides of the counts at which the search takes another round, with empty sequences among the others."""
