@@ -10,17 +10,18 @@
 // which two instructions settle where a prompt's slots lie together.  The search is quadratic, so rows go in
 // launches of kWriteRows, whose order on the stream does the rest.
 //
-// us for rows of 8 + 8 heads of 128 fp16 (4 KB, read and written): 16383 rows 29.4 (4.6 TB/s; a plain copy
-// 27), with every slot somewhere else 38; 48 rows of half that 3.2, of which a launch is 2.6.
+// us for rows of 8 + 8 heads of 128 fp16 (4 KB, read from memory and written): 16383 rows 29.5 (4.55 TB/s; a plain
+// copy 27), with every slot somewhere else 34, and 36 / 45 with stores that stay in the caches; 48 rows of half
+// that 3.2, of which a launch is 2.6.
 #include "biops_common.h"
 
 namespace biops {
 
-constexpr int kWriteRows = 8192;  // rows of a launch; 16384: 32.3 us for the 29.4 above
+constexpr int kWriteRows = 8192;  // rows of a launch; 16384: 33.5 us for the 29.5 above
 
 // Rows of a workgroup: one as long as that does not fill the card, then eight, which share a search.
-// us (one / eight) at 2 KB a row: 48 rows 3.2 / 5.0, 1024 4.1 / 5.3, 2048 5.7 / 5.4; the 16383 rows above 55 / 29
-// (four: 38, sixteen: 35).
+// us (one / eight) at 2 KB a row: 48 rows 3.2 / 5.0, 1024 4.1 / 5.3, 2048 5.7 / 5.4; 16383 rows of 4 KB 55 / 29
+// (four: 38, sixteen: 35; all with cached rows and stores).
 constexpr int kWriteGroup = 8, kWriteFew = 1024;
 
 struct WriteArgs {
@@ -128,7 +129,9 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
       const uint32_t page = (uint32_t)s / a.page, at = (uint32_t)s - page * a.page;
       char* const to = dst + page * dP + at * dS;
       if (whole) {
-        *reinterpret_cast<u32x4_any_t*>(to) = piece[j];
+        // Many rows pass the caches by: they are read again a token later at the earliest.
+        if constexpr (G > 1) __builtin_nontemporal_store(piece[j], reinterpret_cast<u32x4_any_t*>(to));
+        else *reinterpret_cast<u32x4_any_t*>(to) = piece[j];
       } else {
         const char* from = src + (r0 + i) * sT;
         const int left = (value ? a.vbytes : a.kbytes) - e;
