@@ -497,7 +497,12 @@ int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64_t hkv, int
                            int64_t skH, const void* v, int64_t svB, int64_t svT, int64_t svH, void* out, int64_t soB,
                            int64_t soT, int64_t soH, const void* cu_q, int cu_q64, int64_t cu_q_stride, const void* cu_k,
                            int cu_k64, int64_t cu_k_stride, int64_t window, int64_t sinks, float scale, int* flag,
-                           void* stream);
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of a dense biops_window_attention (0: none needed, as for every packed one), -1 for bad sizes.  Up to 64
+ * rows before many keys are cut into ranges of keys, whose results are joined.  Workspace 16-byte aligned. */
+int64_t biops_window_attention_workspace_size(int64_t nseq, int64_t hq, int64_t lq, int64_t lk, int64_t dv, int64_t window,
+                                              int64_t sinks);
 
 #ifdef __cplusplus
 }

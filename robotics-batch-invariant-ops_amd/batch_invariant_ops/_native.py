@@ -119,8 +119,9 @@ _SIGNATURES = {
     "biops_window_attention_max_head": (_i, [_i]),
     "biops_window_attention": (
         _i,
-        [_i, _l, _l, _l, _l, _l, _l, _l] + [_p, _l, _l, _l] * 4 + [_p, _i, _l] * 2 + [_l, _l, _f, _p, _p],
+        [_i, _l, _l, _l, _l, _l, _l, _l] + [_p, _l, _l, _l] * 4 + [_p, _i, _l] * 2 + [_l, _l, _f, _p, _p, _l, _p],
     ),
+    "biops_window_attention_workspace_size": (_l, [_l] * 7),
     "biops_moe_workspace_size": (_l, [_i, _l, _l, _l, _l]),
     "biops_moe": (
         _i,

@@ -535,14 +535,19 @@ def _windowed(q, k, v, out, nseq, lengths, window_size, sinks, scale, offsets, w
     d = q.shape[-1]
     if offsets is None:
         cu = (None, 0, 0, None, 0, 0)
+        need = _fn("biops_window_attention_workspace_size")(nseq, q.shape[2], *lengths, v.shape[-1], window_size or 0x7FFFFFFF,
+                                                            min(int(sinks), 0x7FFFFFFF))
     else:
+        need = 0
         cu = tuple(x for t in offsets for x in (t.data_ptr(), int(t.dtype == torch.int64), t.stride(0)))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     _call("biops_window_attention", nat.dtype_code(q.dtype), nseq, q.shape[2], k.shape[2], *lengths, d,
           v.shape[-1], q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
           v.data_ptr(), vs[0], vs[1], vs[2], out.data_ptr(), os_[0], os_[1], os_[2], *cu,
           window_size or 0x7FFFFFFF, min(int(sinks), 0x7FFFFFFF),
           float(1.0 / math.sqrt(d) if scale is None else scale),
-          None if watch is None else watch.flag.data_ptr(), nat.stream_of(out))
+          None if watch is None else watch.flag.data_ptr(), None if ws is None else ws.data_ptr(), need,
+          nat.stream_of(out))
 
 
 def sliding_window_attention_batch_invariant(

@@ -282,18 +282,18 @@ static PyObject* fast_paged_attention(PyObject* self, PyObject* const* args, Py_
 }
 
 /* window_attention(dtype, nseq, hq, hkv, lq, lk, d, dv, {q, k, v, out: pointer, sB, sT, sH}, cu_q, cu_q64, stride, cu_k,
- *                  cu_k64, stride, window, sinks, scale, flag, stream) */
+ *                  cu_k64, stride, window, sinks, scale, flag, workspace, bytes, stream) */
 static PyObject* fast_window_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
-  int64_t iv[35];
-  void* pv[35];
-  float fv[35];
+  int64_t iv[37];
+  void* pv[37];
+  float fv[37];
   (void)self;
-  if (!parse(args, nargs, "llllllllplllplllplllplllpllpllllfpp", iv, pv, fv)) return NULL;
+  if (!parse(args, nargs, "llllllllplllplllplllplllpllpllllfpplp", iv, pv, fv)) return NULL;
   int rc;
   WITHOUT_GIL(rc, biops_window_attention((int)iv[0], iv[1], iv[2], iv[3], iv[4], iv[5], iv[6], iv[7], pv[8], iv[9],
                                          iv[10], iv[11], pv[12], iv[13], iv[14], iv[15], pv[16], iv[17], iv[18], iv[19],
                                          pv[20], iv[21], iv[22], iv[23], pv[24], (int)iv[25], iv[26], pv[27],
-                                         (int)iv[28], iv[29], iv[30], iv[31], fv[32], (int*)pv[33], pv[34]));
+                                         (int)iv[28], iv[29], iv[30], iv[31], fv[32], (int*)pv[33], pv[34], iv[35], pv[36]));
   return PyLong_FromLong(rc);
 }
 

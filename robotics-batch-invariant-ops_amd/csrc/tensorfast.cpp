@@ -319,10 +319,15 @@ PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   // tokens before heads in memory where the queries have them so
   at::Tensor out = q.stride(1) < q.stride(2) ? at::empty({batch, lq, hq, dv}, q.options()).transpose(1, 2)
                                              : at::empty({batch, hq, lq, dv}, q.options());
+  const int64_t need = biops_window_attention_workspace_size(batch, hq, lq, lk, dv, window, sinks);
+  if (need < 0) Py_RETURN_NONE;
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, q.options().dtype(at::kByte));
   LAUNCH(rc, biops_window_attention(code, batch, hq, hkv, lq, lk, d, dv, ptr(q), q.stride(0), q.stride(2), q.stride(1),
                                     ptr(k), k.stride(0), k.stride(2), k.stride(1), ptr(v), v.stride(0), v.stride(2),
                                     v.stride(1), ptr(out), out.stride(0), out.stride(2), out.stride(1), nullptr, 0, 0,
-                                    nullptr, 0, 0, window, sinks, scale, nullptr, stream_on(device)))
+                                    nullptr, 0, 0, window, sinks, scale, nullptr, need > 0 ? ptr(ws) : nullptr, need,
+                                    stream_on(device)))
   if (rc != BIOPS_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
 }
@@ -354,7 +359,7 @@ PyObject* window_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                     ptr(k), 0, k.stride(1), k.stride(2), ptr(v), 0, v.stride(1), v.stride(2), ptr(out), 0,
                                     out.stride(1), out.stride(2), ptr(cu_q), is_long(cu_q), cu_q.stride(0), ptr(cu_k),
                                     is_long(cu_k), cu_k.stride(0), window, sinks, scale, reinterpret_cast<int*>(flag),
-                                    stream_on(device)))
+                                    nullptr, 0, stream_on(device)))
   if (rc != BIOPS_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
 }

@@ -39,6 +39,9 @@
 namespace biops {
 
 constexpr int kWindowFew = 64;      // rows up to which two wavefronts share them (window_launch_rows)
+// Keys of a range and ranges of a few rows at most (window_splits); a range has at least 16 keys for each of the rows, so that
+// their partial results stay a part of the keys' and values' bytes.
+constexpr int kWindowRange = 512, kWindowRanges = 16;
 constexpr float kWindowSlack = 8.f;  // by how many powers of two weights may pass one (weigh)
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
@@ -56,6 +59,8 @@ struct WindowArgs {
   uint32_t tiles;           // dense: tiles of a sequence; packed: most tiles of a head
   uint32_t hkv, group;
   int d, dv;
+  int splits, per;          // ranges of keys that a tile's workgroups take, blocks of a range
+  float *part, *ml;         // their results: [row][range][dv], [row][range][2]
   int window, sinks;        // window >= 1 (2^31 - 1: all)
   int negate;               // the scale is negative: queries enter with their sign flipped
   float scale;              // |scale| log2 e, > 0
@@ -245,6 +250,13 @@ void window_attn_kernel(WindowArgs a) {
     const uint32_t j = t - first;
     if ((n & 7) == 0) t = first + (j & 7) * (n >> 3) + (j >> 3);
   }
+  int range = 0;
+  if constexpr (KW > 1) {
+    if (a.splits > 1) {
+      range = (int)(t % (uint32_t)a.splits);
+      t /= (uint32_t)a.splits;
+    }
+  }
   WindowTile tile;
   const uint32_t tl = t % a.tiles;
   t /= a.tiles;
@@ -274,7 +286,8 @@ void window_attn_kernel(WindowArgs a) {
   const int ns = kl > 0 ? (a.sinks < start ? a.sinks : start) : 0;
   const int shift = start - ns;
   const int nv = kl > 0 && p1 >= 0 ? p1 + 1 - shift : 0;
-  const int nblk = (nv + BN - 1) / BN;
+  const int all_blocks = (nv + BN - 1) / BN;
+  const int blk0 = range * a.per, nblk = a.per < all_blocks - blk0 ? blk0 + a.per : all_blocks;  // the workgroup's
   // What a row sees of the counted keys: lo .. hi (its window), and v < sv (sinks; all of those in front of the
   // first row's window are before every row, the others are among the window's keys and cut off at hi).
   const int sv = shift > 0 ? ns : a.sinks;
@@ -544,11 +557,11 @@ void window_attn_kernel(WindowArgs a) {
   // higher priority: of two wavefronts of a SIMD one multiplies while the other takes exponentials).  The block's values
   // and the next one's keys are fetched while the wavefronts weigh, when nothing reads the LDS.  Two buffers, filled a turn
   // ahead, were 2 to 12 % slower: every read's address then depends on the block, and so costs an instruction.
-  if (nblk > 0) load_k(0);
+  if (blk0 < nblk) load_k(blk0);
   meet();
-  bool here = sees(0);
+  bool here = sees(blk0);
   if (here) scores();
-  for (int blk = 0; blk < nblk; ++blk) {
+  for (int blk = blk0; blk < nblk; ++blk) {
     meet();
     load_v(blk);
     if (blk + 1 < nblk) load_k(blk + 1);
@@ -596,6 +609,24 @@ void window_attn_kernel(WindowArgs a) {
         for (int e = 0; e < F::OF; ++e)
 #pragma unroll
           for (int r = 0; r < 16; ++r) oacc[e][r] = __builtin_fmaf(o[64 * (16 * e + r)], f, oacc[e][r]);
+      }
+      if (a.splits > 1) {  // this range's part of the rows
+        if (!row_ok) return;
+        const int64_t at = ((b * (a.hkv * a.group) + h) * a.lq + tile.i0 + rloc) * a.splits + range;
+#pragma unroll
+        for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int col = 32 * e + 8 * j + 4 * hf;
+            if (col < a.dv)
+              *reinterpret_cast<f32x4_t*>(a.part + at * a.dv + col) =
+                  f32x4_t{oacc[e][4 * j], oacc[e][4 * j + 1], oacc[e][4 * j + 2], oacc[e][4 * j + 3]};
+          }
+        if (hf == 0) {
+          a.ml[2 * at] = top;
+          a.ml[2 * at + 1] = l;
+        }
+        return;
       }
     }
   }
@@ -649,20 +680,64 @@ void window_attn_kernel(WindowArgs a) {
   }
 }
 
+// Joins the ranges of one row per wavefront, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t row = 4 * (a.first + blockIdx.x) + (threadIdx.x >> 6);
+  if (row >= a.total) return;
+  const int r = (int)(row % (uint32_t)a.lq);
+  const uint32_t heads = a.hkv * a.group, h = row / (uint32_t)a.lq % heads;
+  const int64_t b = row / (uint32_t)a.lq / heads;
+  const float* const ml = a.ml + 2 * (int64_t)row * a.splits;
+  const float* const part = a.part + (int64_t)row * a.splits * a.dv + 4 * lane;
+  const float m = lane < a.splits ? ml[2 * lane] : -INFINITY, sum = lane < a.splits ? ml[2 * lane + 1] : 0.f;
+  const float top = wave_max(m), f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+  float l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int x = 0; x < a.splits; ++x) {
+    const float fx = __shfl(f, x, 64);
+    l = __builtin_fmaf(__shfl(sum, x, 64), fx, l);
+    if (4 * lane < a.dv) o += *reinterpret_cast<const f32x4_t*>(part + (int64_t)x * a.dv) * fx;
+  }
+  char* const out = a.out + b * a.oB + r * a.oT + h * a.oH;
+  const float odd = __builtin_fmaf(o[0], 0.f, o[1] * 0.f) + __builtin_fmaf(o[2], 0.f, o[3] * 0.f);
+  if (l > 0.f && l < INFINITY && __any(odd != 0.f)) {  // not finite over a finite sum
+    const uint32_t hk = h / a.group;
+    window_row<T>(a, a.q + b * a.qB + r * a.qT + h * a.qH, a.k + b * a.kB + hk * a.kH, a.v + b * a.vB + hk * a.vH, out,
+                  a.lk - a.lq + r, a.lk, lane);
+    return;
+  }
+  if (4 * lane >= a.dv) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) Num<T>::store(reinterpret_cast<T*>(out) + 4 * lane + i, l == 0.f ? 0.f : o[i] * inv);
+}
+
 template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
 static int window_launch(WindowArgs a, hipStream_t s) {
   constexpr int rows = 32 * RW / HG;
   // packed: every sequence and the two ends may end in a part of a tile
   const int64_t tiles = a.cu_q ? a.lq / rows + a.nseq + 2 : cdiv(a.lq, rows);
   const int64_t heads = (int64_t)a.hkv * a.group / HG * (a.cu_q ? 1 : a.nseq);
-  if (tiles > INT64_C(0x7fffffff) / heads) return fail(BIOPS_ERR_ARG, "biops_window_attention: more than 2^31 tiles");
+  static_assert(KW == 1 || 32 * NH * KW == 64, "ranges are counted in blocks of 64 keys");
+  if (tiles > INT64_C(0x7fffffff) / heads / a.splits) return fail(BIOPS_ERR_ARG, "biops_window_attention: more than 2^31 tiles");
   a.tiles = (uint32_t)tiles;
-  a.total = (uint32_t)(tiles * heads);
+  a.total = (uint32_t)(tiles * heads * a.splits);
   constexpr uint32_t most = 1 << 22;  // a launch has less than 2^32 threads
   for (a.first = 0; a.first < a.total; a.first += most) {
     const uint32_t n = a.total - a.first < most ? a.total - a.first : most;
     hipLaunchKernelGGL((window_attn_kernel<T, DP, DVP, RW, KW, NH, HG>), dim3(n), dim3(64 * RW * KW), 0, s, a);
     const int rc = check_launch("window_attn_kernel");
+    if (rc != BIOPS_OK) return rc;
+  }
+  if (a.splits == 1) return BIOPS_OK;
+  a.total = (uint32_t)(a.nseq * a.hkv * a.group * a.lq);
+  const uint32_t groups = (a.total + 3) / 4;
+  for (a.first = 0; a.first < groups; a.first += most) {
+    const uint32_t n = groups - a.first < most ? groups - a.first : most;
+    hipLaunchKernelGGL((window_join_kernel<T>), dim3(n), dim3(256), 0, s, a);
+    const int rc = check_launch("window_join_kernel");
     if (rc != BIOPS_OK) return rc;
   }
   return BIOPS_OK;
@@ -717,9 +792,37 @@ static int window_launch_d(const WindowArgs& a, hipStream_t s) {
   return window_launch_rows<T, 128>(a, s);
 }
 
+// Ranges that the keys of a few dense rows are cut into, by sizes that all sequences of a call share; blocks of 64 keys
+// of a range.  A few rows are a few tiles, and each would walk through all keys alone.  us (one tile through all keys /
+// ranges), bf16, 16/4 heads of 128, no window: 16 rows before 2000 keys 39 / 20 (one sequence), 40 / 22 (eight), 61 / 85
+// (64); before 8192 keys 143 / 23, 144 / 46, 254 / 345; 64 rows before 8192 keys 133 / 28, 136 / 68, 445 / 563; float32,
+// 72-wide, 16 rows before 8192 443 / 42, 443 / 117, 806 / 892.  (The batch may not enter: one sequence's bits.)
+static int window_splits(int64_t lq, int64_t lk, int64_t window, int64_t sinks, int* per) {
+  *per = 0x7fffffff;
+  if (lq < 1 || lq > kWindowFew) return 1;
+  const int64_t n = window < lk && sinks < lk - window ? (window + sinks + lq < lk ? window + sinks + lq : lk) : lk;
+  const int64_t each = 16 * lq > kWindowRange ? 16 * lq : kWindowRange;
+  if (n < 2 * each) return 1;
+  const int64_t blocks = (n + 63) / 64, most = n / each < kWindowRanges ? n / each : kWindowRanges;
+  *per = (int)((blocks + most - 1) / most);
+  return (int)((blocks + *per - 1) / *per);
+}
+
 }  // namespace biops
 
 using namespace biops;
+
+extern "C" int64_t biops_window_attention_workspace_size(int64_t nseq, int64_t hq, int64_t lq, int64_t lk, int64_t dv,
+                                                         int64_t window, int64_t sinks) {
+  if (nseq < 0 || hq < 0 || lq < 0 || lk < 0 || dv < 0 || dv > 256 || window < 1 || sinks < 0 || hq > 65536 ||
+      lk > INT64_C(0x7fffffff))
+    return -1;
+  int per;
+  const int splits = window_splits(lq, lk, window, sinks, &per);
+  if (splits == 1 || nseq == 0 || hq == 0) return 0;
+  if (nseq > (INT64_C(1) << 30) / (hq * lq)) return -1;
+  return nseq * hq * lq * splits * (dv + 2) * (int64_t)sizeof(float);
+}
 
 extern "C" int biops_window_attention_max_head(int dtype) {
   return dtype == BIOPS_F32 ? 128 : (dtype == BIOPS_F16 || dtype == BIOPS_BF16 ? 256 : 0);
@@ -730,7 +833,8 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
                                       int64_t skB, int64_t skT, int64_t skH, const void* v, int64_t svB, int64_t svT,
                                       int64_t svH, void* out, int64_t soB, int64_t soT, int64_t soH, const void* cu_q,
                                       int cu_q64, int64_t cu_q_stride, const void* cu_k, int cu_k64, int64_t cu_k_stride,
-                                      int64_t window, int64_t sinks, float scale, int* flag, void* stream) {
+                                      int64_t window, int64_t sinks, float scale, int* flag, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
   const int elt = is_float_dtype(dtype) ? dtype_bytes(dtype) : 0;
   if (elt == 0) return fail(BIOPS_ERR_DTYPE, "biops_window_attention: unsupported dtype %d", dtype);
   if (nseq < 0 || hq < 0 || hkv <= 0 || hq % hkv != 0 || hq > 65536 || lq < 0 || lk < 0)
@@ -770,6 +874,20 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   a.d = (int)d, a.dv = (int)dv;
   const int64_t all = INT64_C(0x7fffffff);
   a.window = (int)(window < all ? window : all), a.sinks = (int)(sinks < all ? sinks : all);
+  a.splits = 1, a.per = 0x7fffffff;
+  a.part = a.ml = nullptr;
+  if (!cu_q && lk > 0) {
+    a.splits = window_splits(lq, lk, window, sinks, &a.per);
+    if (a.splits > 1) {
+      const int64_t need = biops_window_attention_workspace_size(nseq, hq, lq, lk, dv, window, sinks);
+      if (need < 0) return fail(BIOPS_ERR_ARG, "biops_window_attention: more than 2^30 rows");
+      if (!workspace || workspace_bytes < need)
+        return fail(BIOPS_ERR_SIZE, "biops_window_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+      if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BIOPS_ERR_LAYOUT, "biops_window_attention: workspace not 16-byte aligned");
+      a.part = static_cast<float*>(workspace);
+      a.ml = a.part + nseq * hq * lq * a.splits * dv;
+    }
+  }
   a.negate = scale < 0.f;
   // a scale of zero: every weight 1, and 0 * -inf stays out of the masked scores
   const float s = (scale < 0.f ? -scale : scale) * kLog2e;

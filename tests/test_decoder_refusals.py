@@ -221,13 +221,22 @@ def test_host_checks_of_the_entry_points():
     assert size(3, 4, 64, 256, 16, -1, 0, 0) == size(3, 4, 64, 260, 16, -1, 0, 0) == 3 * 4 * 16 * 66 * 4  # the most up to there
     assert size(-1, 4, 64, 8, 16, -1, 0, 0) == -1 and size(3, 4, 264, 8, 16, -1, 0, 0) == -1
 
-    def win(dtype=2, nseq=1, hq=4, hkv=2, lq=5, lk=5, d=64, window=4, sinks=0, scale=1.0, q=p, cu_q=N, flag=p):
+    def win(dtype=2, nseq=1, hq=4, hkv=2, lq=5, lk=5, d=64, window=4, sinks=0, scale=1.0, q=p, cu_q=N, flag=p, ws=N, wsb=0):
         return L.biops_window_attention(dtype, nseq, hq, hkv, lq, lk, d, 64, q, 64, 64, 64, *x, *x, *x, cu_q, 0, 1, N, 0, 1, window,
-                                        sinks, scale, flag, N)
+                                        sinks, scale, flag, ws, wsb, N)
 
     assert win(dtype=3) == 3 and win(hq=5) == 1 and win(hkv=0) == 1 and win(d=36) == 1 and win(dtype=0, d=132) == 1
     assert win(window=0) == 1 and win(sinks=-1) == 1 and win(scale=float("inf")) == 1 and win(q=N) == 1
     assert win(cu_q=p) == 1 and win(lq=1 << 31) == 1 and win(lk=-1) == 1
+    assert win(lk=2000, window=1 << 40) == 5 and win(lk=2000, window=1 << 40, ws=p, wsb=8) == 5
+    assert win(lk=2000, window=1 << 40, ws=p + 4, wsb=1 << 30) == 2
+    size = L.biops_window_attention_workspace_size
+    assert size(3, 4, 5, 1023, 64, 1 << 40, 0) == 0 and size(3, 4, 65, 1 << 20, 64, 1 << 40, 0) == 0
+    assert size(3, 4, 5, 1024, 64, 1 << 40, 0) == 3 * 4 * 5 * 2 * 66 * 4 and size(3, 4, 5, 1 << 20, 64, 1000, 18) == 0
+    assert size(3, 4, 5, 1 << 20, 64, 1000, 19) == size(3, 4, 5, 1024, 64, 1 << 40, 0)
+    assert size(3, 4, 50, 8192, 64, 1 << 40, 1 << 40) == 3 * 4 * 50 * 10 * 66 * 4  # 800 keys a range at least
+    assert size(3, 4, 5, 1 << 30, 64, 1 << 40, 0) == 3 * 4 * 5 * 16 * 66 * 4
+    assert size(-1, 4, 5, 9, 64, 1, 0) == -1 and size(1, 4, 5, 9, 64, 0, 0) == -1 and size(1 << 40, 4, 64, 1 << 20, 64, 1 << 40, 0) == -1
     assert win(lq=0) == 0 and win(nseq=0) == 0 and win(hq=0) == 0
     assert L.biops_window_attention_max_head(nat.F32) == 128 and L.biops_window_attention_max_head(nat.BF16) == 256
 
@@ -244,7 +253,7 @@ def test_fast_call_bindings_match():
     assert fast.paged_attention_workspace_size(*args) == L.biops_paged_attention_workspace_size(*args) > 0
     args = (2, 1, 4, 2, 64, 64, p, 64, 64, *x, *x, 4, 16, p, 0, 2, 1, 64, p, 0, 1, -1, 0, 0, 1.0, p, p, None, 0, None)
     assert fast.paged_attention(*args) == L.biops_paged_attention(*args) == 5
-    args = (2, 1, 5, 2, 5, 5, 64, 64, *x, *x, *x, *x, None, 0, 1, None, 0, 1, 4, 0, 1.0, p, None)
+    args = (2, 1, 5, 2, 5, 5, 64, 64, *x, *x, *x, *x, None, 0, 1, None, 0, 1, 4, 0, 1.0, p, None, 0, None)
     assert fast.window_attention(*args) == L.biops_window_attention(*args) == 1
     for fn in (fast.rotary, fast.paged_write, fast.paged_attention, fast.window_attention):
         with pytest.raises(TypeError):

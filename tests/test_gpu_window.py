@@ -152,6 +152,56 @@ def test_many_sequences():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lq, lk, window, sinks", [
+    (1, 1023, None, 0), (1, 1024, None, 0), (7, 1500, None, 0), (16, 9001, None, 0), (16, 3000, 1100, 4), (5, 3000, 990, 20),
+    (33, 1055, None, 0), (33, 1056, None, 0), (64, 4097, None, 0), (64, 5000, 4090, 64), (3, 2000, 1, 1500), (16, 40, None, 0),
+])
+def test_few_rows_before_many_keys(dtype, lq, lk, window, sinks):
+    """Both sides of the sizes at which the keys are cut into ranges."""
+    for hq, hkv, d, dv in ((4, 2, 64, 64), (3, 1, 128, 72)):
+        check(1, hq, hkv, lq, lk, d, dv, window, sinks, 80, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_rows_of_wide_heads_before_many_keys(dtype):
+    check(2, 4, 1, 20, 2000, 256, 200, None, 0, 81, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ranges_of_keys_joined(dtype):
+    """Their bits in every batch and by strides; masked and infinite keys, values at the end of the range, a graph."""
+    q, k, v = (randn(3, h, n, 64, seed=82 + h, dtype=dtype) for h, n in ((4, 20), (2, 3000), (2, 3000)))
+    out = window_attention(q, k, v, 2500, 3, enable_gqa=True)
+    for b in range(3):
+        assert_bitwise(window_attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], 2500, 3, enable_gqa=True)[0], out[b])
+    turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    assert_bitwise(window_attention(*turned, 2500, 3, enable_gqa=True), out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = window_attention(q, k, v, 2500, 3, enable_gqa=True)
+    for seed in range(3):
+        q.copy_(randn(3, 4, 20, 64, seed=90 + seed, dtype=dtype))
+        graph.replay()
+        assert_bitwise(held, window_attention(q, k, v, 2500, 3, enable_gqa=True))
+        torch.cuda.synchronize()
+    # row 10 is at 2990 and sees keys from 491 on: key 490 and value 2995 must not reach it
+    big = torch.where(v > 0, 0.99, 0.9).to(dtype) * torch.finfo(dtype).max
+    clean = window_attention(q, k, big, 2500, 3, enable_gqa=True)
+    assert bool(torch.isfinite(clean).all())
+    check_window(clean[0], q[0], k[0], big[0], 2500, 3, what="the largest values")
+    k[:, :, 490] = float("nan")
+    v[:, :, 490] = float("inf")
+    v[:, :, 2995] = float("nan")
+    out = window_attention(q, k, v, 2500, 3, enable_gqa=True)
+    assert bool(torch.isnan(out[:, :, :10]).all())  # they see key 490
+    assert bool(torch.isnan(out[:, :, 15:]).all()) and not bool(torch.isnan(out[:, :, 10:15]).any())
+    for t in (k, v):
+        t[:, :, 490] = 0.0
+        t[:, :, 2995] = 0.0
+    check_window(out[0][:, 10:15], q[0][:, 10:15], k[0][:, :2995], v[0][:, :2995], 2500, 3, what="between them")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("group, lq", [(1, 150), (2, 150), (4, 150), (4, 50)])
 def test_a_row_keeps_its_bits_whatever_follows(dtype, group, lq):
     """Other queries, keys and values behind a row, far larger ones among them, in its tile and in its blocks."""
