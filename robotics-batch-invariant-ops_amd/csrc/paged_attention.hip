@@ -6,9 +6,10 @@
 // window first, so that nothing else is loaded or looked up.  They are cut into chunks, a workgroup takes
 // a chunk of one key/value head for all the query heads that share it, and a second kernel joins the
 // chunks in their order (none where no sequence can have more than one):
-//   chunk:  m = max t_v, l = sum exp2(t_v - m), O = sum exp2(t_v - m) V_v,  t_v = (scale log2 e) q.k_v,
-//           t_v - m by one fused multiply-add of the product q.k_v
-//   join:   M = max m_c, o = sum_c exp2(m_c - M) O_c / sum_c exp2(m_c - M) l_c
+//   chunk:  m = max s_v, l = sum exp2(c (s_v - m)), O = sum exp2(c (s_v - m)) V_v,  s_v = q.k_v, c = scale log2 e
+//   join:   M = max m_c, o = sum_c exp2(c (m_c - M)) O_c / sum_c exp2(c (m_c - M)) l_c
+// The difference is taken before the product with c: it is exact next to the maximum however large the scores are, where
+// a fused c s_v - round(c m) would leave the rounding of c m in every weight, powers of two that overflow from 2^31 on.
 // Batch invariance: the chunks follow from n alone, so a sequence's bits are the same in every batch.
 //
 // What bounds it is the stream of keys and values, read once: about 4 G operations per 2-byte element (G
@@ -31,6 +32,7 @@
 //
 // Slots behind the end of a sequence may hold anything: keys of the last tile past the end are read
 // from the last key's row, their scores replaced by -inf and their values by zeros.
+#include <cfloat>
 #include <type_traits>
 
 #include "gemm_core.h"
@@ -231,8 +233,8 @@ void paged_chunk_kernel(PagedArgs a) {
     return lane < 32 ? id * a.kP + at * a.kS : id * a.vP + at * a.vS;
   };
 
-  // of query m16: largest product so far, m * scale, sum (of this lane's keys)
-  float m = -INFINITY, sh = 0.f, l = 0.f;
+  // of query m16: largest product so far, the same or 0 where that is -inf, sum (of this lane's keys)
+  float m = -INFINITY, from = 0.f, l = 0.f;
   f32x4_t acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -305,17 +307,16 @@ void paged_chunk_kernel(PagedArgs a) {
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     if (__any(mx > m)) {
       const float mn = fmaxf(m, mx);
-      const float to = mn == -INFINITY ? 0.f : mn * a.scale;
-      const float corr = mx > m ? (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - to)) : 1.f;
+      const float corr = mx > m ? __builtin_amdgcn_exp2f((m - mn) * a.scale) : 1.f;
       l *= corr;
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t] *= corr;
       m = mn;
-      sh = to;
+      from = mn == -INFINITY ? 0.f : mn;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], a.scale, -sh)) * kDown;
+      p[j] = __builtin_amdgcn_exp2f((p[j] - from) * a.scale) * kDown;
       l += p[j];
     }
     if constexpr (E == 4) {
@@ -355,7 +356,7 @@ void paged_chunk_kernel(PagedArgs a) {
   float* const mls = os + 4 * cols * DVP;
   if (m16 < cols) {
     if (q4 == 0) {
-      mls[2 * (w * cols + m16)] = m == -INFINITY ? m : sh;
+      mls[2 * (w * cols + m16)] = m;
       mls[2 * (w * cols + m16) + 1] = l;
     }
     float* o = os + (w * cols + m16) * DVP;
@@ -382,7 +383,7 @@ void paged_chunk_kernel(PagedArgs a) {
     float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const float f = __builtin_amdgcn_exp2f(mls[2 * (x * cols + col)] - base);
+      const float f = __builtin_amdgcn_exp2f((mls[2 * (x * cols + col)] - base) * a.scale);
       sum = __builtin_fmaf(mls[2 * (x * cols + col) + 1], f, sum);
       o += *reinterpret_cast<const f32x4_t*>(os + (x * cols + col) * DVP + e) * f;
     }
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
         ls = ml[2 * c + 1];
         os = *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * a.dv + 4 * piece);
       }
-      const float f = __builtin_amdgcn_exp2f(ms - base);
+      const float f = __builtin_amdgcn_exp2f((ms - base) * a.scale);
       sum = __builtin_fmaf(ls, f, sum);
       o += os * f;
     }
@@ -594,7 +595,7 @@ extern "C" int biops_paged_attention(int dtype, int64_t batch, int64_t hq, int64
   a.negate = scale < 0.f;
   // a scale of zero: every weight 1, and 0 * -inf stays out of the masked scores
   const float c = (scale < 0.f ? -scale : scale) * kLog2e;
-  a.scale = c > 1e-30f ? c : 1e-30f;
+  a.scale = c > 1e-30f ? (c < FLT_MAX ? c : FLT_MAX) : 1e-30f;  // (no product with 0 is NaN)
   hipStream_t s = static_cast<hipStream_t>(stream);
   BIOPS_DISPATCH_FLOAT(dtype, return paged_launch_d<T>(a, s));
   return BIOPS_OK;

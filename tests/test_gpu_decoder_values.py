@@ -1,0 +1,110 @@
+"""Attention over pages and under a window at the ends of the number range, against the 64-bit definition."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from batch_invariant_ops import check_cache_indices, paged_attention_batch_invariant
+
+from _decoder import HALF, assert_within, attend64, attention_bound, token_rounding
+
+pytestmark = pytest.mark.gpu
+DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _no_error_left():
+    yield
+    check_cache_indices()
+
+
+def randn(*shape, seed, dtype=BF16):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def paged(k, v, page=16):
+    """k [keys, heads, d], v [keys, heads, dv] as caches with their pages backwards, and the table."""
+    n = k.shape[0]
+    count = max(1, -(-n // page))
+    caches = []
+    for x in (k, v):
+        c = torch.full((count, page, *x.shape[1:]), float("nan"), dtype=x.dtype)
+        c.flatten(0, 1)[:n] = x
+        caches.append(c.flip(0).contiguous().cuda())
+    return *caches, torch.arange(count - 1, -1, -1, dtype=torch.int32).view(1, count).cuda()
+
+
+def token(q, k, v, **kw):
+    """q [hq, d] against k [keys, hkv, d], v [keys, hkv, dv] (on the CPU)."""
+    kc, vc, table = paged(k, v)
+    lengths = torch.tensor([k.shape[0]], dtype=torch.int32).cuda()
+    return paged_attention_batch_invariant(q.unsqueeze(0).cuda(), kc, vc, table, lengths, **kw)[0]
+
+
+def exact_scores(out, q, k, v, visible, scale, rounding, what):
+    """As the definition for scores that are exact in 32 bits: they add nothing to the bound.  out, q [rows, d], k, v
+    [keys, d] of one head."""
+    o, mag, err, tail = attend64(q, k, v, visible, scale)
+    assert_within(out, o, attention_bound(out.dtype, o, mag, torch.zeros_like(err), tail, int(visible.sum(1).max()), *rounding), what)
+
+
+# An element of the queries, one of the keys, the head size, the type.  All keys of a kind have the same score to the bit,
+# and those of the other kind one so far away that its weight is 0 in 64 bits too.
+HUGE = [
+    (19968.0, 19968.0, 128, BF16), (20096.0, 18944.0, 128, BF16), (-20096.0, 18944.0, 128, BF16), (5736.0, 5736.0, 128, F16),
+    (6832.0, 6832.0, 64, F16), (-6832.0, 6832.0, 64, F16), (2.0**40, 1.5 * 2.0**40, 64, BF16), (3.0 * 2.0**50, 5.0 * 2.0**40, 72, F32),
+    (20001.0, 20001.0, 64, F32), (2.0**60, 2.0**60, 128, F32),
+]
+
+
+@pytest.mark.parametrize("x, y, d, dtype", HUGE)
+@pytest.mark.parametrize("n", [1, 40, 700, 2500])
+def test_token_attention_of_huge_scores(x, y, d, dtype, n):
+    """Every third key has the largest score, all others far smaller ones: the mean of those values."""
+    q = torch.full((2, d), x, dtype=dtype)
+    k = torch.full((n, 1, d), y, dtype=dtype)
+    other = torch.arange(n) % 3 != 0 if x > 0 else torch.arange(n) % 3 == 0
+    k[other] = k[other] / 2
+    v = randn(n, 1, 64, seed=n, dtype=dtype)
+    out = token(q, k, v)
+    for h in range(2):
+        exact_scores(out[h:h + 1], q[h:h + 1], k[:, 0], v[:, 0], torch.ones(1, n, dtype=torch.bool), d**-0.5, token_rounding(dtype),
+                     f"head {h}")
+
+
+def steps(n, dtype, seed, sign=1.0):
+    """Scores 4096 a + 16 b + j, exact in 32 bits, j random in -60 .. 60 and the rest near 2^20 / log2 e: arguments of 2^x on
+    both sides of 2^20.  (q [1, 8 or 16 bytes of elements], k.)"""
+    g = torch.Generator().manual_seed(seed)
+    j = torch.randint(-60, 61, (n,), generator=g)
+    d = 8
+    q, k = torch.zeros(1, d), torch.zeros(n, 1, d)
+    q[0, :3] = torch.tensor([4096.0, 16.0, 1.0])
+    k[:, 0, 0], k[:, 0, 1], k[:, 0, 2] = 177.0 * sign, 114.0 * sign, j.float()
+    return q.to(dtype), k.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, sign", [(50, 1.0), (3000, 1.0), (700, -1.0)])
+def test_token_attention_of_large_scores_close_together(dtype, n, sign):
+    q, k = steps(n, dtype, n, sign)
+    v = randn(n, 1, 64, seed=n + 1, dtype=dtype)
+    exact_scores(token(q, k, v, scale=1.0), q, k[:, 0], v[:, 0], torch.ones(1, n, dtype=torch.bool), 1.0, token_rounding(dtype), "")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [1e12, -1e12, 1e37, 3e38])
+def test_token_attention_with_a_huge_scale(dtype, scale):
+    """The value of the one key with the largest product."""
+    n, d = 300, 64
+    q, k, v = randn(2, d, seed=1, dtype=dtype), randn(n, 1, d, seed=2, dtype=dtype), randn(n, 1, d, seed=3, dtype=dtype)
+    out = token(q, k, v, scale=scale)
+    s = (k[:, 0].double() @ q.double().T) * math.copysign(1.0, scale)
+    top = s.topk(2, dim=0).values
+    assert float((top[0] - top[1]).min()) > 1e-3  # far more than the 32-bit sums' error
+    want = v[s.argmax(0), 0].double()
+    assert_within(out, want, HALF[dtype] * want.abs() + 2.0**-22 * want.abs())
