@@ -31,6 +31,7 @@
 // a 16-bit type; two or three wavefronts of a SIMD overlap the two in part.  bf16, 16/4 heads of 128, 2 x 8192 tokens
 // under a window of 2048: 288 us, 837 TF/s of visible pairs; fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 31 us.  float32 products
 // run at 1/16 of the 16-bit rate and bound it alone: 3 x 257 rows of 1281 keys, 16 heads of 72, window 500: 37 us.
+#include <cfloat>
 #include <type_traits>
 
 #include "gemm_core.h"
@@ -43,6 +44,10 @@ constexpr int kWindowFew = 64;      // rows up to which two wavefronts share the
 // their partial results stay a part of the keys' and values' bytes.
 constexpr int kWindowRange = 512, kWindowRanges = 16;
 constexpr float kWindowSlack = 8.f;  // by how many powers of two weights may pass one (weigh)
+// A weight is 2^(c s - c m) by one fused multiply-add with c m rounded.  The rounding is the same factor in all weights of a
+// row, and no more than 2^(1/16) up to this size of c m; past it the difference s - m is taken first (with an instruction
+// more), or the factor would leave the range: by 2^28 fp16's, by 2^31 float's.
+constexpr float kWindowLarge = 0x1p20f;
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
 struct WindowArgs {
@@ -178,6 +183,16 @@ struct WindowShape {
   }
 };
 
+// Exponent that turns weights relative to the score m into those relative to the score top; c = a.scale.  (The products are
+// the rounded ones that the weights have seen: no fused multiply-add may take their place.)
+__device__ __forceinline__ float window_ratio(float m, float top, float c) {
+#pragma clang fp contract(off)
+  const float a = m * c, t = top * c;
+  const bool la = fabsf(a) > kWindowLarge, lt = fabsf(t) > kWindowLarge;
+  if (!la && !lt) return a - t;
+  return (m - top) * c - (la ? 0.f : __builtin_fmaf(m, c, -a)) + (lt ? 0.f : __builtin_fmaf(top, c, -t));
+}
+
 // One row over exactly the keys that it sees, a wavefront together: the mean so far is kept normalised,
 // so that values near the end of the type's range do not overflow either.
 template <typename T>
@@ -191,7 +206,7 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const char* q, c
     if (a.negate) x[i] = -x[i];
     o[i] = 0.f;
   }
-  float sh = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f;
   const int64_t start = (int64_t)p - a.window + 1;
   const int last = p < kl - 1 ? p : kl - 1;
   for (int j = 0; j <= last; ++j) {
@@ -204,12 +219,12 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const char* q, c
 #pragma unroll
     for (int i = 0; i < MOST; ++i)
       if (lane + 64 * i < a.d) s = __builtin_fmaf(x[i], Num<T>::load(kr + lane + 64 * i), s);
-    s = wave_sum(s) * a.scale;
+    s = wave_sum(s);
     if (s == -INFINITY) continue;
-    const float top = fmaxf(sh, s);
-    const float old = l * __builtin_amdgcn_exp2f(sh - top), add = __builtin_amdgcn_exp2f(s - top);
+    const float top = fmaxf(m, s);
+    const float old = l * __builtin_amdgcn_exp2f((m - top) * a.scale), add = __builtin_amdgcn_exp2f((s - top) * a.scale);
     l = old + add;
-    sh = top;
+    m = top;
     const float f = old / l, g = add / l;
     const T* vr = reinterpret_cast<const T*>(v + j * a.vT);
 #pragma unroll
@@ -395,9 +410,9 @@ void window_attn_kernel(WindowArgs a) {
     }
   }
 
-  // m: the score (raw) that weights are relative to, sh = m * scale, l: this lane's part of the row's sum
+  // m: the score (raw) that weights are relative to, sh = m * scale (0 before the first), l: this lane's part of the row's sum
   float m = -INFINITY, sh = 0.f, l = 0.f;
-  const float slack = kWindowSlack / a.scale;
+  const float slack = fminf(kWindowSlack / a.scale, FLT_MAX);
   f32x16_t oacc[F::OF];  // O^T: register r of block e is column 32e + 8(r/4) + 4hf + r%4 of row l32
 #pragma unroll
   for (int e = 0; e < F::OF; ++e)
@@ -464,12 +479,12 @@ void window_attn_kernel(WindowArgs a) {
     // A row's maximum is followed when it has grown by more than 2^kWindowSlack in its weights: until then they are that
     // much larger than one at most, and nothing is rescaled
     // (2 to 5 % of the time; 16 % with 256-wide heads and few rows).  Each row by itself, so that no row's bits depend on another.
-    const bool grown = mx > m + slack;
+    const bool grown = mx - m > slack;
     if (__any(grown)) {
       const float mn = grown ? mx : m;
       const float to = mn == -INFINITY ? 0.f : mn * a.scale;
       if (__any(m > -INFINITY)) {  // (nothing is summed before a row's first keys)
-        const float corr = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(sh - to) : 1.f;
+        const float corr = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(window_ratio(m, mn, a.scale)) : 1.f;
         l *= corr;
 #pragma unroll
         for (int e = 0; e < F::OF; ++e)
@@ -479,11 +494,20 @@ void window_attn_kernel(WindowArgs a) {
       m = mn;
       sh = to;
     }
+    const bool large = fabsf(sh) > kWindowLarge;
+    if (__any(large)) {
+      const float less = large ? m : 0.f;
+#pragma unroll
+      for (int x = 0; x < NH; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[x][r] -= less;
+    }
+    const float off = large ? 0.f : sh;
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        sc[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][r], a.scale, -sh));
+        sc[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][r], a.scale, -off));
         if constexpr (E == 4) l += sc[x][r];
       }
       if constexpr (E == 2) {
@@ -585,16 +609,16 @@ void window_attn_kernel(WindowArgs a) {
       for (int e = 0; e < F::OF; ++e)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[64 * (16 * e + r)] = oacc[e][r];
-      o[64 * 16 * F::OF] = m == -INFINITY ? m : sh;
+      o[64 * 16 * F::OF] = m;
       o[64 * (16 * F::OF + 1)] = l;
     }
     __syncthreads();
     if (part == 0) {
-      float top = m == -INFINITY ? m : sh;
+      float top = m;
 #pragma unroll
       for (int x = 1; x < KW; ++x) top = fmaxf(top, js[((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane + 64 * 16 * F::OF]);
-      const float base = top == -INFINITY ? 0.f : top;
-      const float own = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh - base);
+      auto factor = [&](float from) { return from == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(window_ratio(from, top, a.scale)); };
+      const float own = factor(m);
       l *= own;
 #pragma unroll
       for (int e = 0; e < F::OF; ++e)
@@ -603,7 +627,7 @@ void window_attn_kernel(WindowArgs a) {
 #pragma unroll
       for (int x = 1; x < KW; ++x) {
         const float* o = js + ((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane;
-        const float f = __builtin_amdgcn_exp2f(o[64 * 16 * F::OF] - base);
+        const float f = factor(o[64 * 16 * F::OF]);
         l = __builtin_fmaf(o[64 * (16 * F::OF + 1)], f, l);
 #pragma unroll
         for (int e = 0; e < F::OF; ++e)
@@ -692,7 +716,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
   const float* const ml = a.ml + 2 * (int64_t)row * a.splits;
   const float* const part = a.part + (int64_t)row * a.splits * a.dv + 4 * lane;
   const float m = lane < a.splits ? ml[2 * lane] : -INFINITY, sum = lane < a.splits ? ml[2 * lane + 1] : 0.f;
-  const float top = wave_max(m), f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+  const float top = wave_max(m), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(window_ratio(m, top, a.scale));
   float l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int x = 0; x < a.splits; ++x) {
@@ -891,7 +915,7 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   a.negate = scale < 0.f;
   // a scale of zero: every weight 1, and 0 * -inf stays out of the masked scores
   const float s = (scale < 0.f ? -scale : scale) * kLog2e;
-  a.scale = s > 1e-30f ? s : 1e-30f;
+  a.scale = s > 1e-30f ? (s < FLT_MAX ? s : FLT_MAX) : 1e-30f;  // (no product with 0 is NaN)
   BIOPS_DISPATCH_FLOAT(dtype, return window_launch_d<T>(a, static_cast<hipStream_t>(stream)));
   return BIOPS_OK;
 }

@@ -7,9 +7,11 @@ import math
 import pytest
 import torch
 
-from batch_invariant_ops import check_cache_indices, paged_attention_batch_invariant
+from batch_invariant_ops import (check_cache_indices, paged_attention_batch_invariant,
+                                 sliding_window_attention_batch_invariant as window_attention,
+                                 varlen_sliding_window_attention_batch_invariant as packed_attention)
 
-from _decoder import HALF, assert_within, attend64, attention_bound, token_rounding
+from _decoder import HALF, assert_within, attend64, attention_bound, prompt_rounding, token_rounding, window_visible
 
 pytestmark = pytest.mark.gpu
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -108,3 +110,57 @@ def test_token_attention_with_a_huge_scale(dtype, scale):
     assert float((top[0] - top[1]).min()) > 1e-3  # far more than the 32-bit sums' error
     want = v[s.argmax(0), 0].double()
     assert_within(out, want, HALF[dtype] * want.abs() + 2.0**-22 * want.abs())
+
+
+# Rows and keys of the kinds of tiles: few rows, few before keys in ranges, many.
+TILES = [(1, 1), (7, 40), (4, 3000), (130, 200)]
+
+
+def prompt(q, k, v, window=None, sinks=0, **kw):
+    """q [rows, hq, d], k and v [keys, hkv, ...] on the CPU: dense output [rows, hq, dv]; the packed one has to agree where it
+    takes the same tiles, and has to hold by itself where it does not."""
+    dense = window_attention(*(x.transpose(0, 1).unsqueeze(0).cuda() for x in (q, k, v)), window, sinks, enable_gqa=True, **kw)
+    offsets = [torch.tensor([0, x.shape[0]], dtype=torch.int32).cuda() for x in (q, k)]
+    packed = packed_attention(*(x.unsqueeze(0).cuda() for x in (q, k, v)), *offsets, window, sinks, **kw)
+    return dense[0].transpose(0, 1), packed[0]
+
+
+@pytest.mark.parametrize("x, y, d, dtype", HUGE)
+@pytest.mark.parametrize("lq, lk", TILES)
+def test_prompts_of_huge_scores(x, y, d, dtype, lq, lk):
+    q = torch.full((lq, 2, d), x, dtype=dtype)
+    k = torch.full((lk, 1, d), y, dtype=dtype)
+    k[torch.arange(lk) % 3 != 0 if x > 0 else torch.arange(lk) % 3 == 0] /= 2
+    v = randn(lk, 1, 64, seed=lk, dtype=dtype)
+    for window, sinks in ((None, 0), (9, 1)):
+        visible = window_visible(lq, lk, window, sinks)
+        for out in prompt(q, k, v, window, sinks):
+            for h in range(2):
+                exact_scores(out[:, h], q[:, h], k[:, 0], v[:, 0], visible, d**-0.5, prompt_rounding(dtype), f"head {h}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lq, lk, sign", [(5, 60, 1.0), (6, 3000, 1.0), (5, 700, -1.0), (140, 300, 1.0)])
+def test_prompts_of_large_scores_close_together(dtype, lq, lk, sign):
+    q, k = steps(lk, dtype, lk, sign)
+    q, v = q.unsqueeze(0).expand(lq, 1, -1).contiguous(), randn(lk, 1, 64, seed=lk + 1, dtype=dtype)
+    visible = window_visible(lq, lk, None, 0)
+    for out in prompt(q, k, v, scale=1.0):
+        exact_scores(out[:, 0], q[:, 0], k[:, 0], v[:, 0], visible, 1.0, prompt_rounding(dtype), "")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [1e12, -1e12, 1e37, 3e38])
+@pytest.mark.parametrize("lq", [3, 90])
+def test_prompts_with_a_huge_scale(dtype, scale, lq):
+    n, d = 300, 64
+    q = randn(1, 2, d, seed=1, dtype=dtype).expand(lq, 2, d).contiguous()
+    k, v = randn(n, 1, d, seed=2, dtype=dtype), randn(n, 1, d, seed=3, dtype=dtype)
+    s = (k[:, 0].double() @ q[0].double().T) * math.copysign(1.0, scale)
+    for out in prompt(q, k, v, scale=scale):
+        for r in range(lq):
+            seen = n - lq + r + 1
+            top = s[:seen].topk(2, dim=0).values
+            assert float((top[0] - top[1]).min()) > 1e-3  # far more than the 32-bit sums' error
+            want = v[s[:seen].argmax(0), 0].double()
+            assert_within(out[r], want, HALF[dtype] * want.abs() + 2.0**-22 * want.abs(), f"row {r}")
