@@ -32,11 +32,11 @@
 //
 // Slots behind the end of a sequence may hold anything: keys of the last tile past the end are read
 // from the last key's row, their scores replaced by -inf and their values by zeros.
-#include <cfloat>
 #include <type_traits>
 
 #include "gemm_core.h"
 #include "rowops.h"
+#include "scores.h"
 
 namespace biops {
 
@@ -60,8 +60,8 @@ struct PagedArgs {
   int d, dv, chunks;                       // chunks: most chunks of a sequence
   int window, sinks;                       // window 0: all
   int table64, lengths64;
-  int negate;                              // the scale is negative: queries enter with their sign flipped
-  float scale;                             // |scale| log2 e, > 0
+  int negate, zero;                        // the scale is negative, or 0 (score_scale)
+  float scale;                             // c > 0
 };
 
 struct PagedSpan {
@@ -210,7 +210,7 @@ void paged_chunk_kernel(PagedArgs a) {
     for (int s = 0; s < KS; ++s) {
       const int d0 = KW * s + VEC * q4;
       qf[s] = m16 < cols && d0 < a.d ? load_16(qr + E * d0) : zero4;
-      if (a.negate) qf[s] ^= E == 2 ? 0x80008000u : 0x80000000u;
+      if (a.negate | a.zero) qf[s] = score_query<T>(qf[s], a.negate, a.zero);
     }
   }
   __syncthreads();  // bad_page is clear
@@ -592,10 +592,7 @@ extern "C" int biops_paged_attention(int dtype, int64_t batch, int64_t hq, int64
   a.d = (int)d, a.dv = (int)dv;
   a.window = (int)(window < all ? window : all), a.sinks = (int)(sinks < all ? sinks : all);
   a.table64 = table64 != 0, a.lengths64 = lengths64 != 0;
-  a.negate = scale < 0.f;
-  // a scale of zero: every weight 1, and 0 * -inf stays out of the masked scores
-  const float c = (scale < 0.f ? -scale : scale) * kLog2e;
-  a.scale = c > 1e-30f ? (c < FLT_MAX ? c : FLT_MAX) : 1e-30f;  // (no product with 0 is NaN)
+  a.scale = score_scale(scale, &a.negate, &a.zero);
   hipStream_t s = static_cast<hipStream_t>(stream);
   BIOPS_DISPATCH_FLOAT(dtype, return paged_launch_d<T>(a, s));
   return BIOPS_OK;

@@ -31,11 +31,11 @@
 // a 16-bit type; two or three wavefronts of a SIMD overlap the two in part.  bf16, 16/4 heads of 128, 2 x 8192 tokens
 // under a window of 2048: 288 us, 837 TF/s of visible pairs; fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 31 us.  float32 products
 // run at 1/16 of the 16-bit rate and bound it alone: 3 x 257 rows of 1281 keys, 16 heads of 72, window 500: 37 us.
-#include <cfloat>
 #include <type_traits>
 
 #include "gemm_core.h"
 #include "rowops.h"
+#include "scores.h"
 
 namespace biops {
 
@@ -67,8 +67,8 @@ struct WindowArgs {
   int splits, per;          // ranges of keys that a tile's workgroups take, blocks of a range
   float *part, *ml;         // their results: [row][range][dv], [row][range][2]
   int window, sinks;        // window >= 1 (2^31 - 1: all)
-  int negate;               // the scale is negative: queries enter with their sign flipped
-  float scale;              // |scale| log2 e, > 0
+  int negate, zero;         // the scale is negative, or 0 (score_scale)
+  float scale;              // c > 0
 };
 
 struct WindowTile {
@@ -204,6 +204,7 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const char* q, c
   for (int i = 0; i < MOST; ++i) {
     x[i] = lane + 64 * i < a.d ? Num<T>::load(reinterpret_cast<const T*>(q) + lane + 64 * i) : 0.f;
     if (a.negate) x[i] = -x[i];
+    if (a.zero) x[i] *= 0.f;
     o[i] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
@@ -331,9 +332,9 @@ void window_attn_kernel(WindowArgs a) {
 #pragma unroll
       for (int c = 0; c < F::QF; ++c) qf[c] = F::VEC * (2 * c + hf) < a.d ? load_16(qr + 16 * (2 * c + hf)) : zero4;
     }
-    if (a.negate) {
+    if (a.negate | a.zero) {
 #pragma unroll
-      for (int c = 0; c < F::QF; ++c) qf[c] ^= E == 2 ? 0x80008000u : 0x80000000u;
+      for (int c = 0; c < F::QF; ++c) qf[c] = score_query<T>(qf[c], a.negate, a.zero);
     }
   }
 
@@ -912,10 +913,7 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
       a.ml = a.part + nseq * hq * lq * a.splits * dv;
     }
   }
-  a.negate = scale < 0.f;
-  // a scale of zero: every weight 1, and 0 * -inf stays out of the masked scores
-  const float s = (scale < 0.f ? -scale : scale) * kLog2e;
-  a.scale = s > 1e-30f ? (s < FLT_MAX ? s : FLT_MAX) : 1e-30f;  // (no product with 0 is NaN)
+  a.scale = score_scale(scale, &a.negate, &a.zero);
   BIOPS_DISPATCH_FLOAT(dtype, return window_launch_d<T>(a, static_cast<hipStream_t>(stream)));
   return BIOPS_OK;
 }

@@ -164,3 +164,37 @@ def test_prompts_with_a_huge_scale(dtype, scale, lq):
             assert float((top[0] - top[1]).min()) > 1e-3  # far more than the 32-bit sums' error
             want = v[s[:seen].argmax(0), 0].double()
             assert_within(out[r], want, HALF[dtype] * want.abs() + 2.0**-22 * want.abs(), f"row {r}")
+
+
+# Products of queries and keys reach 1e36 and more, where any scale but 0 counts.
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-45, 1e-39, -3e-37, 2e-36])
+@pytest.mark.parametrize("lq", [3, 90])
+def test_tiny_scales(dtype, scale, lq):
+    n, d = 300, 64
+    q, k = (1e18 * randn(x, 2, d, seed=x, dtype=F32) for x in (lq, n))
+    q, k, v = q.to(dtype), k.to(dtype), randn(n, 2, d, seed=9, dtype=dtype)
+    held = float(torch.tensor(scale, dtype=F32))  # as the kernels hold it
+    outs = [(o, window_visible(lq, n, None, 0), prompt_rounding(dtype)) for o in prompt(q, k, v, scale=scale)]
+    outs.append((token(q[-1], k, v, scale=scale).unsqueeze(0), window_visible(1, n, None, 0), token_rounding(dtype)))
+    for out, visible, rounding in outs:
+        for h in range(2):
+            parts = attend64(q[-len(out):, h], k[:, h], v[:, h], visible, held)
+            assert_within(out[:, h], parts[0], attention_bound(dtype, *parts, n, *rounding), f"head {h}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_scale_of_zero_and_infinities(dtype):
+    """0 times a product that is not finite is NaN."""
+    q, k, v = (randn(x, 1, 64, seed=x, dtype=dtype) for x in (5, 70, 71))
+    v = v[:70]
+    q[2, 0, 9], q[3, 0, 1] = float("nan"), float("inf")
+    for bad in (None, 3):
+        if bad is not None:
+            k[68, 0, 0] = float("-inf")
+        visible = window_visible(5, 70, 20, 0)
+        for out in prompt(q, k, v, 20, scale=0.0):
+            parts = attend64(q[:, 0], k[:, 0], v[:, 0], visible, 0.0)
+            assert_within(out[:, 0], parts[0], torch.nan_to_num(attention_bound(dtype, *parts, 20, *prompt_rounding(dtype)), 0.0))
+        for r in (0, 2, 3):
+            assert bool(torch.isnan(token(q[r], k, v, scale=0.0)).all()) == (r > 0 or bad is not None)
