@@ -17,11 +17,16 @@ inline float score_scale(float scale, int* negate, int* zero) {
   return c == 0.f ? 1.f : (c < FLT_MAX ? c : FLT_MAX);
 }
 
+// Exponent bits of an element: all of them are set where it is not finite.
+template <typename T>
+__host__ __device__ constexpr uint32_t score_inf() {
+  return Num<T>::kBytes == 4 ? 0x7f800000u : (std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u);
+}
+
 // 0 * x of packed elements: 0, and NaN where x is not finite.
 template <typename T>
 __device__ __forceinline__ u32x4_t times_zero(u32x4_t v) {
-  constexpr uint32_t inf = Num<T>::kBytes == 4 ? 0x7f800000u : (std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u);
-  constexpr uint32_t nan = inf | inf >> 1;
+  constexpr uint32_t inf = score_inf<T>(), nan = inf | inf >> 1;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (Num<T>::kBytes == 4) v[i] = (v[i] & inf) == inf ? nan : 0u;

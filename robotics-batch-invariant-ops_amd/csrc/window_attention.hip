@@ -18,10 +18,11 @@
 // the transposing read.  16-bit weights are rounded once to the type for the product (half a step, as the
 // output's own rounding); statistics and sums are 32-bit.
 //
-// A masked key never reaches a row.  Scores are replaced, not added to; keys past the sequence's end are
-// zeros in LDS.  What is left is a value that is not finite at a key which one row of a block sees and
-// another does not (0 * inf): a row whose sum is finite and whose output is not is computed again, key by
-// key over what it sees (window_row).
+// A masked key never reaches a row, to the bit.  Its scores are replaced, not added to, and 0 times its values adds nothing
+// unless one of them is not finite: a row whose sum is finite and whose output is not is computed again, in the same blocks
+// and order over values whose infinities and NaN are zeros (mode 1), and those that the row sees are then set in its output
+// (window_mark).  If it still is not finite, its sum passed float's range where the mean does not: once more with smaller
+// weights (mode 2).  Rows behind a sequence's last key are read from that key and masked.
 //
 // Batch invariance: a tile's keys, blocks and order follow from its own sequence's lengths, and the variant from
 // sizes that a call's sequences share.
@@ -48,6 +49,10 @@ constexpr float kWindowSlack = 8.f;  // by how many powers of two weights may pa
 // row, and no more than 2^(1/16) up to this size of c m; past it the difference s - m is taken first (with an instruction
 // more), or the factor would leave the range: by 2^28 fp16's, by 2^31 float's.
 constexpr float kWindowLarge = 0x1p20f;
+// Weights of mode 2 are 2^-40 times their size: of fewer than 2^31 values times weights of up to 2^kWindowSlack no sum passes
+// the largest one.
+constexpr float kWindowDown = 40.f;
+template <typename T> constexpr int kWindowLast = std::is_same<T, f16_t>::value ? 1 : 2;  // (no sum of fp16 values passes float's range)
 constexpr int kWindowOrder = 512;  // tiles that are dealt to the XCDs in runs
 
 struct WindowArgs {
@@ -184,57 +189,115 @@ struct WindowShape {
 };
 
 // Exponent that turns weights relative to the score m into those relative to the score top; c = a.scale.  (The products are
-// the rounded ones that the weights have seen: no fused multiply-add may take their place.)
-__device__ __forceinline__ float window_ratio(float m, float top, float c) {
+// the rounded ones that the weights have seen: no fused multiply-add may take their place.  `exact`: mode 2, where all
+// differences are taken first.)
+__device__ __forceinline__ float window_ratio(float m, float top, float c, bool exact) {
 #pragma clang fp contract(off)
   const float a = m * c, t = top * c;
-  const bool la = fabsf(a) > kWindowLarge, lt = fabsf(t) > kWindowLarge;
+  const bool la = exact || fabsf(a) > kWindowLarge, lt = exact || fabsf(t) > kWindowLarge;
   if (!la && !lt) return a - t;
   return (m - top) * c - (la ? 0.f : __builtin_fmaf(m, c, -a)) + (lt ? 0.f : __builtin_fmaf(top, c, -t));
 }
 
-// One row over exactly the keys that it sees, a wavefront together: the mean so far is kept normalised,
-// so that values near the end of the type's range do not overflow either.
+// Infinities and NaN of 16 bytes as zeros.
 template <typename T>
-__device__ __forceinline__ void window_row(const WindowArgs& a, const char* q, const char* k, const char* v, char* out,
-                                           int p, int kl, int lane) {
-  constexpr int MOST = 4;  // 256 / 64
-  float x[MOST], o[MOST];
+__device__ __forceinline__ u32x4_t finite_or_zero(u32x4_t v) {
+  constexpr uint32_t inf = score_inf<T>();
 #pragma unroll
-  for (int i = 0; i < MOST; ++i) {
-    x[i] = lane + 64 * i < a.d ? Num<T>::load(reinterpret_cast<const T*>(q) + lane + 64 * i) : 0.f;
-    if (a.negate) x[i] = -x[i];
-    if (a.zero) x[i] *= 0.f;
-    o[i] = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Num<T>::kBytes == 4) v[i] = (v[i] & inf) == inf ? 0u : v[i];
+    else v[i] = ((v[i] & inf) == inf ? 0u : v[i] & 0xffffu) | ((v[i] & inf << 16) == inf << 16 ? 0u : v[i] & 0xffff0000u);
   }
-  float m = -INFINITY, l = 0.f;
-  const int64_t start = (int64_t)p - a.window + 1;
-  const int last = p < kl - 1 ? p : kl - 1;
-  for (int j = 0; j <= last; ++j) {
-    if (j >= a.sinks && j < start) {
-      j = (int)start - 1;
-      continue;
+  return v;
+}
+
+// What a wavefront's part of a tile is (the same for all its lanes).
+struct WindowPart {
+  WindowTile tile;
+  int64_t b;
+  int h, w, range;  // head, wavefront of the workgroup, range of keys
+};
+
+// The keys of a tile, counted through from 0: v is key v < ns ? v : v + shift (sinks, then everything from the first row's
+// window on).
+struct WindowKeys {
+  int p0, qrows;     // position of the tile's first row; its rows
+  int ns, shift, nv; // nv: how many there are
+  int sv;            // every row sees v < sv, up to its own position: sinks
+  int blk0, nblk;    // blocks that the workgroup takes
+};
+__device__ __forceinline__ WindowKeys window_keys(const WindowArgs& a, const WindowPart& part, int rows, int block) {
+  const WindowTile& tile = part.tile;
+  WindowKeys k;
+  k.qrows = tile.ql - tile.i0 < rows ? tile.ql - tile.i0 : rows;
+  k.p0 = tile.kl - tile.ql + tile.i0;
+  const int p1 = k.p0 + k.qrows - 1;
+  const int64_t begin = (int64_t)k.p0 - a.window + 1;
+  const int start = begin > 0 ? (int)begin : 0;
+  k.ns = tile.kl > 0 ? (a.sinks < start ? a.sinks : start) : 0;
+  k.shift = start - k.ns;
+  k.nv = tile.kl > 0 && p1 >= 0 ? p1 + 1 - k.shift : 0;
+  const int all = (k.nv + block - 1) / block;
+  k.blk0 = part.range * a.per;
+  k.nblk = a.per < all - k.blk0 ? k.blk0 + a.per : all;
+  // (sinks in front of the first row's window are before every row; the others are among the window's keys)
+  k.sv = k.shift > 0 ? k.ns : a.sinks;
+  return k;
+}
+
+// Infinities and NaN among the values that rows see, set in their outputs whatever the weights: +inf and -inf in one column
+// make NaN.  Rows `odd` of the wavefront's 32.  A lane keeps a bit for each of them in its columns.
+template <typename T, int OF>
+__device__ __forceinline__ void window_mark(const WindowArgs& a, const WindowPart& part, int r0, int rows, int block, uint32_t odd, int lane) {
+  constexpr int N = (OF + 1) / 2, AHEAD = 8;
+  const WindowKeys keys = window_keys(a, part, rows, block);
+  const char* const v = a.v + part.b * a.vB + part.tile.krow * a.vT + part.h / (int)a.group * a.vH;
+  const int first = keys.blk0 * block, last = keys.nblk * block < keys.nv ? keys.nblk * block : keys.nv;
+  const int64_t hi = (int64_t)keys.p0 + r0 - keys.shift;  // the last counted key that row 0 sees
+  uint32_t up[N], down[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) up[i] = down[i] = 0u;
+  auto below = [](int64_t n) -> uint32_t { return n <= 0 ? 0u : ~0u >> (n < 32 ? 32 - n : 0); };  // the n lowest bits
+#pragma unroll 1
+  for (int k = first; k < last; k += AHEAD) {
+    float x[AHEAD][N];
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) {
+      const int c = k + t < last ? k + t : last - 1;
+      const T* row = reinterpret_cast<const T*>(v + (int64_t)(c < keys.ns ? c : c + keys.shift) * a.vT);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[t][i] = lane + 64 * i < a.dv ? Num<T>::load(row + lane + 64 * i) : 0.f;
     }
-    float s = 0.f;
-    const T* kr = reinterpret_cast<const T*>(k + j * a.kT);
 #pragma unroll
-    for (int i = 0; i < MOST; ++i)
-      if (lane + 64 * i < a.d) s = __builtin_fmaf(x[i], Num<T>::load(kr + lane + 64 * i), s);
-    s = wave_sum(s);
-    if (s == -INFINITY) continue;
-    const float top = fmaxf(m, s);
-    const float old = l * __builtin_amdgcn_exp2f((m - top) * a.scale), add = __builtin_amdgcn_exp2f((s - top) * a.scale);
-    l = old + add;
-    m = top;
-    const float f = old / l, g = add / l;
-    const T* vr = reinterpret_cast<const T*>(v + j * a.vT);
+    for (int t = 0; t < AHEAD; ++t) {
+      const int64_t c = k + t < last ? k + t : last - 1;
+      const uint32_t see = odd & ~below(c - hi) & (c < keys.sv ? ~0u : below(c + a.window - hi));
 #pragma unroll
-    for (int i = 0; i < MOST; ++i)
-      if (lane + 64 * i < a.dv) o[i] = __builtin_fmaf(Num<T>::load(vr + lane + 64 * i), g, o[i] * f);
+      for (int i = 0; i < N; ++i) {
+        if (!(x[t][i] < INFINITY)) up[i] |= see;  // (NaN: both)
+        if (!(x[t][i] > -INFINITY)) down[i] |= see;
+      }
+    }
   }
+  auto store = [&](auto* to, int64_t step) {
 #pragma unroll
-  for (int i = 0; i < MOST; ++i)
-    if (lane + 64 * i < a.dv) Num<T>::store(reinterpret_cast<T*>(out) + lane + 64 * i, o[i]);
+    for (int i = 0; i < N; ++i) {
+      const int col = lane + 64 * i;
+      if (col >= a.dv) continue;
+      for (uint32_t rest = up[i] | down[i]; rest != 0; rest &= rest - 1) {
+        const int r = __builtin_ctz(rest);
+        const float x = (up[i] & down[i]) >> r & 1 ? NAN : (up[i] >> r & 1 ? INFINITY : -INFINITY);
+        Num<std::remove_pointer_t<decltype(to)>>::store(to + r * step + col, x);
+      }
+    }
+  };
+  if (a.splits > 1) {
+    const int64_t row = (part.b * (a.hkv * a.group) + part.h) * a.lq + part.tile.i0 + r0;
+    store(a.part + (row * a.splits + part.range) * a.dv, (int64_t)a.splits * a.dv);
+  } else {
+    char* const out = a.out + part.b * a.oB + (int64_t)(part.tile.qrow + part.tile.i0 + r0) * a.oT + part.h * a.oH;
+    store(reinterpret_cast<T*>(out), a.oT / (int64_t)sizeof(T));
+  }
 }
 
 // Wavefronts per SIMD that registers are given out for.
@@ -243,70 +306,30 @@ constexpr int window_waves() {
   return DP > 128 || DVP > 128 ? 1 : (sizeof(T) == 2 && DP <= 64 && DVP <= 64 ? (NH == 1 ? 4 : 3) : 2);
 }
 
-template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
-__global__ __launch_bounds__(64 * RW * KW)
-__attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP, NH>(), window_waves<T, DP, DVP, NH>())))
-void window_attn_kernel(WindowArgs a) {
+// Rows `left` of the wavefront's 32 in one pass over the tile's keys, stored.  Returns those without a result, which take
+// another mode.  Mode 0 is a function of its own (AGAIN false), so that what the others need costs it no registers.
+template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG, bool AGAIN>
+__device__ __forceinline__ uint32_t window_pass(const WindowArgs& a, char* smem, const WindowPart& own_part, int tid, uint32_t left, int mode_) {
   using F = WindowShape<T, DP, DVP, RW, KW, NH, HG>;
   constexpr int E = F::E, BN = F::BN;
-  __shared__ __attribute__((aligned(16))) char smem[F::LDS_BYTES];
-  // What is the same for a wavefront is told to the compiler, and then computed once for it.
-  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63, hf = lane >> 5, l32 = lane & 31;
+  const int mode = AGAIN ? mode_ : 0;
+  const WindowTile& tile = own_part.tile;
+  const int64_t b = own_part.b;
+  const int w = own_part.w, h = own_part.h, hk = h / (int)a.group, range = own_part.range;
+  const int lane = tid & 63, hf = lane >> 5, l32 = lane & 31;
   const int rw = w % RW, part = w / RW;  // row group, turn at the keys
   const int r0 = 32 * (rw / HG);         // its first row
   const u32x4_t zero4 = {0u, 0u, 0u, 0u};
-
-  // Workgroups are dealt to the 8 XCDs in turn: every XCD takes a run of each kWindowOrder tiles, so that the
-  // heads of a group and neighbouring tiles, which read the same keys, share one L2.
-  uint32_t t = a.first + blockIdx.x;
-  {
-    const uint32_t first = t / kWindowOrder * kWindowOrder;
-    const uint32_t n = a.total - first < kWindowOrder ? a.total - first : kWindowOrder;
-    const uint32_t j = t - first;
-    if ((n & 7) == 0) t = first + (j & 7) * (n >> 3) + (j >> 3);
-  }
-  int range = 0;
-  if constexpr (KW > 1) {
-    if (a.splits > 1) {
-      range = (int)(t % (uint32_t)a.splits);
-      t /= (uint32_t)a.splits;
-    }
-  }
-  WindowTile tile;
-  const uint32_t tl = t % a.tiles;
-  t /= a.tiles;
-  const uint32_t htiles = a.hkv * a.group / HG;
-  const int h = (int)(t % htiles) * HG + rw % HG, hk = h / (int)a.group;
-  const int64_t b = t / htiles;
-  if (a.cu_q) {
-    const bool work = window_find<F::ROWS>(a, (int)tl, lane, tile);
-    if (h < HG && tl <= a.nseq && w == RW * KW - 1 && !window_offsets_ok(a, tl)) *a.flag = 1;
-    if (!work) return;
-  } else {
-    tile.i0 = (int)(a.tiles - 1 - tl) * F::ROWS;  // longest ranges first
-    tile.qrow = tile.krow = 0;
-    tile.ql = a.lq;
-    tile.kl = a.lk;
-  }
-  const int kl = tile.kl, qrows = tile.ql - tile.i0 < F::ROWS ? tile.ql - tile.i0 : F::ROWS;
+  const WindowKeys keys = window_keys(a, own_part, F::ROWS, BN);
+  const int qrows = keys.qrows, p0 = keys.p0, ns = keys.ns, shift = keys.shift, nv = keys.nv;
+  const int blk0 = keys.blk0, nblk = keys.nblk;
   const char* const qb = a.q + b * a.qB + (int64_t)(tile.qrow + tile.i0) * a.qT + h * a.qH;
   const char* const kb = a.k + b * a.kB + tile.krow * a.kT + hk * a.kH;
   const char* const vb = a.v + b * a.vB + tile.krow * a.vT + hk * a.vH;
   char* const ob = a.out + b * a.oB + (int64_t)(tile.qrow + tile.i0) * a.oT + h * a.oH;
 
-  // positions of the tile's first and last row; keys of v: v < ns ? v : v + shift
-  const int p0 = kl - tile.ql + tile.i0, p1 = p0 + qrows - 1;
-  const int64_t begin = (int64_t)p0 - a.window + 1;
-  const int start = begin > 0 ? (int)begin : 0;
-  const int ns = kl > 0 ? (a.sinks < start ? a.sinks : start) : 0;
-  const int shift = start - ns;
-  const int nv = kl > 0 && p1 >= 0 ? p1 + 1 - shift : 0;
-  const int all_blocks = (nv + BN - 1) / BN;
-  const int blk0 = range * a.per, nblk = a.per < all_blocks - blk0 ? blk0 + a.per : all_blocks;  // the workgroup's
-  // What a row sees of the counted keys: lo .. hi (its window), and v < sv (sinks; all of those in front of the
-  // first row's window are before every row, the others are among the window's keys and cut off at hi).
-  const int sv = shift > 0 ? ns : a.sinks;
+  // What a row sees of the counted keys: lo .. hi (its window), and v < sv (sinks; cut off at hi).
+  const int sv = keys.sv;
   auto row_lo = [&](int p) -> int {
     const int64_t x = (int64_t)p - a.window + 1 - shift;
     return x > 0 ? (int)x : 0;
@@ -485,7 +508,7 @@ void window_attn_kernel(WindowArgs a) {
       const float mn = grown ? mx : m;
       const float to = mn == -INFINITY ? 0.f : mn * a.scale;
       if (__any(m > -INFINITY)) {  // (nothing is summed before a row's first keys)
-        const float corr = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(window_ratio(m, mn, a.scale)) : 1.f;
+        const float corr = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(window_ratio(m, mn, a.scale, mode == 2)) : 1.f;
         l *= corr;
 #pragma unroll
         for (int e = 0; e < F::OF; ++e)
@@ -495,15 +518,15 @@ void window_attn_kernel(WindowArgs a) {
       m = mn;
       sh = to;
     }
-    const bool large = fabsf(sh) > kWindowLarge;
+    const bool large = mode == 2 || fabsf(sh) > kWindowLarge;
     if (__any(large)) {
-      const float less = large ? m : 0.f;
+      const float less = large && m > -INFINITY ? m : 0.f;
 #pragma unroll
       for (int x = 0; x < NH; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[x][r] -= less;
     }
-    const float off = large ? 0.f : sh;
+    const float off = large ? (mode == 2 ? kWindowDown : 0.f) : sh;
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
 #pragma unroll
@@ -593,6 +616,12 @@ void window_attn_kernel(WindowArgs a) {
     if (here) weigh(blk);
     const bool then = sees(blk + 1);
     meet();
+    if constexpr (AGAIN) {
+      u32x4_t* const p = reinterpret_cast<u32x4_t*>(vbuf) + tid;
+#pragma unroll 1
+      for (int i = 0; i < F::VL; ++i) p[F::THREADS * i] = finite_or_zero<T>(p[F::THREADS * i]);
+      meet();
+    }
     __builtin_amdgcn_s_setprio(1);
     if (here) gather();
     if (then) scores();
@@ -618,7 +647,9 @@ void window_attn_kernel(WindowArgs a) {
       float top = m;
 #pragma unroll
       for (int x = 1; x < KW; ++x) top = fmaxf(top, js[((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane + 64 * 16 * F::OF]);
-      auto factor = [&](float from) { return from == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(window_ratio(from, top, a.scale)); };
+      auto factor = [&](float from) {
+        return from == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(window_ratio(from, top, a.scale, mode == 2));
+      };
       const float own = factor(m);
       l *= own;
 #pragma unroll
@@ -635,26 +666,10 @@ void window_attn_kernel(WindowArgs a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) oacc[e][r] = __builtin_fmaf(o[64 * (16 * e + r)], f, oacc[e][r]);
       }
-      if (a.splits > 1) {  // this range's part of the rows
-        if (!row_ok) return;
-        const int64_t at = ((b * (a.hkv * a.group) + h) * a.lq + tile.i0 + rloc) * a.splits + range;
-#pragma unroll
-        for (int e = 0; e < F::OF; ++e)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int col = 32 * e + 8 * j + 4 * hf;
-            if (col < a.dv)
-              *reinterpret_cast<f32x4_t*>(a.part + at * a.dv + col) =
-                  f32x4_t{oacc[e][4 * j], oacc[e][4 * j + 1], oacc[e][4 * j + 2], oacc[e][4 * j + 3]};
-          }
-        if (hf == 0) {
-          a.ml[2 * at] = top;
-          a.ml[2 * at + 1] = l;
-        }
-        return;
-      }
+      m = top;
     }
   }
+  uint32_t again = 0;
   if (part == 0) {
     if (__any(l == 0.f)) {  // rows that see nothing, or only scores of -inf
 #pragma unroll
@@ -669,39 +684,142 @@ void window_attn_kernel(WindowArgs a) {
     for (int e = 0; e < F::OF; ++e)
 #pragma unroll
       for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(oacc[e][r], 0.f, odd);
-    const uint64_t again = __ballot(row_ok && l > 0.f && l < INFINITY && odd != 0.f);
-    const bool mine_again = (again >> l32 | again >> (l32 + 32)) & 1;
-    if (row_ok && !mine_again) {
-      char* orow = ob + rloc * a.oT;
-      auto put = [&](int e, int j) {
-        const int col = 32 * e + 8 * j + 4 * hf;
-        float x[4];
+    const uint64_t bad = __ballot(row_ok && l > 0.f && l < INFINITY && odd != 0.f);
+    again = mode < kWindowLast<T> ? ((uint32_t)bad | (uint32_t)(bad >> 32)) & left : 0u;
+    if (row_ok && (left & ~again) >> l32 & 1) {
+      if constexpr (KW > 1) {
+        if (a.splits > 1) {  // this range's part of the row: its own mean, and what that counts for
+          const int64_t at = ((b * (a.hkv * a.group) + h) * a.lq + tile.i0 + rloc) * a.splits + range;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = oacc[e][4 * j + i] * inv;
-        if constexpr (E == 4) {
-          *reinterpret_cast<u32x4_any_t*>(orow + E * col) =
-              u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
-        } else {
-          *reinterpret_cast<u32x2_any_t*>(orow + E * col) = u32x2_t{window_pack<T>(x[0], x[1]), window_pack<T>(x[2], x[3])};
+          for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int col = 32 * e + 8 * j + 4 * hf;
+              if (col < a.dv)
+                *reinterpret_cast<f32x4_t*>(a.part + at * a.dv + col) =
+                    f32x4_t{oacc[e][4 * j] * inv, oacc[e][4 * j + 1] * inv, oacc[e][4 * j + 2] * inv, oacc[e][4 * j + 3] * inv};
+            }
+          if (hf == 0) {
+            if (mode == 2) {  // as the weights of the other modes
+              const float c = m * a.scale;
+              l *= __builtin_amdgcn_exp2f(kWindowDown + (fabsf(c) > kWindowLarge ? 0.f : __builtin_fmaf(m, a.scale, -c)));
+            }
+            a.ml[2 * at] = m;
+            a.ml[2 * at + 1] = l;
+          }
         }
-      };
-      if (a.dv == 32 * F::OF) {
+      }
+      if (KW == 1 || a.splits == 1) {
+        char* orow = ob + rloc * a.oT;
+        auto put = [&](int e, int j) {
+          const int col = 32 * e + 8 * j + 4 * hf;
+          float x[4];
 #pragma unroll
-        for (int e = 0; e < F::OF; ++e)
+          for (int i = 0; i < 4; ++i) x[i] = oacc[e][4 * j + i] * inv;
+          if constexpr (E == 4) {
+            *reinterpret_cast<u32x4_any_t*>(orow + E * col) =
+                u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+          } else {
+            *reinterpret_cast<u32x2_any_t*>(orow + E * col) = u32x2_t{window_pack<T>(x[0], x[1]), window_pack<T>(x[2], x[3])};
+          }
+        };
+        if (a.dv == 32 * F::OF) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) put(e, j);
-      } else {
+          for (int e = 0; e < F::OF; ++e)
 #pragma unroll
-        for (int e = 0; e < F::OF; ++e)
+            for (int j = 0; j < 4; ++j) put(e, j);
+        } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (32 * e + 8 * j + 4 * hf < a.dv) put(e, j);
+          for (int e = 0; e < F::OF; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (32 * e + 8 * j + 4 * hf < a.dv) put(e, j);
+        }
       }
     }
-    for (uint64_t rest = (again | again >> 32) & 0xffffffffull; rest != 0; rest &= rest - 1) {
-      const int r = r0 + __builtin_ctzll(rest);
-      window_row<T>(a, qb + r * a.qT, kb, vb, ob + r * a.oT, p0 + r, kl, lane);
+  }
+  return again;
+}
+
+// The part of wavefront w in workgroup `at` of the call; false where there is none.
+template <int ROWS, int RW, int KW, int HG>
+__device__ __forceinline__ bool window_part(const WindowArgs& a, uint32_t at, int w, int lane, WindowPart& p) {
+  // Workgroups are dealt to the 8 XCDs in turn: every XCD takes a run of each kWindowOrder tiles, so that the
+  // heads of a group and neighbouring tiles, which read the same keys, share one L2.
+  uint32_t t = at;
+  {
+    const uint32_t first = t / kWindowOrder * kWindowOrder;
+    const uint32_t n = a.total - first < kWindowOrder ? a.total - first : kWindowOrder;
+    const uint32_t j = t - first;
+    if ((n & 7) == 0) t = first + (j & 7) * (n >> 3) + (j >> 3);
+  }
+  p.w = w;
+  p.range = 0;
+  if constexpr (KW > 1) {
+    if (a.splits > 1) {
+      p.range = (int)(t % (uint32_t)a.splits);
+      t /= (uint32_t)a.splits;
     }
+  }
+  const uint32_t tl = t % a.tiles;
+  t /= a.tiles;
+  const uint32_t htiles = a.hkv * a.group / HG;
+  p.h = (int)(t % htiles) * HG + w % RW % HG;
+  p.b = t / htiles;
+  if (a.cu_q) {
+    const bool work = window_find<ROWS>(a, (int)tl, lane, p.tile);
+    if (p.h < HG && tl <= a.nseq && w == RW * KW - 1 && !window_offsets_ok(a, tl)) *a.flag = 1;
+    return work;
+  }
+  p.tile.i0 = (int)(a.tiles - 1 - tl) * ROWS;  // longest ranges first
+  p.tile.qrow = p.tile.krow = 0;
+  p.tile.ql = a.lq;
+  p.tile.kl = a.lk;
+  return true;
+}
+
+template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
+__global__ __launch_bounds__(64 * RW * KW)
+__attribute__((amdgpu_waves_per_eu(window_waves<T, DP, DVP, NH>(), window_waves<T, DP, DVP, NH>())))
+void window_attn_kernel(WindowArgs a) {
+  using F = WindowShape<T, DP, DVP, RW, KW, NH, HG>;
+  __shared__ __attribute__((aligned(16))) char smem[F::LDS_BYTES];
+  __shared__ int again_in[2];  // whether a row is left after mode 0, 1
+  uint32_t odd;                // rows that were not finite in mode 0
+  {
+    const int tid = threadIdx.x;
+    WindowPart p;  // (the wavefront's number is the same for its lanes, as the compiler is told)
+    if (!window_part<F::ROWS, RW, KW, HG>(a, a.first + blockIdx.x, __builtin_amdgcn_readfirstlane(tid >> 6), tid & 63, p)) return;
+    if (tid < 2) again_in[tid] = 0;
+    odd = window_pass<T, DP, DVP, RW, KW, NH, HG, false>(a, smem, p, tid, ~0u, 0);
+    if (odd != 0 && (tid & 63) == 0) again_in[0] = 1;
+    __syncthreads();
+    if (again_in[0] == 0) return;
+  }
+  // Arguments, thread and part are found again, so that none of them is kept in registers through the first pass.
+  auto* at = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  uint32_t block = blockIdx.x;
+  int tid = threadIdx.x;
+  asm volatile("" : "+s"(at), "+s"(block));
+  asm volatile("" : "+v"(tid));
+  uint32_t words[sizeof(WindowArgs) / 4];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(WindowArgs) / 4); ++i) words[i] = at[i];
+  const WindowArgs again = __builtin_bit_cast(WindowArgs, words);
+  WindowPart p;
+  window_part<F::ROWS, RW, KW, HG>(again, again.first + block, __builtin_amdgcn_readfirstlane(tid >> 6), tid & 63, p);
+  uint32_t left = odd;
+#pragma unroll 1
+  for (int mode = 1; mode <= kWindowLast<T>; ++mode) {
+    left = window_pass<T, DP, DVP, RW, KW, NH, HG, true>(again, smem, p, tid, left, mode);
+    if (mode == kWindowLast<T>) break;
+    if (left != 0 && (tid & 63) == 0) again_in[mode] = 1;
+    __syncthreads();
+    if (again_in[mode] == 0) break;
+  }
+  if (odd != 0) {
+    __builtin_amdgcn_s_waitcnt(0);  // the rows' stores come first
+    window_mark<T, F::OF>(again, p, 32 * (p.w % RW / HG), F::ROWS, F::BN, odd, tid & 63);
   }
 }
 
@@ -717,26 +835,23 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
   const float* const ml = a.ml + 2 * (int64_t)row * a.splits;
   const float* const part = a.part + (int64_t)row * a.splits * a.dv + 4 * lane;
   const float m = lane < a.splits ? ml[2 * lane] : -INFINITY, sum = lane < a.splits ? ml[2 * lane + 1] : 0.f;
-  const float top = wave_max(m), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(window_ratio(m, top, a.scale));
-  float l = 0.f;
-  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int x = 0; x < a.splits; ++x) {
-    const float fx = __shfl(f, x, 64);
-    l = __builtin_fmaf(__shfl(sum, x, 64), fx, l);
-    if (4 * lane < a.dv) o += *reinterpret_cast<const f32x4_t*>(part + (int64_t)x * a.dv) * fx;
-  }
-  char* const out = a.out + b * a.oB + r * a.oT + h * a.oH;
-  const float odd = __builtin_fmaf(o[0], 0.f, o[1] * 0.f) + __builtin_fmaf(o[2], 0.f, o[3] * 0.f);
-  if (l > 0.f && l < INFINITY && __any(odd != 0.f)) {  // not finite over a finite sum
-    const uint32_t hk = h / a.group;
-    window_row<T>(a, a.q + b * a.qB + r * a.qT + h * a.qH, a.k + b * a.kB + hk * a.kH, a.v + b * a.vB + hk * a.vH, out,
-                  a.lk - a.lq + r, a.lk, lane);
-    return;
-  }
-  if (4 * lane >= a.dv) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  f32x4_t mean[kWindowRanges];  // on their way while the shares are found
 #pragma unroll
-  for (int i = 0; i < 4; ++i) Num<T>::store(reinterpret_cast<T*>(out) + 4 * lane + i, l == 0.f ? 0.f : o[i] * inv);
+  for (int x = 0; x < kWindowRanges; ++x)
+    if (x < a.splits && 4 * lane < a.dv) mean[x] = *reinterpret_cast<const f32x4_t*>(part + (int64_t)x * a.dv);
+  const float top = wave_max(m);
+  // what each range's mean counts for
+  const float own = m == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(window_ratio(m, top, a.scale, false));
+  const float l = wave_sum(own);
+  const float share = l == 0.f ? 0.f : own / l;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < kWindowRanges; ++x)
+    if (x < a.splits) o += mean[x] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), x));
+  if (4 * lane >= a.dv) return;
+  char* const out = a.out + b * a.oB + r * a.oT + h * a.oH;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) Num<T>::store(reinterpret_cast<T*>(out) + 4 * lane + i, o[i]);
 }
 
 template <typename T, int DP, int DVP, int RW, int KW, int NH, int HG>
