@@ -6,8 +6,8 @@
 // window first, so that nothing else is loaded or looked up.  They are cut into chunks, a workgroup takes
 // a chunk of one key/value head for all the query heads that share it, and a second kernel joins the
 // chunks in their order (none where no sequence can have more than one):
-//   chunk:  m = max s_v, l = sum exp2(c (s_v - m)), O = sum exp2(c (s_v - m)) V_v,  s_v = q.k_v, c = scale log2 e
-//   join:   M = max m_c, o = sum_c exp2(c (m_c - M)) O_c / sum_c exp2(c (m_c - M)) l_c
+//   chunk:  m = max s_v, l = sum exp2(c (s_v - m)), o = sum exp2(c (s_v - m)) V_v / l,  s_v = q.k_v, c = scale log2 e
+//   join:   M = max m_c, L_c = exp2(c (m_c - M)) l_c, o = sum_c (L_c / sum L) o_c
 // The difference is taken before the product with c: it is exact next to the maximum however large the scores are, where
 // a fused c s_v - round(c m) would leave the rounding of c m in every weight, powers of two that overflow from 2^31 on.
 // Batch invariance: the chunks follow from n alone, so a sequence's bits are the same in every batch.
@@ -22,8 +22,9 @@
 //     elements (16 bytes; 8 with 64-wide heads) of value rows 8q .. 8q + 7 at column W m -- whole
 //     rows, contiguous over the lanes -- and turns its own 8 x W block with byte permutes: row m of output
 //     block t is column W m + t.
-// Weights are kept 2^-31 times their size where the type has float's range, so that sums of values near its end
-// stay finite (of fewer than 2^31 keys none can pass the largest value); fp16's cannot get there.
+// Parts are joined as means, which stay in the range of their values; a wavefront whose own sum has left it goes through its
+// keys once more, with weights so much smaller that as many of the largest values stay in it (always so, small values would
+// lose bits).  Sums of fp16 values cannot get there.
 // 16-bit weights go in as a rounded part and the rounded rest (two MFMAs), which leaves an error of
 // 2^-16 (bf16) instead of 2^-8 where the matrix cores have the time.
 //
@@ -163,7 +164,6 @@ void paged_chunk_kernel(PagedArgs a) {
   constexpr int W = E == 2 && DVP <= 64 ? 4 : VEC;      // elements of a value load
   constexpr int NB = DVP / (16 * W), NT = NB * W;       // value blocks of a row; 16-column output blocks
   constexpr int VD = W * E / 4;                         // dwords of a value load
-  constexpr float kDown = std::is_same<T, f16_t>::value ? 1.f : 0x1p-31f;
   extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][cols][DVP] O, then [4][cols][2] m, l
   __shared__ __attribute__((aligned(16))) int64_t offs[4][2][32];
   __shared__ int bad_page;
@@ -233,131 +233,146 @@ void paged_chunk_kernel(PagedArgs a) {
     return lane < 32 ? id * a.kP + at * a.kS : id * a.vP + at * a.vS;
   };
 
-  // of query m16: largest product so far, the same or 0 where that is -inf, sum (of this lane's keys)
-  float m = -INFINITY, from = 0.f, l = 0.f;
-  f32x4_t acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const char* const kb = a.kc + hk * a.kH;
   const char* const vb = a.vc + hk * a.vH;
-
-  int64_t off = w < tiles ? lookup(w) : 0;
-  for (int tile = w; tile < tiles; tile += 4) {
-    offs[w][lane >> 5][lane & 31] = off;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    u32x4_t kf[2][KS];
+  // of query m16: largest product so far, the same or 0 where that is -inf, sum (of this lane's keys)
+  float m, from, l;
+  f32x4_t acc[NT];
+  float down = 0.f;  // powers of two that are off the weights
+  for (;;) {
+    m = -INFINITY, from = 0.f, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const char* p = kb + offs[w][0][8 * (m16 >> 2) + 4 * i + (m16 & 3)];
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    int64_t off = w < tiles ? lookup(w) : 0;
+    for (int tile = w; tile < tiles; tile += 4) {
+      offs[w][lane >> 5][lane & 31] = off;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      u32x4_t kf[2][KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d0 = KW * s + VEC * q4;
-        kf[i][s] = d0 < a.d ? load_16(p + E * d0) : zero4;
-      }
-    }
-    uint32_t vf[NB][8][VD];
+      for (int i = 0; i < 2; ++i) {
+        const char* p = kb + offs[w][0][8 * (m16 >> 2) + 4 * i + (m16 & 3)];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const char* p = vb + offs[w][1][8 * q4 + j];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int e0 = 16 * W * n + W * m16;
-        if constexpr (VD == 4) {
-          const u32x4_t x = e0 < a.dv ? load_16(p + E * e0) : zero4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vf[n][j][i] = x[i];
-        } else {
-          const u32x2_t x = e0 < a.dv ? *reinterpret_cast<const u32x2_any_t*>(p + E * e0) : u32x2_t{0u, 0u};
-          vf[n][j][0] = x[0];
-          vf[n][j][1] = x[1];
+        for (int s = 0; s < KS; ++s) {
+          const int d0 = KW * s + VEC * q4;
+          kf[i][s] = d0 < a.d ? load_16(p + E * d0) : zero4;
         }
       }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (tile + 4 < tiles) off = lookup(tile + 4);
-
-    f32x4_t sc[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) mfma16<T>(sc[i], kf[i][s], qf[s]);
-    }
-    float p[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = sc[j >> 2][j & 3];
-    const int left = nkeys - 32 * tile;
-    if (left < 32) {
+      uint32_t vf[NB][8][VD];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const bool in = 8 * q4 + j < left;
-        p[j] = in ? p[j] : -INFINITY;
+        const char* p = vb + offs[w][1][8 * q4 + j];
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < NB; ++n) {
+          const int e0 = 16 * W * n + W * m16;
+          if constexpr (VD == 4) {
+            const u32x4_t x = e0 < a.dv ? load_16(p + E * e0) : zero4;
 #pragma unroll
-          for (int i = 0; i < VD; ++i) vf[n][j][i] = in ? vf[n][j][i] : 0u;
-      }
-    }
-    float mx = p[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, p[j]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__any(mx > m)) {
-      const float mn = fmaxf(m, mx);
-      const float corr = mx > m ? __builtin_amdgcn_exp2f((m - mn) * a.scale) : 1.f;
-      l *= corr;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] *= corr;
-      m = mn;
-      from = mn == -INFINITY ? 0.f : mn;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f((p[j] - from) * a.scale) * kDown;
-      l += p[j];
-    }
-    if constexpr (E == 4) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int t = 0; t < W; ++t)
-            acc[W * n + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[n][j][t]), p[j], acc[W * n + t], 0, 0, 0);
-    } else {
-      u32x4_t hi, lo;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        hi[i] = pack_pair<T>(p[2 * i], p[2 * i + 1]);
-        lo[i] = pack_pair<T>(p[2 * i] - Num<T>::from_bits(hi[i] & 0xffffu), p[2 * i + 1] - Num<T>::from_bits(hi[i] >> 16));
-      }
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int t = 0; t < W; ++t) {
-          u32x4_t va;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            va[i] = __builtin_amdgcn_perm(vf[n][2 * i + 1][t >> 1], vf[n][2 * i][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-          mfma16<T>(acc[W * n + t], va, hi);
-          mfma16<T>(acc[W * n + t], va, lo);
+            for (int i = 0; i < 4; ++i) vf[n][j][i] = x[i];
+          } else {
+            const u32x2_t x = e0 < a.dv ? *reinterpret_cast<const u32x2_any_t*>(p + E * e0) : u32x2_t{0u, 0u};
+            vf[n][j][0] = x[0];
+            vf[n][j][1] = x[1];
+          }
         }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (tile + 4 < tiles) off = lookup(tile + 4);
+
+      f32x4_t sc[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) mfma16<T>(sc[i], kf[i][s], qf[s]);
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = sc[j >> 2][j & 3];
+      const int left = nkeys - 32 * tile;
+      if (left < 32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = 8 * q4 + j < left;
+          p[j] = in ? p[j] : -INFINITY;
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < VD; ++i) vf[n][j][i] = in ? vf[n][j][i] : 0u;
+        }
+      }
+      float mx = p[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, p[j]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      if (__any(mx > m)) {
+        const float mn = fmaxf(m, mx);
+        const float corr = mx > m ? __builtin_amdgcn_exp2f((m - mn) * a.scale) : 1.f;
+        l *= corr;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] *= corr;
+        m = mn;
+        from = mn == -INFINITY ? 0.f : mn;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j] - from, a.scale, -down));
+        l += p[j];
+      }
+      if constexpr (E == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int t = 0; t < W; ++t)
+              acc[W * n + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[n][j][t]), p[j], acc[W * n + t], 0, 0, 0);
+      } else {
+        u32x4_t hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          hi[i] = pack_pair<T>(p[2 * i], p[2 * i + 1]);
+          lo[i] = pack_pair<T>(p[2 * i] - Num<T>::from_bits(hi[i] & 0xffffu), p[2 * i + 1] - Num<T>::from_bits(hi[i] >> 16));
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int t = 0; t < W; ++t) {
+            u32x4_t va;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              va[i] = __builtin_amdgcn_perm(vf[n][2 * i + 1][t >> 1], vf[n][2 * i][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+            mfma16<T>(acc[W * n + t], va, hi);
+            mfma16<T>(acc[W * n + t], va, lo);
+          }
+      }
     }
+    if constexpr (std::is_same<T, f16_t>::value) break;
+    float odd = 0.f;  // NaN where a sum of the query is not finite
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) odd = __builtin_fmaf(acc[t][i], 0.f, odd);
+    odd += __shfl_xor(odd, 16, 64);
+    odd += __shfl_xor(odd, 32, 64);
+    const bool past = odd != 0.f && down == 0.f && m16 < cols;
+    if (!__any(past)) break;
+    if (past) down = (float)(32 - __builtin_clz((uint32_t)span.chunk / 4));  // (a wavefront has a quarter of the chunk's keys)
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   if (bad) bad_page = 1;
 
-  // the four wavefronts' results, joined in order
+  // the four wavefronts' results: means and what they count for, joined in order
   float* const os = reinterpret_cast<float*>(smem);
   float* const mls = os + 4 * cols * DVP;
   if (m16 < cols) {
     if (q4 == 0) {
       mls[2 * (w * cols + m16)] = m;
-      mls[2 * (w * cols + m16) + 1] = l;
+      mls[2 * (w * cols + m16) + 1] = l * __builtin_amdgcn_exp2f(down);
     }
     float* o = os + (w * cols + m16) * DVP;
 #pragma unroll
@@ -367,7 +382,7 @@ void paged_chunk_kernel(PagedArgs a) {
 #pragma unroll
         for (int t = 0; t < W; t += 4)
           *reinterpret_cast<f32x4_t*>(o + 16 * W * n + W * (4 * q4 + i) + t) =
-              f32x4_t{acc[W * n + t][i], acc[W * n + t + 1][i], acc[W * n + t + 2][i], acc[W * n + t + 3][i]};
+              f32x4_t{acc[W * n + t][i], acc[W * n + t + 1][i], acc[W * n + t + 2][i], acc[W * n + t + 3][i]} * inv;
   }
   __syncthreads();
   const bool void_ = bad_page != 0;
@@ -380,19 +395,20 @@ void paged_chunk_kernel(PagedArgs a) {
     for (int x = 0; x < 4; ++x) M = fmaxf(M, mls[2 * (x * cols + col)]);
     const float base = M == -INFINITY ? 0.f : M;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
+    float f[4], sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const float f = __builtin_amdgcn_exp2f((mls[2 * (x * cols + col)] - base) * a.scale);
-      sum = __builtin_fmaf(mls[2 * (x * cols + col) + 1], f, sum);
-      o += *reinterpret_cast<const f32x4_t*>(os + (x * cols + col) * DVP + e) * f;
+      f[x] = mls[2 * (x * cols + col) + 1] * __builtin_amdgcn_exp2f((mls[2 * (x * cols + col)] - base) * a.scale);
+      sum += f[x];
     }
+    const float share = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o += *reinterpret_cast<const f32x4_t*>(os + (x * cols + col) * DVP + e) * (f[x] * share);
     const int64_t row = b * heads + h0 + col;
     if (a.chunks == 1) {
-      const float inv = void_ || sum == 0.f ? 0.f : 1.f / sum;
       T* dst = reinterpret_cast<T*>(a.out) + row * a.dv + e;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) Num<T>::store(dst + x, inv == 0.f ? 0.f : o[x] * inv);
+      for (int x = 0; x < 4; ++x) Num<T>::store(dst + x, void_ ? 0.f : o[x]);
     } else {
       const int64_t at = row * a.chunks + c;
       *reinterpret_cast<f32x4_t*>(a.part + at * a.dv + e) = o;
@@ -408,10 +424,9 @@ void paged_chunk_kernel(PagedArgs a) {
 // ... for four columns; the splits are then added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-  __shared__ float top;
+  __shared__ float top, total;
   __shared__ int void_row;
   __shared__ __attribute__((aligned(16))) f32x4_t so[256];
-  __shared__ float sl[256];
   const int tid = threadIdx.x;
   const int64_t row = a.first + blockIdx.x;
   const float* ml = a.ml + 2 * row * a.chunks;
@@ -439,15 +454,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     const bool there = tid < span.chunks;
     const float mx = wave_max(there ? m0 : -INFINITY);
     const bool bad = __any(there && l0 == -1.f);
+    const float all = wave_sum(there ? l0 * __builtin_amdgcn_exp2f((m0 - (mx == -INFINITY ? 0.f : mx)) * a.scale) : 0.f);
     if (tid == 0) {
-      top = mx;
-      void_row = bad;
+      top = mx == -INFINITY ? 0.f : mx;
+      total = all;
+      void_row = bad || all == 0.f;
     }
   }
   __syncthreads();
-  const float base = top == -INFINITY ? 0.f : top;
+  const float base = top, sum = total;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
   if (split < splits)
     for (int c = split; c < span.chunks; c += splits) {
       if (c != split) {
@@ -455,22 +471,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
         ls = ml[2 * c + 1];
         os = *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * a.dv + 4 * piece);
       }
-      const float f = __builtin_amdgcn_exp2f((ms - base) * a.scale);
-      sum = __builtin_fmaf(ls, f, sum);
-      o += os * f;
+      o += os * (ls * __builtin_amdgcn_exp2f((ms - base) * a.scale) / sum);  // (of one chunk 1 exactly)
     }
   so[tid] = o;
-  sl[tid] = sum;
   __syncthreads();
   if (split == 0) {
     const int filled = span.chunks < splits ? span.chunks : splits;
-    for (int s = 1; s < filled; ++s) {
-      o += so[s * pieces + piece];
-      sum += sl[s * pieces + piece];
-    }
-    const float inv = void_row || sum == 0.f ? 0.f : 1.f / sum;
+    for (int s = 1; s < filled; ++s) o += so[s * pieces + piece];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) Num<T>::store(dst + 4 * piece + x, inv == 0.f ? 0.f : o[x] * inv);
+    for (int x = 0; x < 4; ++x) Num<T>::store(dst + 4 * piece + x, void_row ? 0.f : o[x]);
   }
 }
 

@@ -198,3 +198,39 @@ def test_a_scale_of_zero_and_infinities(dtype):
             assert_within(out[:, 0], parts[0], torch.nan_to_num(attention_bound(dtype, *parts, 20, *prompt_rounding(dtype)), 0.0))
         for r in (0, 2, 3):
             assert bool(torch.isnan(token(q[r], k, v, scale=0.0)).all()) == (r > 0 or bad is not None)
+
+
+@pytest.mark.parametrize("dtype, down", [(BF16, 117), (F32, 117), (F16, 6)])
+@pytest.mark.parametrize("n", [1, 40, 700, 2500])
+def test_token_attention_of_small_values(dtype, down, n):
+    """Equal weights: the mean of values near the type's smallest normal numbers, down to its own rounding.  (Without the
+    1e-30 that the general bound adds.  Sums of n products in 32 bits, their mean and the shares of its parts: 2 (n + 8) 2^-24
+    of the mean magnitude; products below 2^-126 lose 2^-149 each.)"""
+    q = torch.zeros(3, 64, dtype=dtype)
+    k, v = randn(n, 1, 64, seed=n, dtype=dtype), randn(n, 1, 64, seed=n + 1, dtype=F32)
+    v = ((v + v.sign() / 16) * 2.0**-down).to(dtype)
+    o = v[:, 0].double().mean(0)
+    bound = HALF[dtype] * o.abs() + 2 * (n + 8) * 2.0**-24 * v[:, 0].double().abs().mean(0) + 2.0**-149
+    assert_within(token(q, k, v), o.expand(3, 64), bound.expand(3, 64))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n", [40, 700, 2500, 40000])
+def test_token_attention_of_the_largest_and_the_smallest_values(dtype, n):
+    """Columns whose sums pass the range, in some chunks and not in others, beside columns of small values; each query by itself,
+    one of which hardly sees the large values (weights below 2^-400).  Sums that pass the range are of weights 2^-9 times their
+    size at most (256 keys of a wavefront): products that lose 2^-150 leave 2^-141 in the means."""
+    d = 64
+    q, k = torch.zeros(2, d, dtype=dtype), torch.zeros(n, 1, d, dtype=dtype)
+    small = float(torch.tensor(1.2345 * 2.0**-117, dtype=dtype))
+    v = torch.full((n, 1, d), small, dtype=dtype)
+    large = torch.arange(n) < max(20, n // 3)
+    v[large, 0, ::2] = 0.96 * torch.finfo(dtype).max
+    k[large, 0, 0] = -300.0
+    q[1, 0] = 8.0  # scores of -300 at the large values
+    out = token(q, k, v).double().cpu()
+    o = v[:, 0].double().mean(0)
+    relative = HALF[dtype] + 2 * (n + 8) * 2.0**-24
+    assert_within(out[:1], o.unsqueeze(0), (relative * o.abs() + 2.0**-141).unsqueeze(0))
+    want = torch.full((1, d), small, dtype=torch.float64)
+    assert_within(out[1:], want, relative * want + 2.0**-141)
