@@ -491,7 +491,7 @@ int biops_window_attention_max_head(int dtype);
  * of lq query rows and cu_k[s] .. cu_k[s + 1] of lk key rows (device offsets, int32 or int64, by strides; batch strides
  * unused); rows outside of all sequences become zeros; bad offsets set the flag.  d and dv: multiples of 16 bytes up
  * to biops_window_attention_max_head; unit stride in dim; the scale is finite.  Rows of k and v lie at multiples of 16
- * bytes, at most 2^23 elements apart (BIOPS_ERR_LAYOUT otherwise). */
+ * bytes, at most 2^23 elements apart (BIOPS_ERR_LAYOUT otherwise); strides of dimensions with one element are not used. */
 int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64_t hkv, int64_t lq, int64_t lk, int64_t d, int64_t dv,
                            const void* q, int64_t sqB, int64_t sqT, int64_t sqH, const void* k, int64_t skB, int64_t skT,
                            int64_t skH, const void* v, int64_t svB, int64_t svT, int64_t svH, void* out, int64_t soB,

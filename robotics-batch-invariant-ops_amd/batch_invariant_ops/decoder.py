@@ -522,7 +522,7 @@ _MOST_ROW_STRIDE = 1 << 23  # elements between key rows that the kernel's 32-bit
 def _fetchable(t: torch.Tensor) -> bool:
     """Whether keys or values ``[batch, tokens, heads, dim]`` go straight to LDS: rows at multiples of 16 bytes."""
     vec = 16 // t.element_size()
-    return (t.stride(1) <= _MOST_ROW_STRIDE and t.data_ptr() % 16 == 0
+    return ((t.stride(1) <= _MOST_ROW_STRIDE or t.shape[1] == 1) and t.data_ptr() % 16 == 0
             and all(t.stride(i) % vec == 0 or t.shape[i] == 1 for i in range(3)))
 
 

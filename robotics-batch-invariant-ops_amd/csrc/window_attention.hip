@@ -986,6 +986,10 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   if (!(scale - scale == 0.f)) return fail(BIOPS_ERR_ARG, "biops_window_attention: scale is not finite");
   const int64_t longest = INT64_C(0x7fffffff) - 1024;  // tiles and blocks may round positions up
   if (lq > longest || lk > longest || nseq > longest) return fail(BIOPS_ERR_ARG, "biops_window_attention: more than 2^31 rows");
+  // strides of a single element are never used
+  if (cu_q || nseq == 1) skB = svB = 0;
+  if (lk == 1) skT = svT = 0;
+  if (hkv == 1) skH = svH = 0;
   // a block's rows are addressed by 32-bit offsets
   if (skT < 0 || svT < 0 || skT > (1 << 23) || svT > (1 << 23))
     return fail(BIOPS_ERR_LAYOUT, "biops_window_attention: key and value rows more than 2^23 elements apart");
