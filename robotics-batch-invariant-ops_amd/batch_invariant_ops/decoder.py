@@ -201,6 +201,7 @@ def _rotate(query, key, positions, plan: _RotaryPlan, inverse: bool):
     """Rotated copies of ``query`` and ``key`` (either may be None), leading dimensions [tokens] or
     [batch, tokens]."""
     outs, args = [], []
+    held = []  # copies, until the launch
     some = query if query is not None else key
     for x in (query, key):
         if x is None:
@@ -208,6 +209,7 @@ def _rotate(query, key, positions, plan: _RotaryPlan, inverse: bool):
             args += (0, (None, 0, 0, 0, None, 0, 0, 0))
             continue
         x = _unit_last(x)
+        held.append(x)
         y = torch.empty_like(x)
         if y.stride(-1) != 1 and y.shape[-1] > 1:
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
