@@ -208,7 +208,7 @@ def _rotate(query, key, positions, plan: _RotaryPlan, inverse: bool):
             outs.append(None)
             args += (0, (None, 0, 0, 0, None, 0, 0, 0))
             continue
-        x = _unit_last(x)
+        x = _unit_last(x.resolve_neg())  # (a gradient comes as the engine has it)
         held.append(x)
         y = torch.empty_like(x)
         if y.stride(-1) != 1 and y.shape[-1] > 1:

@@ -85,9 +85,13 @@ struct Rotation {
   int neighbours;
 };
 
-// Rotated copies of [tokens, heads, dim] or [batch, tokens, heads, dim] tensors (either may be undefined); any strides.
+// Rotated copies of [tokens, heads, dim] or [batch, tokens, heads, dim] tensors (either may be undefined); any strides, and
+// lazily negated (a gradient comes as the engine has it).
 std::pair<at::Tensor, at::Tensor> rotated(const at::Tensor& query, const at::Tensor& key, const at::Tensor& p, const Rotation& r, bool inverse) {
-  auto unit = [](const at::Tensor& t) { return !t.defined() || unit_last(t) ? t : t.contiguous(); };
+  auto unit = [](const at::Tensor& x) {
+    const at::Tensor t = x.defined() ? x.resolve_neg() : x;
+    return !t.defined() || unit_last(t) ? t : t.contiguous();
+  };
   auto like = [](const at::Tensor& t) {
     if (!t.defined()) return t;
     at::Tensor y = at::empty_like(t);
