@@ -13,7 +13,8 @@ range: the row it belongs to is zeros (a written row is left out), and the error
 which waits, raises ``RuntimeError``.
 
 Only ``multi_axis_rotary`` has a gradient.  The other functions refuse tensors that require one while
-grad mode is on.
+grad mode is on.  None has a forward-mode derivative or can be recorded by ``torch.jit.trace``: both are
+refused.
 """
 
 from __future__ import annotations
@@ -26,6 +27,7 @@ from collections.abc import Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .moe import _IndexWatch
@@ -116,6 +118,14 @@ def _watch(device: torch.device) -> _CacheWatch:
         watch = _CacheWatch.of(device)
     watch.poll()
     return watch
+
+
+def _refuse_transforms(what: str, *tensors) -> None:
+    """A launch is no operator that a trace records, and a tangent would be lost."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be recorded by torch.jit.trace")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no forward-mode derivative")
 
 
 def _check_tensors(what: str, *tensors) -> torch.device:
@@ -286,6 +296,7 @@ def multi_axis_rotary(
         if out is not None:
             return out
     tensors = (query,) if key is None else (query, key)
+    _refuse_transforms("multi_axis_rotary", *tensors, positions)
     for x in tensors:
         if x.dim() < 2:
             raise ValueError(f"rotary tensors have shape [..., heads, head_dim], got {tuple(x.shape)}")
@@ -376,6 +387,7 @@ def paged_cache_write(
     if module and module.paged_write(key, value, key_cache, value_cache, slots, watch.flag_at):
         watch.after_call()
         return
+    _refuse_transforms("paged_cache_write", key, value, key_cache, value_cache)
     _check_caches(key_cache, value_cache)
     if key.dim() < 2 or value.dim() != key.dim() or key.shape[:-1] != value.shape[:-1]:
         raise ValueError("key and value must have shapes [..., kv_heads, dim] with the same leading dimensions")
@@ -467,6 +479,7 @@ def paged_attention_batch_invariant(
         if out is not None:
             watch.after_call()
             return out
+    _refuse_transforms("paged_attention_batch_invariant", query, key_cache, value_cache)
     _check_caches(key_cache, value_cache)
     if query.dim() != 3:
         raise ValueError(f"query must have shape [batch, heads, head_dim], got {tuple(query.shape)}")
@@ -579,6 +592,7 @@ def sliding_window_attention_batch_invariant(
         out = module.window_attention(query, key, value, 0x7FFFFFFF if window is None else window, sinks, scale, enable_gqa)
         if out is not None:
             return out
+    _refuse_transforms("sliding_window_attention_batch_invariant", query, key, value)
     if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
         raise ValueError("sliding-window attention expects rank-4 query, key, and value")
     if query.dtype != key.dtype or query.dtype != value.dtype:
@@ -640,6 +654,7 @@ def varlen_sliding_window_attention_batch_invariant(
         if out is not None:
             watch.after_call()
             return out
+    _refuse_transforms("varlen_sliding_window_attention_batch_invariant", query, key, value)
     if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
         raise ValueError("varlen attention expects rank-4 query, key, and value")
     if query.shape[0] != 1 or key.shape[0] != 1 or value.shape[0] != 1:

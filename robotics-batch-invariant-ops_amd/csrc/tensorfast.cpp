@@ -5,6 +5,7 @@
 // Python functions then do what is left, and raise the errors.  Optional: without this module they do all.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -33,11 +34,13 @@ int is_long(const at::Tensor& t) { return t.scalar_type() == at::kLong ? 1 : 0; 
 bool unit_last(const at::Tensor& t) { return t.stride(-1) == 1; }
 
 bool needs_grad(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
-// A plain tensor with elements on the current device that needs no gradient here (`grad`: or does).
+// A plain tensor with elements on the current device that needs no gradient here (`grad`: or does) and has no tangent.
 const at::Tensor* take(PyObject* o, c10::DeviceIndex device, bool grad = false) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.is_cuda() || t.layout() != at::kStrided || t.get_device() != device || t.numel() == 0 || t.is_neg()) return nullptr;
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.get_device() != device || t.numel() == 0 || t.is_neg() ||
+      t._fw_grad(0).defined())
+    return nullptr;
   return !grad && needs_grad(t) ? nullptr : &t;
 }
 bool number(PyObject* o, int64_t* v) {
@@ -372,6 +375,7 @@ PyObject* window_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   try {
+    if (at::tracer::impl::is_dispatch_enabled()) Py_RETURN_NONE;  // (refused in Python)
     return F(self, args, n);
   } catch (...) {
     PyErr_Clear();
