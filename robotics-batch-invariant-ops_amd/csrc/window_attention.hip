@@ -143,14 +143,20 @@ __device__ __forceinline__ bool window_find(const WindowArgs& a, int tl, int lan
   }
 }
 
-// Whether sequence i's offsets rise and stay inside the tensors (i = nseq: whether the first one is zero and the last one
-// inside).
+// Whether sequence i's offsets rise and stay inside the tensors (i = nseq: whether the first ones are zero and the last one
+// of the queries inside).
 __device__ __forceinline__ bool window_offsets_ok(const WindowArgs& a, int64_t i) {
   auto q = [&](int64_t x) { return window_offset(a.cu_q, a.cu_q64, a.cu_q_stride, x); };
   auto k = [&](int64_t x) { return window_offset(a.cu_k, a.cu_k64, a.cu_k_stride, x); };
-  if (i == a.nseq) return q(0) == 0 && q(i) <= a.lq;
+  if (i == a.nseq) return q(0) == 0 && k(0) == 0 && q(i) <= a.lq;
   const int64_t ks = k(i), ke = k(i + 1);
   return q(i) <= q(i + 1) && ks >= 0 && ks <= ke && ke <= a.lk;
+}
+
+// The check alone, for calls without query rows or heads.
+__global__ __launch_bounds__(256) void window_offsets_kernel(WindowArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i <= a.nseq && !window_offsets_ok(a, i)) *a.flag = 1;
 }
 
 // DP, DVP: head and value size rounded up to whole fragments; RW row groups of 32 (of HG heads) by KW wavefronts that
@@ -999,8 +1005,9 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
     const int64_t all_v = (int64_t)reinterpret_cast<uintptr_t>(v) | elt * svB | elt * svT | elt * svH;
     if ((all_k | all_v) & 15) return fail(BIOPS_ERR_LAYOUT, "biops_window_attention: keys or values not aligned to 16 bytes");
   }
-  if (hq == 0 || lq == 0 || (!cu_q && nseq == 0)) return BIOPS_OK;
-  if (!q || !out || (lk > 0 && (!k || !v)) || (cu_q && (!cu_k || !flag)))
+  const bool empty = hq == 0 || lq == 0;
+  if (!cu_q && (empty || nseq == 0)) return BIOPS_OK;
+  if ((!empty && (!q || !out || (lk > 0 && (!k || !v)))) || (cu_q && (!cu_k || !flag)))
     return fail(BIOPS_ERR_ARG, "biops_window_attention: null pointer");
   WindowArgs a;
   a.q = static_cast<const char*>(q), a.k = static_cast<const char*>(k), a.v = static_cast<const char*>(v);
@@ -1014,6 +1021,10 @@ extern "C" int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64
   a.flag = flag;
   a.nseq = nseq;
   a.lq = (int)lq, a.lk = (int)lk;
+  if (empty) {
+    hipLaunchKernelGGL(window_offsets_kernel, dim3((unsigned)(nseq / 256 + 1)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    return check_launch("window_offsets_kernel");
+  }
   a.hkv = (uint32_t)hkv, a.group = (uint32_t)(hq / hkv);
   a.d = (int)d, a.dv = (int)dv;
   const int64_t all = INT64_C(0x7fffffff);
