@@ -286,7 +286,8 @@ def multi_axis_rotary(
     Angles are computed in 64 bits, the rotation in 32, with one rounding to the tensors' type.  Returns new
     tensors ``(query, key)``, or the rotated query alone when ``key`` is None.  Differentiable with respect
     to ``query`` and ``key`` (not to ``positions``).  A capture into a graph is refused while a leaf among them has a
-    living autograd graph from another stream, whose backward pass the capture would run into.
+    living autograd graph from another stream, whose backward pass the capture would run into (without the tensor module, which
+    can tell, of every leaf that requires a gradient).
     """
     plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(map(float, inv_freq)),
                         bool(interleaved_axes), bool(interleaved_pairs))
@@ -322,6 +323,15 @@ def multi_axis_rotary(
         with torch.cuda.device(query.device):
             return multi_axis_rotary(query, key, positions, sections, base=base, inv_freq=inv_freq,
                                      interleaved_axes=interleaved_axes, interleaved_pairs=interleaved_pairs)
+
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        leaves = [x for x in tensors if x.requires_grad and x.is_leaf]
+        if leaves and not module:
+            raise RuntimeError("multi_axis_rotary: without its tensor module a capture cannot tell whether another graph of a "
+                               "leaf is alive: rotate a tensor that is not a leaf, or one without a gradient")
+        if leaves and module.held(*leaves) is not False:
+            raise RuntimeError("multi_axis_rotary: a graph of this leaf from outside of the capture is still alive; "
+                               "delete its outputs (or capture on the stream that they were made on)")
 
     lead = query.shape[:-2]
     q, k, p = query, key, positions

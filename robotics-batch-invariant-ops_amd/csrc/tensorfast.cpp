@@ -177,6 +177,13 @@ bool capturing(c10::DeviceIndex device) {
   return hipStreamIsCapturing((hipStream_t)stream_on(device), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
 }
 
+// held(tensors...) -> whether one of them is such a leaf, for the rotations that the Python function launches
+PyObject* held(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (THPVariable_Check(args[i]) && held_elsewhere(THPVariable_Unpack(args[i]), c10::hip::current_device())) Py_RETURN_TRUE;
+  Py_RETURN_FALSE;
+}
+
 // rotary(query, key or None, positions, axes, pairs, turns, axis, neighbours) -> query or (query, key)
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 8) Py_RETURN_NONE;
@@ -388,6 +395,7 @@ PyCFunction fast() {
 }
 
 PyMethodDef methods[] = {
+    {"held", fast<held>(), METH_FASTCALL, "whether a graph of a leaf is alive on another stream, or None"},
     {"rotary", fast<rotary>(), METH_FASTCALL, "biops_rotary on tensors, or None"},
     {"paged_write", fast<paged_write>(), METH_FASTCALL, "biops_paged_write on tensors, or None"},
     {"paged_attention", fast<paged_attention>(), METH_FASTCALL, "biops_paged_attention on tensors, or None"},

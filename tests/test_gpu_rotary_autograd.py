@@ -48,3 +48,46 @@ def test_lazily_negated_gradients(path):
         check_rotated(gg, g[0], p, (8, 4))
     (gq,) = torch.autograd.grad(torch._neg_view(multi_axis_rotary(q, None, p, (8, 4))), q, g[0])
     check_rotated(gq, -g[0], p, (8, 4), inverse=True)
+
+
+class Plain(torch.Tensor):
+    """A subclass, which the tensor module leaves to the Python function."""
+
+
+def test_captures_beside_a_living_graph_on_the_python_path():
+    p = torch.randint(0, 99, (1, 5)).cuda()
+    q = randn(5, 2, 16, seed=1).as_subclass(Plain).requires_grad_()
+    want = multi_axis_rotary(q.detach(), None, p, (8,))
+    alive = q * 2.0
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            multi_axis_rotary(q, None, p, (8,))
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = multi_axis_rotary(q, None, p, (8,)).detach()
+    graph.replay()
+    assert_bitwise(got, want)
+
+
+def test_captures_without_the_module(monkeypatch):
+    """What cannot be told is refused; what has no leaf's gradient is captured."""
+    monkeypatch.setattr(decoder, "_tensor_module", False)
+    monkeypatch.setattr(decoder, "_direct", lambda: False)
+    p = torch.randint(0, 99, (1, 5)).cuda()
+    q = randn(5, 2, 16, seed=2).requires_grad_()
+    want = multi_axis_rotary(q.detach(), None, p, (8,))
+    for inputs in ((q, None), (q.detach(), q)):
+        with pytest.raises(RuntimeError, match="tensor module"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                multi_axis_rotary(*inputs, p, (8,))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = multi_axis_rotary(q.detach(), None, p, (8,))
+        with torch.no_grad():
+            second = multi_axis_rotary(q, None, p, (8,))
+    graph.replay()
+    assert_bitwise(first, want)
+    assert_bitwise(second, want)
