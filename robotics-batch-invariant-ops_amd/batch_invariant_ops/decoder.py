@@ -377,6 +377,42 @@ def _overlaps(t: torch.Tensor) -> bool:
     return False
 
 
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an element of the key cache may lie where one of the value cache does (two views of one allocation may be
+    interleaved in any dimension, if their slots have the same strides)."""
+    if a.numel() == 0 or b.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+    if a.storage_offset() > b.storage_offset():
+        a, b = b, a
+    gap = b.storage_offset() - a.storage_offset()
+    if gap > sum((n - 1) * s for n, s in zip(a.shape, a.stride())):
+        return False
+    dims = [(s, n) for s, n in zip(a.stride()[:3], a.shape[:3]) if n > 1]
+    if dims != [(s, n) for s, n in zip(b.stride()[:3], b.shape[:3]) if n > 1]:
+        return True
+    # both at once, as one tensor with a dimension more, whose two entries are `gap` apart
+    low, high = a.shape[3] - 1, b.shape[3] - 1  # how far each reaches
+    for stride, size in sorted([*dims, (gap, 0)]):
+        if size == 0:
+            if gap <= low:
+                return True
+            low = high = max(low, gap + high)
+        elif stride <= max(low, high):
+            return True
+        else:
+            low, high = low + stride * (size - 1), high + stride * (size - 1)
+    return False
+
+
+def _part(a: torch.Tensor, b: torch.Tensor) -> int | None:
+    """The element of ``a``'s rows at which ``b``'s rows begin, where one's rows are a part of the other's."""
+    at = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if a.stride() != b.stride() or a.shape[:-1] != b.shape[:-1]:
+        return None
+    inside = 0 <= at <= a.shape[-1] - b.shape[-1] or 0 <= -at <= b.shape[-1] - a.shape[-1]
+    return at if inside else None
+
+
 def paged_cache_write(
     key: torch.Tensor,
     value: torch.Tensor,
@@ -391,7 +427,8 @@ def paged_cache_write(
     place``.  A negative slot leaves its row out (padding).  A slot past the cache is left out too and reported
     as an error later (see the module).  Of several rows that name one slot the last one stays.  ``key`` and
     ``value`` may be rows of the caches themselves (a page that is copied) as long as no slot that is written is
-    among them.
+    among them.  The caches may be interleaved views of one allocation.  They must not share
+    elements, unless the new rows do in the same way (values that are a part of the keys).
     """
     module, watch = _direct_watch()
     if module and module.paged_write(key, value, key_cache, value_cache, slots, watch.flag_at):
@@ -410,6 +447,9 @@ def paged_cache_write(
     device = _check_tensors("paged_cache_write", key, value, key_cache, value_cache, slots)
     if _overlaps(key_cache) or _overlaps(value_cache):
         raise ValueError("caches must not overlap themselves (an expanded view?)")
+    if _share(key_cache, value_cache) and (
+            _part(key_cache, value_cache) is None or _part(key_cache, value_cache) != _part(key, value)):
+        raise ValueError("the key and the value cache must not share memory")
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return paged_cache_write(key, value, key_cache, value_cache, slots)

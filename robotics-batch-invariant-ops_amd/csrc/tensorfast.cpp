@@ -258,8 +258,10 @@ PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!number(args[5], &flag) || code < 0 || !caches(kc, vc) || k.scalar_type() != kc.scalar_type() ||
       v.scalar_type() != kc.scalar_type())
     Py_RETURN_NONE;
-  // (an overlapping cache is refused in Python)
+  // (caches that overlap themselves or one another are refused in Python)
   if (!kc.is_non_overlapping_and_dense() || !vc.is_non_overlapping_and_dense()) Py_RETURN_NONE;
+  const int64_t gap = vc.storage_offset() - kc.storage_offset();
+  if (kc.is_alias_of(vc) && gap < kc.numel() && -gap < vc.numel()) Py_RETURN_NONE;
   if (k.dim() != 3 || v.dim() != 3 || !unit_last(k) || !unit_last(v) || k.size(0) != v.size(0) || k.size(1) != kc.size(2) ||
       v.size(1) != kc.size(2) || k.size(2) != kc.size(3) || v.size(2) != vc.size(3))
     Py_RETURN_NONE;

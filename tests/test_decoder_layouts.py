@@ -83,3 +83,97 @@ def test_one_page_one_head_one_row():
     for a, b in zip(bio.multi_axis_rotary(odd(new, 0), odd(new, 1), odd(p, 1), (32,)), want):
         assert_bitwise(a, b)
     bio.check_cache_indices()
+
+
+def brute(a, b):
+    def places(t):
+        at = torch.full((1,), t.storage_offset())
+        for n, s in zip(t.shape, t.stride()):
+            at = (at.view(-1, 1) + torch.arange(n) * s).flatten()
+        return set(at.tolist())
+
+    return bool(places(a) & places(b))
+
+
+def pairs():
+    """Views of one allocation, with whether they are fit for keys and values."""
+    base = torch.zeros(4000)
+
+    def at(offset, shape, strides):
+        return base.as_strided(shape, strides, offset)
+
+    kv = base[:1536].view(2, 3, 4, 4, 16)
+    yield kv[0], kv[1], True
+    yield kv[1], kv[0], True
+    yield kv[0], kv[0], False
+    for dim in range(1, 5):
+        two = base[:1536].view(*[(3, 4, 4, 16)[i] for i in range(dim - 1)], 2, *[(3, 4, 4, 16)[i] for i in range(dim - 1, 4)])
+        yield two.select(dim - 1, 0), two.select(dim - 1, 1), True
+        yield two.select(dim - 1, 1), two.select(dim - 1, 0), True
+    fused = base[:3 * 4 * 2 * 40].view(3, 4, 2, 40)
+    yield fused[..., :16], fused[..., 16:], True
+    yield fused[..., :24], fused[..., 24:], True
+    yield fused[..., :24], fused[..., 16:], False
+    yield fused[..., 8:16], fused[..., :16], False
+    heads = base[:3 * 4 * 6 * 16].view(3, 4, 6, 16)
+    yield heads[:, :, :3], heads[:, :, 3:], True
+    yield heads[:, :, :4], heads[:, :, 2:], False
+    yield heads[:, :, 0::2], heads[:, :, 1::2], True
+    pages = base[:3 * 4 * 2 * 16].view(3, 4, 2, 16)
+    yield pages[:2], pages[1:], False
+    yield pages[:1], pages[2:], True
+    yield pages[:, :2], pages[:, 2:], True
+    yield pages[:1, :, :1], pages[:1, :, 1:], True
+    turned = base[:768].view(2, 3, 2, 4, 16).transpose(2, 3)
+    yield turned[0], turned[1], True
+    yield at(0, (2, 2, 2, 8), (64, 16, 8, 1)), at(40, (2, 2, 2, 8), (64, 16, 8, 1)), False
+    yield at(0, (2, 2, 2, 8), (64, 16, 8, 1)), at(32, (2, 2, 2, 8), (64, 16, 8, 1)), True
+
+
+def test_caches_that_share_memory_are_recognised():
+    for i, (a, b, fit) in enumerate(pairs()):
+        assert decoder._share(a, b) is not fit, i
+        if fit:
+            assert not brute(a, b), i  # what is taken never overlaps
+    assert not decoder._share(torch.zeros(2, 2, 2, 8), torch.zeros(2, 2, 2, 8))
+    assert not decoder._share(torch.zeros(0, 2, 2, 8), torch.zeros(0, 2, 2, 8))
+
+
+@pytest.mark.gpu
+def test_shared_caches_are_refused_and_interleaved_ones_written():
+    slots = torch.tensor([5, 0, 11]).cuda()
+    for i, (a, b, fit) in enumerate(pairs()):
+        if a.shape[2] != b.shape[2] or a.shape[:3] != b.shape[:3]:
+            continue
+        base = torch.zeros(4000, dtype=BF16).cuda()
+        kc, vc = (base.as_strided(t.shape, t.stride(), t.storage_offset()) for t in (a, b))
+        k, v = (randn(3, t.shape[2], t.shape[3], seed=i + j) for j, t in enumerate((a, b)))
+        at = slots % (kc.shape[0] * kc.shape[1])
+        if not fit:
+            with pytest.raises(ValueError, match="share memory"):
+                bio.paged_cache_write(k, v, kc, vc, at)
+            continue
+        bio.paged_cache_write(k, v, kc, vc, at)
+        for r, s in enumerate(at.tolist()):
+            if s in at.tolist()[r + 1:]:
+                continue
+            assert_bitwise(kc[s // kc.shape[1], s % kc.shape[1]], k[r])
+            assert_bitwise(vc[s // kc.shape[1], s % kc.shape[1]], v[r])
+    bio.check_cache_indices()
+
+
+@pytest.mark.gpu
+def test_values_that_are_a_part_of_the_keys():
+    """The same elements of the same rows: one cache for both."""
+    slots = torch.tensor([5, 0, 11]).cuda()
+    for part in (slice(0, 64), slice(0, 48), slice(16, 64), slice(8, 56)):
+        kc, k = torch.zeros(3, 4, 2, 64, dtype=BF16).cuda(), randn(3, 2, 64, seed=30 + part.stop)
+        bio.paged_cache_write(k, k[..., part], kc, kc[..., part], slots)
+        assert_bitwise(kc.flatten(0, 1)[slots], k)
+        assert int((kc != 0).any(-1).any(-1).sum()) == 3
+        bio.paged_cache_write(k[..., part], k, kc[..., part], kc, slots.flip(0))
+        assert_bitwise(kc.flatten(0, 1)[slots.flip(0)], k)
+        for other in (k.clone()[..., part], k[..., slice(part.start + 8, part.stop + 8)] if part.stop <= 56 else k.flip(0)[..., part]):
+            with pytest.raises(ValueError, match="share memory"):
+                bio.paged_cache_write(k, other, kc, kc[..., part], slots)
+    bio.check_cache_indices()
