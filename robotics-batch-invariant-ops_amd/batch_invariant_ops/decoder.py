@@ -67,14 +67,11 @@ class _CacheWatch(_IndexWatch):
             super().after_call(nat.stream_of(self.flag) if stream is None else stream)
 
 
-def check_cache_indices(device: torch.device | int | None = None) -> None:
+def check_cache_indices(device: torch.device | str | int | None = None) -> None:
     """Raise ``RuntimeError`` if a call of this module on ``device`` (default: the current device) met an
     index outside its tensor since the last report.  Waits for the work queued on that device's current
     stream."""
-    if device is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    elif isinstance(device, int):
-        device = torch.device("cuda", device)
+    device = _CacheWatch.device(device)
     with torch.cuda.device(device):
         _CacheWatch.of(device).check()
 

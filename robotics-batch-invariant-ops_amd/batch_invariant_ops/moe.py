@@ -33,6 +33,14 @@ class _IndexWatch:
         self.last = 0.0
         self.copy = nat.fast_copy_d2h()
 
+    @staticmethod
+    def device(device: torch.device | str | int | None) -> torch.device:
+        """A device with its number: the current one where none is given."""
+        if device is None or isinstance(device, int):
+            return torch.device("cuda", torch.cuda.current_device() if device is None else device)
+        device = torch.device(device)
+        return device if device.index is not None else torch.device(device.type, torch.cuda.current_device())
+
     @classmethod
     def of(cls, device: torch.device) -> "_IndexWatch":
         watch = cls._by_device.get(device.index)
@@ -79,14 +87,11 @@ class _IndexWatch:
         self._raise_if_set(int(self.flag.item()))
 
 
-def check_moe_indices(device: torch.device | int | None = None) -> None:
+def check_moe_indices(device: torch.device | str | int | None = None) -> None:
     """Raise ``RuntimeError`` if a ``deterministic_token_choice_moe`` call on ``device``
     (default: the current device) met an expert index outside [0, num_experts) since the last
     report.  Waits for the work queued on that device's current stream."""
-    if device is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    elif isinstance(device, int):
-        device = torch.device("cuda", device)
+    device = _IndexWatch.device(device)
     with torch.cuda.device(device):
         _IndexWatch.of(device).check()
 
