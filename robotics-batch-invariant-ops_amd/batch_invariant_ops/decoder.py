@@ -242,8 +242,10 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.plan, ctx.inverse = plan, inverse
         ctx.set_materialize_grads(False)
-        out_q, out_k = _rotate(query, key, positions, plan, inverse)
-        return out_q, out_k
+        outs = _rotate(query, key, positions, plan, inverse)
+        # what comes of a tensor without a gradient has none
+        ctx.mark_non_differentiable(*(y for y, needs in zip(outs, ctx.needs_input_grad) if y is not None and not needs))
+        return tuple(outs)
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):

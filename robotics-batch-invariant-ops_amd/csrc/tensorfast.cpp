@@ -136,6 +136,9 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     auto y = rotated(q, k, p, r, inverse);
     torch::autograd::variable_list out{y.first};
     if (k.defined()) out.push_back(y.second);
+    // what comes of a tensor without a gradient has none
+    if (!q.requires_grad()) ctx->mark_non_differentiable({y.first});
+    else if (k.defined() && !k.requires_grad()) ctx->mark_non_differentiable({y.second});
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {

@@ -91,3 +91,28 @@ def test_captures_without_the_module(monkeypatch):
     graph.replay()
     assert_bitwise(first, want)
     assert_bitwise(second, want)
+
+
+def test_outputs_of_inputs_without_a_gradient_have_none(path):
+    """Their keys can go straight into a cache, for one."""
+    p = torch.randint(0, 99, (1, 5)).cuda()
+    q, k = randn(5, 2, 16, seed=3), randn(5, 2, 16, seed=4)
+    g = randn(5, 2, 16, seed=5)
+    for which in (0, 1):
+        inputs = [x.clone().requires_grad_() if i == which else x for i, x in enumerate((q, k))]
+        out = multi_axis_rotary(*inputs, p, (8,))
+        assert out[which].requires_grad and not out[1 - which].requires_grad and out[1 - which].grad_fn is None
+        for a, b in zip(out, multi_axis_rotary(q, k, p, (8,))):
+            assert_bitwise(a.detach(), b)
+        (got,) = torch.autograd.grad(out[which], inputs[which], g)
+        check_rotated(got, g, p, (8,), inverse=True)
+        cache = torch.zeros(1, 5, 2, 16).cuda()
+        bio.paged_cache_write(out[1 - which], out[1 - which], cache, cache.clone(), torch.arange(5).cuda())
+        assert_bitwise(cache[0], out[1 - which])
+        # a gradient of the gradient, with the other output used beside it
+        held = g.clone().requires_grad_()
+        (got,) = torch.autograd.grad(multi_axis_rotary(*inputs, p, (8,))[which], inputs[which], held, create_graph=True)
+        (gg,) = torch.autograd.grad(got, held, g)
+        check_rotated(gg, g, p, (8,))
+    both = multi_axis_rotary(q.clone().requires_grad_(), k.clone().requires_grad_(), p, (8,))
+    assert both[0].requires_grad and both[1].requires_grad
