@@ -632,9 +632,9 @@ def sliding_window_attention_batch_invariant(
     Rows that see nothing (more queries than keys) are zeros.  Work and memory grow with the window, not
     with the square of the length.  ``enable_gqa`` lets groups of query heads share a key/value head.
 
-    A key that is masked for a row never reaches it, whatever its key and value hold.  Scores and sums are
-    in 32 bits; 16-bit products take weights rounded to the type.  Output rows depend on their own sequence
-    only.
+    A key that is masked for a row changes none of its bits, whatever its key and value hold; an infinity or
+    NaN in a value reaches every row that sees it, whatever its weight.  Scores and sums are in 32 bits; 16-bit
+    products take weights rounded to the type.  Output rows depend on their own sequence only.
     """
     module = _tensor_module or _direct()
     if module:

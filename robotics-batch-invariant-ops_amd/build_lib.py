@@ -6,7 +6,8 @@ Each csrc/*.hip file is compiled to an object with hipcc for gfx950, then linked
 batch_invariant_ops/libbiops.so next to the Python package that loads it.  csrc/pyfast.c, a
 CPython fast-call binding of the most frequent entry points, is compiled with the host C
 compiler into batch_invariant_ops/_biops_fast (linked against libbiops.so beside it), and
-csrc/tensorfast.cpp, the decoder operators on torch tensors, against torch into _biops_tensor.
+csrc/tensorfast.cpp, the decoder operators on torch tensors, against torch into _biops_tensor.  The build
+fails where one of them does; the package runs without these two, more slowly.
 """
 
 from __future__ import annotations

@@ -28,8 +28,8 @@
 // 16-bit weights go in as a rounded part and the rounded rest (two MFMAs), which leaves an error of
 // 2^-16 (bf16) instead of 2^-8 where the matrix cores have the time.
 //
-// bf16, 16/4 heads of 128, 64 sequences of 250 to 16384 keys: 113 us, 4.55 TB/s (a copy of as many bytes: 103), and 5 for
-// the join; one sequence of 2047 keys 7 and 4; fp16, 8/2 heads of 64, 100 sequences under a window of 1024: 11.4 and 4.
+// bf16, 16/4 heads of 128, 64 sequences of 250 to 16384 keys: 114 us, 4.5 TB/s (a copy of as many bytes: 103), and 5 for
+// the join; one sequence of 2047 keys 7 and 4; fp16, 8/2 heads of 64, 100 sequences under a window of 1024: 11.6 and 4.
 //
 // Slots behind the end of a sequence may hold anything: keys of the last tile past the end are read
 // from the last key's row, their scores replaced by -inf and their values by zeros.

@@ -2,7 +2,8 @@
 // some sixty of them in a call): a call whose tensors are as the kernels take them is checked, given its
 // output and workspace, and launched here.  Every function returns None where it does not take the call
 // as it is -- other layouts, empty tensors, what needs a gradient, and everything that is refused: the
-// Python functions then do what is left, and raise the errors.  Optional: without this module they do all.
+// Python functions then do what is left, and raise the errors.  The package runs without this module: they then do all, and
+// refuse captured rotations of leaves, whose living graphs only the module sees.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>

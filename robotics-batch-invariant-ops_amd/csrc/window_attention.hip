@@ -30,7 +30,7 @@
 // What bounds it: the vector units and the matrix cores in turn.  A score costs about seven vector slots
 // (maximum, fused multiply-add, exponential at a quarter of the rate, conversion, sum) and 4 D / 1024 matrix cycles of
 // a 16-bit type; two or three wavefronts of a SIMD overlap the two in part.  bf16, 16/4 heads of 128, 2 x 8192 tokens
-// under a window of 2048: 288 us, 837 TF/s of visible pairs; fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 31 us.  float32 products
+// under a window of 2048: 286 us, 842 TF/s of visible pairs; fp16, 8/2 heads of 64, 32 packed prompts of 19533 tokens, window 256: 30 us.  float32 products
 // run at 1/16 of the 16-bit rate and bound it alone: 3 x 257 rows of 1281 keys, 16 heads of 72, window 500: 37 us.
 #include <type_traits>
 
@@ -905,9 +905,9 @@ static int window_launch(WindowArgs a, hipStream_t s) {
 //   64-wide, 50 rows of 700 keys, 1 / 64 sequences
 //                                     16 / 23   16 / 23   15 / 33   12 / 25   12 / 24
 //   128-wide, the same                20 / 33   20 / 32   19 / 45   16 / 41   16 / 41
-//   float32                          <4,1,1,4> <4,1,1,2> <4,1,1,1> <2,2,1,2> <2,2,1,1> <2,4,1,2> <2,4,1,1>
-//   64-wide, 1 x 700 / 4 x 2048       49 / 161  52 / 174  55 / 191  28 / 165  30 / 187  27 / 196  30 / 212
-//   72-wide, the same                 63 / 210  67 / 227  69 / 251  37 / 224  40 / 256  38 / 269  40 / 288
+//   float32 (<4,1,1,1>, without turns, beside them)          <4,1,1,1> <2,2,1,2> <2,2,1,1>
+//   64-wide, 1 x 700 / 4 x 2048                              55 / 191  28 / 165  30 / 187
+//   72-wide, the same                                        69 / 251  37 / 224  40 / 256
 template <typename T, int DP>
 static int window_launch_rows(const WindowArgs& a, hipStream_t s) {
   const bool pairs = a.group % 2 == 0, fours = a.group % 4 == 0;
@@ -940,9 +940,9 @@ static int window_launch_d(const WindowArgs& a, hipStream_t s) {
 
 // Ranges that the keys of a few dense rows are cut into, by sizes that all sequences of a call share; blocks of 64 keys
 // of a range.  A few rows are a few tiles, and each would walk through all keys alone.  us (one tile through all keys /
-// ranges), bf16, 16/4 heads of 128, no window: 16 rows before 2000 keys 39 / 20 (one sequence), 40 / 22 (eight), 61 / 85
-// (64); before 8192 keys 143 / 23, 144 / 46, 254 / 345; 64 rows before 8192 keys 133 / 28, 136 / 68, 445 / 563; float32,
-// 72-wide, 16 rows before 8192 443 / 42, 443 / 117, 806 / 892.  (The batch may not enter: one sequence's bits.)
+// ranges), bf16, 16/4 heads of 128, no window: 16 rows before 2000 keys 39 / 21 (one sequence), 40 / 23 (eight), 61 / 83
+// (64); before 8192 keys 143 / 19, 144 / 42, 254 / 327; 64 rows before 8192 keys 133 / 26, 136 / 65, 445 / 538; float32,
+// 72-wide, 16 rows before 8192 443 / 37, 443 / 114, 806 / 882.  (The batch may not enter: one sequence's bits.)
 static int window_splits(int64_t lq, int64_t lk, int64_t window, int64_t sinks, int* per) {
   *per = 0x7fffffff;
   if (lq < 1 || lq > kWindowFew) return 1;
