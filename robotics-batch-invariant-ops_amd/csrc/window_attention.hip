@@ -532,6 +532,9 @@ __device__ __forceinline__ uint32_t window_pass(const WindowArgs& a, char* smem,
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[x][r] -= less;
     }
+    // A block's 16-bit weights are added up by themselves: one by one, those below 2^-25 of the sum so far would not count in
+    // it, as they do in the product's sums, 16 keys at a time.  (float32 products add two keys at a time.)
+    float sum = 0.f;
     const float off = large ? (mode == 2 ? kWindowDown : 0.f) : sh;
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
@@ -544,10 +547,11 @@ __device__ __forceinline__ uint32_t window_pass(const WindowArgs& a, char* smem,
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           pw[x][i >> 2][i & 3] = window_pack<T>(sc[x][2 * i], sc[x][2 * i + 1]);
-          l = window_add_pair<T>(pw[x][i >> 2][i & 3], l);
+          sum = window_add_pair<T>(pw[x][i >> 2][i & 3], sum);
         }
       }
     }
+    l += sum;
   };
   // What the weights add to the output.
   auto gather = [&]() {

@@ -234,3 +234,26 @@ def test_token_attention_of_the_largest_and_the_smallest_values(dtype, n):
     assert_within(out[:1], o.unsqueeze(0), (relative * o.abs() + 2.0**-141).unsqueeze(0))
     want = torch.full((1, d), small, dtype=torch.float64)
     assert_within(out[1:], want, relative * want + 2.0**-141)
+
+
+@pytest.mark.parametrize("dtype, n, top", [(BF16, 600000, 17.375)])
+def test_prompts_of_many_small_weights(dtype, n, top):
+    """Keys of weight 2^-25.1 beside one of 1, which make 2^-6 (600000 keys) or 2^-8 (100000) of the output together.  Values are
+    positive, so that a sum's error is 2^-24 for each of the additions on a value's way: one for each block of 64 keys and 64 in a
+    block, in the numerator and the denominator.  The many weights are rounded once to the type: all alike, the other one is 1."""
+    lq, d = 65, 8
+    q, k = torch.zeros(lq, 1, d, dtype=dtype), torch.zeros(n, 1, d, dtype=dtype)
+    q[:, 0, 0] = 8.0
+    k[50, 0, 0] = top
+    v = randn(n, 1, d, seed=78, dtype=dtype).abs() + 1
+    v[50] = 1.0
+    rows = [0, 40, 64]
+    visible = window_visible(1, n, None, 0).expand(3, n).clone()
+    for i, r in enumerate(rows):
+        visible[i, n - lq + r + 1:] = False
+    o, mag, err, tail = attend64(q[rows, 0], k[:, 0], v[:, 0], visible, 0.125)
+    share = (o - 1).abs()  # of the many, at least: their values are over 1
+    relative = 2.0**-20 + 2 * err + 2 * (n / 64 + 64) * 2.0**-24
+    bound = HALF[dtype] * o.abs() + (1 + HALF[dtype]) * (relative * mag + HALF[dtype] * 4 * share)
+    for out in prompt(q, k, v, scale=0.125):
+        assert_within(out[rows, 0], o, bound)
