@@ -49,6 +49,9 @@ constexpr float kWindowSlack = 8.f;  // by how many powers of two weights may pa
 // row, and no more than 2^(1/16) up to this size of c m; past it the difference s - m is taken first (with an instruction
 // more), or the factor would leave the range: by 2^28 fp16's, by 2^31 float's.
 constexpr float kWindowLarge = 0x1p20f;
+// fp16 weights are 2^7 times their size, which with the slack is near the end of their range: those down to 2^-32 of the largest
+// count (2^-25 without it, which 100000 keys add up to 2^-8 of a row).
+template <typename T> constexpr float kWindowUp = std::is_same<T, f16_t>::value ? 7.f : 0.f;
 // Weights of mode 2 are 2^-40 times their size: of fewer than 2^31 values times weights of up to 2^kWindowSlack no sum passes
 // the largest one.
 constexpr float kWindowDown = 40.f;
@@ -194,15 +197,23 @@ struct WindowShape {
   }
 };
 
-// Exponent that turns weights relative to the score m into those relative to the score top; c = a.scale.  (The products are
-// the rounded ones that the weights have seen: no fused multiply-add may take their place.  `exact`: mode 2, where all
-// differences are taken first.)
+// c m as weights take it off, less the powers of two that these are larger by; c = a.scale.
+template <typename T>
+__device__ __forceinline__ float window_shift(float m, float c) {
+  if constexpr (kWindowUp<T> == 0.f) return m * c;
+  else return __builtin_fmaf(m, c, -kWindowUp<T>);
+}
+// Exponent that turns weights relative to the score m into those relative to the score top.  (The shifts are the rounded ones
+// that the weights have seen: no fused multiply-add may take their place.  `exact`: mode 2, where all differences are
+// taken first.)
+template <typename T>
 __device__ __forceinline__ float window_ratio(float m, float top, float c, bool exact) {
 #pragma clang fp contract(off)
-  const float a = m * c, t = top * c;
+  const float a = window_shift<T>(m, c), t = window_shift<T>(top, c);
   const bool la = exact || fabsf(a) > kWindowLarge, lt = exact || fabsf(t) > kWindowLarge;
   if (!la && !lt) return a - t;
-  return (m - top) * c - (la ? 0.f : __builtin_fmaf(m, c, -a)) + (lt ? 0.f : __builtin_fmaf(top, c, -t));
+  auto rounding = [&](float x, float shift) { return __builtin_fmaf(x, c, -shift) - kWindowUp<T>; };
+  return (m - top) * c - (la ? 0.f : rounding(m, a)) + (lt ? 0.f : rounding(top, t));
 }
 
 // Infinities and NaN of 16 bytes as zeros.
@@ -440,7 +451,7 @@ __device__ __forceinline__ uint32_t window_pass(const WindowArgs& a, char* smem,
     }
   }
 
-  // m: the score (raw) that weights are relative to, sh = m * scale (0 before the first), l: this lane's part of the row's sum
+  // m: the score (raw) that weights are relative to, sh = window_shift of it (0 before the first), l: this lane's part of the row's sum
   float m = -INFINITY, sh = 0.f, l = 0.f;
   const float slack = fminf(kWindowSlack / a.scale, FLT_MAX);
   f32x16_t oacc[F::OF];  // O^T: register r of block e is column 32e + 8(r/4) + 4hf + r%4 of row l32
@@ -512,9 +523,9 @@ __device__ __forceinline__ uint32_t window_pass(const WindowArgs& a, char* smem,
     const bool grown = mx - m > slack;
     if (__any(grown)) {
       const float mn = grown ? mx : m;
-      const float to = mn == -INFINITY ? 0.f : mn * a.scale;
+      const float to = mn == -INFINITY ? 0.f : window_shift<T>(mn, a.scale);
       if (__any(m > -INFINITY)) {  // (nothing is summed before a row's first keys)
-        const float corr = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(window_ratio(m, mn, a.scale, mode == 2)) : 1.f;
+        const float corr = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(window_ratio<T>(m, mn, a.scale, mode == 2)) : 1.f;
         l *= corr;
 #pragma unroll
         for (int e = 0; e < F::OF; ++e)
@@ -535,7 +546,7 @@ __device__ __forceinline__ uint32_t window_pass(const WindowArgs& a, char* smem,
     // A block's 16-bit weights are added up by themselves: one by one, those below 2^-25 of the sum so far would not count in
     // it, as they do in the product's sums, 16 keys at a time.  (float32 products add two keys at a time.)
     float sum = 0.f;
-    const float off = large ? (mode == 2 ? kWindowDown : 0.f) : sh;
+    const float off = large ? (mode == 2 ? kWindowDown : -kWindowUp<T>) : sh;
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
 #pragma unroll
@@ -658,7 +669,7 @@ __device__ __forceinline__ uint32_t window_pass(const WindowArgs& a, char* smem,
 #pragma unroll
       for (int x = 1; x < KW; ++x) top = fmaxf(top, js[((x - 1) * RW + rw) * 64 * (16 * F::OF + 2) + lane + 64 * 16 * F::OF]);
       auto factor = [&](float from) {
-        return from == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(window_ratio(from, top, a.scale, mode == 2));
+        return from == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(window_ratio<T>(from, top, a.scale, mode == 2));
       };
       const float own = factor(m);
       l *= own;
@@ -851,7 +862,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
     if (x < a.splits && 4 * lane < a.dv) mean[x] = *reinterpret_cast<const f32x4_t*>(part + (int64_t)x * a.dv);
   const float top = wave_max(m);
   // what each range's mean counts for
-  const float own = m == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(window_ratio(m, top, a.scale, false));
+  const float own = m == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(window_ratio<T>(m, top, a.scale, false));
   const float l = wave_sum(own);
   const float share = l == 0.f ? 0.f : own / l;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};

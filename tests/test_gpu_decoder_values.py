@@ -236,11 +236,12 @@ def test_token_attention_of_the_largest_and_the_smallest_values(dtype, n):
     assert_within(out[1:], want, relative * want + 2.0**-141)
 
 
-@pytest.mark.parametrize("dtype, n, top", [(BF16, 600000, 17.375)])
+@pytest.mark.parametrize("dtype, n, top", [(BF16, 600000, 17.375), (F16, 100000, 17.40625)])
 def test_prompts_of_many_small_weights(dtype, n, top):
     """Keys of weight 2^-25.1 beside one of 1, which make 2^-6 (600000 keys) or 2^-8 (100000) of the output together.  Values are
     positive, so that a sum's error is 2^-24 for each of the additions on a value's way: one for each block of 64 keys and 64 in a
-    block, in the numerator and the denominator.  The many weights are rounded once to the type: all alike, the other one is 1."""
+    block, in the numerator and the denominator.  The many weights are rounded once to the type: all alike, the other one is 1.  (fp16's
+    smallest step is 2^-24, half of it 2^-25, and weights are 2^7 times their size in it: 2^-32 each.)"""
     lq, d = 65, 8
     q, k = torch.zeros(lq, 1, d, dtype=dtype), torch.zeros(n, 1, d, dtype=dtype)
     q[:, 0, 0] = 8.0
@@ -254,6 +255,6 @@ def test_prompts_of_many_small_weights(dtype, n, top):
     o, mag, err, tail = attend64(q[rows, 0], k[:, 0], v[:, 0], visible, 0.125)
     share = (o - 1).abs()  # of the many, at least: their values are over 1
     relative = 2.0**-20 + 2 * err + 2 * (n / 64 + 64) * 2.0**-24
-    bound = HALF[dtype] * o.abs() + (1 + HALF[dtype]) * (relative * mag + HALF[dtype] * 4 * share)
+    bound = HALF[dtype] * o.abs() + (1 + HALF[dtype]) * (relative * mag + HALF[dtype] * 4 * share + (2.0**-32 if dtype == F16 else 0.0) * tail)
     for out in prompt(q, k, v, scale=0.125):
         assert_within(out[rows, 0], o, bound)
