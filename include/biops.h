@@ -504,6 +504,72 @@ int biops_window_attention(int dtype, int64_t nseq, int64_t hq, int64_t hkv, int
 int64_t biops_window_attention_workspace_size(int64_t nseq, int64_t hq, int64_t lq, int64_t lk, int64_t dv, int64_t window,
                                               int64_t sinks);
 
+/* -------------------------------------------------- served decoder with fewer bits ---- */
+
+/* A cache in 4 bits: kc [pages, page_size, heads, d / 2] and its scales ks [..., d / 32], vc and vs the same of dv, all
+ * bytes with strides in bytes.  32 elements are a block: a scale byte x, 2^(x - 127), 255 for a block that is not finite, and
+ * two elements to a byte (the first in the low half), each a sign, two exponent bits and a mantissa bit (0, 0.5, 1, 1.5, 2, 3,
+ * 4, 6).  The power is the smallest of which no element is more than 7, within [2^-125, 2^125] (bf16 rows) or
+ * [2^-23, 2^13] (fp16 rows); elements go to the nearest level, ties to the even code, past 6 to 6. */
+
+/* biops_rotary of q [rows, hq, d] (-> oq) and k [rows, hk, d], and biops_paged_write of the rotated keys and of v [rows, hk, dv],
+ * with their bits, in one launch for each 8192 rows.  ks and vs null: caches of dtype; otherwise caches in 4 bits (fp16 or
+ * bf16 rows, d and dv multiples of 32), of rotated keys rounded to dtype.  hq may be 0, and pairs 0 (positions, turns and axis
+ * then null).  Rows and caches must not share memory. */
+int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t hk, int64_t d, int64_t dv,
+                       const void* q, int64_t sqT, int64_t sqH, void* oq, int64_t soqT, int64_t soqH,
+                       const void* k, int64_t skT, int64_t skH, const void* v, int64_t svT, int64_t svH,
+                       void* kc, int64_t skcP, int64_t skcS, int64_t skcH, void* ks, int64_t sksP, int64_t sksS, int64_t sksH,
+                       void* vc, int64_t svcP, int64_t svcS, int64_t svcH, void* vs, int64_t svsP, int64_t svsS, int64_t svsH,
+                       int64_t pages, int64_t page_size, const void* slots, int slots64, int64_t slot_stride,
+                       const void* positions, int pos_type, int64_t spA, int64_t spT, int64_t pairs, const double* turns,
+                       const uint8_t* axis, int neighbours, int* flag, void* stream);
+
+/* Keys ok [rows, heads, d] and values ov [rows, heads, dv] (contiguous, fp16 or bf16) of the slots of a cache in 4 bits.
+ * Negative slots give zeros; slots past the cache too, with the flag. */
+int biops_paged_read_fp4(int dtype, int64_t rows, int64_t heads, int64_t d, int64_t dv,
+                         const void* kc, int64_t skcP, int64_t skcS, int64_t skcH, const void* ks, int64_t sksP, int64_t sksS,
+                         int64_t sksH, const void* vc, int64_t svcP, int64_t svcS, int64_t svcH, const void* vs, int64_t svsP,
+                         int64_t svsS, int64_t svsH, int64_t pages, int64_t page_size, const void* slots, int slots64,
+                         int64_t slot_stride, void* ok, void* ov, int* flag, void* stream);
+
+/* biops_paged_attention over a cache in 4 bits: q fp16 or bf16, d and dv multiples of 32 up to 256, the same workspace
+ * (biops_paged_attention_workspace_size). */
+int biops_paged_attention_fp4(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t dv,
+                              const void* q, int64_t sqB, int64_t sqH,
+                              const void* kc, int64_t skP, int64_t skS, int64_t skH, const void* ks, int64_t sksP, int64_t sksS,
+                              int64_t sksH, const void* vc, int64_t svP, int64_t svS, int64_t svH, const void* vs,
+                              int64_t svsP, int64_t svsS, int64_t svsH, int64_t pages, int64_t page_size,
+                              const void* table, int table64, int64_t stB, int64_t stW, int64_t width,
+                              const void* lengths, int lengths64, int64_t slB, int64_t max_length, int64_t window,
+                              int64_t sinks, float scale, void* out, int* flag, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
+/* Workspace bytes of biops_sample, -1 for bad sizes (more than 2^20 tokens or 65536 rows). */
+int64_t biops_sample_workspace_size(int64_t rows, int64_t vocab);
+
+/* The next token of each row of logits [rows, vocab] (rows `ld` elements apart) from u[row] in [0, 1).  Weights are
+ * w_i = exp((l_i - max) / T).  Of the tokens ranked by logit (equal ones by index) stay the first k, those before which less than
+ * p of the weight of the first k has gone (the first always), and those with w_i >= min_p; the token is the first index at
+ * which the running sum of what stays exceeds u times all of it.  T <= 0: the most likely token.  Each setting comes from an
+ * array (by its stride, in elements) or, where that is null, for all rows from t0, k0 (0: all), p0 (1: all) and m0.  NaN
+ * logits count as -inf; a row without any other gives -1.  Workspace 16-byte aligned. */
+int biops_sample(int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, int64_t u_s,
+                 const float* temperature, int64_t t_s, double t0, const void* top_k, int k64, int64_t k_s, int64_t k0,
+                 const float* top_p, int64_t p_s, double p0, const float* min_p, int64_t m_s, double m0, int64_t* out,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows x [rows, k] (`ld` elements apart) as 8-bit integers q [rows, k] (contiguous) with a step for each: m = max |x|
+ * (at least 2^-100), scale = m / 127, q = round(x (127 / m)), ties to even.  A row that is not finite: zeros, scale NaN.
+ * At most 131071 elements. */
+int biops_quantize_int8(int dtype, int64_t rows, int64_t k, const void* x, int64_t ld, int8_t* q, float* scale, void* stream);
+
+/* y [M, N] (contiguous, of dtype) = (x . w^T) xs[m] ws[n] + bias[n] of 8-bit integers x [M, K] and w [N, K] (unit stride in K,
+ * rows ldx and ldw bytes apart): exact integer sums, 32-bit floats, one rounding.  bias (of dtype) may be null.  K of
+ * at most 131071. */
+int biops_linear_int8(int dtype, int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, const float* xs, int64_t xs_s,
+                      const int8_t* w, int64_t ldw, const float* ws, int64_t ws_s, const void* bias, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

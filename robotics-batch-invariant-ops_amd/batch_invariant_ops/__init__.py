@@ -35,6 +35,15 @@ from .decoder import (  # noqa: F401
     varlen_sliding_window_attention_batch_invariant,
     check_cache_indices,
 )
+from .served import (  # noqa: F401
+    rotary_cache_write,
+    paged_cache_write_fp4,
+    paged_cache_read_fp4,
+    paged_attention_fp4_batch_invariant,
+    sample_tokens_batch_invariant,
+    quantize_tokens_int8,
+    linear_int8_batch_invariant,
+)
 
 __version__ = "0.2.0"
 

@@ -36,6 +36,7 @@ _i = ctypes.c_int
 _l = ctypes.c_int64
 _p = ctypes.c_void_p
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 _SIGNATURES = {
     "biops_version": (ctypes.c_char_p, []),
@@ -122,6 +123,24 @@ _SIGNATURES = {
         [_i, _l, _l, _l, _l, _l, _l, _l] + [_p, _l, _l, _l] * 4 + [_p, _i, _l] * 2 + [_l, _l, _f, _p, _p, _l, _p],
     ),
     "biops_window_attention_workspace_size": (_l, [_l] * 7),
+    "biops_rotary_write": (
+        _i,
+        [_i, _l, _l, _l, _l, _l] + [_p, _l, _l] * 4 + [_p, _l, _l, _l] * 4 + [_l, _l, _p, _i, _l] + [_p, _i, _l, _l, _l, _p, _p, _i]
+        + [_p, _p],
+    ),
+    "biops_paged_read_fp4": (_i, [_i, _l, _l, _l, _l] + [_p, _l, _l, _l] * 4 + [_l, _l, _p, _i, _l] + [_p] * 4),
+    "biops_paged_attention_fp4": (
+        _i,
+        [_i, _l, _l, _l, _l, _l] + [_p, _l, _l] + [_p, _l, _l, _l] * 4 + [_l, _l]
+        + [_p, _i, _l, _l, _l] + [_p, _i, _l] + [_l, _l, _l, _f, _p, _p, _p, _l, _p],
+    ),
+    "biops_sample_workspace_size": (_l, [_l, _l]),
+    "biops_sample": (
+        _i,
+        [_i, _l, _l, _p, _l, _p, _l, _p, _l, _d, _p, _i, _l, _l, _p, _l, _d, _p, _l, _d, _p, _p, _l, _p],
+    ),
+    "biops_quantize_int8": (_i, [_i, _l, _l, _p, _l, _p, _p, _p]),
+    "biops_linear_int8": (_i, [_i, _l, _l, _l, _p, _l, _p, _l, _p, _l, _p, _l, _p, _p, _p]),
     "biops_moe_workspace_size": (_l, [_i, _l, _l, _l, _l]),
     "biops_moe": (
         _i,

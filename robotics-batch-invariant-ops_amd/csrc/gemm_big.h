@@ -47,17 +47,17 @@ namespace biops {
 // entries (lds_off_n) and the B fragments come through the transposing LDS reads.
 template <typename T, int BM, int BN, int SB, bool BKM = true>
 struct BigTile {
-  static_assert(sizeof(T) == 2, "16-bit operands");
+  static_assert(sizeof(T) == 2 || (sizeof(T) == 1 && BKM), "16-bit operands, or K-major 8-bit integers");
   static_assert(BKM || BN >= 64, "N-major stage rows of at least 8 chunks");
   static_assert(SB == 128, "whole K step per stage");
   static constexpr int THREADS = 256;
   static constexpr int WM = BM / 2, WN = BN / 2;
   static constexpr int FM = WM / 32, FN = WN / 32;
   static constexpr int NM = FM * FN;              // MFMAs per chunk pair
-  static constexpr int VEC = 8;
+  static constexpr int VEC = 16 / (int)sizeof(T);
   static constexpr int CPR = SB / 16;             // 16-byte chunks per row of a stage
   static constexpr int P = CPR / 2;               // chunk pairs per stage
-  static constexpr int STAGE_ELEMS = SB / 2;      // K elements per stage
+  static constexpr int STAGE_ELEMS = SB / (int)sizeof(T);  // K elements per stage
   static constexpr int LDS_A = BM * SB;
   static constexpr int LDS_STAGE = (BM + BN) * SB;
   static constexpr int LDS_MAX = 160 * 1024;
@@ -75,7 +75,7 @@ struct BigTile {
   static_assert(STAGES >= 2, "ring");
   static_assert((STAGES - 1) * LOADS < 64, "vmcnt range");
   static_assert(SMEM_BYTES <= LDS_MAX, "LDS");
-  typedef f32x16_t Acc;
+  typedef typename Mfma<T>::Acc Acc;
 
   struct Frags {
     u32x4_t a[FM];
@@ -325,7 +325,7 @@ struct BigTile {
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
     const int64_t H = K / STAGE_ELEMS;  // stages
     if (H == 0) return;
     const Src src = make_src(A, lda, rows, B, ldb, cols);

@@ -30,12 +30,14 @@ typedef __attribute__((address_space(1))) const void global_cvoid_t;
 // One 32x32 output block, one chunk pair of the step (32 x 32 fp32 accumulators: 16 per lane).
 template <typename T> struct Mfma;
 template <> struct Mfma<bf16_t> {
+  typedef f32x16_t Acc;
   __device__ static __forceinline__ void step(f32x16_t& acc, const u32x4_t& a, const u32x4_t& b) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                    __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);
   }
 };
 template <> struct Mfma<f16_t> {
+  typedef f32x16_t Acc;
   __device__ static __forceinline__ void step(f32x16_t& acc, const u32x4_t& a, const u32x4_t& b) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
                                                   __builtin_bit_cast(f16x8_t, b), acc, 0, 0, 0);

@@ -13,11 +13,11 @@
 // us for rows of 8 + 8 heads of 128 fp16 (4 KB, read from memory and written): 16383 rows 29.5 (4.55 TB/s; a plain
 // copy 27), with every slot somewhere else 34, and 36 / 45 with stores that stay in the caches; 48 rows of half
 // that 3.2, of which a launch is 2.6.
-#include "biops_common.h"
+#include "cache_slots.h"
 
 namespace biops {
 
-constexpr int kWriteRows = 8192;  // rows of a launch; 16384: 33.5 us for the 29.5 above
+// (kWriteRows of 16384: 33.5 us for the 29.5 above)
 
 // Rows of a workgroup: one as long as that does not fill the card, then eight, which share a search.
 // us (one / eight) at 2 KB a row: 48 rows 3.2 / 5.0, 1024 4.1 / 5.3, 2048 5.7 / 5.4; 16383 rows of 4 KB 55 / 29
@@ -82,42 +82,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
       if (active && whole && i < n) piece[j] = load_16(src + (r0 + i) * sT);
     }
     if (base == 0) {  // the rows are on their way: which of them stay?
-      if (tid < G) {
-        if (first >= (int64_t)a.total) {
-          *a.flag = 1;
-          first = -1;
-        }
-        place[tid] = first;
-        again[tid] = 0;
-      }
-      __syncthreads();
-      int64_t lo = -1, hi = -1;
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const int64_t s = place[i];
-        if (s < 0) continue;
-        lo = lo < 0 || s < lo ? s : lo;
-        hi = s > hi ? s : hi;
-      }
-      if (hi >= 0) {
-        constexpr int kAhead = 4;
-        for (int r = r0 + 1; r < a.rows; r += 256 * kAhead) {
-          int64_t s[kAhead];
-          int at[kAhead];
-#pragma unroll
-          for (int j = 0; j < kAhead; ++j) {
-            at[j] = r + tid + 256 * j < a.rows ? r + tid + 256 * j : a.rows - 1;
-            s[j] = slot(at[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < kAhead; ++j) {
-            if (s[j] < lo || s[j] > hi) continue;
-            for (int i = 0; i < G; ++i)
-              if (s[j] == place[i] && at[j] > r0 + i) again[i] = 1;
-          }
-        }
-      }
-      __syncthreads();
+      slots_that_stay<G>(slot, r0, a.rows, first, a.total, a.flag, place, again);
     }
     if (!active) continue;
 #pragma unroll

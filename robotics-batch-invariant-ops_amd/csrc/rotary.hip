@@ -15,17 +15,9 @@
 // The video case (32768 tokens, 16 + 4 heads of 128 in bf16, 336 MB): 66.5 us, 5.05 TB/s, the rate of a plain
 // copy.  4100 tokens of 16 + 16 float32 heads of 72: 17.4 us (a copy 15).  16 tokens: 3.5 us, a launch.
 // (Stores past the caches take 3 to 25 % less by themselves, and nothing off the rotation and its reader together.)
-#include "biops_common.h"
+#include "rotary.h"
 
 namespace biops {
-
-constexpr int kRotaryPairs = 128;  // most pairs (a head size of 256 rotated whole)
-
-struct RotaryTensor {
-  const char* x;
-  char* y;
-  int64_t xB, xT, xH, yB, yT, yH;  // byte strides: batch, token, head
-};
 
 struct RotaryArgs {
   double turns[kRotaryPairs];  // f_i / 2 pi
@@ -42,42 +34,6 @@ struct RotaryArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ void unpack(const u32x4_t& v, float (&x)[16 / sizeof(T)]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = Num<T>::from_bits(v[i] & 0xffffu);
-      x[2 * i + 1] = Num<T>::from_bits(v[i] >> 16);
-    }
-  }
-}
-template <typename T>
-__device__ __forceinline__ u32x4_t pack(const float (&x)[16 / sizeof(T)]) {
-  u32x4_t v;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(x[i]);
-  } else if constexpr (std::is_same<T, bf16_t>::value) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = f32x2_to_bf16x2_bits(x[2 * i], x[2 * i + 1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = f32x2_to_f16x2_bits(x[2 * i], x[2 * i + 1]);
-  }
-  return v;
-}
-__device__ __forceinline__ void store_16(void* p, const u32x4_t& v) { *reinterpret_cast<u32x4_any_t*>(p) = v; }
-
-__device__ __forceinline__ void turn(float& x0, float& x1, float c, float s) {
-  const float y0 = __builtin_fmaf(x0, c, -(x1 * s)), y1 = __builtin_fmaf(x1, c, x0 * s);
-  x0 = y0;
-  x1 = y1;
-}
-
-template <typename T>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   extern __shared__ __attribute__((aligned(16))) float table[];  // [token][cos, sin][pairs padded to 8]
   constexpr int E = sizeof(T), VEC = 16 / E;
@@ -86,8 +42,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   const int tid = threadIdx.x;
   const int S = a.pairs, SP = (S + 7) & ~7;
   const int heads = a.heads[0] + a.heads[1];
-  // pieces of a head: VEC pairs (both halves) or VEC / 2 neighbouring pairs, then what is copied
-  const int np = a.neighbours ? (2 * S + VEC - 1) / VEC : (S + VEC - 1) / VEC;
+  const int np = rotary_pieces<T>(S, a.neighbours);
   const int units = np + (a.d - 2 * S + VEC - 1) / VEC;
   for (int64_t t0 = (int64_t)blockIdx.x * a.group; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.group) {
     const int n = a.tokens - t0 < a.group ? (int)(a.tokens - t0) : a.group;
@@ -95,13 +50,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       const int tok = i / S, j = i - tok * S;
       const int64_t t = t0 + tok, b = t / a.per_batch;
       const int64_t at = args->axis[j] * a.pA + b * a.pB + (t - b * a.per_batch) * a.pT;
-      double p;
-      if (a.pos_type == 0) p = (double)reinterpret_cast<const int64_t*>(a.pos)[at];
-      else if (a.pos_type == 1) p = (double)reinterpret_cast<const int32_t*>(a.pos)[at];
-      else p = (double)reinterpret_cast<const float*>(a.pos)[at];
-      const double r = p * args->turns[j];
       float s, c;
-      sincospif(2.f * (float)(r - rint(r)), &s, &c);
+      rotary_angle(a.pos, a.pos_type, at, args->turns[j], c, s);
       table[tok * 2 * SP + j] = c;
       table[tok * 2 * SP + SP + j] = s * a.sign;
     }
@@ -117,46 +67,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       const T* src = reinterpret_cast<const T*>(x.x + b * x.xB + tb * x.xT + h * x.xH);
       T* dst = reinterpret_cast<T*>(x.y + b * x.yB + tb * x.yT + h * x.yH);
       const float* cs = table + tok * 2 * SP;
-      if (c >= np) {  // copied
-        const int e0 = 2 * S + (c - np) * VEC;
-        if (e0 + VEC <= a.d) store_16(dst + e0, load_16(src + e0));
-        else
-          for (int e = e0; e < a.d; ++e) dst[e] = src[e];
-      } else if (a.neighbours) {
-        const int e0 = c * VEC;
-        if (e0 + VEC <= 2 * S) {
-          float v[VEC];
-          unpack<T>(load_16(src + e0), v);
-#pragma unroll
-          for (int i = 0; i < VEC / 2; ++i) turn(v[2 * i], v[2 * i + 1], cs[e0 / 2 + i], cs[SP + e0 / 2 + i]);
-          store_16(dst + e0, pack<T>(v));
-        } else {
-          for (int e = e0; e < 2 * S; e += 2) {
-            float v0 = Num<T>::load(src + e), v1 = Num<T>::load(src + e + 1);
-            turn(v0, v1, cs[e / 2], cs[SP + e / 2]);
-            Num<T>::store(dst + e, v0);
-            Num<T>::store(dst + e + 1, v1);
-          }
-        }
-      } else {
-        const int e0 = c * VEC;
-        if (e0 + VEC <= S) {
-          float v0[VEC], v1[VEC];
-          unpack<T>(load_16(src + e0), v0);
-          unpack<T>(load_16(src + S + e0), v1);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) turn(v0[i], v1[i], cs[e0 + i], cs[SP + e0 + i]);
-          store_16(dst + e0, pack<T>(v0));
-          store_16(dst + S + e0, pack<T>(v1));
-        } else {
-          for (int e = e0; e < S; ++e) {
-            float v0 = Num<T>::load(src + e), v1 = Num<T>::load(src + S + e);
-            turn(v0, v1, cs[e], cs[SP + e]);
-            Num<T>::store(dst + e, v0);
-            Num<T>::store(dst + S + e, v1);
-          }
-        }
-      }
+      rotary_piece<T>(c, np, src, dst, cs, S, SP, a.d, a.neighbours);
     }
     __syncthreads();
   }
