@@ -512,8 +512,11 @@ int64_t biops_window_attention_workspace_size(int64_t nseq, int64_t hq, int64_t 
  * 4, 6).  The power is the smallest of which no element is more than 7, within [2^-125, 2^125] (bf16 rows) or
  * [2^-23, 2^13] (fp16 rows); elements go to the nearest level, ties to the even code, past 6 to 6. */
 
+/* Workspace bytes of biops_rotary_write (0: none needed), 8-byte aligned. */
+int64_t biops_rotary_write_workspace_size(int64_t rows);
+
 /* biops_rotary of q [rows, hq, d] (-> oq) and k [rows, hk, d], and biops_paged_write of the rotated keys and of v [rows, hk, dv],
- * with their bits, in one launch for each 8192 rows.  ks and vs null: caches of dtype; otherwise caches in 4 bits (fp16 or
+ * with their bits, in one launch (more than 1024 rows: two for each 65536).  ks and vs null: caches of dtype; otherwise caches in 4 bits (fp16 or
  * bf16 rows, d and dv multiples of 32), of rotated keys rounded to dtype.  hq may be 0, and pairs 0 (positions, turns and axis
  * then null).  Rows and caches must not share memory. */
 int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t hk, int64_t d, int64_t dv,
@@ -523,7 +526,7 @@ int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t hk, int64_t 
                        void* vc, int64_t svcP, int64_t svcS, int64_t svcH, void* vs, int64_t svsP, int64_t svsS, int64_t svsH,
                        int64_t pages, int64_t page_size, const void* slots, int slots64, int64_t slot_stride,
                        const void* positions, int pos_type, int64_t spA, int64_t spT, int64_t pairs, const double* turns,
-                       const uint8_t* axis, int neighbours, int* flag, void* stream);
+                       const uint8_t* axis, int neighbours, int* flag, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Keys ok [rows, heads, d] and values ov [rows, heads, dv] (contiguous, fp16 or bf16) of the slots of a cache in 4 bits.
  * Negative slots give zeros; slots past the cache too, with the flag. */

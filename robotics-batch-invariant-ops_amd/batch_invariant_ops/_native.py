@@ -126,8 +126,9 @@ _SIGNATURES = {
     "biops_rotary_write": (
         _i,
         [_i, _l, _l, _l, _l, _l] + [_p, _l, _l] * 4 + [_p, _l, _l, _l] * 4 + [_l, _l, _p, _i, _l] + [_p, _i, _l, _l, _l, _p, _p, _i]
-        + [_p, _p],
+        + [_p, _p, _l, _p],
     ),
+    "biops_rotary_write_workspace_size": (_l, [_l]),
     "biops_paged_read_fp4": (_i, [_i, _l, _l, _l, _l] + [_p, _l, _l, _l] * 4 + [_l, _l, _p, _i, _l] + [_p] * 4),
     "biops_paged_attention_fp4": (
         _i,

@@ -26,6 +26,7 @@ from collections.abc import Sequence
 import torch
 
 from . import _native as nat
+from . import decoder
 from .decoder import (
     _INDEX_TYPES,
     _POSITION_CODE,
@@ -34,6 +35,8 @@ from .decoder import (
     _check_scale,
     _check_tensors,
     _check_window,
+    _direct,
+    _direct_watch,
     _fn,
     _overlaps,
     _refuse_transforms,
@@ -122,6 +125,8 @@ def _write(what, query, key, value, caches, scales, slots, positions, plan):
     def at(t, first):
         return (None, *([0] * (t.dim() - 1 - first))) if t is None else (t.data_ptr(), *t.stride()[first:-1])
 
+    need = _fn("biops_rotary_write_workspace_size")(rows)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     kc, vc = caches
     ks, vs = scales if scales is not None else (None, None)
     none4 = (None, 0, 0, 0)
@@ -132,7 +137,7 @@ def _write(what, query, key, value, caches, scales, slots, positions, plan):
           *((None, 0, 0, 0, 0, None, None, 0) if q is None else
             (positions.data_ptr(), _POSITION_CODE[positions.dtype], positions.stride(0), positions.stride(1), plan.pairs,
              plan.turns_at, plan.axis_at, plan.neighbours)),
-          watch.flag.data_ptr(), nat.stream_of(k))
+          watch.flag.data_ptr(), None if ws is None else ws.data_ptr(), need, nat.stream_of(k))
     # autograd has to know of the change, as of any other in place
     torch.autograd.graph.increment_version([c for c in (*caches, *(scales or ())) if not c.is_inference()])
     watch.after_call(nat.stream_of(k))
@@ -186,6 +191,13 @@ def rotary_cache_write(
     """
     plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(map(float, inv_freq)),
                         bool(interleaved_axes), bool(interleaved_pairs))
+    module, watch = _direct_watch()
+    if module:
+        out = module.rotary_write(query, key, value, key_cache, value_cache, slots, positions, key_scales, value_scales, len(sections),
+                                  plan.pairs, plan.turns_at, plan.axis_at, plan.neighbours, watch.flag_at)
+        if out is not None:
+            watch.after_call()
+            return out
     if (key_scales is None) != (value_scales is None):
         raise ValueError("key_scales and value_scales are given together, or neither")
     scales = () if key_scales is None else (key_scales, value_scales)
@@ -227,6 +239,11 @@ def paged_cache_write_fp4(
     """``paged_cache_write`` into a cache in 4 bits (see the module): rows of bfloat16 or float16 keys ``[..., kv_heads,
     head_dim]`` and values ``[..., kv_heads, value_dim]``, each block to its power of two and its elements to the nearest level
     (ties to the even code), in place.  Slots are as there; the rows must not lie in the memory of the caches."""
+    module, watch = _direct_watch()
+    if module and module.rotary_write(None, key, value, key_cache, value_cache, slots, None, key_scales, value_scales, 0, 0, 0, 0, 0,
+                                      watch.flag_at):
+        watch.after_call()
+        return
     _refuse_transforms("paged_cache_write_fp4", key, value, key_cache, key_scales, value_cache, value_scales)
     _check_rows(key, value, slots)
     _check_fp4_rows(key, value, key_cache, key_scales, value_cache, value_scales)
@@ -249,6 +266,12 @@ def paged_cache_read_fp4(
     cache in 4 bits (see the module), as attention sees them: for the prefix of a longer prompt, for example.  Exact in the
     type of the rows that were written.  A negative slot gives zeros; one past the cache too, and is reported as an error
     later."""
+    module, watch = _direct_watch()
+    if module and dtype in _HALVES:
+        out = module.paged_read4(key_cache, key_scales, value_cache, value_scales, slots, nat.DIRECT_DTYPES[dtype], watch.flag_at)
+        if out is not None:
+            watch.after_call()
+            return out
     _refuse_transforms("paged_cache_read_fp4", key_cache, key_scales, value_cache, value_scales)
     d, dv = _check_fp4(key_cache, key_scales, value_cache, value_scales)
     if dtype not in _HALVES:
@@ -291,6 +314,13 @@ def paged_attention_fp4_batch_invariant(
     and sums are in 32 bits, with one rounding to the output's type, and products take the weights as two 16-bit parts.
     Returns ``[batch, heads, value_dim]``.
     """
+    module, watch = _direct_watch()
+    if module and window != 0 and (max_length is None or max_length >= 0):
+        out = module.paged_attention4(query, key_cache, key_scales, value_cache, value_scales, block_table, lengths, scale,
+                                      0 if window is None else window, sinks, -1 if max_length is None else max_length, watch.flag_at)
+        if out is not None:
+            watch.after_call()
+            return out
     _refuse_transforms("paged_attention_fp4_batch_invariant", query, key_cache, key_scales, value_cache, value_scales)
     d, dv = _check_fp4(key_cache, key_scales, value_cache, value_scales)
     if query.dim() != 3:
@@ -381,6 +411,11 @@ def sample_tokens_batch_invariant(
     Logits of NaN count as -inf, which are never chosen; a row without any other gives -1.  Where logits are +inf only those
     can be chosen.  Sums are of 64-bit weights and exact, so a token does not depend on the batch.  Up to 2**20 tokens and 65536 rows.
     """
+    module = decoder._tensor_module or _direct()
+    if module:
+        out = module.sample(logits, uniforms, temperature, top_k, top_p, min_p)
+        if out is not None:
+            return out
     settings = [x for x in (temperature, top_k, top_p, min_p) if isinstance(x, torch.Tensor)]
     _refuse_transforms("sample_tokens_batch_invariant", logits, uniforms)
     if logits.dim() < 1 or logits.dtype not in nat.DIRECT_DTYPES:
@@ -426,6 +461,11 @@ def quantize_tokens_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     (float32, ``[...]``): with ``m`` the row's largest magnitude, ``step = m / 127`` and ``q = round(x * (127 / m))``, in 32-bit
     arithmetic, ties to even.  (``m`` counts as at least 2**-100.)  A row with an infinity or NaN has a step of NaN and
     zeros.  At most 131071 features."""
+    module = decoder._tensor_module or _direct()
+    if module:
+        out = module.quantize8(x)
+        if out is not None:
+            return out
     _refuse_transforms("quantize_tokens_int8", x)
     if x.dim() < 1 or x.dtype not in nat.DIRECT_DTYPES:
         raise ValueError(f"rows must be float32, float16 or bfloat16 of shape [..., features], got {x.dtype} {tuple(x.shape)}")
@@ -458,6 +498,11 @@ def linear_int8_batch_invariant(
 
     The integer sums are exact (32 bits; at most 131071 terms), what follows is in 32-bit floats with one rounding, so the
     bits depend neither on the other rows nor on how the work is split."""
+    module = decoder._tensor_module or _direct()
+    if module:
+        out = module.linear8(x, x_scale, weight, weight_scale, bias, nat.DIRECT_DTYPES.get(dtype, -1))
+        if out is not None:
+            return out
     tensors = (x, x_scale, weight, weight_scale) if bias is None else (x, x_scale, weight, weight_scale, bias)
     _refuse_transforms("linear_int8_batch_invariant", *tensors)
     if x.dim() < 1 or weight.dim() != 2 or x.dtype != torch.int8 or weight.dtype != torch.int8:

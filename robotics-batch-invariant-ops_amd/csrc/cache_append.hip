@@ -27,6 +27,7 @@ struct AppendArgs {
   const void *pos, *slots;
   int64_t pA, pT, slot_stride;                               // element strides
   int* flag;
+  uint8_t* stays;                                            // [row][kStayParts] whether no part of the later rows has its slot (null: to be found here)
   uint32_t total, page;                                      // slots of the cache, slots of a page
   int rows, hq, hk, d, dv, pairs, pos_type, neighbours, slots64;
 };
@@ -89,8 +90,78 @@ __device__ __forceinline__ void store_eight(const float (&y)[8], int e0, char* d
   if (e0 % kFp4Block == 0) exponents[e0 / kFp4Block] = (char)e;
 }
 
-// FOUR: the cache is in 4 bits (T: bf16 or fp16); G: rows of a workgroup.
-template <typename T, bool FOUR, int G>
+__device__ __forceinline__ int64_t slot_of(const AppendArgs& a, int r) {
+  return a.slots64 ? reinterpret_cast<const int64_t*>(a.slots)[r * a.slot_stride]
+                   : (int64_t) reinterpret_cast<const int32_t*>(a.slots)[r * a.slot_stride];
+}
+
+// Which of many rows stay.  A workgroup has 256 rows and one part of the later ones: its slots go into a table in LDS, with the
+// last of its rows that names each, and the later slots are looked up there where they lie between the smallest and the
+// largest of its own.
+constexpr int kStayRows = 65536;  // rows of a launch: the later ones are read by every workgroup
+constexpr int kStayParts = 8;
+__global__ __launch_bounds__(256) void stays_kernel(AppendArgs a) {
+  constexpr int kPlaces = 1024;
+  constexpr uint32_t kNone = 0xffffffffu;
+  __shared__ uint32_t slots[kPlaces];
+  __shared__ int last[kPlaces];
+  __shared__ uint32_t lows[4], highs[4];
+  const int tid = threadIdx.x, part = blockIdx.x % kStayParts, first = blockIdx.x / kStayParts * 256, r = first + tid;
+  for (int i = tid; i < kPlaces; i += 256) {
+    slots[i] = kNone;
+    last[i] = -1;
+  }
+  const int64_t named = r < a.rows ? slot_of(a, r) : -1;
+  const bool inside = named >= 0 && named < (int64_t)a.total;
+  if (named >= (int64_t)a.total) *a.flag = 1;
+  const uint32_t slot = (uint32_t)named;
+  auto place = [](uint32_t s) { return (s * 2654435761u) >> 22; };
+  uint32_t low = inside ? slot : kNone, high = inside ? slot : 0u;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t x = (uint32_t)__shfl_xor((int)low, o, 64), y = (uint32_t)__shfl_xor((int)high, o, 64);
+    low = x < low ? x : low;
+    high = y > high ? y : high;
+  }
+  if ((tid & 63) == 0) {
+    lows[tid >> 6] = low;
+    highs[tid >> 6] = high;
+  }
+  __syncthreads();
+  uint32_t at = 0;
+  if (inside) {
+    for (at = place(slot);; at = (at + 1) % kPlaces) {  // (at most 256 of the 1024 places are taken)
+      const uint32_t was = atomicCAS(&slots[at], kNone, slot);
+      if (was == kNone || was == slot) break;
+    }
+    atomicMax(&last[at], r);
+  }
+  for (int i = 0; i < 4; ++i) {
+    low = lows[i] < low ? lows[i] : low;
+    high = highs[i] > high ? highs[i] : high;
+  }
+  __syncthreads();
+  constexpr int kAhead = 8;
+  for (int base = first + 256 + 256 * kAhead * part; base < a.rows && low <= high; base += 256 * kAhead * kStayParts) {
+    int64_t s[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) s[j] = base + 256 * j + tid < a.rows ? slot_of(a, base + 256 * j + tid) : -1;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (s[j] < (int64_t)low || s[j] > (int64_t)high) continue;
+      for (uint32_t i = place((uint32_t)s[j]); slots[i] != kNone; i = (i + 1) % kPlaces)
+        if (slots[i] == (uint32_t)s[j]) {
+          last[i] = a.rows;
+          break;
+        }
+    }
+  }
+  __syncthreads();
+  if (r < a.rows) a.stays[(int64_t)r * kStayParts + part] = inside && last[at] == r;
+}
+
+// FOUR: the cache is in 4 bits (T: bf16 or fp16); G: rows of a workgroup; FEW: which rows stay is found here.
+template <typename T, bool FOUR, int G, bool FEW>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   extern __shared__ __attribute__((aligned(16))) float table[];  // [row][cos, sin][pairs padded to 8]
   __shared__ int64_t place[G];
@@ -102,12 +173,14 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int r0 = blockIdx.x * G;
   const int n = a.rows - r0 < G ? a.rows - r0 : G;
   const int S = a.pairs, SP = (S + 7) & ~7;
-  auto slot = [&](int r) -> int64_t {
-    return a.slots64 ? reinterpret_cast<const int64_t*>(a.slots)[r * a.slot_stride]
-                     : (int64_t) reinterpret_cast<const int32_t*>(a.slots)[r * a.slot_stride];
-  };
   int64_t first = -1;
-  if (tid < n) first = slot(r0 + tid);
+  if (tid < n) first = slot_of(a, r0 + tid);
+  if constexpr (!FEW)
+    if (tid < G) {
+      static_assert(kStayParts == 8, "a row's parts in 8 bytes");
+      place[tid] = tid < n && reinterpret_cast<const uint64_t*>(a.stays)[r0 + tid] == 0x0101010101010101ull ? first : -1;
+      again[tid] = 0;
+    }
   for (int i = tid; i < n * S; i += 256) {
     const int r = i / S, j = i - r * S;
     float c, s;
@@ -115,7 +188,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     table[r * 2 * SP + j] = c;
     table[r * 2 * SP + SP + j] = s;
   }
-  slots_that_stay<G>(slot, r0, a.rows, first, a.total, a.flag, place, again);
+  if constexpr (FEW) slots_that_stay<G>([&](int r) { return slot_of(a, r); }, r0, a.rows, first, a.total, a.flag, place, again);
+  else __syncthreads();
 
   // pieces: keys, values (in 4 bits a multiple of four each, so that a block's four lanes are together), queries
   const int np = rotary_pieces<T>(S, a.neighbours), whole = np + (a.d - 2 * S + VEC - 1) / VEC;
@@ -162,14 +236,19 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   }
 }
 
+constexpr int kStayFew = 1024;  // rows up to which each workgroup looks for later rows itself
+
 template <typename T, bool FOUR>
 static int append_launch(const AppendArgs& a, hipStream_t s) {
-  constexpr int kFew = 1024, kGroup = 4;
-  const int group = a.rows <= kFew ? 1 : kGroup;
-  const dim3 grid((unsigned)cdiv(a.rows, group));
-  const unsigned lds = (unsigned)(group * 2 * ((a.pairs + 7) & ~7) * sizeof(float));
-  if (group == 1) hipLaunchKernelGGL((append_kernel<T, FOUR, 1>), grid, dim3(256), lds, s, a);
-  else hipLaunchKernelGGL((append_kernel<T, FOUR, kGroup>), grid, dim3(256), lds, s, a);
+  constexpr int kGroup = 4;
+  const unsigned table = (unsigned)(2 * ((a.pairs + 7) & ~7) * sizeof(float));
+  if (a.stays == nullptr) {
+    hipLaunchKernelGGL((append_kernel<T, FOUR, 1, true>), dim3((unsigned)a.rows), dim3(256), table, s, a);
+    return check_launch("append_kernel");
+  }
+  hipLaunchKernelGGL(stays_kernel, dim3((unsigned)(cdiv(a.rows, 256) * kStayParts)), dim3(256), 0, s, a);
+  if (const int rc = check_launch("stays_kernel")) return rc;
+  hipLaunchKernelGGL((append_kernel<T, FOUR, kGroup, false>), dim3((unsigned)cdiv(a.rows, kGroup)), dim3(256), kGroup * table, s, a);
   return check_launch("append_kernel");
 }
 
@@ -186,32 +265,51 @@ struct ReadArgs {
   int heads, d, dv, slots64;
 };
 
-// Eight elements a thread and step; pieces of a row are its heads' keys, then its heads' values.
+// Eight elements a piece; pieces of a row are its heads' keys, then its heads' values.  A thread has kReadAhead pieces, 256 apart,
+// whose loads go out together.
+constexpr int kReadAhead = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void read4_kernel(ReadArgs a) {
   const int kn = a.heads * (a.d / 8), per_row = kn + a.heads * (a.dv / 8);
   const int64_t all = a.rows * per_row;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < all; u += (int64_t)gridDim.x * 256) {
-    const int64_t r = u / per_row;
+  const int64_t u0 = (int64_t)blockIdx.x * (256 * kReadAhead) + threadIdx.x;
+  int64_t s[kReadAhead];
+  int h[kReadAhead], e0[kReadAhead];
+  bool value[kReadAhead];
+  char* to[kReadAhead];
+#pragma unroll
+  for (int i = 0; i < kReadAhead; ++i) {
+    const int64_t u = u0 + 256 * i, r = u / per_row;
     int x = (int)(u - r * per_row);
-    const bool value = x >= kn;
-    if (value) x -= kn;
-    const int width = value ? a.dv : a.d;
-    const int h = x / (width / 8), e0 = 8 * (x - h * (width / 8));
-    const int64_t s = a.slots64 ? reinterpret_cast<const int64_t*>(a.slots)[r * a.slot_stride]
-                                : (int64_t) reinterpret_cast<const int32_t*>(a.slots)[r * a.slot_stride];
-    u32x4_t y = {0u, 0u, 0u, 0u};
-    if (s >= 0 && s < (int64_t)a.total) {
-      const uint32_t page = (uint32_t)s / a.page, at = (uint32_t)s - page * a.page;
-      const char* data = value ? a.vc + page * a.vcP + at * a.vcS + h * a.vcH : a.kc + page * a.kcP + at * a.kcS + h * a.kcH;
-      const char* exps = value ? a.vs + page * a.vsP + at * a.vsS + h * a.vsH : a.ks + page * a.ksP + at * a.ksS + h * a.ksH;
-      const uint32_t e = (uint8_t)exps[e0 / kFp4Block];
-      y = fp4_values<T>(*reinterpret_cast<const u32_byte_t*>(data + (e0 >> 1)), __uint_as_float(e << 23));
-    } else if (s >= 0) {
+    value[i] = x >= kn;
+    if (value[i]) x -= kn;
+    const int width = value[i] ? a.dv : a.d;
+    h[i] = x / (width / 8);
+    e0[i] = 8 * (x - h[i] * (width / 8));
+    to[i] = (value[i] ? a.ov : a.ok) + 2 * ((r * a.heads + h[i]) * width + e0[i]);
+    s[i] = -1;
+    if (u < all)
+      s[i] = a.slots64 ? reinterpret_cast<const int64_t*>(a.slots)[r * a.slot_stride]
+                       : (int64_t) reinterpret_cast<const int32_t*>(a.slots)[r * a.slot_stride];
+  }
+  uint32_t codes[kReadAhead], e[kReadAhead];
+#pragma unroll
+  for (int i = 0; i < kReadAhead; ++i) {
+    codes[i] = 0u;
+    e[i] = 127u;
+    if (s[i] >= 0 && s[i] < (int64_t)a.total) {
+      const uint32_t page = (uint32_t)s[i] / a.page, at = (uint32_t)s[i] - page * a.page;
+      const char* data = value[i] ? a.vc + page * a.vcP + at * a.vcS + h[i] * a.vcH : a.kc + page * a.kcP + at * a.kcS + h[i] * a.kcH;
+      const char* exps = value[i] ? a.vs + page * a.vsP + at * a.vsS + h[i] * a.vsH : a.ks + page * a.ksP + at * a.ksS + h[i] * a.ksH;
+      codes[i] = *reinterpret_cast<const u32_byte_t*>(data + (e0[i] >> 1));
+      e[i] = (uint8_t)exps[e0[i] / kFp4Block];
+    } else if (s[i] >= 0) {
       *a.flag = 1;
     }
-    store_16((value ? a.ov : a.ok) + 2 * ((r * a.heads + h) * width + e0), y);
   }
+#pragma unroll
+  for (int i = 0; i < kReadAhead; ++i)
+    if (u0 + 256 * i < all) store_16(to[i], fp4_values<T>(codes[i], __uint_as_float(e[i] << 23)));
 }
 
 }  // namespace biops
@@ -227,6 +325,10 @@ static int append_sizes(const char* what, int64_t rows, int64_t hq, int64_t hk, 
   return BIOPS_OK;
 }
 
+extern "C" int64_t biops_rotary_write_workspace_size(int64_t rows) {
+  return rows <= kStayFew ? 0 : (rows < kStayRows ? rows : kStayRows) * kStayParts;
+}
+
 extern "C" int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t hk, int64_t d, int64_t dv, const void* q,
                                   int64_t sqT, int64_t sqH, void* oq, int64_t soqT, int64_t soqH, const void* k, int64_t skT,
                                   int64_t skH, const void* v, int64_t svT, int64_t svH, void* kc, int64_t skcP, int64_t skcS,
@@ -234,7 +336,7 @@ extern "C" int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t h
                                   int64_t svcS, int64_t svcH, void* vs, int64_t svsP, int64_t svsS, int64_t svsH, int64_t pages,
                                   int64_t page_size, const void* slots, int slots64, int64_t slot_stride, const void* positions,
                                   int pos_type, int64_t spA, int64_t spT, int64_t pairs, const double* turns, const uint8_t* axis,
-                                  int neighbours, int* flag, void* stream) {
+                                  int neighbours, int* flag, void* workspace, int64_t workspace_bytes, void* stream) {
   const int elt = is_float_dtype(dtype) ? dtype_bytes(dtype) : 0;
   const bool four = ks != nullptr || vs != nullptr;
   if (elt == 0 || (four && elt != 2)) return fail(BIOPS_ERR_DTYPE, "biops_rotary_write: unsupported dtype %d", dtype);
@@ -250,7 +352,12 @@ extern "C" int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t h
     return fail(BIOPS_ERR_ARG, "biops_rotary_write: null pointer");
   if (pages * page_size > 0 && ((hk * d > 0 && (!kc || (four && !ks))) || (hk * dv > 0 && (!vc || (four && !vs)))))
     return fail(BIOPS_ERR_ARG, "biops_rotary_write: null cache");
+  const int64_t need = biops_rotary_write_workspace_size(rows);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(BIOPS_ERR_SIZE, "biops_rotary_write: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  if (need > 0 && reinterpret_cast<uintptr_t>(workspace) % 8) return fail(BIOPS_ERR_LAYOUT, "biops_rotary_write: workspace not 8-byte aligned");
   AppendArgs a;
+  a.stays = need > 0 ? static_cast<uint8_t*>(workspace) : nullptr;
   for (int i = 0; i < kRotaryPairs; ++i) {
     a.turns[i] = i < pairs ? turns[i] : 0.0;
     a.axis[i] = i < pairs ? axis[i] : 0;
@@ -267,8 +374,8 @@ extern "C" int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t h
   a.hq = (int)hq, a.hk = (int)hk, a.d = (int)d, a.dv = (int)dv, a.pairs = (int)pairs;
   a.pos_type = pos_type, a.neighbours = neighbours != 0, a.slots64 = slots64 != 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  for (int64_t r = 0; r < rows; r += kWriteRows) {
-    a.rows = (int)(rows - r < kWriteRows ? rows - r : kWriteRows);
+  for (int64_t r = 0; r < rows; r += kStayRows) {
+    a.rows = (int)(rows - r < kStayRows ? rows - r : kStayRows);
     a.q = static_cast<const char*>(q) + r * a.qT, a.oq = static_cast<char*>(oq) + r * a.oqT;
     a.k = static_cast<const char*>(k) + r * a.kT, a.v = static_cast<const char*>(v) + r * a.vT;
     a.pos = static_cast<const char*>(positions) + r * spT * (pos_type == 0 ? 8 : 4);
@@ -303,8 +410,9 @@ extern "C" int biops_paged_read_fp4(int dtype, int64_t rows, int64_t heads, int6
   a.slots = slots, a.slot_stride = slot_stride, a.flag = flag, a.slots64 = slots64 != 0;
   a.total = (uint32_t)(pages * page_size), a.page = page_size > 0 ? (uint32_t)page_size : 1u;
   a.rows = rows, a.heads = (int)heads, a.d = (int)d, a.dv = (int)dv;
-  const int64_t blocks = cdiv(rows * heads * ((d + dv) / 8), 256);
-  const dim3 grid((unsigned)(blocks < (1 << 22) ? blocks : (1 << 22)));
+  const int64_t blocks = cdiv(rows * heads * ((d + dv) / 8), 256 * kReadAhead);
+  if (blocks >= (1 << 24)) return fail(BIOPS_ERR_SIZE, "biops_paged_read_fp4: more than 2^24 blocks of 8192 elements");  // (2^32 threads)
+  const dim3 grid((unsigned)blocks);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == BIOPS_F16) hipLaunchKernelGGL((read4_kernel<f16_t>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((read4_kernel<bf16_t>), grid, dim3(256), 0, s, a);

@@ -384,6 +384,259 @@ PyObject* window_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// ---- the operators of a decoder served with fewer bits ----
+bool bytes4(const at::Tensor& t) { return t.scalar_type() == at::kByte && t.dim() == 4 && unit_last(t); }
+// Caches in 4 bits and their scales that belong together.
+bool caches4(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs) {
+  if (!bytes4(kc) || !bytes4(ks) || !bytes4(vc) || !bytes4(vs)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (ks.size(i) != kc.size(i) || vc.size(i) != kc.size(i) || vs.size(i) != kc.size(i)) return false;
+  return kc.size(3) == 16 * ks.size(3) && vc.size(3) == 16 * vs.size(3);
+}
+// Tensors that a call writes: each whole in memory, and no allocation shared with another one or with what is read.
+template <size_t N, size_t M>
+bool apart(const at::Tensor* const (&written)[N], const at::Tensor* const (&read)[M]) {
+  for (size_t i = 0; i < N; ++i) {
+    if (!written[i]) continue;
+    if (!written[i]->is_non_overlapping_and_dense()) return false;
+    for (size_t j = i + 1; j < N; ++j)
+      if (written[j] && written[i]->is_alias_of(*written[j])) return false;
+    for (const at::Tensor* r : read)
+      if (r && written[i]->is_alias_of(*r)) return false;
+  }
+  return true;
+}
+struct Strides4 {
+  char* at;
+  int64_t p, s, h;
+};
+Strides4 strides4(const at::Tensor* t) {
+  return t ? Strides4{ptr(*t), t->stride(0), t->stride(1), t->stride(2)} : Strides4{nullptr, 0, 0, 0};
+}
+void changed(const at::Tensor& t) {  // autograd has to know of the change, as of any other in place
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// rotary_write(query or None, key, value, key_cache, value_cache, slots, positions or None, key_scales or None, value_scales or
+//              None, axes, pairs, turns, axis, neighbours, flag) -> rotated query, or True without one   (three dimensions)
+PyObject* rotary_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 15) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  const bool rotates = args[0] != Py_None, four = args[7] != Py_None;
+  TAKE(k, args[1]);
+  TAKE(v, args[2]);
+  TAKE(kc, args[3]);
+  TAKE(vc, args[4]);
+  TAKE(slots, args[5]);
+  const at::Tensor* q = rotates ? take(args[0], device) : nullptr;
+  const at::Tensor* p = rotates ? take(args[6], device) : nullptr;
+  const at::Tensor* ks = four ? take(args[7], device) : nullptr;
+  const at::Tensor* vs = four ? take(args[8], device) : nullptr;
+  if ((rotates && (!q || !p)) || (four && (!ks || !vs)) || (!four && args[8] != Py_None)) Py_RETURN_NONE;
+  int64_t axes, pairs, turns, axis, neighbours, flag;
+  if (!number(args[9], &axes) || !number(args[10], &pairs) || !number(args[11], &turns) || !number(args[12], &axis) ||
+      !number(args[13], &neighbours) || !number(args[14], &flag))
+    Py_RETURN_NONE;
+  const int code = type_code(k.scalar_type());
+  if (code < 0 || v.scalar_type() != k.scalar_type() || k.dim() != 3 || v.dim() != 3 || !unit_last(k) || !unit_last(v) ||
+      k.size(0) != v.size(0) || k.size(1) != v.size(1))
+    Py_RETURN_NONE;
+  const int64_t rows = k.size(0), hk = k.size(1), d = k.size(2), dv = v.size(2);
+  if (slots.dim() != 1 || !is_index(slots) || slots.size(0) != rows) Py_RETURN_NONE;
+  if (four) {
+    if (code == BIOPS_F32 || !caches4(kc, *ks, vc, *vs) || kc.size(2) != hk || 2 * kc.size(3) != d || 2 * vc.size(3) != dv) Py_RETURN_NONE;
+  } else if (!caches(kc, vc) || kc.scalar_type() != k.scalar_type() || kc.size(2) != hk || kc.size(3) != d || vc.size(3) != dv) {
+    Py_RETURN_NONE;
+  }
+  if (rotates) {
+    if (q->dim() != 3 || !unit_last(*q) || q->scalar_type() != k.scalar_type() || q->size(0) != rows || q->size(2) != d || 2 * pairs > d)
+      Py_RETURN_NONE;
+    const bool known = p->scalar_type() == at::kLong || p->scalar_type() == at::kInt || p->scalar_type() == at::kFloat;
+    if (!known || p->dim() != 2 || p->size(0) != axes || p->size(1) != rows) Py_RETURN_NONE;
+  }
+  const at::Tensor *const written[] = {&kc, &vc, ks, vs}, *const read[] = {&k, &v, &slots, q, p};
+  if (!apart(written, read)) Py_RETURN_NONE;
+  at::Tensor out, ws;
+  if (rotates) out = at::empty(q->sizes(), q->options());
+  const int64_t need = biops_rotary_write_workspace_size(rows);
+  if (need > 0) ws = at::empty({need}, k.options().dtype(at::kByte));
+  const Strides4 a = strides4(&kc), b = strides4(ks), c = strides4(&vc), e = strides4(vs);
+  const int pos = !rotates || p->scalar_type() == at::kLong ? 0 : p->scalar_type() == at::kInt ? 1 : 2;
+  LAUNCH(rc, biops_rotary_write(
+                 code, rows, rotates ? q->size(1) : 0, hk, d, dv, rotates ? ptr(*q) : nullptr, rotates ? q->stride(0) : 0,
+                 rotates ? q->stride(1) : 0, rotates ? ptr(out) : nullptr, rotates ? out.stride(0) : 0, rotates ? out.stride(1) : 0,
+                 ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), a.at, a.p, a.s, a.h, b.at, b.p, b.s, b.h, c.at, c.p,
+                 c.s, c.h, e.at, e.p, e.s, e.h, kc.size(0), kc.size(1), ptr(slots), is_long(slots), slots.stride(0),
+                 rotates ? ptr(*p) : nullptr, pos, rotates ? p->stride(0) : 0, rotates ? p->stride(1) : 0, rotates ? pairs : 0,
+                 reinterpret_cast<const double*>(turns), reinterpret_cast<const uint8_t*>(axis), (int)neighbours,
+                 reinterpret_cast<int*>(flag), need > 0 ? ptr(ws) : nullptr, need, stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  for (const at::Tensor* t : written)
+    if (t) changed(*t);
+  if (!rotates) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// paged_read4(key_cache, key_scales, value_cache, value_scales, slots, dtype code, flag) -> (key, value)
+PyObject* paged_read4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(kc, args[0]);
+  TAKE(ks, args[1]);
+  TAKE(vc, args[2]);
+  TAKE(vs, args[3]);
+  TAKE(slots, args[4]);
+  int64_t code, flag;
+  if (!number(args[5], &code) || !number(args[6], &flag) || (code != BIOPS_F16 && code != BIOPS_BF16) || !caches4(kc, ks, vc, vs) ||
+      slots.dim() != 1 || !is_index(slots))
+    Py_RETURN_NONE;
+  const int64_t rows = slots.size(0), heads = kc.size(2), d = 2 * kc.size(3), dv = 2 * vc.size(3);
+  const auto options = kc.options().dtype(code == BIOPS_F16 ? at::kHalf : at::kBFloat16);
+  at::Tensor ok = at::empty({rows, heads, d}, options), ov = at::empty({rows, heads, dv}, options);
+  const Strides4 a = strides4(&kc), b = strides4(&ks), c = strides4(&vc), e = strides4(&vs);
+  LAUNCH(rc, biops_paged_read_fp4((int)code, rows, heads, d, dv, a.at, a.p, a.s, a.h, b.at, b.p, b.s, b.h, c.at, c.p, c.s, c.h, e.at, e.p,
+                                  e.s, e.h, kc.size(0), kc.size(1), ptr(slots), is_long(slots), slots.stride(0), ptr(ok), ptr(ov),
+                                  reinterpret_cast<int*>(flag), stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(ok)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(ov)));
+  return pair;
+}
+
+// paged_attention4(query, key_cache, key_scales, value_cache, value_scales, table, lengths, scale or None, window or 0, sinks,
+//                  max_length or -1, flag) -> output
+PyObject* paged_attention4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 12) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(q, args[0]);
+  TAKE(kc, args[1]);
+  TAKE(ks, args[2]);
+  TAKE(vc, args[3]);
+  TAKE(vs, args[4]);
+  TAKE(table, args[5]);
+  TAKE(lengths, args[6]);
+  int64_t window, sinks, bound, flag;
+  float scale;
+  const int code = type_code(q.scalar_type());
+  if (code < 0 || code == BIOPS_F32 || q.dim() != 3 || !unit_last(q) || !caches4(kc, ks, vc, vs)) Py_RETURN_NONE;
+  const int64_t batch = q.size(0), hq = q.size(1), hkv = kc.size(2), d = q.size(2), dv = 2 * vc.size(3);
+  if (!scale_of(args[7], d, &scale) || !number(args[8], &window) || !number(args[9], &sinks) || !number(args[10], &bound) ||
+      !number(args[11], &flag) || window < 0 || sinks < 0)
+    Py_RETURN_NONE;
+  if (d != 2 * kc.size(3) || hq % hkv != 0 || table.dim() != 2 || table.size(0) != batch || !is_index(table) || lengths.dim() != 1 ||
+      lengths.size(0) != batch || !is_index(lengths))
+    Py_RETURN_NONE;
+  const int64_t page = kc.size(1), width = table.size(1);
+  const int64_t need = biops_paged_attention_workspace_size(batch, hq, dv, width, page, bound, window, sinks);
+  if (need < 0) Py_RETURN_NONE;
+  at::Tensor out = at::empty({batch, hq, dv}, q.options());
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, kc.options());
+  const Strides4 a = strides4(&kc), b = strides4(&ks), c = strides4(&vc), e = strides4(&vs);
+  LAUNCH(rc, biops_paged_attention_fp4(code, batch, hq, hkv, d, dv, ptr(q), q.stride(0), q.stride(1), a.at, a.p, a.s, a.h, b.at, b.p, b.s,
+                                       b.h, c.at, c.p, c.s, c.h, e.at, e.p, e.s, e.h, kc.size(0), page, ptr(table), is_long(table),
+                                       table.stride(0), table.stride(1), width, ptr(lengths), is_long(lengths), lengths.stride(0), bound,
+                                       window, sinks, scale, ptr(out), reinterpret_cast<int*>(flag), need > 0 ? ptr(ws) : nullptr, need,
+                                       stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// A setting of sampling: a tensor with a value for each row, a number for all, or None.
+struct Setting {
+  const at::Tensor* each = nullptr;
+  double all = 0.0;
+  const void* at() const { return each ? each->data_ptr() : nullptr; }
+  int64_t stride() const { return each ? each->stride(0) : 0; }
+};
+bool setting(PyObject* o, int64_t rows, c10::DeviceIndex device, bool index, double otherwise, Setting* s) {
+  s->all = otherwise;
+  if (o == Py_None) return true;
+  if (PyFloat_CheckExact(o)) {
+    s->all = PyFloat_AS_DOUBLE(o);
+    return !index;
+  }
+  if (PyLong_CheckExact(o)) {
+    int64_t x;
+    if (!number(o, &x) || x > (INT64_C(1) << 52) || x < 0) return false;
+    s->all = (double)x;
+    return true;
+  }
+  s->each = take(o, device);
+  return s->each && s->each->dim() == 1 && s->each->size(0) == rows && (index ? is_index(*s->each) : s->each->scalar_type() == at::kFloat);
+}
+
+// sample(logits, uniforms, temperature, top_k, top_p, min_p) -> tokens   ([rows, vocab])
+PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(x, args[0]);
+  TAKE(u, args[1]);
+  const int code = type_code(x.scalar_type());
+  if (code < 0 || x.dim() != 2 || !unit_last(x) || u.scalar_type() != at::kFloat || u.dim() != 1 || u.size(0) != x.size(0)) Py_RETURN_NONE;
+  const int64_t rows = x.size(0), vocab = x.size(1);
+  Setting t, k, p, m;
+  if (!setting(args[2], rows, device, false, 1.0, &t) || !setting(args[3], rows, device, true, 0.0, &k) ||
+      !setting(args[4], rows, device, false, 1.0, &p) || !setting(args[5], rows, device, false, 0.0, &m))
+    Py_RETURN_NONE;
+  if (args[2] == Py_None || !(t.all >= 0.0 && t.all < INFINITY) || (args[3] != Py_None && !k.each && k.all < 1.0) ||
+      !(p.all > 0.0 && p.all <= 1.0) || !(m.all >= 0.0 && m.all <= 1.0))
+    Py_RETURN_NONE;
+  const int64_t need = biops_sample_workspace_size(rows, vocab);
+  if (need < 0) Py_RETURN_NONE;
+  at::Tensor out = at::empty({rows}, x.options().dtype(at::kLong)), ws = at::empty({need}, x.options().dtype(at::kByte));
+  LAUNCH(rc, biops_sample(code, rows, vocab, ptr(x), x.stride(0), u.const_data_ptr<float>(), u.stride(0), (const float*)t.at(), t.stride(),
+                          t.all, k.at(), k.each ? is_long(*k.each) : 0, k.stride(), (int64_t)std::min(k.all, 2097152.0),
+                          (const float*)p.at(), p.stride(), p.all, (const float*)m.at(), m.stride(), m.all, out.data_ptr<int64_t>(),
+                          ptr(ws), need, stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// quantize8(x) -> (integers, steps)   ([rows, features])
+PyObject* quantize8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 1) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(x, args[0]);
+  const int code = type_code(x.scalar_type());
+  if (code < 0 || x.dim() != 2 || !unit_last(x)) Py_RETURN_NONE;
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar)), s = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  LAUNCH(rc, biops_quantize_int8(code, x.size(0), x.size(1), ptr(x), x.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(q)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(s)));
+  return pair;
+}
+
+// linear8(x, x_scale, weight, weight_scale, bias or None, dtype code) -> output   ([rows, features])
+PyObject* linear8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) Py_RETURN_NONE;
+  const auto device = c10::hip::current_device();
+  TAKE(x, args[0]);
+  TAKE(xs, args[1]);
+  TAKE(w, args[2]);
+  TAKE(ws, args[3]);
+  const at::Tensor* bias = args[4] == Py_None ? nullptr : take(args[4], device);
+  int64_t code;
+  if ((!bias && args[4] != Py_None) || !number(args[5], &code)) Py_RETURN_NONE;
+  const auto type = code == BIOPS_F32 ? at::kFloat : code == BIOPS_F16 ? at::kHalf : at::kBFloat16;
+  if (code < BIOPS_F32 || code > BIOPS_BF16 || x.dim() != 2 || w.dim() != 2 || x.scalar_type() != at::kChar || w.scalar_type() != at::kChar ||
+      !unit_last(x) || !unit_last(w) || x.size(1) != w.size(1) || xs.dim() != 1 || ws.dim() != 1 || xs.scalar_type() != at::kFloat ||
+      ws.scalar_type() != at::kFloat || xs.size(0) != x.size(0) || ws.size(0) != w.size(0))
+    Py_RETURN_NONE;
+  if (bias && (bias->dim() != 1 || bias->size(0) != w.size(0) || bias->scalar_type() != type || !bias->is_contiguous())) Py_RETURN_NONE;
+  at::Tensor y = at::empty({x.size(0), w.size(0)}, x.options().dtype(type));
+  LAUNCH(rc, biops_linear_int8((int)code, x.size(0), w.size(0), x.size(1), (const int8_t*)ptr(x), x.stride(0), (const float*)ptr(xs), xs.stride(0),
+                               (const int8_t*)ptr(w), w.stride(0), (const float*)ptr(ws), ws.stride(0), bias ? ptr(*bias) : nullptr, ptr(y),
+                               stream_on(device)))
+  if (rc != BIOPS_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+}
+
 // C++ exceptions (out of memory) end here: the Python function then meets the same condition and raises it.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
@@ -407,6 +660,12 @@ PyMethodDef methods[] = {
     {"paged_attention", fast<paged_attention>(), METH_FASTCALL, "biops_paged_attention on tensors, or None"},
     {"window_attention", fast<window_attention>(), METH_FASTCALL, "biops_window_attention on dense tensors, or None"},
     {"window_packed", fast<window_packed>(), METH_FASTCALL, "biops_window_attention on packed tensors, or None"},
+    {"rotary_write", fast<rotary_write>(), METH_FASTCALL, "biops_rotary_write on tensors, or None"},
+    {"paged_read4", fast<paged_read4>(), METH_FASTCALL, "biops_paged_read_fp4 on tensors, or None"},
+    {"paged_attention4", fast<paged_attention4>(), METH_FASTCALL, "biops_paged_attention_fp4 on tensors, or None"},
+    {"sample", fast<sample>(), METH_FASTCALL, "biops_sample on tensors, or None"},
+    {"quantize8", fast<quantize8>(), METH_FASTCALL, "biops_quantize_int8 on tensors, or None"},
+    {"linear8", fast<linear8>(), METH_FASTCALL, "biops_linear_int8 on tensors, or None"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_biops_tensor", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -226,7 +226,7 @@ def rotary_write(dtype=2, rows=1, hq=2, hk=1, d=64, dv=64, q=P, k=P, kc=P, ks=No
     turns, axis = (ctypes.c_double * 128)(), (ctypes.c_uint8 * 128)()
     return entry("biops_rotary_write")(
         dtype, rows, hq, hk, d, dv, q, 1, 1, q, 1, 1, k, 1, 1, k, 1, 1, kc, 1, 1, 1, ks, 1, 1, 1, kc, 1, 1, 1, vs, 1, 1, 1, pages, page,
-        slots, 1, 1, pos, pos_type, 1, 1, pairs, ctypes.cast(turns, ctypes.c_void_p), ctypes.cast(axis, ctypes.c_void_p), 0, flag, None)
+        slots, 1, 1, pos, pos_type, 1, 1, pairs, ctypes.cast(turns, ctypes.c_void_p), ctypes.cast(axis, ctypes.c_void_p), 0, flag, None, 0, None)
 
 
 @pytest.mark.parametrize("kw, code, message", [
@@ -234,7 +234,7 @@ def rotary_write(dtype=2, rows=1, hq=2, hk=1, d=64, dv=64, q=P, k=P, kc=P, ks=No
     (dict(pages=1 << 30, page=16), 1, "2^31"), (dict(hq=1 << 20, d=128), 1, "2^22"), (dict(pairs=33), 1, "pairs"),
     (dict(pairs=129, d=512), 1, "pairs"), (dict(pos_type=3), 3, "position"), (dict(ks=P, vs=P, d=48), 1, "multiples of 32"),
     (dict(q=None), 1, "null"), (dict(slots=None), 1, "null"), (dict(flag=None), 1, "null"), (dict(pos=None), 1, "null"),
-    (dict(kc=None), 1, "null cache"), (dict(ks=P), 1, "null cache"),
+    (dict(kc=None), 1, "null cache"), (dict(ks=P), 1, "null cache"), (dict(rows=1025), 5, "workspace"),
 ])
 def test_rotary_write_entry(kw, code, message):
     refused(rotary_write(**kw), code, message)
