@@ -5,37 +5,40 @@
 // less than p of the weight of the first k has gone (top-p), those with w_i >= min-p.  The token is the first index whose
 // running sum of the weights that stay is past u times all of them.
 //
-// Sums decide between neighbours, so they are exact: a weight is a 64-bit exponential rounded once to a multiple of 2^-43,
+// Sums decide between neighbours, so they are exact: a weight is formed in 64 bits and rounded once to a multiple of 2^-43,
 // and sums of those are integers, the same in any order.  A row's token depends on its own row only.
 //
-// Three launches share a row's tokens among `segs` workgroups.  sample_top finds a segment's largest and smallest logit.
-// sample_bins counts tokens and weights in 1024 bins of log2 of the weight; the last workgroup of a row to end adds them up
-// and finds the bins that a border can lie in.  sample_pick sums the weights in front of those bins for every 512 tokens and lists
-// the tokens inside of them; the last workgroup of a row finds the border in the list (by bisection, first of the logit,
-// then of the index among equal ones), completes the sums, and finds the token.  Where the list is too long (thousands of
-// tokens in a bin: equal logits) that workgroup reads the row instead, at each step.
-//
-// What bounds it: the first launch reads the row from memory; then 16 operations in 64 bits a token, twice, and three
-// launches with two joins, which is all there is for few rows.
+// A row's tokens are shared among `segs` workgroups, in five launches (one where a workgroup has a whole row):
+//   top     a segment's largest and smallest logit;
+//   bins    tokens by log2 of their weight in 2048 bins, each with its count and the sum of the places inside of it, which
+//           bound its weight to 2^-11 (one 32-bit sum a token: 64-bit ones for the weights took three times as long);
+//   join    the bins over all segments, and those that a border can lie in;
+//   sums    the weights in front of those bins, for every 512 tokens, and a list of the tokens inside of them;
+//   finish  the list sorted, the borders in its running sums, the sums of 512 tokens completed, and the token.
+// (Joins by the last workgroup of a launch took longer than launches of their own: what makes one XCD's writes visible to
+// another inside of a kernel cost 70 us a launch with 512 workgroups.)  Calls without top-k and top-p go without bins and join.
+// Where the list is too long (thousands of tokens in a bin: equal logits, mostly) finish finds the borders by bisection over the row.
 #include "biops_common.h"
 
 namespace biops {
 
-constexpr int kSampleBins = 1024, kSampleList = 2048, kSampleSub = 512;
+constexpr int kSampleThreads = 512, kSampleWaves = kSampleThreads / 64;
+constexpr int kSampleBins = 2048, kSampleInside = 32, kSampleList = 2048, kSampleSub = 512;
 constexpr int kSampleMost = 1 << 20;           // tokens of a row: sums of that many weights fit 64 bits
 constexpr int kSampleSubs = kSampleMost / kSampleSub;
-constexpr double kSampleOctaves = 32.0;        // what the bins cover at most, as powers of two of the weight
+constexpr int kSampleTable = 1024;
+constexpr int kSampleSeg = 8192;               // most tokens of a segment: 14 bits of a bin's word count, 18 add up places
+constexpr int kSamplePlace = 18;
 constexpr uint32_t kNoIndex = 0xffffffffu;
 
-struct SampleRow {
-  double c, bins, min_p, p;         // log2 e / T; bins per octave; p >= 1: all
-  uint64_t k, weight, before, all;  // k 0: all; weight in front of bin bk, and of plo; of all tokens
-  float top;
-  int state;                        // 0: to be sampled; 1: done
-  int plo, phi, bk;                 // bins of the border of top-p (or of top-k alone), of top-k
-  uint32_t count;                   // tokens in front of bin bk
-  uint32_t listed;                  // tokens of those bins
-  int unused;
+struct SampleRow {   // what join finds
+  int plo, phi, bk;   // bins of the border of top-p (of top-k, where there is no top-p), of top-k; -1: none
+  uint32_t count;     // tokens in front of bin bk
+};
+struct SampleSeg {                // of a segment
+  uint64_t top;                   // rank of the largest logit, 0 where nothing counts
+  uint64_t all, before, weight;   // weight of all tokens, in front of bin plo, in front of bin bk
+  float low;
 };
 
 struct SampleArgs {
@@ -47,12 +50,13 @@ struct SampleArgs {
   double t0, p0, m0;                            // of all rows
   int64_t k0;
   int64_t* out;
-  int rows, vocab, segs, seg, subs, k64;        // seg: tokens of a workgroup, a multiple of kSampleSub
+  int rows, vocab, segs, seg, subs, k64;        // seg: tokens of a workgroup, a multiple of kSampleSub * kSampleWaves
+  int filters;                                  // there is a top-k or a top-p
   // workspace
   SampleRow* row;
-  uint64_t *tops, *weights, *sub, *list;        // [rows][segs], [rows][segs][bins], [rows][subs], [rows][kSampleList]
-  uint32_t *counts, *ends;                      // [rows][segs][bins]; [rows][3]: workgroups that ended, entries of the list
-  float* lows;                                  // [rows][segs]
+  SampleSeg* part;                              // [rows][segs]
+  uint64_t *sub, *list;                         // [rows][subs], [rows][kSampleList]
+  uint32_t *bins, *listed;                      // [rows][segs][bins]; [rows] entries of the list
 };
 
 // Larger logits have larger keys; equal ones equal keys.
@@ -60,7 +64,9 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);  // (-0 is 0)
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ bool counts_at_all(float x) { return x > -INFINITY; }  // not -inf, not NaN
+__device__ __forceinline__ float float_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+// A token's place in the order: larger ones first.
+__device__ __forceinline__ uint64_t rank_of(float x, uint32_t index) { return (uint64_t)key_of(x) << 32 | (kNoIndex - index); }
 
 // Eight logits from element i of a row on; -inf behind its end.
 template <typename T>
@@ -87,41 +93,41 @@ __device__ __forceinline__ void eight_logits(const T* row, int i, int vocab, flo
   }
 }
 
-// The weight 2^-y of a logit in units of 2^-43, with 2^(-i / 64) from a table and the rest by its series: relative error
-// below 2^-47.
+// Weights.  y = (M - l) log2 e / T in units of 2^-40 (at most 50, which is a weight of 0: logits of -inf and NaN have that);
+// 2^-y from a table of 2^(-i / 1024) and 1 - 2^-r = t - t^2 / 2 + t^3 / 6, t = r ln 2 < 2^-10.5, which 32 bits hold to
+// 2^-33: relative error of a weight, and of a sum at most that.
 struct SampleWeight {
-  double top, c, bins;
+  double top, c;
+  bool infinite;            // M is infinite: only logits of that count, alike
+  uint32_t scale;           // places of 2^-26 octaves, times 2^32
   const double* table;
-  __device__ __forceinline__ double octaves(float x) const {
-    const double d = top - (double)x;
-    return d > 0.0 ? fmin(d * c, 1000.0) : 0.0;  // (0 * inf and inf - inf are 0)
+  __device__ __forceinline__ uint64_t octaves(float x) const {
+    double y = fmin((top - (double)x) * c, 50.0);
+    if (infinite) y = x == INFINITY ? 0.0 : 50.0;
+    return (uint64_t)__double_as_longlong(y + 4096.0) & 0xfffffffffffffull;
   }
-  __device__ __forceinline__ int bin(double y) const {
-    const double b = y * bins;
-    return b < (double)kSampleBins ? (int)b : kSampleBins - 1;
+  // the place among all places of the bins, kSampleInside of each
+  __device__ __forceinline__ uint32_t place(uint64_t y) const {
+    const uint32_t b = __umulhi((uint32_t)(y >> 14), scale);
+    return b < kSampleBins * kSampleInside ? b : kSampleBins * kSampleInside - 1;
   }
-  __device__ __forceinline__ double weight(double y) const {
-    const double z = y * 64.0, whole = floor(z), r = z - whole;
-    const int n = (int)whole;
-    constexpr double a = 0.010830424696249145;  // ln 2 / 64
-    double e = -a * a * a * a * a / 120.0;
-    e = fma(e, r, a * a * a * a / 24.0);
-    e = fma(e, r, -a * a * a / 6.0);
-    e = fma(e, r, a * a / 2.0);
-    e = fma(e, r, -a);
-    e = fma(e, r, 1.0);
-    return ldexp(e * table[n & 63], -(n >> 6));
-  }
-  __device__ static __forceinline__ uint64_t units(double w) {
-    return (uint64_t)__double_as_longlong(w * 0x1p43 + 0x1p52) & 0xfffffffffffffull;  // to the nearest
+  __device__ __forceinline__ int bin(uint64_t y) const { return (int)(place(y) / kSampleInside); }
+  // in units of 2^-43
+  __device__ __forceinline__ uint64_t units(uint64_t y) const {
+    const uint32_t hi = (uint32_t)(y >> 32), lo = (uint32_t)y;
+    const double t = table[(hi & 255u) << 2 | lo >> 30];
+    const float r = (float)(lo & 0x3fffffffu) * 6.3041396e-13f;  // ln 2 / 2^40
+    const float off = r * __builtin_fmaf(r, __builtin_fmaf(r, 1.f / 6.f, -0.5f), 1.f);
+    const double w = fma(-t, (double)off, t);
+    const double sized = __hiloint2double(__double2hiint(w) + ((43 - (int)(hi >> 8)) << 20), __double2loint(w));
+    return (uint64_t)__double_as_longlong(sized + 0x1p52) & 0xfffffffffffffull;  // to the nearest
   }
 };
-// (a block of at least 64 threads; __syncthreads before use)
+// (__syncthreads before use)
 __device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2(-(double)threadIdx.x / 64.0);
+  for (int i = threadIdx.x; i < kSampleTable; i += kSampleThreads) table[i] = exp2(-(double)i / kSampleTable);
 }
 
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int from) { return (uint64_t)__shfl((unsigned long long)v, from, 64); }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, o, 64);
@@ -137,55 +143,89 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
   }
   return v;
 }
-// Sum over the 256 threads, to all of them.
-__device__ __forceinline__ uint64_t block_sum64(uint64_t v, uint64_t* four) {
-  v = wave_sum64(v);
-  __syncthreads();  // (the last sum has been read)
-  if ((threadIdx.x & 63) == 0) four[threadIdx.x >> 6] = v;
+// The sum in front of this thread and the sum of all, over the workgroup.
+__device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t* waves, uint64_t& all) {
+  const uint64_t scan = wave_scan64(v);
+  __syncthreads();  // (the last sums have been read)
+  if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = scan;
   __syncthreads();
-  return four[0] + four[1] + four[2] + four[3];
-}
-
-// Whether this workgroup is the last of `n` that end here: what the others wrote before is then visible to it.
-__device__ __forceinline__ bool last_to_end(uint32_t* count, int n, uint32_t* flag) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    *flag = __hip_atomic_fetch_add(count, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(n - 1);
+  uint64_t before = scan - v;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < kSampleWaves; ++i) {
+    if (i < (int)(threadIdx.x >> 6)) before += waves[i];
+    all += waves[i];
   }
+  return before;
+}
+__device__ __forceinline__ uint64_t block_sum64(uint64_t v, uint64_t* waves) {
+  v = wave_sum64(v);
+  __syncthreads();  // (the last sums have been read)
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
   __syncthreads();
-  if (*flag == 0) return false;
-  __threadfence();
-  return true;
+  uint64_t all = 0;
+#pragma unroll
+  for (int i = 0; i < kSampleWaves; ++i) all += waves[i];
+  return all;
 }
 
 __device__ __forceinline__ double row_value(const float* p, int64_t s, double all, int r) { return p ? (double)p[r * s] : all; }
 
+// Shared memory of the steps; the table stays from one step to the next.
+struct SampleTop {
+  uint64_t tops[kSampleWaves];
+  float lows[kSampleWaves];
+};
+struct SampleBins {
+  uint32_t bins[kSampleBins];
+};
+struct SampleJoin {
+  int found[3];
+  uint64_t bounds[2];
+  uint32_t count;
+};
+struct SampleSums {
+  uint64_t item[kSampleList];
+  uint32_t met, ready;
+};
+struct SampleFinish {
+  uint64_t sub[kSampleSubs], item[kSampleList];
+  int chosen;
+  uint64_t left;
+};
+struct SampleShared {
+  double table[kSampleTable];
+  uint64_t waves[kSampleWaves];
+  union {
+    SampleTop top;
+    SampleBins bins;
+    SampleJoin join;
+    SampleSums sums;
+    SampleFinish finish;
+  };
+};
+
 // --------------------------------------------------------------------------------- largest logits ----
 template <typename T>
-__global__ __launch_bounds__(256) void sample_top(SampleArgs a) {
-  __shared__ uint64_t tops[4];
-  __shared__ float lows[4];
-  const int seg = blockIdx.x % a.segs, r = blockIdx.x / a.segs, tid = threadIdx.x;
+__device__ __forceinline__ void top_step(const SampleArgs& a, int seg, int r, SampleTop& sh) {
+  const int tid = threadIdx.x;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
   const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
-  uint64_t top = 0;  // (key, ~index): 0 where nothing counts
   float best = -INFINITY, low = INFINITY;
   int at = -1;
-  for (int i = seg * a.seg + 8 * tid; i < end; i += 2048) {
+  for (int i = seg * a.seg + 8 * tid; i < end; i += 8 * kSampleThreads) {
     float x[8];
     eight_logits<T>(row, i, a.vocab, x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (!counts_at_all(x[j])) continue;
+    for (int j = 0; j < 8; ++j) {  // (-inf and NaN do not count)
       if (x[j] > best) {
         best = x[j];
         at = i + j;
       }
-      low = fminf(low, x[j]);
+      low = x[j] > -INFINITY ? fminf(low, x[j]) : low;
     }
   }
-  if (at >= 0) top = (uint64_t)key_of(best) << 32 | (kNoIndex - (uint32_t)at);
+  uint64_t top = at >= 0 ? rank_of(best, at) : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const uint64_t t = (uint64_t)__shfl_xor((unsigned long long)top, o, 64);
@@ -193,423 +233,409 @@ __global__ __launch_bounds__(256) void sample_top(SampleArgs a) {
     low = fminf(low, __shfl_xor(low, o, 64));
   }
   if ((tid & 63) == 0) {
-    tops[tid >> 6] = top;
-    lows[tid >> 6] = low;
+    sh.tops[tid >> 6] = top;
+    sh.lows[tid >> 6] = low;
   }
   __syncthreads();
   if (tid == 0) {
-    for (int i = 1; i < 4; ++i) {
-      top = tops[i] > top ? tops[i] : top;
-      low = fminf(low, lows[i]);
+    for (int i = 1; i < kSampleWaves; ++i) {
+      top = sh.tops[i] > top ? sh.tops[i] : top;
+      low = fminf(low, sh.lows[i]);
     }
-    a.tops[(int64_t)r * a.segs + seg] = top;
-    a.lows[(int64_t)r * a.segs + seg] = low;
-    if (seg == 0)
-      for (int i = 0; i < 3; ++i) a.ends[3 * r + i] = 0u;
+    SampleSeg& out = a.part[(int64_t)r * a.segs + seg];
+    out.top = top;
+    out.low = low;
+    if (seg == 0) a.listed[r] = 0u;
   }
 }
 
-// ------------------------------------------------------------------------------ weights by their size ----
-// The row's largest logit and its first index, its smallest, and its settings, from the segments (all threads alike).
-__device__ __forceinline__ uint64_t row_top(const SampleArgs& a, int r, float& low) {
+// The row's weights, from its segments' largest and smallest logits and its temperature (every wavefront by itself).  False
+// where there is nothing to sample: `token` is then the row's answer.
+__device__ __forceinline__ bool row_weights(const SampleArgs& a, int r, const double* table, SampleWeight& of, int64_t& token) {
   uint64_t top = 0;
-  low = INFINITY;
-  for (int s = 0; s < a.segs; ++s) {
-    const uint64_t t = a.tops[(int64_t)r * a.segs + s];
-    top = t > top ? t : top;
-    low = fminf(low, a.lows[(int64_t)r * a.segs + s]);
+  float low = INFINITY;
+  for (int s = threadIdx.x & 63; s < a.segs; s += 64) {
+    const SampleSeg& part = a.part[(int64_t)r * a.segs + s];
+    top = part.top > top ? part.top : top;
+    low = fminf(low, part.low);
   }
-  return top;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t t = (uint64_t)__shfl_xor((unsigned long long)top, o, 64);
+    top = t > top ? t : top;
+    low = fminf(low, __shfl_xor(low, o, 64));
+  }
+  const double t = row_value(a.temperature, a.t_s, a.t0, r);
+  token = top == 0 ? -1 : (int64_t)(kNoIndex - (uint32_t)top);
+  if (top == 0 || !(t > 0.0)) return false;
+  of.top = (double)float_of((uint32_t)(top >> 32));
+  of.infinite = of.top == INFINITY;
+  of.c = fmin(1.4426950408889634 / t, 1e300);  // (finite: 0 times it is 0)
+  of.table = table;
+  const uint64_t most = 44ull << 40, range = of.infinite ? 0u : of.octaves(low);  // (weights below 2^-44 are 0)
+  const double scale = (double)(kSampleBins * kSampleInside) * 0x1p32 / (double)((range < most ? range : most) / 16384 + 1);
+  of.scale = scale < 4294967295.0 ? (uint32_t)scale : 0xffffffffu;
+  return true;
 }
-__device__ __forceinline__ float float_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 __device__ __forceinline__ uint64_t part(double p, uint64_t weight) {  // the weight that top-p asks for, at least one unit
   const double x = ceil(p * (double)weight);
   return x >= 1.0 ? (uint64_t)x : 1u;
 }
+__device__ __forceinline__ int64_t row_k(const SampleArgs& a, int r) {
+  const int64_t k = !a.top_k ? a.k0
+                    : a.k64  ? reinterpret_cast<const int64_t*>(a.top_k)[r * a.k_s]
+                             : (int64_t) reinterpret_cast<const int32_t*>(a.top_k)[r * a.k_s];
+  return k > 0 && k < a.vocab ? k : 0;  // 0: all
+}
+__device__ __forceinline__ double row_p(const SampleArgs& a, int r) {
+  const double p = row_value(a.top_p, a.p_s, a.p0, r);
+  return p < 1.0 ? p : 1.0;  // 1 (and NaN): all
+}
 
+// ------------------------------------------------------------------------------ weights by their size ----
 template <typename T>
-__global__ __launch_bounds__(256) void sample_bins(SampleArgs a) {
-  __shared__ double table[64];
-  __shared__ uint32_t count[kSampleBins];
-  __shared__ uint64_t weight[kSampleBins];
-  __shared__ uint64_t sums[2][4];
-  __shared__ uint32_t last;
-  __shared__ int found[3];
-  __shared__ uint64_t at_found[2];
-  __shared__ uint32_t count_found[2];
-  const int seg = blockIdx.x % a.segs, r = blockIdx.x / a.segs, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+__device__ __forceinline__ void bins_step(const SampleArgs& a, int seg, int r, double* table, uint64_t* waves, SampleBins& sh) {
+  const int tid = threadIdx.x;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
-  float low;
-  const uint64_t top = row_top(a, r, low);
-  const double t = row_value(a.temperature, a.t_s, a.t0, r);
-  const bool greedy = !(t > 0.0);
-  if (top == 0 || greedy) {  // nothing to choose from, or nothing to choose
-    if (seg == 0 && tid == 0) {
-      a.row[r].state = 1;
-      a.out[r] = top == 0 ? -1 : (int64_t)(kNoIndex - (uint32_t)top);
-    }
-    return;
-  }
   SampleWeight of;
-  of.top = (double)float_of((uint32_t)(top >> 32));
-  of.c = 1.4426950408889634 / t;
-  of.table = table;
-  const bool infinite = of.top == INFINITY;  // only those with the same logit count
-  const double range = infinite ? 0.0 : fmin(of.octaves(low), kSampleOctaves);
-  of.bins = range > 0.0 ? kSampleBins / range : 0.0;
+  int64_t token;
+  if (!row_weights(a, r, table, of, token) || (row_k(a, r) == 0 && row_p(a, r) == 1.0)) return;
   fill_table(table);
-  for (int i = tid; i < kSampleBins; i += 256) {
-    count[i] = 0u;
-    weight[i] = 0u;
-  }
+  for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.bins[i] = 0u;
   __syncthreads();
   const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
-  for (int i = seg * a.seg + 8 * tid; i < end; i += 2048) {
+  uint64_t sum = 0;
+  for (int i = seg * a.seg + 8 * tid; i < end; i += 8 * kSampleThreads) {
     float x[8];
     eight_logits<T>(row, i, a.vocab, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (!counts_at_all(x[j]) || (infinite && x[j] != INFINITY)) continue;
-      const double y = of.octaves(x[j]);
-      const uint64_t units = SampleWeight::units(of.weight(y));
-      if (units == 0) continue;
-      const int b = of.bin(y);
-      atomicAdd(&count[b], 1u);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&weight[b]), (unsigned long long)units);
+      const uint64_t y = of.octaves(x[j]), units = of.units(y);
+      const uint32_t place = of.place(y);
+      sum += units;
+      if (units != 0) atomicAdd(&sh.bins[place / kSampleInside], 1u << kSamplePlace | place % kSampleInside);
     }
   }
-  __syncthreads();
-  const int64_t mine = ((int64_t)r * a.segs + seg) * kSampleBins;
-  for (int i = tid; i < kSampleBins; i += 256) {
-    a.counts[mine + i] = count[i];
-    a.weights[mine + i] = weight[i];
-  }
-  if (!last_to_end(&a.ends[3 * r], a.segs, &last)) return;
+  sum = block_sum64(sum, waves);
+  const int64_t at = (int64_t)r * a.segs + seg;
+  if (tid == 0) a.part[at].all = sum;
+  static_assert(kSampleBins == 4 * kSampleThreads, "four bins a thread");
+  *reinterpret_cast<u32x4_t*>(a.bins + at * kSampleBins + 4 * tid) = *reinterpret_cast<const u32x4_t*>(sh.bins + 4 * tid);
+}
 
-  // four bins a thread, over all segments
-  uint32_t n[4] = {0u, 0u, 0u, 0u};
-  uint64_t s[4] = {0u, 0u, 0u, 0u};
+// The sum of a member over a row's segments (every wavefront by itself).
+template <typename F>
+__device__ __forceinline__ uint64_t over_segments(const SampleArgs& a, int r, F member) {
+  uint64_t v = 0;
+  for (int s = threadIdx.x & 63; s < a.segs; s += 64) v += member(a.part[(int64_t)r * a.segs + s]);
+  return wave_sum64(v);
+}
+
+__device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* waves, SampleJoin& sh) {
+  const int tid = threadIdx.x;
+  SampleWeight of;
+  int64_t token;
+  if (!row_weights(a, r, nullptr, of, token)) return;
+  const uint64_t k = (uint64_t)row_k(a, r);
+  const double p = row_p(a, r);
+  if (k == 0 && p == 1.0) {
+    if (tid == 0) a.row[r] = SampleRow{kSampleBins, -1, -1, 0u};
+    return;
+  }
+  // four bins a thread: their tokens, and bounds of their weights
+  uint32_t n[4] = {0u, 0u, 0u, 0u}, places[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 4
   for (int g = 0; g < a.segs; ++g) {
-    const int64_t at = ((int64_t)r * a.segs + g) * kSampleBins + 4 * tid;
-    const u32x4_t c = *reinterpret_cast<const u32x4_t*>(a.counts + at);
-    const u32x4_t w0 = *reinterpret_cast<const u32x4_t*>(a.weights + at), w1 = *reinterpret_cast<const u32x4_t*>(a.weights + at + 2);
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(a.bins + ((int64_t)r * a.segs + g) * kSampleBins + 4 * tid);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] += c[i];
-    s[0] += (uint64_t)w0[1] << 32 | w0[0];
-    s[1] += (uint64_t)w0[3] << 32 | w0[2];
-    s[2] += (uint64_t)w1[1] << 32 | w1[0];
-    s[3] += (uint64_t)w1[3] << 32 | w1[2];
+    for (int i = 0; i < 4; ++i) {
+      n[i] += v[i] >> kSamplePlace;
+      places[i] += v[i] & ((1u << kSamplePlace) - 1u);
+    }
   }
-  const uint64_t n4 = n[0] + n[1] + n[2] + n[3], s4 = s[0] + s[1] + s[2] + s[3];
-  const uint64_t nscan = wave_scan64(n4), sscan = wave_scan64(s4);
-  if (lane == 63) {
-    sums[0][w] = nscan;
-    sums[1][w] = sscan;
-  }
-  if (tid < 3) found[tid] = kSampleBins;
-  __syncthreads();
-  uint64_t nb = nscan - n4, sb = sscan - s4, total_n = 0, total = 0;
+  // A token of place i has y in [i w, (i + 1) w + 2^-26), w = 2^6 / scale octaves.  2^-y is convex: the sum over tokens whose
+  // places have the mean f is at most the chord's from place 0 to the last, and at least their number times the value at f + 1.
+  const double width = 64.0 / (double)of.scale;
+  uint64_t least[4], most[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (i < w) {
-      nb += sums[0][i];
-      sb += sums[1][i];
-    }
-    total_n += sums[0][i];
-    total += sums[1][i];
+    const double c = (double)n[i], at = (double)((4 * tid + i) * kSampleInside), f = (double)places[i];
+    const double w0 = exp2(43.0 - at * width), w1 = exp2(43.0 - (at + (kSampleInside - 1)) * width);
+    const double high = (c * w0 + (w1 - w0) * f / (kSampleInside - 1)) * 1.000001 + c;  // (and half a unit's rounding each)
+    const double low = n[i] ? c * exp2(43.0 - (at + f / c + 1.0) * width) * 0.999999 - c : 0.0;
+    least[i] = low > 0.0 ? (uint64_t)low : 0u;
+    most[i] = n[i] ? (uint64_t)high + 1u : 0u;
   }
-  int64_t k = a.k0;
-  if (a.top_k) k = a.k64 ? reinterpret_cast<const int64_t*>(a.top_k)[r * a.k_s] : (int64_t) reinterpret_cast<const int32_t*>(a.top_k)[r * a.k_s];
-  const bool by_k = k > 0 && (uint64_t)k < total_n;
-  const double p = row_value(a.top_p, a.p_s, a.p0, r);
-  const bool by_p = p < 1.0;  // (a NaN: all)
+  uint64_t total_n, total_least, total_most;
+  const uint64_t nb = block_scan64((uint64_t)n[0] + n[1] + n[2] + n[3], waves, total_n);
+  const uint64_t lb = block_scan64(least[0] + least[1] + least[2] + least[3], waves, total_least);
+  const uint64_t mb = block_scan64(most[0] + most[1] + most[2] + most[3], waves, total_most);
+  if (tid < 3) sh.found[tid] = kSampleBins - 1;
+  __syncthreads();
+  const bool by_k = k > 0 && k < total_n;
   if (by_k) {  // the bin of the k-th token
-    uint64_t x = nb, y = sb;
+    uint64_t x = nb, low = lb, high = mb;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (x < (uint64_t)k && (uint64_t)k <= x + n[i]) {
-        found[0] = 4 * tid + i;
-        at_found[0] = y;
-        at_found[1] = s[i];
-        count_found[0] = (uint32_t)x;
+      if (x < k && k <= x + n[i]) {
+        sh.found[0] = 4 * tid + i;
+        sh.bounds[0] = low;
+        sh.bounds[1] = high + most[i];
+        sh.count = (uint32_t)x;
       }
       x += n[i];
-      y += s[i];
+      low += least[i];
+      high += most[i];
     }
   }
   __syncthreads();
-  const int bk = by_k ? found[0] : -1;
+  const int bk = by_k ? sh.found[0] : -1;
   int plo = by_k ? bk : kSampleBins, phi = by_k ? bk : -1;
-  if (by_p) {  // the bins that have the border, whatever part of bin bk counts
-    const uint64_t least = part(p, by_k ? at_found[0] : total), most = part(p, by_k ? at_found[0] + at_found[1] : total);
-    uint64_t y = sb;
+  if (p < 1.0) {  // the bins that can have the border
+    const uint64_t all = over_segments(a, r, [](const SampleSeg& s) { return s.all; });
+    const uint64_t first = part(p, by_k ? sh.bounds[0] : all), last = part(p, by_k ? sh.bounds[1] : all);
+    uint64_t low = lb, high = mb;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint64_t z = y + s[i];
-      if (y < least && z >= least) found[1] = 4 * tid + i;
-      if (y < most && z >= most) found[2] = 4 * tid + i;
-      y = z;
+      if (high < first && high + most[i] >= first) sh.found[1] = 4 * tid + i;
+      if (low < last && low + least[i] >= last) sh.found[2] = 4 * tid + i;
+      low += least[i];
+      high += most[i];
     }
     __syncthreads();
-    plo = found[1] < plo ? found[1] : plo;
-    phi = by_k ? (found[2] < bk ? found[2] : bk) : found[2];
+    plo = sh.found[1] < plo ? sh.found[1] : plo;
+    phi = by_k && bk < sh.found[2] ? bk : sh.found[2];
     if (phi < plo) phi = plo;
   }
-  // what is in front of bin plo, and how many tokens the border's bins have
-  uint64_t listed = 0;
-  {
-    uint64_t y = sb;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int b = 4 * tid + i;
-      if (b == plo) a.row[r].before = y;
-      if ((b >= plo && b <= phi) || b == bk) listed += n[i];
-      y += s[i];
-    }
-  }
-  listed = block_sum64(listed, sums[0]);
-  if (tid == 0) {
-    SampleRow& out = a.row[r];
-    out.c = of.c;
-    out.bins = of.bins;
-    out.min_p = fmin(row_value(a.min_p, a.m_s, a.m0, r), 1.0);
-    out.p = by_p ? p : 1.0;
-    out.k = by_k ? (uint64_t)k : 0u;
-    out.weight = by_k ? at_found[0] : 0u;
-    out.all = total;
-    out.top = (float)of.top;
-    out.state = 0;
-    out.plo = plo;
-    out.phi = phi;
-    out.bk = bk;
-    out.count = by_k ? count_found[0] : 0u;
-    out.listed = (uint32_t)listed;
-  }
+  if (tid == 0) a.row[r] = SampleRow{plo, phi, bk, by_k ? sh.count : 0u};
 }
 
 // ---------------------------------------------------------------------------- the border and the token ----
-// A token of the border's bins.
-struct SampleItem {
-  uint32_t key, index;
-  uint64_t units;
-  int bin;
-  bool heavy;  // enough for min-p
+struct SampleBorder {
+  int plo, phi, bk;
+  uint64_t lightest;  // the largest y that min-p lets pass: log2(1 / min-p)
+  __device__ __forceinline__ bool at(int bin) const { return (bin >= plo && bin <= phi) || bin == bk; }
 };
+__device__ __forceinline__ SampleBorder border_of(const SampleArgs& a, int r) {
+  SampleBorder b{kSampleBins, -1, -1, 50ull << 40};
+  if (a.filters) {
+    b.plo = a.row[r].plo;
+    b.phi = a.row[r].phi;
+    b.bk = a.row[r].bk;
+  }
+  const double min_p = fmin(row_value(a.min_p, a.m_s, a.m0, r), 1.0);
+  if (min_p > 0x1p-49) b.lightest = (uint64_t)(-log2(min_p) * 0x1p40 + 0.5);
+  return b;
+}
 
 template <typename T>
-__global__ __launch_bounds__(256) void sample_pick(SampleArgs a) {
-  __shared__ double table[64];
-  __shared__ uint64_t four[4];
-  __shared__ uint32_t last, ready, met;
-  __shared__ uint64_t sub[kSampleSubs];
-  __shared__ uint32_t item_key[kSampleList], item_index[kSampleList];
-  __shared__ uint64_t item_units[kSampleList];
-  __shared__ uint16_t item_bin[kSampleList];
-  __shared__ int chosen;
-  __shared__ uint64_t left;
-  const int seg = blockIdx.x % a.segs, r = blockIdx.x / a.segs, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+__device__ __forceinline__ void sums_step(const SampleArgs& a, int seg, int r, double* table, uint64_t* waves, SampleSums& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
-  const SampleRow& in = a.row[r];
-  if (in.state != 0) return;
   SampleWeight of;
-  of.top = (double)in.top;
-  of.c = in.c;
-  of.bins = in.bins;
-  of.table = table;
-  const bool infinite = of.top == INFINITY;
-  const int plo = in.plo, phi = in.phi, bk = in.bk;
-  const double min_p = in.min_p;
-  const bool fits = in.listed <= kSampleList;
+  int64_t token;
+  if (!row_weights(a, r, table, of, token)) return;
+  const SampleBorder border = border_of(a, r);
+  const int last = border.bk > border.plo ? border.bk : border.plo;  // weights in front of it are needed
   fill_table(table);
-  if (tid == 0) met = 0u;
+  if (tid == 0) sh.met = 0u;
   __syncthreads();
-  // (octaves, bin, weight) of a logit; false where it does not count
-  auto item_of = [&](float x, uint32_t index, SampleItem& t) {
-    if (!counts_at_all(x) || (infinite && x != INFINITY)) return false;
-    const double y = of.octaves(x), weight = of.weight(y);
-    t.key = key_of(x);
-    t.index = index;
-    t.units = SampleWeight::units(weight);
-    t.bin = of.bin(y);
-    t.heavy = !(weight < min_p);
-    return t.units != 0;
-  };
-  auto at_border = [&](int bin) { return (bin >= plo && bin <= phi) || bin == bk; };
-
   const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
-  if (fits)
-    for (int s0 = seg * a.seg + kSampleSub * w; s0 < end; s0 += 4 * kSampleSub) {
-      float x[8];
-      const int i = s0 + 8 * lane;
-      eight_logits<T>(row, i, a.vocab, x);
+  uint64_t before = 0, weight = 0;
+  for (int s0 = seg * a.seg + kSampleSub * w; s0 < end; s0 += kSampleWaves * kSampleSub) {
+    float x[8];
+    const int i = s0 + 8 * lane;
+    eight_logits<T>(row, i, a.vocab, x);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint64_t y = of.octaves(x[j]);
+      const int bin = of.bin(y);
+      const bool near = border.at(bin);
+      if (bin >= last && !near) continue;
+      const uint64_t units = of.units(y);
+      if (bin < border.plo) {
+        before += units;
+        if (y <= border.lightest) sum += units;
+      }
+      if (bin < border.bk) weight += units;
+      if (near && units != 0) {
+        const uint32_t at = atomicAdd(&sh.met, 1u);
+        if (at < kSampleList) sh.item[at] = rank_of(x[j], i + j);
+      }
+    }
+    sum = wave_sum64(sum);
+    if (lane == 0) a.sub[(int64_t)r * a.subs + s0 / kSampleSub] = sum;
+  }
+  if (!a.filters) return;
+  before = block_sum64(before, waves);
+  weight = block_sum64(weight, waves);
+  SampleSeg& out = a.part[(int64_t)r * a.segs + seg];
+  if (tid == 0) {
+    out.before = before;
+    out.weight = weight;
+    if (sh.met > 0) sh.ready = __hip_atomic_fetch_add(&a.listed[r], sh.met, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < sh.met && i < kSampleList && sh.ready < kSampleList - i; i += kSampleThreads)  // in any order
+    a.list[(int64_t)r * kSampleList + sh.ready + i] = sh.item[i];
+}
+
+template <typename T>
+__device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* table, uint64_t* waves, SampleFinish& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
+  SampleWeight of;
+  int64_t token;
+  if (!row_weights(a, r, table, of, token)) {  // nothing to choose from, or nothing to choose
+    if (tid == 0) a.out[r] = token;
+    return;
+  }
+  const SampleBorder border = border_of(a, r);
+  const uint32_t listed = a.listed[r];
+  const bool fits = listed <= kSampleList;
+  fill_table(table);
+  for (int i = tid; i < a.subs; i += kSampleThreads) sh.sub[i] = a.sub[(int64_t)r * a.subs + i];
+  __syncthreads();
+  uint64_t least = 0;  // the rank of the last token that stays
+  if (listed > 0) {
+    const double p = row_p(a, r);
+    const int bk = border.bk, phi = border.phi;
+    const uint64_t want_k = bk >= 0 ? (uint64_t)row_k(a, r) - a.row[r].count : 0;  // tokens of bin bk that stay
+    const uint64_t in_front_of_plo = over_segments(a, r, [](const SampleSeg& s) { return s.before; });
+    uint64_t total = bk >= 0 ? over_segments(a, r, [](const SampleSeg& s) { return s.weight; })
+                             : over_segments(a, r, [](const SampleSeg& s) { return s.all; });
+    if (fits) {
+      // the list from the largest rank down (and zeros behind it)
+      int n = 64;
+      while (n < (int)listed) n *= 2;
+      for (int i = tid; i < n; i += kSampleThreads) sh.item[i] = i < (int)listed ? a.list[(int64_t)r * kSampleList + i] : 0u;
+      __syncthreads();
+      for (int size = 2; size <= n; size *= 2)
+        for (int step = size / 2; step > 0; step /= 2) {
+          for (int i = tid; i < n / 2; i += kSampleThreads) {
+            const int x = 2 * i - (i & (step - 1)), z = x + step;
+            const uint64_t p0 = sh.item[x], p1 = sh.item[z];
+            if ((p0 < p1) == ((x & size) == 0)) {
+              sh.item[x] = p1;
+              sh.item[z] = p0;
+            }
+          }
+          __syncthreads();
+        }
+      // running sums: of four tokens a thread
+      constexpr int kPer = kSampleList / kSampleThreads;
+      uint64_t units[kPer], upto[kPer], y[kPer], all;
+      int in_front = 0, in_range = 0;  // tokens in bins in front of bk; in bins up to phi
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int at = kPer * tid + i;
+        const bool there = at < (int)listed;
+        y[i] = there ? of.octaves(float_of((uint32_t)(sh.item[at] >> 32))) : 0u;
+        units[i] = there ? of.units(y[i]) : 0u;
+        const int bin = of.bin(y[i]);
+        in_front += there && bin < bk;
+        in_range += there && bin <= phi;
+      }
       uint64_t sum = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        SampleItem t;
-        if (!item_of(x[j], i + j, t)) continue;
-        if (t.bin < plo) {
-          if (t.heavy) sum += t.units;
-        } else if (at_border(t.bin)) {
-          const uint32_t at = atomicAdd(&met, 1u);
-          if (at < kSampleList) {  // (always: sample_bins counted them)
-            item_key[at] = t.key;
-            item_index[at] = t.index;
-          }
-        }
+      for (int i = 0; i < kPer; ++i) sum += units[i];
+      uint64_t before = block_scan64(sum, waves, all);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        upto[i] = before;
+        before += units[i];
       }
-      sum = wave_sum64(sum);
-      if (lane == 0) a.sub[(int64_t)r * a.subs + s0 / kSampleSub] = sum;
-    }
-  __syncthreads();
-  if (met > 0) {  // this segment's part of the list, in any order
-    if (tid == 0) ready = __hip_atomic_fetch_add(&a.ends[3 * r + 2], met, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    for (uint32_t i = tid; i < met && ready + i < kSampleList; i += 256)
-      a.list[(int64_t)r * kSampleList + ready + i] = (uint64_t)item_key[i] << 32 | item_index[i];
-  }
-  if (!last_to_end(&a.ends[3 * r + 1], a.segs, &last)) return;
-
-  const int listed = fits ? (int)in.listed : 0;
-  for (int i = tid; i < listed; i += 256) {
-    const uint64_t e = a.list[(int64_t)r * kSampleList + i];
-    SampleItem t;
-    item_of(float_of((uint32_t)(e >> 32)), (uint32_t)e, t);
-    item_key[i] = t.key;
-    item_index[i] = t.index;
-    item_units[i] = t.heavy ? t.units : t.units | 1ull << 63;  // (units stay below 2^44)
-    item_bin[i] = (uint16_t)t.bin;
-  }
-  for (int i = tid; i < a.subs; i += 256) sub[i] = fits ? a.sub[(int64_t)r * a.subs + i] : 0u;
-  __syncthreads();
-  // f(item) for this thread's share of the border's tokens
-  auto each = [&](auto f) {
-    if (fits) {
-      for (int i = tid; i < listed; i += 256) {
-        const uint64_t u = item_units[i];
-        f(SampleItem{item_key[i], item_index[i], u & ~(1ull << 63), (int)item_bin[i], u >> 63 == 0});
+      const uint64_t counts = block_sum64((uint64_t)in_front << 32 | (uint32_t)in_range, waves);
+      const int front = (int)(counts >> 32), range = (int)(uint32_t)counts;
+      int cut = (int)listed;  // tokens of the list that stay
+      if (bk >= 0) {
+        cut = front + (int)want_k;
+        uint64_t s = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s += kPer * tid + i >= front && kPer * tid + i < cut ? units[i] : 0u;
+        total += block_sum64(s, waves);
+      }
+      if (p < 1.0) {
+        const uint64_t want = part(p, total);
+        const int most = range < cut ? range : cut;
+        uint64_t s = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s += kPer * tid + i < most && in_front_of_plo + upto[i] < want;
+        cut = (int)block_sum64(s, waves);  // (the border may be the end of bin phi: what is behind it goes)
+      }
+      least = sh.item[cut > 0 ? cut - 1 : 0];  // (at least one: less weight than asked for is in front of bin plo)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int at = kPer * tid + i;
+        if (at < cut && y[i] <= border.lightest)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sub[(kNoIndex - (uint32_t)sh.item[at]) / kSampleSub]), (unsigned long long)units[i]);
       }
     } else {
-      for (int i = 8 * tid; i < a.vocab; i += 2048) {
-        float x[8];
-        eight_logits<T>(row, i, a.vocab, x);
-        for (int j = 0; j < 8; ++j) {
-          SampleItem t;
-          if (item_of(x[j], i + j, t) && at_border(t.bin)) f(t);
-        }
-      }
-    }
-  };
-  // the sum of f(item) over them
-  auto sum_of = [&](auto f) {
-    uint64_t s = 0;
-    each([&](const SampleItem& t) { s += f(t); });
-    return block_sum64(s, four);
-  };
-  // the largest x with f(x), which holds at 0 and, where it holds, for everything smaller
-  auto largest = [&](uint32_t lo, uint32_t hi, auto f) {  // f(lo) holds
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      if (f(mid)) lo = mid;
-      else hi = mid - 1;
-    }
-    return lo;
-  };
-  // the bounds of the border's keys
-  uint32_t key_lo = kNoIndex, key_hi = 0u;
-  each([&](const SampleItem& t) {
-    key_lo = t.key < key_lo ? t.key : key_lo;
-    key_hi = t.key > key_hi ? t.key : key_hi;
-  });
+      // f(rank, y, bin) of the border's tokens, summed
+      auto sum_of = [&](auto f) {
+        uint64_t s = 0;
+        for (int i = 8 * tid; i < a.vocab; i += 8 * kSampleThreads) {
+          float x[8];
+          eight_logits<T>(row, i, a.vocab, x);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t x = (uint32_t)__shfl_xor((int)key_lo, o, 64), y = (uint32_t)__shfl_xor((int)key_hi, o, 64);
-    key_lo = x < key_lo ? x : key_lo;
-    key_hi = y > key_hi ? y : key_hi;
-  }
-  __syncthreads();
-  if (lane == 0) four[w] = (uint64_t)key_hi << 32 | key_lo;
-  __syncthreads();
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = (uint32_t)four[i], y = (uint32_t)(four[i] >> 32);
-    key_lo = x < key_lo ? x : key_lo;
-    key_hi = y > key_hi ? y : key_hi;
-  }
-  __syncthreads();
-
-  // what stays: larger keys, and of those with this key the ones at smaller indices
-  uint32_t key = 0u, below = kNoIndex;
-  auto stays = [&](const SampleItem& t) { return t.key > key || (t.key == key && t.index < below); };
-  // the first `n` of the tokens with key `x` that stay so far: the index behind them
-  auto first_of = [&](uint32_t x, uint64_t n) {
-    const auto equal = [&](const SampleItem& t) { return t.key == x && stays(t); };
-    if (n >= sum_of([&](const SampleItem& t) { return (uint64_t)equal(t); })) return kNoIndex;
-    // the last of them is the largest index in front of which there are fewer than n
-    return 1u + largest(0u, (uint32_t)a.vocab, [&](uint32_t i) {
-      return sum_of([&](const SampleItem& t) { return (uint64_t)(equal(t) && t.index < i); }) < n;
-    });
-  };
-  uint64_t weight = in.all;
-  if (bk >= 0) {
-    const uint64_t want = in.k - in.count;  // tokens of bin bk that stay
-    const uint32_t t = largest(key_lo, key_hi, [&](uint32_t x) {
-      return sum_of([&](const SampleItem& i) { return (uint64_t)(i.bin == bk && i.key >= x); }) >= want;
-    });
-    const uint64_t over = sum_of([&](const SampleItem& i) { return (uint64_t)(i.bin == bk && i.key > t); });
-    const uint32_t cut = first_of(t, want - over);
-    key = t;
-    below = cut;
-    weight = in.weight + sum_of([&](const SampleItem& i) { return i.bin == bk && stays(i) ? i.units : 0ull; });
-  }
-  if (in.p < 1.0) {
-    const uint64_t want = part(in.p, weight);
-    const auto upto = [&](uint32_t x) {  // weight of the tokens with keys of at least x
-      return in.before + sum_of([&](const SampleItem& i) { return i.bin >= plo && i.bin <= phi && i.key >= x && stays(i) ? i.units : 0ull; });
-    };
-    if (upto(key_lo) >= want) {
-      const uint32_t t = largest(key_lo, key_hi, [&](uint32_t x) { return upto(x) >= want; });
-      const uint64_t over = t == kNoIndex ? in.before : upto(t + 1u);
-      SampleItem one;
-      item_of(float_of(t), 0u, one);  // (t is the key of a token)
-      const uint32_t cut = first_of(t, (want - over + one.units - 1) / one.units);
-      below = t == key ? (cut < below ? cut : below) : cut;
-      key = t;
-    }
-  }
-  // the sums of 512 tokens each, with the border's
-  if (fits) {
-    each([&](const SampleItem& t) {
-      if (stays(t) && t.heavy) atomicAdd(reinterpret_cast<unsigned long long*>(&sub[t.index / kSampleSub]), (unsigned long long)t.units);
-    });
-  } else {
-    for (int s0 = kSampleSub * w; s0 < a.vocab; s0 += 4 * kSampleSub) {
-      float x[8];
-      const int i = s0 + 8 * lane;
-      eight_logits<T>(row, i, a.vocab, x);
-      uint64_t sum = 0;
-      for (int j = 0; j < 8; ++j) {
-        SampleItem t;
-        if (item_of(x[j], i + j, t) && stays(t) && t.heavy) sum += t.units;
+          for (int j = 0; j < 8; ++j) {
+            const uint64_t y = of.octaves(x[j]);
+            const int bin = of.bin(y);
+            if (border.at(bin) && of.units(y) != 0) s += f(rank_of(x[j], i + j), y, bin);
+          }
+        }
+        return block_sum64(s, waves);
+      };
+      // the largest rank x with f(x), which holds at 0 and, where it holds, for everything smaller
+      auto largest = [&](auto f) {
+        uint64_t lo = 0, hi = ~0ull;
+        while (lo < hi) {
+          const uint64_t mid = lo + (hi - lo) / 2 + 1;
+          if (f(mid)) lo = mid;
+          else hi = mid - 1;
+        }
+        return lo;
+      };
+      if (bk >= 0) {
+        least = largest([&](uint64_t x) {
+          return sum_of([&](uint64_t rank, uint64_t, int bin) { return (uint64_t)(bin == bk && rank >= x); }) >= want_k;
+        });
+        total += sum_of([&](uint64_t rank, uint64_t y, int bin) { return bin == bk && rank >= least ? of.units(y) : 0ull; });
       }
-      sum = wave_sum64(sum);
-      if (lane == 0) sub[s0 / kSampleSub] = sum;
+      if (p < 1.0) {
+        const uint64_t want = part(p, total), stays = least;
+        const auto upto = [&](uint64_t x) {  // weight of the tokens with ranks of at least x
+          return in_front_of_plo + sum_of([&](uint64_t rank, uint64_t y, int bin) { return bin <= phi && rank >= x && rank >= stays ? of.units(y) : 0ull; });
+        };
+        if (upto(0) >= want) least = largest([&](uint64_t x) { return upto(x) >= want; });
+      }
+      for (int s0 = kSampleSub * w; s0 < a.vocab; s0 += kSampleWaves * kSampleSub) {
+        float x[8];
+        const int i = s0 + 8 * lane;
+        eight_logits<T>(row, i, a.vocab, x);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t y = of.octaves(x[j]);
+          if (y <= border.lightest && rank_of(x[j], i + j) >= least) sum += of.units(y);
+        }
+        sum = wave_sum64(sum);
+        if (lane == 0) sh.sub[s0 / kSampleSub] = sum;
+      }
     }
   }
   __syncthreads();
   // which of them the random number falls into
-  constexpr int kPer = kSampleSubs / 256;
-  uint64_t mine[kPer], sum = 0;
+  constexpr int kPer = kSampleSubs / kSampleThreads;
+  uint64_t mine[kPer], sum = 0, all;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    mine[i] = kPer * tid + i < a.subs ? sub[kPer * tid + i] : 0u;
+    mine[i] = kPer * tid + i < a.subs ? sh.sub[kPer * tid + i] : 0u;
     sum += mine[i];
   }
-  const uint64_t scan = wave_scan64(sum);
-  if (lane == 63) four[w] = scan;
-  __syncthreads();
-  uint64_t before = scan - sum;
-  for (int i = 0; i < w; ++i) before += four[i];
-  const uint64_t all = four[0] + four[1] + four[2] + four[3];
+  uint64_t before = block_scan64(sum, waves, all);
   const double u = (double)a.u[r * a.u_s];
   const double aim = u > 0.0 ? floor(u * (double)all) : 0.0;  // (a NaN: 0)
   uint64_t target = aim < (double)all ? (uint64_t)aim : all - 1;
@@ -617,22 +643,23 @@ __global__ __launch_bounds__(256) void sample_pick(SampleArgs a) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (before <= target && target < before + mine[i]) {
-      chosen = kPer * tid + i;
-      left = target - before;
+      sh.chosen = kPer * tid + i;
+      sh.left = target - before;
     }
     before += mine[i];
   }
   __syncthreads();
   if (w != 0) return;
-  const int i0 = kSampleSub * chosen + 8 * lane;
+  const int i0 = kSampleSub * sh.chosen + 8 * lane;
+  const uint64_t left = sh.left;
   float x[8];
   eight_logits<T>(row, i0, a.vocab, x);
   uint64_t units[8];
   sum = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    SampleItem t;
-    units[j] = item_of(x[j], i0 + j, t) && stays(t) && t.heavy ? t.units : 0u;
+    const uint64_t y = of.octaves(x[j]);
+    units[j] = y <= border.lightest && rank_of(x[j], i0 + j) >= least ? of.units(y) : 0u;
     sum += units[j];
   }
   uint64_t upto = wave_scan64(sum) - sum;
@@ -643,15 +670,64 @@ __global__ __launch_bounds__(256) void sample_pick(SampleArgs a) {
   }
 }
 
-// Tokens of a workgroup: enough workgroups for the card, where there are that many tokens.
+// --------------------------------------------------------------------------------------- launches ----
+template <typename T>
+__global__ __launch_bounds__(kSampleThreads) void sample_top(SampleArgs a) {
+  __shared__ SampleTop sh;
+  top_step<T>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, sh);
+}
+template <typename T>
+__global__ __launch_bounds__(kSampleThreads) void sample_bins(SampleArgs a) {
+  __shared__ double table[kSampleTable];
+  __shared__ uint64_t waves[kSampleWaves];
+  __shared__ __attribute__((aligned(16))) SampleBins sh;
+  bins_step<T>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
+}
+__global__ __launch_bounds__(kSampleThreads) void sample_join(SampleArgs a) {
+  __shared__ uint64_t waves[kSampleWaves];
+  __shared__ SampleJoin sh;
+  join_step(a, blockIdx.x, waves, sh);
+}
+template <typename T>
+__global__ __launch_bounds__(kSampleThreads) void sample_sums(SampleArgs a) {
+  __shared__ double table[kSampleTable];
+  __shared__ uint64_t waves[kSampleWaves];
+  __shared__ SampleSums sh;
+  sums_step<T>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
+}
+template <typename T>
+__global__ __launch_bounds__(kSampleThreads) void sample_finish(SampleArgs a) {
+  __shared__ double table[kSampleTable];
+  __shared__ uint64_t waves[kSampleWaves];
+  __shared__ SampleFinish sh;
+  finish_step<T>(a, blockIdx.x, table, waves, sh);
+}
+// All steps of a row that is one segment, by one workgroup, which sees its own writes behind a barrier.
+template <typename T>
+__global__ __launch_bounds__(kSampleThreads) void sample_whole(SampleArgs a) {
+  __shared__ __attribute__((aligned(16))) SampleShared sh;
+  const int r = blockIdx.x;
+  top_step<T>(a, 0, r, sh.top);
+  __syncthreads();
+  if (a.filters) {
+    bins_step<T>(a, 0, r, sh.table, sh.waves, sh.bins);
+    __syncthreads();
+    join_step(a, r, sh.waves, sh.join);
+    __syncthreads();
+  }
+  sums_step<T>(a, 0, r, sh.table, sh.waves, sh.sums);
+  __syncthreads();
+  finish_step<T>(a, r, sh.table, sh.waves, sh.finish);
+}
+
+// Tokens of a workgroup: enough workgroups for the card where there are that many tokens, at most kSampleSeg.
 static int sample_seg(int64_t rows, int64_t vocab) {
-  int64_t seg = cdiv(cdiv(vocab * rows, 1024), 4 * kSampleSub) * 4 * kSampleSub;
-  const int64_t whole = cdiv(vocab, 4 * kSampleSub) * 4 * kSampleSub;
-  return (int)(seg < whole ? seg : whole);
+  constexpr int64_t step = kSampleWaves * kSampleSub;
+  return vocab > step && rows * vocab > 512 * step ? kSampleSeg : (int)step;
 }
 
 struct SampleSpace {
-  int64_t row, tops, weights, sub, list, counts, ends, lows, bytes;
+  int64_t row, part, sub, list, bins, listed, bytes;
 };
 static SampleSpace sample_space(int64_t rows, int64_t vocab) {
   const int64_t segs = cdiv(vocab, sample_seg(rows, vocab)), subs = cdiv(vocab, kSampleSub);
@@ -659,30 +735,38 @@ static SampleSpace sample_space(int64_t rows, int64_t vocab) {
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t x = at;
-    at += (bytes + 15) & ~INT64_C(15);
+    at += (bytes + 15) & ~INT64_C(15);  // (16-byte loads)
     return x;
   };
   s.row = take(rows * sizeof(SampleRow));
-  s.tops = take(rows * segs * 8);
-  s.weights = take(rows * segs * kSampleBins * 8);
+  s.part = take(rows * segs * sizeof(SampleSeg));
   s.sub = take(rows * subs * 8);
   s.list = take(rows * kSampleList * 8);
-  s.counts = take(rows * segs * kSampleBins * 4);
-  s.ends = take(rows * 3 * 4);
-  s.lows = take(rows * segs * 4);
+  s.bins = take(rows * segs * kSampleBins * 4);
+  s.listed = take(rows * 4);
   s.bytes = at;
   return s;
 }
 
 template <typename T>
 static int sample_launch(const SampleArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.rows * a.segs));
-  hipLaunchKernelGGL((sample_top<T>), grid, dim3(256), 0, s, a);
+  const dim3 rows((unsigned)a.rows), all((unsigned)(a.rows * a.segs)), threads(kSampleThreads);
+  if (a.segs == 1) {
+    hipLaunchKernelGGL((sample_whole<T>), rows, threads, 0, s, a);
+    return check_launch("sample_whole");
+  }
+  hipLaunchKernelGGL((sample_top<T>), all, threads, 0, s, a);
   if (const int rc = check_launch("sample_top")) return rc;
-  hipLaunchKernelGGL((sample_bins<T>), grid, dim3(256), 0, s, a);
-  if (const int rc = check_launch("sample_bins")) return rc;
-  hipLaunchKernelGGL((sample_pick<T>), grid, dim3(256), 0, s, a);
-  return check_launch("sample_pick");
+  if (a.filters) {
+    hipLaunchKernelGGL((sample_bins<T>), all, threads, 0, s, a);
+    if (const int rc = check_launch("sample_bins")) return rc;
+    hipLaunchKernelGGL(sample_join, rows, threads, 0, s, a);
+    if (const int rc = check_launch("sample_join")) return rc;
+  }
+  hipLaunchKernelGGL((sample_sums<T>), all, threads, 0, s, a);
+  if (const int rc = check_launch("sample_sums")) return rc;
+  hipLaunchKernelGGL((sample_finish<T>), rows, threads, 0, s, a);
+  return check_launch("sample_finish");
 }
 
 }  // namespace biops
@@ -712,14 +796,13 @@ extern "C" int biops_sample(int dtype, int64_t rows, int64_t vocab, const void* 
   a.u = u, a.temperature = temperature, a.top_p = top_p, a.min_p = min_p, a.top_k = top_k;
   a.u_s = u_s, a.t_s = t_s, a.k_s = k_s, a.p_s = p_s, a.m_s = m_s;
   a.t0 = t0, a.p0 = p0, a.m0 = m0, a.k0 = k0, a.k64 = k64 != 0;
+  a.filters = top_k || top_p || (k0 > 0 && k0 < vocab) || p0 < 1.0;
   a.out = out, a.rows = (int)rows, a.vocab = (int)vocab;
   a.seg = sample_seg(rows, vocab), a.segs = (int)cdiv(vocab, a.seg), a.subs = (int)cdiv(vocab, kSampleSub);
   char* const base = static_cast<char*>(workspace);
-  a.row = reinterpret_cast<SampleRow*>(base + x.row);
-  a.tops = reinterpret_cast<uint64_t*>(base + x.tops), a.weights = reinterpret_cast<uint64_t*>(base + x.weights);
+  a.row = reinterpret_cast<SampleRow*>(base + x.row), a.part = reinterpret_cast<SampleSeg*>(base + x.part);
   a.sub = reinterpret_cast<uint64_t*>(base + x.sub), a.list = reinterpret_cast<uint64_t*>(base + x.list);
-  a.counts = reinterpret_cast<uint32_t*>(base + x.counts), a.ends = reinterpret_cast<uint32_t*>(base + x.ends);
-  a.lows = reinterpret_cast<float*>(base + x.lows);
+  a.bins = reinterpret_cast<uint32_t*>(base + x.bins), a.listed = reinterpret_cast<uint32_t*>(base + x.listed);
   hipStream_t s = static_cast<hipStream_t>(stream);
   BIOPS_DISPATCH_FLOAT(dtype, return sample_launch<T>(a, s));
   return BIOPS_OK;
