@@ -31,9 +31,14 @@ constexpr int kSampleSeg = 8192;               // most tokens of a segment: 14 b
 constexpr int kSamplePlace = 18;
 constexpr uint32_t kNoIndex = 0xffffffffu;
 
-struct SampleRow {   // what join finds
-  int plo, phi, bk;   // bins of the border of top-p (of top-k, where there is no top-p), of top-k; -1: none
-  uint32_t count;     // tokens in front of bin bk
+struct SampleRow {    // what join finds, and what several workgroups would have to compute again
+  double top, c;       // SampleWeight
+  uint64_t lightest;   // the largest y that min-p lets pass: log2(1 / min-p)
+  int64_t token;       // the answer where there is nothing to sample, -2 elsewhere
+  uint32_t scale;
+  int plo, phi, bk;    // bins of the border of top-p (of top-k, where there is no top-p), of top-k; -1: none
+  uint32_t count;      // tokens in front of bin bk
+  int unused;
 };
 struct SampleSeg {                // of a segment
   uint64_t top;                   // rank of the largest logit, 0 where nothing counts
@@ -123,9 +128,25 @@ struct SampleWeight {
     return (uint64_t)__double_as_longlong(sized + 0x1p52) & 0xfffffffffffffull;  // to the nearest
   }
 };
+// The table, by the exponential's series for 2^(-i / 1024) = e^(-i ln 2 / 1024): 24 terms leave less than 2^-80.
+struct SampleTable {
+  double value[kSampleTable];
+};
+constexpr SampleTable make_table() {
+  SampleTable t{};
+  for (int i = 0; i < kSampleTable; ++i) {
+    const double x = -0.6931471805599453 * i / kSampleTable;
+    double sum = 1.0;
+    for (int n = 24; n > 0; --n) sum = 1.0 + sum * x / n;
+    t.value[i] = sum;
+  }
+  return t;
+}
+__device__ const SampleTable kTable = make_table();
 // (__syncthreads before use)
 __device__ __forceinline__ void fill_table(double* table) {
-  for (int i = threadIdx.x; i < kSampleTable; i += kSampleThreads) table[i] = exp2(-(double)i / kSampleTable);
+  static_assert(kSampleTable == 2 * kSampleThreads, "16 bytes a thread");
+  reinterpret_cast<u32x4_t*>(table)[threadIdx.x] = reinterpret_cast<const u32x4_t*>(kTable.value)[threadIdx.x];
 }
 
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
@@ -189,7 +210,7 @@ struct SampleSums {
   uint32_t met, ready;
 };
 struct SampleFinish {
-  uint64_t sub[kSampleSubs], item[kSampleList];
+  uint64_t sub[kSampleSubs], item[kSampleList], other[kSampleThreads];
   int chosen;
   uint64_t left;
 };
@@ -249,33 +270,69 @@ __device__ __forceinline__ void top_step(const SampleArgs& a, int seg, int r, Sa
   }
 }
 
-// The row's weights, from its segments' largest and smallest logits and its temperature (every wavefront by itself).  False
-// where there is nothing to sample: `token` is then the row's answer.
-__device__ __forceinline__ bool row_weights(const SampleArgs& a, int r, const double* table, SampleWeight& of, int64_t& token) {
-  uint64_t top = 0;
-  float low = INFINITY;
+// What a row's segments have found, together.
+struct SampleWhole {
+  uint64_t top, all, before, weight;
+  float low;
+};
+// (every wavefront by itself; all that is asked for is read at once)
+template <bool ALL, bool PARTS>
+__device__ __forceinline__ SampleWhole over_segments(const SampleArgs& a, int r) {
+  SampleWhole v{0, 0, 0, 0, INFINITY};
   for (int s = threadIdx.x & 63; s < a.segs; s += 64) {
-    const SampleSeg& part = a.part[(int64_t)r * a.segs + s];
-    top = part.top > top ? part.top : top;
-    low = fminf(low, part.low);
+    const SampleSeg part = a.part[(int64_t)r * a.segs + s];
+    v.top = part.top > v.top ? part.top : v.top;
+    v.low = fminf(v.low, part.low);
+    if (ALL) v.all += part.all;
+    if (PARTS) {
+      v.before += part.before;
+      v.weight += part.weight;
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t t = (uint64_t)__shfl_xor((unsigned long long)top, o, 64);
-    top = t > top ? t : top;
-    low = fminf(low, __shfl_xor(low, o, 64));
+    const uint64_t t = (uint64_t)__shfl_xor((unsigned long long)v.top, o, 64);
+    v.top = t > v.top ? t : v.top;
+    v.low = fminf(v.low, __shfl_xor(v.low, o, 64));
+    if (ALL) v.all += (uint64_t)__shfl_xor((unsigned long long)v.all, o, 64);
+    if (PARTS) {
+      v.before += (uint64_t)__shfl_xor((unsigned long long)v.before, o, 64);
+      v.weight += (uint64_t)__shfl_xor((unsigned long long)v.weight, o, 64);
+    }
   }
-  const double t = row_value(a.temperature, a.t_s, a.t0, r);
-  token = top == 0 ? -1 : (int64_t)(kNoIndex - (uint32_t)top);
-  if (top == 0 || !(t > 0.0)) return false;
-  of.top = (double)float_of((uint32_t)(top >> 32));
+  return v;
+}
+
+// The row's weights, from its largest and smallest logits and its temperature.  False where there is nothing to sample: `token`
+// is then the row's answer.
+__device__ __forceinline__ bool row_weights(const SampleWhole& whole, double t, const double* table, SampleWeight& of, int64_t& token) {
+  token = whole.top == 0 ? -1 : (int64_t)(kNoIndex - (uint32_t)whole.top);
+  if (whole.top == 0 || !(t > 0.0)) return false;
+  of.top = (double)float_of((uint32_t)(whole.top >> 32));
   of.infinite = of.top == INFINITY;
   of.c = fmin(1.4426950408889634 / t, 1e300);  // (finite: 0 times it is 0)
   of.table = table;
-  const uint64_t most = 44ull << 40, range = of.infinite ? 0u : of.octaves(low);  // (weights below 2^-44 are 0)
+  const uint64_t most = 44ull << 40, range = of.infinite ? 0u : of.octaves(whole.low);  // (weights below 2^-44 are 0)
   const double scale = (double)(kSampleBins * kSampleInside) * 0x1p32 / (double)((range < most ? range : most) / 16384 + 1);
   of.scale = scale < 4294967295.0 ? (uint32_t)scale : 0xffffffffu;
   return true;
+}
+__device__ __forceinline__ double row_t(const SampleArgs& a, int r) { return row_value(a.temperature, a.t_s, a.t0, r); }
+// A row without borders.
+__device__ __forceinline__ SampleRow plain_row(const SampleArgs& a, int r, const SampleWhole& whole) {
+  const double min_p = fmin(row_value(a.min_p, a.m_s, a.m0, r), 1.0);
+  SampleRow row{0.0, 0.0, 50ull << 40, -2, 0u, kSampleBins, -1, -1, 0u, 0};
+  SampleWeight of;
+  int64_t token;
+  if (!row_weights(whole, row_t(a, r), nullptr, of, token)) {
+    row.token = token;
+    return row;
+  }
+  row.top = of.top;
+  row.c = of.c;
+  row.scale = of.scale;
+  if (min_p > 0x1p-49) row.lightest = (uint64_t)(-log2(min_p) * 0x1p40 + 0.5);
+  return row;
 }
 
 __device__ __forceinline__ uint64_t part(double p, uint64_t weight) {  // the weight that top-p asks for, at least one unit
@@ -298,17 +355,23 @@ template <typename T>
 __device__ __forceinline__ void bins_step(const SampleArgs& a, int seg, int r, double* table, uint64_t* waves, SampleBins& sh) {
   const int tid = threadIdx.x;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
-  SampleWeight of;
-  int64_t token;
-  if (!row_weights(a, r, table, of, token) || (row_k(a, r) == 0 && row_p(a, r) == 1.0)) return;
+  const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
+  float next[8];  // (on their way while the row's settings are)
+  eight_logits<T>(row, seg * a.seg + 8 * tid, a.vocab, next);
   fill_table(table);
   for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.bins[i] = 0u;
+  const int64_t k = row_k(a, r);
+  const double p = row_p(a, r);
+  SampleWeight of;
+  int64_t token;
+  if (!row_weights(over_segments<false, false>(a, r), row_t(a, r), table, of, token) || (k == 0 && p == 1.0)) return;
   __syncthreads();
-  const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
   uint64_t sum = 0;
   for (int i = seg * a.seg + 8 * tid; i < end; i += 8 * kSampleThreads) {
     float x[8];
-    eight_logits<T>(row, i, a.vocab, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = next[j];
+    if (i + 8 * kSampleThreads < end) eight_logits<T>(row, i + 8 * kSampleThreads, a.vocab, next);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint64_t y = of.octaves(x[j]), units = of.units(y);
@@ -324,28 +387,13 @@ __device__ __forceinline__ void bins_step(const SampleArgs& a, int seg, int r, d
   *reinterpret_cast<u32x4_t*>(a.bins + at * kSampleBins + 4 * tid) = *reinterpret_cast<const u32x4_t*>(sh.bins + 4 * tid);
 }
 
-// The sum of a member over a row's segments (every wavefront by itself).
-template <typename F>
-__device__ __forceinline__ uint64_t over_segments(const SampleArgs& a, int r, F member) {
-  uint64_t v = 0;
-  for (int s = threadIdx.x & 63; s < a.segs; s += 64) v += member(a.part[(int64_t)r * a.segs + s]);
-  return wave_sum64(v);
-}
-
 __device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* waves, SampleJoin& sh) {
   const int tid = threadIdx.x;
-  SampleWeight of;
-  int64_t token;
-  if (!row_weights(a, r, nullptr, of, token)) return;
   const uint64_t k = (uint64_t)row_k(a, r);
   const double p = row_p(a, r);
-  if (k == 0 && p == 1.0) {
-    if (tid == 0) a.row[r] = SampleRow{kSampleBins, -1, -1, 0u};
-    return;
-  }
   // four bins a thread: their tokens, and bounds of their weights
   uint32_t n[4] = {0u, 0u, 0u, 0u}, places[4] = {0u, 0u, 0u, 0u};
-#pragma unroll 4
+#pragma unroll 8
   for (int g = 0; g < a.segs; ++g) {
     const u32x4_t v = *reinterpret_cast<const u32x4_t*>(a.bins + ((int64_t)r * a.segs + g) * kSampleBins + 4 * tid);
 #pragma unroll
@@ -354,16 +402,24 @@ __device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* 
       places[i] += v[i] & ((1u << kSamplePlace) - 1u);
     }
   }
+  const SampleWhole whole = over_segments<true, false>(a, r);
+  SampleRow row = plain_row(a, r, whole);
+  if (row.token != -2 || (k == 0 && p == 1.0)) {  // (there are no bins)
+    if (tid == 0) a.row[r] = row;
+    return;
+  }
   // A token of place i has y in [i w, (i + 1) w + 2^-26), w = 2^6 / scale octaves.  2^-y is convex: the sum over tokens whose
   // places have the mean f is at most the chord's from place 0 to the last, and at least their number times the value at f + 1.
-  const double width = 64.0 / (double)of.scale;
+  const double width = 64.0 / (double)row.scale;
   uint64_t least[4], most[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const double c = (double)n[i], at = (double)((4 * tid + i) * kSampleInside), f = (double)places[i];
-    const double w0 = exp2(43.0 - at * width), w1 = exp2(43.0 - (at + (kSampleInside - 1)) * width);
-    const double high = (c * w0 + (w1 - w0) * f / (kSampleInside - 1)) * 1.000001 + c;  // (and half a unit's rounding each)
-    const double low = n[i] ? c * exp2(43.0 - (at + f / c + 1.0) * width) * 0.999999 - c : 0.0;
+    // (32-bit powers of arguments below 64: 2^-24 64 ln 2 of the argument's rounding and 2^-22 of their own, less than 1e-5)
+    const double w0 = __builtin_amdgcn_exp2f((float)(43.0 - at * width)), w1 = __builtin_amdgcn_exp2f((float)(43.0 - (at + (kSampleInside - 1)) * width));
+    const double high = (c * w0 + (w1 - w0) * f * (1.0 / (kSampleInside - 1))) * 1.00001 + c;  // (and half a unit's rounding each)
+    const double mean = f * (double)(1.f / (float)n[i]) * 1.0000003;
+    const double low = n[i] ? c * (double)__builtin_amdgcn_exp2f((float)(43.0 - (at + mean + 1.0) * width)) * 0.99999 - c : 0.0;
     least[i] = low > 0.0 ? (uint64_t)low : 0u;
     most[i] = n[i] ? (uint64_t)high + 1u : 0u;
   }
@@ -393,8 +449,7 @@ __device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* 
   const int bk = by_k ? sh.found[0] : -1;
   int plo = by_k ? bk : kSampleBins, phi = by_k ? bk : -1;
   if (p < 1.0) {  // the bins that can have the border
-    const uint64_t all = over_segments(a, r, [](const SampleSeg& s) { return s.all; });
-    const uint64_t first = part(p, by_k ? sh.bounds[0] : all), last = part(p, by_k ? sh.bounds[1] : all);
+    const uint64_t first = part(p, by_k ? sh.bounds[0] : whole.all), last = part(p, by_k ? sh.bounds[1] : whole.all);
     uint64_t low = lb, high = mb;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -408,74 +463,74 @@ __device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* 
     phi = by_k && bk < sh.found[2] ? bk : sh.found[2];
     if (phi < plo) phi = plo;
   }
-  if (tid == 0) a.row[r] = SampleRow{plo, phi, bk, by_k ? sh.count : 0u};
+  row.plo = plo;
+  row.phi = phi;
+  row.bk = bk;
+  row.count = by_k ? sh.count : 0u;
+  if (tid == 0) a.row[r] = row;
 }
 
 // ---------------------------------------------------------------------------- the border and the token ----
-struct SampleBorder {
-  int plo, phi, bk;
-  uint64_t lightest;  // the largest y that min-p lets pass: log2(1 / min-p)
-  __device__ __forceinline__ bool at(int bin) const { return (bin >= plo && bin <= phi) || bin == bk; }
-};
-__device__ __forceinline__ SampleBorder border_of(const SampleArgs& a, int r) {
-  SampleBorder b{kSampleBins, -1, -1, 50ull << 40};
-  if (a.filters) {
-    b.plo = a.row[r].plo;
-    b.phi = a.row[r].phi;
-    b.bk = a.row[r].bk;
-  }
-  const double min_p = fmin(row_value(a.min_p, a.m_s, a.m0, r), 1.0);
-  if (min_p > 0x1p-49) b.lightest = (uint64_t)(-log2(min_p) * 0x1p40 + 0.5);
-  return b;
+__device__ __forceinline__ bool at_border(const SampleRow& row, int bin) { return (bin >= row.plo && bin <= row.phi) || bin == row.bk; }
+__device__ __forceinline__ SampleWeight weights_of(const SampleRow& row, const double* table) {
+  return SampleWeight{row.top, row.c, row.top == INFINITY, row.scale, table};
 }
 
 template <typename T>
 __device__ __forceinline__ void sums_step(const SampleArgs& a, int seg, int r, double* table, uint64_t* waves, SampleSums& sh) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
-  SampleWeight of;
-  int64_t token;
-  if (!row_weights(a, r, table, of, token)) return;
-  const SampleBorder border = border_of(a, r);
-  const int last = border.bk > border.plo ? border.bk : border.plo;  // weights in front of it are needed
+  const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
+  float next[8];  // (on their way while the row's settings are)
+  eight_logits<T>(row, seg * a.seg + kSampleSub * w + 8 * lane, a.vocab, next);
   fill_table(table);
   if (tid == 0) sh.met = 0u;
+  const SampleRow border = a.filters ? a.row[r] : plain_row(a, r, over_segments<false, false>(a, r));
+  if (border.token != -2) return;
+  const SampleWeight of = weights_of(border, table);
   __syncthreads();
-  const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
   uint64_t before = 0, weight = 0;
   for (int s0 = seg * a.seg + kSampleSub * w; s0 < end; s0 += kSampleWaves * kSampleSub) {
     float x[8];
     const int i = s0 + 8 * lane;
-    eight_logits<T>(row, i, a.vocab, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = next[j];
+    if (s0 + kSampleWaves * kSampleSub < end) eight_logits<T>(row, i + kSampleWaves * kSampleSub, a.vocab, next);
     uint64_t sum = 0;
+    uint32_t near = 0u;  // of the eight, those at the border
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint64_t y = of.octaves(x[j]);
+      const uint64_t y = of.octaves(x[j]), units = of.units(y);
       const int bin = of.bin(y);
-      const bool near = border.at(bin);
-      if (bin >= last && !near) continue;
-      const uint64_t units = of.units(y);
-      if (bin < border.plo) {
-        before += units;
-        if (y <= border.lightest) sum += units;
-      }
-      if (bin < border.bk) weight += units;
-      if (near && units != 0) {
-        const uint32_t at = atomicAdd(&sh.met, 1u);
-        if (at < kSampleList) sh.item[at] = rank_of(x[j], i + j);
-      }
+      const uint64_t mine = bin < border.plo ? units : 0u;
+      before += mine;
+      sum += y <= border.lightest ? mine : 0u;
+      if (border.bk >= 0) weight += bin < border.bk ? units : 0u;
+      near |= (uint32_t)(at_border(border, bin) && units != 0) << j;
+    }
+    if (near != 0u) {
+      uint32_t at = atomicAdd(&sh.met, (uint32_t)__builtin_popcount(near));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (near >> j & 1u) {
+          if (at < kSampleList) sh.item[at] = rank_of(x[j], i + j);
+          ++at;
+        }
     }
     sum = wave_sum64(sum);
     if (lane == 0) a.sub[(int64_t)r * a.subs + s0 / kSampleSub] = sum;
   }
   if (!a.filters) return;
+  __syncthreads();
+  uint32_t ready = 0u;  // (the sums go on while it comes)
+  if (tid == 0 && sh.met > 0) ready = __hip_atomic_fetch_add(&a.listed[r], sh.met, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   before = block_sum64(before, waves);
   weight = block_sum64(weight, waves);
   SampleSeg& out = a.part[(int64_t)r * a.segs + seg];
   if (tid == 0) {
     out.before = before;
     out.weight = weight;
-    if (sh.met > 0) sh.ready = __hip_atomic_fetch_add(&a.listed[r], sh.met, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sh.ready = ready;
   }
   __syncthreads();
   for (uint32_t i = tid; i < sh.met && i < kSampleList && sh.ready < kSampleList - i; i += kSampleThreads)  // in any order
@@ -486,44 +541,66 @@ template <typename T>
 __device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* table, uint64_t* waves, SampleFinish& sh) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
-  SampleWeight of;
-  int64_t token;
-  if (!row_weights(a, r, table, of, token)) {  // nothing to choose from, or nothing to choose
-    if (tid == 0) a.out[r] = token;
-    return;
-  }
-  const SampleBorder border = border_of(a, r);
+  // what is read from memory goes out together: a wait for one after another is most of a small row's time
   const uint32_t listed = a.listed[r];
-  const bool fits = listed <= kSampleList;
+  const uint64_t some = a.list[(int64_t)r * kSampleList + tid];  // (its place exists; looked at up to `listed`)
+  const double u = (double)a.u[r * a.u_s];
   fill_table(table);
   for (int i = tid; i < a.subs; i += kSampleThreads) sh.sub[i] = a.sub[(int64_t)r * a.subs + i];
+  const double p = row_p(a, r);
+  const uint64_t k = (uint64_t)row_k(a, r);
+  const SampleWhole whole = over_segments<true, true>(a, r);  // (before and weight are there where there are filters)
+  const SampleRow border = a.filters ? a.row[r] : plain_row(a, r, whole);
+  if (border.token != -2) {  // nothing to choose from, or nothing to choose
+    if (tid == 0) a.out[r] = border.token;
+    return;
+  }
+  const SampleWeight of = weights_of(border, table);
+  const bool fits = listed <= kSampleList;
   __syncthreads();
   uint64_t least = 0;  // the rank of the last token that stays
   if (listed > 0) {
-    const double p = row_p(a, r);
     const int bk = border.bk, phi = border.phi;
-    const uint64_t want_k = bk >= 0 ? (uint64_t)row_k(a, r) - a.row[r].count : 0;  // tokens of bin bk that stay
-    const uint64_t in_front_of_plo = over_segments(a, r, [](const SampleSeg& s) { return s.before; });
-    uint64_t total = bk >= 0 ? over_segments(a, r, [](const SampleSeg& s) { return s.weight; })
-                             : over_segments(a, r, [](const SampleSeg& s) { return s.all; });
+    const uint64_t want_k = bk >= 0 ? k - border.count : 0;  // tokens of bin bk that stay
+    const uint64_t in_front_of_plo = whole.before;
+    uint64_t total = bk >= 0 ? whole.weight : whole.all;
     if (fits) {
-      // the list from the largest rank down (and zeros behind it)
-      int n = 64;
-      while (n < (int)listed) n *= 2;
-      for (int i = tid; i < n; i += kSampleThreads) sh.item[i] = i < (int)listed ? a.list[(int64_t)r * kSampleList + i] : 0u;
-      __syncthreads();
-      for (int size = 2; size <= n; size *= 2)
-        for (int step = size / 2; step > 0; step /= 2) {
-          for (int i = tid; i < n / 2; i += kSampleThreads) {
-            const int x = 2 * i - (i & (step - 1)), z = x + step;
-            const uint64_t p0 = sh.item[x], p1 = sh.item[z];
-            if ((p0 < p1) == ((x & size) == 0)) {
-              sh.item[x] = p1;
-              sh.item[z] = p0;
+      // the list from the largest rank down
+      if (listed <= kSampleThreads) {  // a token a thread, to the place behind all larger ones
+        sh.other[tid] = tid < (int)listed ? some : 0u;
+        __syncthreads();
+        int at = 0;
+        for (int i = 0; i < (int)listed; i += 4)  // (zeros behind the list)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) at += sh.other[i + j] > some;
+        if (tid < (int)listed) sh.item[at] = some;
+        __syncthreads();
+      } else {  // in pairs, and zeros behind it
+        int n = 2 * kSampleThreads;
+        while (n < (int)listed) n *= 2;
+        for (int i = tid; i < n; i += kSampleThreads)
+          sh.item[i] = i >= (int)listed ? 0u : (i == tid ? some : a.list[(int64_t)r * kSampleList + i]);
+        __syncthreads();
+        for (int size = 2; size <= n; size *= 2)
+          for (int step = size / 2; step > 0; step /= 2) {
+            for (int i = tid; i < n / 2; i += kSampleThreads) {
+              const int x = 2 * i - (i & (step - 1)), z = x + step;
+              const uint64_t p0 = sh.item[x], p1 = sh.item[z];
+              if ((p0 < p1) == ((x & size) == 0)) {
+                sh.item[x] = p1;
+                sh.item[z] = p0;
+              }
+            }
+            // up to steps of 64 a wavefront stays within 128 tokens of its own
+            if (step > 64 || (step == 1 && size >= 128)) {
+              __syncthreads();
+            } else {
+              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+              __builtin_amdgcn_wave_barrier();
             }
           }
-          __syncthreads();
-        }
+        __syncthreads();
+      }
       // running sums: of four tokens a thread
       constexpr int kPer = kSampleList / kSampleThreads;
       uint64_t units[kPer], upto[kPer], y[kPer], all;
@@ -583,7 +660,7 @@ __device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* 
           for (int j = 0; j < 8; ++j) {
             const uint64_t y = of.octaves(x[j]);
             const int bin = of.bin(y);
-            if (border.at(bin) && of.units(y) != 0) s += f(rank_of(x[j], i + j), y, bin);
+            if (at_border(border, bin) && of.units(y) != 0) s += f(rank_of(x[j], i + j), y, bin);
           }
         }
         return block_sum64(s, waves);
@@ -636,7 +713,6 @@ __device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* 
     sum += mine[i];
   }
   uint64_t before = block_scan64(sum, waves, all);
-  const double u = (double)a.u[r * a.u_s];
   const double aim = u > 0.0 ? floor(u * (double)all) : 0.0;  // (a NaN: 0)
   uint64_t target = aim < (double)all ? (uint64_t)aim : all - 1;
   if (target >= all) target = all - 1;  // (a sum that its double is larger than)
@@ -678,7 +754,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_top(SampleArgs a) {
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void sample_bins(SampleArgs a) {
-  __shared__ double table[kSampleTable];
+  __shared__ __attribute__((aligned(16))) double table[kSampleTable];
   __shared__ uint64_t waves[kSampleWaves];
   __shared__ __attribute__((aligned(16))) SampleBins sh;
   bins_step<T>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
@@ -690,14 +766,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_join(SampleArgs a) {
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void sample_sums(SampleArgs a) {
-  __shared__ double table[kSampleTable];
+  __shared__ __attribute__((aligned(16))) double table[kSampleTable];
   __shared__ uint64_t waves[kSampleWaves];
   __shared__ SampleSums sh;
   sums_step<T>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void sample_finish(SampleArgs a) {
-  __shared__ double table[kSampleTable];
+  __shared__ __attribute__((aligned(16))) double table[kSampleTable];
   __shared__ uint64_t waves[kSampleWaves];
   __shared__ SampleFinish sh;
   finish_step<T>(a, blockIdx.x, table, waves, sh);
