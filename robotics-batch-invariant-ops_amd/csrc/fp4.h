@@ -19,22 +19,18 @@ struct Fp4Range {
   static constexpr int kLow = 127 + (kHalf ? -23 : -125), kHigh = 127 + (kHalf ? 13 : 125);
 };
 
-// Eight elements of a block (`word`) times its power of two (a float of the exponent byte in its place), in T.
+// Elements 2 I and 2 I + 1 of the eight in a word of a block times its power of two (a float of the exponent byte in its place), in T.
+template <typename T, int I>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t word, float power) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    return __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, I));
+  else
+    return __builtin_bit_cast(uint32_t, (f16x2_t)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, power, I));
+}
+// All eight.
 template <typename T>
 __device__ __forceinline__ u32x4_t fp4_values(uint32_t word, float power) {
-  u32x4_t v;
-  if constexpr (std::is_same<T, bf16_t>::value) {
-    v[0] = __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 0));
-    v[1] = __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 1));
-    v[2] = __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 2));
-    v[3] = __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 3));
-  } else {
-    v[0] = __builtin_bit_cast(uint32_t, (f16x2_t)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, power, 0));
-    v[1] = __builtin_bit_cast(uint32_t, (f16x2_t)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, power, 1));
-    v[2] = __builtin_bit_cast(uint32_t, (f16x2_t)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, power, 2));
-    v[3] = __builtin_bit_cast(uint32_t, (f16x2_t)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, power, 3));
-  }
-  return v;
+  return u32x4_t{fp4_pair<T, 0>(word, power), fp4_pair<T, 1>(word, power), fp4_pair<T, 2>(word, power), fp4_pair<T, 3>(word, power)};
 }
 
 // The biased exponent of a block whose largest magnitude has the float bits `top`: the smallest power of two of which every

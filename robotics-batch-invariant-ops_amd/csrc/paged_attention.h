@@ -70,7 +70,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedArgs& a, int len) {
   s.shift = start - s.ns;
   s.n = s.ns + l - start;
   s.chunk = paged_chunk(s.n);
-  s.chunks = s.n > 0 ? (s.n - 1) / s.chunk + 1 : 0;
+  // (a power of two up to the length from which a sequence has all its chunks: a division is 20 instructions)
+  s.chunks = s.n <= 4 * kPagedKeys * kPagedChunks ? (s.n + s.chunk - 1) >> (31 - __builtin_clz((uint32_t)s.chunk)) : (s.n - 1) / s.chunk + 1;
   return s;
 }
 

@@ -17,6 +17,7 @@ namespace biops {
 struct Paged4Args : PagedArgs {
   const char *ks, *vs;                       // exponents
   int64_t ksP, ksS, ksH, vsP, vsS, vsH;      // byte strides
+  uint32_t page_factor, page_shift;          // key / page_size = key page_factor >> page_shift
 };
 
 typedef u32x4_t u32x4_byte_t __attribute__((aligned(1)));
@@ -24,14 +25,17 @@ typedef u32x2_t u32x2_byte_t __attribute__((aligned(1)));
 typedef uint32_t u32_byte_t __attribute__((aligned(1)));
 typedef uint16_t u16_byte_t __attribute__((aligned(1)));
 
+constexpr float kSlack = 8.f;  // powers of two that a weight may be larger than 1
+
 // Wavefronts per SIMD that registers are given out for.
 template <int DP, int DVP>
 constexpr int paged4_waves() {
   constexpr int wide = DP > DVP ? DP : DVP;
-  return wide <= 64 ? 5 : (wide <= 128 ? 3 : 2);
+  return wide <= 64 ? 4 : (wide <= 128 ? 3 : 2);
 }
 
-template <typename T, int DP, int DVP>
+// WHOLE: the head sizes are DP and DVP (and no lane is without elements).
+template <typename T, int DP, int DVP, bool WHOLE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged4_waves<DP, DVP>(), paged4_waves<DP, DVP>())))
 void paged4_chunk_kernel(Paged4Args a) {
   constexpr int KB = DP <= 64 ? 1 : DP / 128;           // blocks (or halves of one) of a key that a lane has
@@ -50,9 +54,9 @@ void paged4_chunk_kernel(Paged4Args a) {
 
   // Workgroups go round over the eight XCDs: the heads of a chunk, whose rows share lines of memory, to the same one.
   const uint32_t across = a.hkv * a.zs, id = a.first + blockIdx.x;
-  const uint32_t r = (id >> 3) % across, item = 8 * ((id >> 3) / across) + (id & 7);
+  const uint32_t r = (id >> 3) % across;
   const uint32_t z = r % a.zs, hk = r / a.zs;
-  uint32_t b = item;
+  uint32_t b = 8 * ((id >> 3) / across) + (id & 7);
   int c = 0, length;
   if (a.chunks == 1) {
     if (b >= a.batch) return;
@@ -88,55 +92,31 @@ void paged4_chunk_kernel(Paged4Args a) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d0 = element(s);
-      qf[s] = m16 < cols && d0 < a.d ? load_16(qr + 2 * d0) : u32x4_t{0u, 0u, 0u, 0u};
+      qf[s] = m16 < cols && (WHOLE || d0 < a.d) ? load_16(qr + 2 * d0) : u32x4_t{0u, 0u, 0u, 0u};
       if (a.negate | a.zero) qf[s] = score_query<T>(qf[s], a.negate, a.zero);
     }
   }
   __syncthreads();  // bad_page is clear
 
-  // Key `lane % 32` of a tile: the byte offset of its keys (lanes 0-31) or values, and their exponents (1 behind the end).
-  struct Place {
-    int64_t off;
-    uint32_t exps[XW];
-  };
-  bool bad = false;
+  // Key `lane % 32` of a tile: its page, then the byte offset of its keys (lanes 0-31) or values, and their exponents (1
+  // behind the end).
   const bool is_key = lane < 32;
   const int blocks = (is_key ? a.d : a.dv) >> 5;
-  const bool words = a.d == 128 && a.dv == 128;
   const int64_t rowP = is_key ? a.kP : a.vP, rowS = is_key ? a.kS : a.vS;
   const int64_t expP = is_key ? a.ksP : a.vsP, expS = is_key ? a.ksS : a.vsS;
   const char* const eb = is_key ? a.ks + hk * a.ksH : a.vs + hk * a.vsH;
-  auto lookup = [&](int tile) {
-    Place p;
-    int i = 32 * tile + (lane & 31);
-    const bool behind = i >= nkeys;
-    if (behind) i = nkeys - 1;
-    const int v = v0 + i;
-    const uint32_t key = (uint32_t)(v < span.ns ? v : v + span.shift);
-    const uint32_t page = key / a.page_size, at = key - page * a.page_size;
-    const int64_t e = b * a.tB + page * a.tW;
-    int64_t at_page = a.table64 ? reinterpret_cast<const int64_t*>(a.table)[e]
-                                : (int64_t) reinterpret_cast<const int32_t*>(a.table)[e];
-    if (at_page < 0 || at_page >= a.pages) {
-      bad = true;
-      at_page = 0;
-    }
-    p.off = at_page * rowP + at * rowS;
-    const char* x = eb + at_page * expP + at * expS;
-    if (words) {
-      p.exps[0] = *reinterpret_cast<const u32_byte_t*>(x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < XW; ++j) p.exps[j] = 0x7f7f7f7fu;
-#pragma unroll
-      for (int j = 0; j < 4 * XW; ++j)
-        if (j < blocks) p.exps[j >> 2] = (p.exps[j >> 2] & ~(255u << (8 * (j & 3)))) | (uint32_t)(uint8_t)x[j] << (8 * (j & 3));
-    }
-    if (behind)
-#pragma unroll
-      for (int j = 0; j < XW; ++j) p.exps[j] = 0x7f7f7f7fu;
-    return p;
+  auto key_at = [&](int tile) {
+    const int i = 32 * tile + (lane & 31), v = v0 + (i < nkeys ? i : nkeys - 1);
+    return (uint32_t)(v < span.ns ? v : v + span.shift);
   };
+  auto page_of = [&](int tile) -> int64_t {
+    const int64_t e = b * a.tB + (uint32_t)((uint64_t)key_at(tile) * a.page_factor >> a.page_shift) * a.tW;
+    return a.table64 ? reinterpret_cast<const int64_t*>(a.table)[e] : (int64_t) reinterpret_cast<const int32_t*>(a.table)[e];
+  };
+  struct Exps {
+    uint32_t word[XW];
+  };
+  bool bad = false;
 
   struct Tile {
     uint32_t k[2][KB][KW];
@@ -144,10 +124,26 @@ void paged4_chunk_kernel(Paged4Args a) {
   };
   const char* const kb = a.kc + hk * a.kH;
   const char* const vb = a.vc + hk * a.vH;
-  auto fetch = [&](Tile& t, int64_t off) {
-    offs[w][lane >> 5][lane & 31] = off;
+  // the loads of a tile whose pages are `id`
+  auto fetch = [&](Tile& t, Exps& x, int tile, int64_t id) {
+    if (id < 0 || id >= a.pages) {
+      bad = true;
+      id = 0;
+    }
+    const uint32_t key = key_at(tile), at = key - (uint32_t)((uint64_t)key * a.page_factor >> a.page_shift) * a.page_size;
+    offs[w][lane >> 5][lane & 31] = id * rowP + at * rowS;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    const char* e = eb + id * expP + at * expS;
+    if constexpr (WHOLE && DP == 128 && DVP == 128) {
+      x.word[0] = *reinterpret_cast<const u32_byte_t*>(e);
+    } else {
+#pragma unroll
+      for (int j = 0; j < XW; ++j) x.word[j] = 0x7f7f7f7fu;
+#pragma unroll
+      for (int j = 0; j < (DP > DVP ? DP : DVP) / 32; ++j)
+        if ((WHOLE && DP == DVP) || j < blocks) x.word[j >> 2] = (x.word[j >> 2] & ~(255u << (8 * (j & 3)))) | (uint32_t)(uint8_t)e[j] << (8 * (j & 3));
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const char* p = kb + offs[w][0][8 * (m16 >> 2) + 4 * i + (m16 & 3)];
@@ -155,11 +151,11 @@ void paged4_chunk_kernel(Paged4Args a) {
       for (int s = 0; s < KB; ++s) {
         const int d0 = element(s * KW);
         if constexpr (KW == 4) {
-          const u32x4_t x = d0 < a.d ? u32x4_t(*reinterpret_cast<const u32x4_byte_t*>(p + (d0 >> 1))) : u32x4_t{0u, 0u, 0u, 0u};
+          const u32x4_t x = WHOLE || d0 < a.d ? u32x4_t(*reinterpret_cast<const u32x4_byte_t*>(p + (d0 >> 1))) : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
           for (int j = 0; j < 4; ++j) t.k[i][s][j] = x[j];
         } else {
-          const u32x2_t x = d0 < a.d ? u32x2_t(*reinterpret_cast<const u32x2_byte_t*>(p + (d0 >> 1))) : u32x2_t{0u, 0u};
+          const u32x2_t x = WHOLE || d0 < a.d ? u32x2_t(*reinterpret_cast<const u32x2_byte_t*>(p + (d0 >> 1))) : u32x2_t{0u, 0u};
           t.k[i][s][0] = x[0];
           t.k[i][s][1] = x[1];
         }
@@ -171,8 +167,8 @@ void paged4_chunk_kernel(Paged4Args a) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         const int e0 = 16 * W * n + W * m16;
-        if constexpr (W == 8) t.v[n][j] = e0 < a.dv ? *reinterpret_cast<const u32_byte_t*>(p + (e0 >> 1)) : 0u;
-        else t.v[n][j] = e0 < a.dv ? (uint32_t)*reinterpret_cast<const u16_byte_t*>(p + (e0 >> 1)) : 0u;
+        if constexpr (W == 8) t.v[n][j] = WHOLE || e0 < a.dv ? *reinterpret_cast<const u32_byte_t*>(p + (e0 >> 1)) : 0u;
+        else t.v[n][j] = WHOLE || e0 < a.dv ? (uint32_t)*reinterpret_cast<const u16_byte_t*>(p + (e0 >> 1)) : 0u;
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -191,21 +187,24 @@ void paged4_chunk_kernel(Paged4Args a) {
     m = -INFINITY, from = 0.f, l = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    // One wait a tile: while it is worked on, the next one's rows and the pages of the one after it are on their way.
     Tile cur, next;
-    Place here, there;
+    Exps here, there;
+    int64_t id = 0;
     if (w < tiles) {
-      here = lookup(w);
-      fetch(cur, here.off);
-      if (w + 4 < tiles) there = lookup(w + 4);
+      fetch(cur, here, w, page_of(w));
+      if (w + 4 < tiles) id = page_of(w + 4);
     }
     for (int tile = w; tile < tiles; tile += 4) {
-      Place later = there;
-      if (tile + 4 < tiles) {
-        fetch(next, there.off);
-        if (tile + 8 < tiles) later = lookup(tile + 8);
-      }
+      if (32 * tile + (lane & 31) >= nkeys)
 #pragma unroll
-      for (int j = 0; j < XW; ++j) exps[w][j][lane >> 5][lane & 31] = here.exps[j];
+        for (int j = 0; j < XW; ++j) here.word[j] = 0x7f7f7f7fu;
+#pragma unroll
+      for (int j = 0; j < XW; ++j) exps[w][j][lane >> 5][lane & 31] = here.word[j];
+      if (tile + 4 < tiles) {
+        fetch(next, there, tile + 4, id);
+        if (tile + 8 < tiles) id = page_of(tile + 8);
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       f32x4_t sc[2];
@@ -237,7 +236,8 @@ void paged4_chunk_kernel(Paged4Args a) {
       for (int j = 1; j < 8; ++j) mx = fmaxf(mx, p[j]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      if (__any(mx > m)) {
+      // The sums are rescaled where a product has grown past the last maximum by 2^kSlack in its weight: weights go up to that.
+      if (__any((mx - m) * a.scale > kSlack || (mx > m && m == -INFINITY))) {
         const float mn = fmaxf(m, mx);
         const float corr = mx > m ? __builtin_amdgcn_exp2f((m - mn) * a.scale) : 1.f;
         l *= corr;
@@ -259,25 +259,38 @@ void paged4_chunk_kernel(Paged4Args a) {
       }
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        u32x4_t rows[8];  // 8 columns (4: the first two words) of value rows 8 q4 .. 8 q4 + 7
+        float power_of[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          rows[j] = fp4_values<T>(cur.v[n][j], power(exps[w][n][1][8 * q4 + j], W == 8 ? m16 >> 2 : m16 >> 3));
+        for (int j = 0; j < 8; ++j) power_of[j] = power(exps[w][n][1][8 * q4 + j], W == 8 ? m16 >> 2 : m16 >> 3);
+        // four columns of value rows 8 q4 .. 8 q4 + 7 at a time (all eight take registers of a whole wavefront)
+        auto columns = [&](auto half) {
+          constexpr int H = decltype(half)::value;
+          uint32_t rows[8][2];
 #pragma unroll
-        for (int t = 0; t < W; ++t) {
-          u32x4_t va;
+          for (int j = 0; j < 8; ++j) {
+            rows[j][0] = fp4_pair<T, 2 * H>(cur.v[n][j], power_of[j]);
+            rows[j][1] = fp4_pair<T, 2 * H + 1>(cur.v[n][j], power_of[j]);
+          }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            va[i] = __builtin_amdgcn_perm(rows[2 * i + 1][t >> 1], rows[2 * i][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-          mfma16<T>(acc[W * n + t], va, hi);
-          mfma16<T>(acc[W * n + t], va, lo);
+          for (int t = 0; t < 4; ++t) {
+            u32x4_t va;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              va[i] = __builtin_amdgcn_perm(rows[2 * i + 1][t >> 1], rows[2 * i][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+            mfma16<T>(acc[W * n + 4 * H + t], va, hi);
+            mfma16<T>(acc[W * n + 4 * H + t], va, lo);
+          }
+        };
+        columns(std::integral_constant<int, 0>());
+        if constexpr (W == 8) {
+          __builtin_amdgcn_sched_barrier(0);
+          columns(std::integral_constant<int, 1>());
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       cur = next;
       here = there;
-      there = later;
     }
     if constexpr (std::is_same<T, f16_t>::value) break;
     float odd = 0.f;  // NaN where a sum of the query is not finite
@@ -289,7 +302,7 @@ void paged4_chunk_kernel(Paged4Args a) {
     odd += __shfl_xor(odd, 32, 64);
     const bool past = odd != 0.f && down == 0.f && m16 < cols;
     if (!__any(past)) break;
-    if (past) down = (float)(32 - __builtin_clz((uint32_t)span.chunk / 4));  // (a wavefront has a quarter of the chunk's keys)
+    if (past) down = kSlack + (float)(32 - __builtin_clz((uint32_t)span.chunk / 4));  // (a wavefront has a quarter of the chunk's keys)
   }
   paged_finish<T, DVP, W>(a, smem, &bad_page, m, l, down, bad, acc, b, h0, c, cols);
 }
@@ -303,7 +316,8 @@ static int paged4_launch(Paged4Args a, hipStream_t s) {
   const uint32_t total = ((items + 7) & ~7u) * (a.hkv * a.zs);
   for (a.first = 0; a.first < total; a.first += most) {
     const uint32_t n = total - a.first < most ? total - a.first : most;
-    hipLaunchKernelGGL((paged4_chunk_kernel<T, DP, DVP>), dim3(n), dim3(256), lds, s, a);
+    if (a.d == DP && a.dv == DVP) hipLaunchKernelGGL((paged4_chunk_kernel<T, DP, DVP, true>), dim3(n), dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((paged4_chunk_kernel<T, DP, DVP, false>), dim3(n), dim3(256), lds, s, a);
     const int rc = check_launch("paged4_chunk_kernel");
     if (rc != BIOPS_OK) return rc;
   }
@@ -373,6 +387,11 @@ extern "C" int biops_paged_attention_fp4(int dtype, int64_t batch, int64_t hq, i
   a.tB = stB, a.tW = stW, a.lB = slB;
   a.pages = pages, a.page_size = (uint32_t)page_size;
   a.d = (int)d, a.dv = (int)dv;
+  // keys are below 2^31: with 2^l >= page_size the factor floor(2^(31 + l) / page_size) + 1 is off by at most 2^l / 2^(31 + l)
+  int bits = 0;
+  while ((INT64_C(1) << bits) < page_size) ++bits;
+  a.page_shift = 31 + bits;
+  a.page_factor = (uint32_t)((UINT64_C(1) << a.page_shift) / (uint64_t)page_size + 1);
   a.window = (int)(window < all ? window : all), a.sinks = (int)(sinks < all ? sinks : all);
   a.table64 = table64 != 0, a.lengths64 = lengths64 != 0;
   a.scale = score_scale(scale, &a.negate, &a.zero);
