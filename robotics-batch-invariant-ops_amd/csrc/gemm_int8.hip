@@ -170,7 +170,8 @@ __device__ __forceinline__ u32x4_t row_bytes(const int8_t* row, int64_t k, int64
 }
 
 // MB blocks of 16 rows; WAVES wavefronts share K.
-template <typename T, int MB, int WAVES>
+// WHOLE: K is a whole number of steps.
+template <typename T, int MB, int WAVES, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(Int8Args a) {
   __shared__ __attribute__((aligned(16))) i32x4_t part[WAVES][MB][64];
   constexpr int AHEAD = 8 / MB < 2 ? 2 : 8 / MB;  // K steps of 64 bytes whose loads go out together
@@ -193,16 +194,26 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(Int8Args a) {
     u32x4_t b[AHEAD], x[AHEAD][MB];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const int64_t k = s + j < s1 ? 64 * (s + j) + 16 * q4 : a.K;  // (behind the part: zeros)
-      b[j] = row_bytes(wr, k, a.K);
+      if constexpr (WHOLE) {
+        if (s + j >= s1) break;
+        const int64_t k = 64 * (s + j) + 16 * q4;
+        b[j] = *reinterpret_cast<const u32x4_byte_t*>(wr + k);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) x[j][i] = row_bytes(xr[i], k, a.K);
+        for (int i = 0; i < MB; ++i) x[j][i] = *reinterpret_cast<const u32x4_byte_t*>(xr[i] + k);
+      } else {
+        const int64_t k = s + j < s1 ? 64 * (s + j) + 16 * q4 : a.K;  // (behind the part: zeros)
+        b[j] = row_bytes(wr, k, a.K);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) x[j][i] = row_bytes(xr[i], k, a.K);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
+    for (int j = 0; j < AHEAD; ++j) {
+      if (WHOLE && s + j >= s1) break;
 #pragma unroll
       for (int i = 0; i < MB; ++i)
         acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, x[j][i]), __builtin_bit_cast(i32x4_t, b[j]), acc[i], 0, 0, 0);
+    }
   }
 #pragma unroll
   for (int i = 0; i < MB; ++i) part[w][i][lane] = acc[i];
@@ -291,32 +302,39 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
     xr[i] = a.x + m * a.ldx;
     wr[i] = a.w + n * a.ldw;
   }
-  u32x4_t x[2], v[2];
-  auto fetch = [&](int64_t k) {
+  constexpr int AHEAD = 4;  // steps whose loads are on their way
+  u32x4_t x[AHEAD][2], v[AHEAD][2];
+  auto fetch = [&](int s, int64_t k) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x[i] = row_bytes(xr[i], k + 16 * chunk, a.K);
-      v[i] = row_bytes(wr[i], k + 16 * chunk, a.K);
+      x[s][i] = row_bytes(xr[i], k + 16 * chunk, a.K);
+      v[s][i] = row_bytes(wr[i], k + 16 * chunk, a.K);
     }
   };
   i32x16_t acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0;
-  fetch(0);
-  int cur = 0;
-  for (int64_t k = 0; k < a.K; k += 128, cur ^= 1) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      *reinterpret_cast<u32x4_t*>(smem[cur][0] + lds_off(row + 32 * i, chunk)) = x[i];
-      *reinterpret_cast<u32x4_t*>(smem[cur][1] + lds_off(row + 32 * i, chunk)) = v[i];
+  for (int s = 0; s < AHEAD; ++s)
+    if (128 * s < a.K) fetch(s, 128 * s);
+  for (int64_t k0 = 0; k0 < a.K; k0 += 128 * AHEAD)
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      const int64_t k = k0 + 128 * s;
+      if (k >= a.K) break;
+      const int cur = s & 1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<u32x4_t*>(smem[cur][0] + lds_off(row + 32 * i, chunk)) = x[s][i];
+        *reinterpret_cast<u32x4_t*>(smem[cur][1] + lds_off(row + 32 * i, chunk)) = v[s][i];
+      }
+      __syncthreads();  // (two buffers: what is written next was read before this barrier)
+      if (k + 128 * AHEAD < a.K) fetch(s, k + 128 * AHEAD);
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        Mfma<i8_t>::step(acc, *reinterpret_cast<const u32x4_t*>(smem[cur][0] + lds_off(wm + lr, 2 * p + half)),
+                         *reinterpret_cast<const u32x4_t*>(smem[cur][1] + lds_off(wn + lr, 2 * p + half)));
     }
-    __syncthreads();  // (two buffers: what is written next was read before this barrier)
-    if (k + 128 < a.K) fetch(k + 128);
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-      Mfma<i8_t>::step(acc, *reinterpret_cast<const u32x4_t*>(smem[cur][0] + lds_off(wm + lr, 2 * p + half)),
-                       *reinterpret_cast<const u32x4_t*>(smem[cur][1] + lds_off(wn + lr, 2 * p + half)));
-  }
   const int64_t col = n0 + wn + lr;
   if (col >= a.N) return;
   const float ws = a.ws[col * a.ws_s], bias = a.bias ? Num<T>::load(static_cast<const T*>(a.bias) + col) : 0.f;
@@ -327,11 +345,16 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
   }
 }
 
+template <typename T, int MB, int WAVES>
+static void int8_few_waves(const Int8Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(a.N, 16)), threads(64 * WAVES);
+  if (a.K % 64 == 0) hipLaunchKernelGGL((int8_few_kernel<T, MB, WAVES, true>), grid, threads, 0, s, a);
+  else hipLaunchKernelGGL((int8_few_kernel<T, MB, WAVES, false>), grid, threads, 0, s, a);
+}
 template <typename T, int MB>
 static int int8_few(const Int8Args& a, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv(a.N, 16));
-  if (a.K > 4096 && a.N <= 4096) hipLaunchKernelGGL((int8_few_kernel<T, MB, 16>), grid, dim3(1024), 0, s, a);
-  else hipLaunchKernelGGL((int8_few_kernel<T, MB, 4>), grid, dim3(256), 0, s, a);
+  if (a.K > 4096 && a.N <= 4096) int8_few_waves<T, MB, 16>(a, s);
+  else int8_few_waves<T, MB, 4>(a, s);
   return check_launch("int8_few_kernel");
 }
 static void int8_tiles(Int8Args& a, int BM, int BN) {
