@@ -27,12 +27,13 @@ struct AppendArgs {
   const void *pos, *slots;
   int64_t pA, pT, slot_stride;                               // element strides
   int* flag;
-  uint8_t* stays;                                            // [row][kStayParts] whether no part of the later rows has its slot (null: to be found here)
+  uint8_t* stays;                                            // [kStayParts][rows] whether no part of the later rows has its slot (null: to be found here)
   uint32_t total, page;                                      // slots of the cache, slots of a page
   int rows, hq, hk, d, dv, pairs, pos_type, neighbours, slots64;
 };
 
 typedef uint32_t u32_byte_t __attribute__((aligned(1)));
+typedef u32x2_t u32x2_byte_t __attribute__((aligned(1)));
 
 // Elements e0 .. e0 + 7 (e0 a multiple of 8) of a head after its rotation, rounded to T.
 template <typename T>
@@ -70,23 +71,26 @@ __device__ __forceinline__ void rotated_eight(const T* src, int e0, const float*
   for (int i = 0; i < 8; ++i) y[i] = Num<T>::round(y[i]);
 }
 
-// Eight elements of a block (the next three lanes have the others, or those before) to `data`, its exponent to `exponents`.
-template <typename T>
-__device__ __forceinline__ void store_eight(const float (&y)[8], int e0, char* data, char* exponents, bool stays) {
+// 8 H elements of a block (4 / H lanes side by side have all of it) to `data`, the block's exponent to `exponents`.
+template <typename T, int H>
+__device__ __forceinline__ void store_part(const float (&y)[H][8], int e0, char* data, char* exponents, bool stays) {
   uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t x = __float_as_uint(y[i]) & 0x7fffffffu;
-    top = x > top ? x : top;
-  }
+  for (int h = 0; h < H; ++h)
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = __float_as_uint(y[h][i]) & 0x7fffffffu;
+      top = x > top ? x : top;
+    }
+#pragma unroll
+  for (int o = 1; o < 4 / H; o <<= 1) {
     const uint32_t x = (uint32_t)__shfl_xor((int)top, o, 64);
     top = x > top ? x : top;
   }
   const int e = fp4_exponent<T>(top);
   if (!stays) return;
-  *reinterpret_cast<u32_byte_t*>(data + (e0 >> 1)) = fp4_pack(y, e);
+  if constexpr (H == 2) *reinterpret_cast<u32x2_byte_t*>(data + (e0 >> 1)) = u32x2_t{fp4_pack(y[0], e), fp4_pack(y[1], e)};
+  else *reinterpret_cast<u32_byte_t*>(data + (e0 >> 1)) = fp4_pack(y[0], e);
   if (e0 % kFp4Block == 0) exponents[e0 / kFp4Block] = (char)e;
 }
 
@@ -142,13 +146,22 @@ __global__ __launch_bounds__(256) void stays_kernel(AppendArgs a) {
   }
   __syncthreads();
   constexpr int kAhead = 8;
+  auto row_at = [&](int i) { return i < a.rows ? i : a.rows - 1; };
   for (int base = first + 256 + 256 * kAhead * part; base < a.rows && low <= high; base += 256 * kAhead * kStayParts) {
     int64_t s[kAhead];
+    if (a.slots64) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) s[j] = base + 256 * j + tid < a.rows ? slot_of(a, base + 256 * j + tid) : -1;
+      for (int j = 0; j < kAhead; ++j) s[j] = reinterpret_cast<const int64_t*>(a.slots)[row_at(base + 256 * j + tid) * a.slot_stride];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) s[j] = reinterpret_cast<const int32_t*>(a.slots)[row_at(base + 256 * j + tid) * a.slot_stride];
+    }
+    uint32_t met[kAhead];  // (three of four places are free: most slots end here)
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) met[j] = slots[place((uint32_t)s[j])];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (s[j] < (int64_t)low || s[j] > (int64_t)high) continue;
+      if (met[j] == kNone || s[j] < (int64_t)low || s[j] > (int64_t)high || base + 256 * j + tid >= a.rows) continue;
       for (uint32_t i = place((uint32_t)s[j]); slots[i] != kNone; i = (i + 1) % kPlaces)
         if (slots[i] == (uint32_t)s[j]) {
           last[i] = a.rows;
@@ -157,7 +170,7 @@ __global__ __launch_bounds__(256) void stays_kernel(AppendArgs a) {
     }
   }
   __syncthreads();
-  if (r < a.rows) a.stays[(int64_t)r * kStayParts + part] = inside && last[at] == r;
+  if (r < a.rows) a.stays[part * a.rows + r] = inside && last[at] == r;
 }
 
 // FOUR: the cache is in 4 bits (T: bf16 or fp16); G: rows of a workgroup; FEW: which rows stay is found here.
@@ -175,12 +188,17 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int S = a.pairs, SP = (S + 7) & ~7;
   int64_t first = -1;
   if (tid < n) first = slot_of(a, r0 + tid);
-  if constexpr (!FEW)
+  bool stays = true;
+  if constexpr (!FEW) {
+    static_assert(kStayParts * G <= 256, "a thread for each part of a row");
+    if (tid < kStayParts * n) stays = a.stays[(tid / n) * a.rows + r0 + tid % n] != 0;
     if (tid < G) {
-      static_assert(kStayParts == 8, "a row's parts in 8 bytes");
-      place[tid] = tid < n && reinterpret_cast<const uint64_t*>(a.stays)[r0 + tid] == 0x0101010101010101ull ? first : -1;
+      place[tid] = first;
       again[tid] = 0;
     }
+    __syncthreads();
+    if (!stays) again[tid % n] = 1;
+  }
   for (int i = tid; i < n * S; i += 256) {
     const int r = i / S, j = i - r * S;
     float c, s;
@@ -191,9 +209,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   if constexpr (FEW) slots_that_stay<G>([&](int r) { return slot_of(a, r); }, r0, a.rows, first, a.total, a.flag, place, again);
   else __syncthreads();
 
-  // pieces: keys, values (in 4 bits a multiple of four each, so that a block's four lanes are together), queries
+  // pieces: keys, values (in 4 bits quarters of blocks, or halves where there are many rows; a block's lanes are together), queries
   const int np = rotary_pieces<T>(S, a.neighbours), whole = np + (a.d - 2 * S + VEC - 1) / VEC;
-  const int kn = FOUR ? a.d / 8 : whole, vn = FOUR ? a.dv / 8 : (a.dv + VEC - 1) / VEC;
+  constexpr int H = FEW ? 1 : 2;
+  const int kn = FOUR ? a.d / (8 * H) : whole, vn = FOUR ? a.dv / (8 * H) : (a.dv + VEC - 1) / VEC;
   const int keys = n * a.hk * kn, values = n * a.hk * vn, queries = n * a.hq * whole;
   for (int u = tid; u < keys + values + queries; u += 256) {
     if (u < keys) {
@@ -204,11 +223,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       const uint32_t s = stays ? (uint32_t)place[r] : 0u, page = s / a.page, at = s - page * a.page;
       char* const dst = a.kc + page * a.kcP + at * a.kcS + h * a.kcH;
       if constexpr (FOUR) {
-        float y[8];
-        rotated_eight<T>(src, 8 * c, cs, S, SP, a.neighbours, y);
-        store_eight<T>(y, 8 * c, dst, a.ks + page * a.ksP + at * a.ksS + h * a.ksH, stays);
+        float y[H][8];
+#pragma unroll
+        for (int i = 0; i < H; ++i) rotated_eight<T>(src, 8 * (H * c + i), cs, S, SP, a.neighbours, y[i]);
+        store_part<T, H>(y, 8 * H * c, dst, a.ks + page * a.ksP + at * a.ksS + h * a.ksH, stays);
       } else if (stays) {
-        rotary_piece<T>(c, np, src, reinterpret_cast<T*>(dst), cs, S, SP, a.d, a.neighbours);
+        rotary_piece<T, !FEW>(c, np, src, reinterpret_cast<T*>(dst), cs, S, SP, a.d, a.neighbours);
       }
     } else if (u < keys + values) {
       const int x = u - keys;
@@ -218,19 +238,20 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       const uint32_t s = stays ? (uint32_t)place[r] : 0u, page = s / a.page, at = s - page * a.page;
       char* const dst = a.vc + page * a.vcP + at * a.vcS + h * a.vcH;
       if constexpr (FOUR) {
-        float y[8];
-        unpack<T>(load_16(src + 8 * c), y);
-        store_eight<T>(y, 8 * c, dst, a.vs + page * a.vsP + at * a.vsS + h * a.vsH, stays);
+        float y[H][8];
+#pragma unroll
+        for (int i = 0; i < H; ++i) unpack<T>(load_16(src + 8 * (H * c + i)), y[i]);
+        store_part<T, H>(y, 8 * H * c, dst, a.vs + page * a.vsP + at * a.vsS + h * a.vsH, stays);
       } else if (stays) {
         T* const to = reinterpret_cast<T*>(dst);
-        if (VEC * (c + 1) <= a.dv) store_16(to + VEC * c, load_16(src + VEC * c));
+        if (VEC * (c + 1) <= a.dv) put_16<!FEW>(to + VEC * c, load_16(src + VEC * c));
         else
           for (int e = VEC * c; e < a.dv; ++e) to[e] = src[e];
       }
     } else {
       const int x = u - keys - values;
       const int c = x % whole, rh = x / whole, h = rh % a.hq, r = rh / a.hq;
-      rotary_piece<T>(c, np, reinterpret_cast<const T*>(a.q + (r0 + r) * a.qT + h * a.qH),
+      rotary_piece<T, !FEW>(c, np, reinterpret_cast<const T*>(a.q + (r0 + r) * a.qT + h * a.qH),
                       reinterpret_cast<T*>(a.oq + (r0 + r) * a.oqT + h * a.oqH), table + r * 2 * SP, S, SP, a.d, a.neighbours);
     }
   }
@@ -240,7 +261,7 @@ constexpr int kStayFew = 1024;  // rows up to which each workgroup looks for lat
 
 template <typename T, bool FOUR>
 static int append_launch(const AppendArgs& a, hipStream_t s) {
-  constexpr int kGroup = 4;
+  constexpr int kGroup = FOUR ? 16 : 4;
   const unsigned table = (unsigned)(2 * ((a.pairs + 7) & ~7) * sizeof(float));
   if (a.stays == nullptr) {
     hipLaunchKernelGGL((append_kernel<T, FOUR, 1, true>), dim3((unsigned)a.rows), dim3(256), table, s, a);
@@ -265,20 +286,19 @@ struct ReadArgs {
   int heads, d, dv, slots64;
 };
 
-// Eight elements a piece; pieces of a row are its heads' keys, then its heads' values.  A thread has kReadAhead pieces, 256 apart,
+// Eight elements a piece; pieces of a row are its heads' keys, then its heads' values.  A thread has AHEAD pieces, 256 apart,
 // whose loads go out together.
-constexpr int kReadAhead = 4;
-template <typename T>
+template <typename T, int AHEAD>
 __global__ __launch_bounds__(256) void read4_kernel(ReadArgs a) {
   const int kn = a.heads * (a.d / 8), per_row = kn + a.heads * (a.dv / 8);
   const int64_t all = a.rows * per_row;
-  const int64_t u0 = (int64_t)blockIdx.x * (256 * kReadAhead) + threadIdx.x;
-  int64_t s[kReadAhead];
-  int h[kReadAhead], e0[kReadAhead];
-  bool value[kReadAhead];
-  char* to[kReadAhead];
+  const int64_t u0 = (int64_t)blockIdx.x * (256 * AHEAD) + threadIdx.x;
+  int64_t s[AHEAD];
+  int h[AHEAD], e0[AHEAD];
+  bool value[AHEAD];
+  char* to[AHEAD];
 #pragma unroll
-  for (int i = 0; i < kReadAhead; ++i) {
+  for (int i = 0; i < AHEAD; ++i) {
     const int64_t u = u0 + 256 * i, r = u / per_row;
     int x = (int)(u - r * per_row);
     value[i] = x >= kn;
@@ -292,9 +312,9 @@ __global__ __launch_bounds__(256) void read4_kernel(ReadArgs a) {
       s[i] = a.slots64 ? reinterpret_cast<const int64_t*>(a.slots)[r * a.slot_stride]
                        : (int64_t) reinterpret_cast<const int32_t*>(a.slots)[r * a.slot_stride];
   }
-  uint32_t codes[kReadAhead], e[kReadAhead];
+  uint32_t codes[AHEAD], e[AHEAD];
 #pragma unroll
-  for (int i = 0; i < kReadAhead; ++i) {
+  for (int i = 0; i < AHEAD; ++i) {
     codes[i] = 0u;
     e[i] = 127u;
     if (s[i] >= 0 && s[i] < (int64_t)a.total) {
@@ -308,8 +328,8 @@ __global__ __launch_bounds__(256) void read4_kernel(ReadArgs a) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < kReadAhead; ++i)
-    if (u0 + 256 * i < all) store_16(to[i], fp4_values<T>(codes[i], __uint_as_float(e[i] << 23)));
+  for (int i = 0; i < AHEAD; ++i)
+    if (u0 + 256 * i < all) __builtin_nontemporal_store(fp4_values<T>(codes[i], __uint_as_float(e[i] << 23)), reinterpret_cast<u32x4_any_t*>(to[i]));
 }
 
 }  // namespace biops
@@ -410,11 +430,18 @@ extern "C" int biops_paged_read_fp4(int dtype, int64_t rows, int64_t heads, int6
   a.slots = slots, a.slot_stride = slot_stride, a.flag = flag, a.slots64 = slots64 != 0;
   a.total = (uint32_t)(pages * page_size), a.page = page_size > 0 ? (uint32_t)page_size : 1u;
   a.rows = rows, a.heads = (int)heads, a.d = (int)d, a.dv = (int)dv;
-  const int64_t blocks = cdiv(rows * heads * ((d + dv) / 8), 256 * kReadAhead);
-  if (blocks >= (1 << 24)) return fail(BIOPS_ERR_SIZE, "biops_paged_read_fp4: more than 2^24 blocks of 8192 elements");  // (2^32 threads)
-  const dim3 grid((unsigned)blocks);
+  const int64_t pieces = rows * heads * ((d + dv) / 8);
+  if (pieces >= INT64_C(1) << 34) return fail(BIOPS_ERR_SIZE, "biops_paged_read_fp4: more than 2^37 elements");  // (2^32 threads)
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == BIOPS_F16) hipLaunchKernelGGL((read4_kernel<f16_t>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((read4_kernel<bf16_t>), grid, dim3(256), 0, s, a);
+  // One piece a thread spreads few of them over the card.
+  if (pieces < 256 * 1024) {
+    const dim3 grid((unsigned)cdiv(pieces, 256));
+    if (dtype == BIOPS_F16) hipLaunchKernelGGL((read4_kernel<f16_t, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((read4_kernel<bf16_t, 1>), grid, dim3(256), 0, s, a);
+    return check_launch("read4_kernel");
+  }
+  const dim3 grid((unsigned)cdiv(pieces, 1024));
+  if (dtype == BIOPS_F16) hipLaunchKernelGGL((read4_kernel<f16_t, 4>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((read4_kernel<bf16_t, 4>), grid, dim3(256), 0, s, a);
   return check_launch("read4_kernel");
 }

@@ -42,6 +42,12 @@ __device__ __forceinline__ u32x4_t pack(const float (&x)[16 / sizeof(T)]) {
   return v;
 }
 __device__ __forceinline__ void store_16(void* p, const u32x4_t& v) { *reinterpret_cast<u32x4_any_t*>(p) = v; }
+// (PAST: past the caches)
+template <bool PAST>
+__device__ __forceinline__ void put_16(void* p, const u32x4_t& v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any_t*>(p));
+  else store_16(p, v);
+}
 
 __device__ __forceinline__ void turn(float& x0, float& x1, float c, float s) {
   const float y0 = __builtin_fmaf(x0, c, -(x1 * s)), y1 = __builtin_fmaf(x1, c, x0 * s);
@@ -66,12 +72,12 @@ __device__ __forceinline__ int rotary_pieces(int S, int neighbours) {
   return neighbours ? (2 * S + VEC - 1) / VEC : (S + VEC - 1) / VEC;
 }
 // Piece c of a head from src to dst, np of them rotated; cs: S cosines, and the sines SP places behind them.
-template <typename T>
+template <typename T, bool PAST = false>
 __device__ __forceinline__ void rotary_piece(int c, int np, const T* src, T* dst, const float* cs, int S, int SP, int d, int neighbours) {
   constexpr int VEC = 16 / sizeof(T);
   if (c >= np) {  // copied
     const int e0 = 2 * S + (c - np) * VEC;
-    if (e0 + VEC <= d) store_16(dst + e0, load_16(src + e0));
+    if (e0 + VEC <= d) put_16<PAST>(dst + e0, load_16(src + e0));
     else
       for (int e = e0; e < d; ++e) dst[e] = src[e];
   } else if (neighbours) {
@@ -81,7 +87,7 @@ __device__ __forceinline__ void rotary_piece(int c, int np, const T* src, T* dst
       unpack<T>(load_16(src + e0), v);
 #pragma unroll
       for (int i = 0; i < VEC / 2; ++i) turn(v[2 * i], v[2 * i + 1], cs[e0 / 2 + i], cs[SP + e0 / 2 + i]);
-      store_16(dst + e0, pack<T>(v));
+      put_16<PAST>(dst + e0, pack<T>(v));
     } else {
       for (int e = e0; e < 2 * S; e += 2) {
         float v0 = Num<T>::load(src + e), v1 = Num<T>::load(src + e + 1);
@@ -98,8 +104,8 @@ __device__ __forceinline__ void rotary_piece(int c, int np, const T* src, T* dst
       unpack<T>(load_16(src + S + e0), v1);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) turn(v0[i], v1[i], cs[e0 + i], cs[SP + e0 + i]);
-      store_16(dst + e0, pack<T>(v0));
-      store_16(dst + S + e0, pack<T>(v1));
+      put_16<PAST>(dst + e0, pack<T>(v0));
+      put_16<PAST>(dst + S + e0, pack<T>(v1));
     } else {
       for (int e = e0; e < S; ++e) {
         float v0 = Num<T>::load(src + e), v1 = Num<T>::load(src + S + e);
