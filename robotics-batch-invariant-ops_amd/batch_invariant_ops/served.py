@@ -192,7 +192,7 @@ def rotary_cache_write(
     plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(map(float, inv_freq)),
                         bool(interleaved_axes), bool(interleaved_pairs))
     module, watch = _direct_watch()
-    if module:
+    if module and query is not None:
         out = module.rotary_write(query, key, value, key_cache, value_cache, slots, positions, key_scales, value_scales, len(sections),
                                   plan.pairs, plan.turns_at, plan.axis_at, plan.neighbours, watch.flag_at)
         if out is not None:
@@ -240,7 +240,7 @@ def paged_cache_write_fp4(
     head_dim]`` and values ``[..., kv_heads, value_dim]``, each block to its power of two and its elements to the nearest level
     (ties to the even code), in place.  Slots are as there; the rows must not lie in the memory of the caches."""
     module, watch = _direct_watch()
-    if module and module.rotary_write(None, key, value, key_cache, value_cache, slots, None, key_scales, value_scales, 0, 0, 0, 0, 0,
+    if module and key_scales is not None and module.rotary_write(None, key, value, key_cache, value_cache, slots, None, key_scales, value_scales, 0, 0, 0, 0, 0,
                                       watch.flag_at):
         watch.after_call()
         return
@@ -409,7 +409,8 @@ def sample_tokens_batch_invariant(
     less the most likely token, and a ``min_p`` above 1 means 1.  Random numbers outside of [0, 1) count as the nearest inside.
 
     Logits of NaN count as -inf, which are never chosen; a row without any other gives -1.  Where logits are +inf only those
-    can be chosen.  Sums are of 64-bit weights and exact, so a token does not depend on the batch.  Up to 2**20 tokens and 65536 rows.
+    can be chosen.  Weights are multiples of 2**-43 (what is less than half of that is never chosen, and not counted) and their
+    sums are exact, so a token does not depend on the batch.  Up to 2**20 tokens and 65536 rows.
     """
     module = decoder._tensor_module or _direct()
     if module:

@@ -214,7 +214,7 @@ def test_empty_calls():
         same(a, b)
 
 
-@pytest.mark.parametrize("tokens", [64, 20001])
+@pytest.mark.parametrize("tokens", [64, 1025, 20001, 70001])
 def test_of_rows_for_one_slot_the_last_stays(tokens):
     """Inside a workgroup's rows, across workgroups and across launches."""
     slots = torch.randint(0, 40, (tokens,), generator=torch.Generator().manual_seed(40))
@@ -229,6 +229,33 @@ def test_of_rows_for_one_slot_the_last_stays(tokens):
         assert_bitwise(got, rq)
         for a, b in zip(caches, want):
             same(a, b)
+
+
+@pytest.mark.parametrize("tokens", [1500, 66000])
+def test_far_apart_rows_for_one_slot(tokens):
+    """Pages in any order, one repeated slot for each distance between its rows, padding and slots past the cache."""
+    g = torch.Generator().manual_seed(44)
+    pages = -(-tokens // 8) + 3
+    slots = (torch.randperm(pages, generator=g).view(-1, 1) * 8 + torch.arange(8)).view(-1)[:tokens]
+    for i, far in enumerate((1, 3, 4, 15, 16, 255, 256, 257, 1023, 1400)):
+        slots[i * 5 + far] = slots[i * 5]
+    slots[-1] = slots[7]
+    slots[700:720] = -1
+    slots[725] = pages * 8
+    k, v = randn(tokens, 1, 32, seed=45), randn(tokens, 1, 32, seed=46)
+    q, p = randn(tokens, 2, 32, seed=47), torch.arange(tokens, device="cuda").view(1, -1)
+    rq, rk = multi_axis_rotary(q, k, p, (16,))
+    kc, vc = randn(pages, 8, 1, 32, seed=48), randn(pages, 8, 1, 32, seed=49)
+    want = kc.clone(), vc.clone()
+    paged_cache_write(rk, v, *want, slots.cuda())
+    with pytest.raises(RuntimeError, match="outside its tensor"):
+        check_cache_indices()
+    got = rotary_cache_write(q, k, v, kc, vc, slots.cuda().to(torch.int32), p, (16,))
+    with pytest.raises(RuntimeError, match="outside its tensor"):
+        check_cache_indices()
+    assert_bitwise(got, rq)
+    assert_bitwise(kc, want[0])
+    assert_bitwise(vc, want[1])
 
 
 def test_slots_past_the_cache_are_left_out_and_reported():

@@ -132,6 +132,51 @@ def test_prompts_then_tokens(dtype):
         tokens = new
 
 
+@pytest.fixture
+def in_python(monkeypatch):
+    """Without the tensor module: the Python functions do all."""
+    from batch_invariant_ops import decoder
+
+    monkeypatch.setattr(decoder, "_tensor_module", False)
+    monkeypatch.setattr(decoder, "_direct", lambda: False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_both_host_paths(dtype, request):
+    """The same answer and the same bits in the cache; rows in a cache of the model's type too."""
+    def plain():
+        g = torch.Generator().manual_seed(7)
+        q, k, v = (torch.randn(1500, n, 64, generator=g).to(dtype).cuda() for n in (4, 2, 2))
+        kc, vc = (torch.zeros(100, 16, 2, 64, dtype=dtype, device="cuda") for _ in range(2))
+        slots = torch.randint(-3, 1600, (1500,), generator=g).cuda()
+        return rotary_cache_write(q, k, v, kc, vc, slots, torch.arange(1500, device="cuda").view(1, -1), (32,)), kc, vc
+
+    m = Model(dtype)
+    tokens, rows = m.run(), plain()
+    request.getfixturevalue("in_python")
+    again = Model(dtype)
+    assert torch.equal(again.run(), tokens)
+    for a, b in zip(again.caches, m.caches):
+        assert torch.equal(a, b)
+    for a, b in zip(plain(), rows):
+        assert_bitwise(a, b)
+    logits = torch.randn(3, 9000, generator=torch.Generator().manual_seed(8)).cuda()
+    each = dict(temperature=torch.full((3,), 0.7).cuda(), top_k=torch.tensor([5, 0, 900]).cuda(), top_p=torch.tensor([1.0, 0.9, 0.5]).cuda(),
+                min_p=torch.tensor([0.0, 0.1, 0.0]).cuda())
+    got = sample_tokens_batch_invariant(logits, torch.tensor([0.1, 0.5, 0.9]).cuda(), **each)
+    want = [int(sample_tokens_batch_invariant(logits[i:i + 1], torch.tensor([u]).cuda(), temperature=float(each["temperature"][i]),
+                                              top_k=[5, None, 900][i], top_p=float(each["top_p"][i]), min_p=float(each["min_p"][i])))
+            for i, u in enumerate((0.1, 0.5, 0.9))]
+    assert got.tolist() == want
+
+
+def test_a_query_is_needed():
+    with pytest.raises(AttributeError):
+        rotary_cache_write(None, *(torch.zeros(3, 2, 64, device="cuda") for _ in range(2)),
+                           *(torch.zeros(4, 16, 2, 64, device="cuda") for _ in range(2)), torch.arange(3, device="cuda"),
+                           torch.zeros(1, 3, dtype=torch.int64, device="cuda"), (32,))
+
+
 def test_a_sequence_alone_gives_the_same_tokens():
     whole = Model().run()
     for b, n in enumerate(Model().lengths):
