@@ -159,19 +159,27 @@ __device__ __forceinline__ void put_value(T* p, float v) {
   else Num<T>::store(p, v);
 }
 
-// 16 bytes of a row from byte k on; zeros from byte K on.
+// 16 bytes of a row from byte k on; zeros from byte K on.  (The last ones come as the row's last 16, shifted: byte for byte they
+// took a fifth of the time of 3000 x 4001 x 1032.)
 __device__ __forceinline__ u32x4_t row_bytes(const int8_t* row, int64_t k, int64_t K) {
   if (k + 16 <= K) return *reinterpret_cast<const u32x4_byte_t*>(row + k);
   u32x4_t v = {0u, 0u, 0u, 0u};
+  if (k >= K) return v;
+  if (K < 16) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (k + j < K) v[j >> 2] |= (uint32_t)(uint8_t)row[k + j] << (8 * (j & 3));
-  return v;
+    for (int j = 0; j < 16; ++j)
+      if (k + j < K) v[j >> 2] |= (uint32_t)(uint8_t)row[k + j] << (8 * (j & 3));
+    return v;
+  }
+  v = *reinterpret_cast<const u32x4_byte_t*>(row + K - 16);
+  const int by = 8 * (int)(16 - (K - k));  // 8 .. 120
+  const uint64_t low = (uint64_t)v[1] << 32 | v[0], high = (uint64_t)v[3] << 32 | v[2];
+  const uint64_t first = by < 64 ? low >> by | high << (64 - by) : high >> (by - 64), second = by < 64 ? high >> by : 0u;
+  return u32x4_t{(uint32_t)first, (uint32_t)(first >> 32), (uint32_t)second, (uint32_t)(second >> 32)};
 }
 
 // MB blocks of 16 rows; WAVES wavefronts share K.
-// WHOLE: K is a whole number of steps.
-template <typename T, int MB, int WAVES, bool WHOLE>
+template <typename T, int MB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(Int8Args a) {
   __shared__ __attribute__((aligned(16))) i32x4_t part[WAVES][MB][64];
   constexpr int AHEAD = 8 / MB < 2 ? 2 : 8 / MB;  // K steps of 64 bytes whose loads go out together
@@ -188,32 +196,35 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(Int8Args a) {
   i32x4_t acc[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
-  const int64_t steps = (a.K + 63) / 64, per = (steps + WAVES - 1) / WAVES;
+  const int64_t steps = a.K / 64, per = (steps + WAVES - 1) / WAVES;  // whole steps, of 64 bytes
   const int64_t s1 = (w + 1) * per < steps ? (w + 1) * per : steps;
+  auto product = [&](const u32x4_t& b, const u32x4_t (&x)[MB]) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+      acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, x[i]), __builtin_bit_cast(i32x4_t, b), acc[i], 0, 0, 0);
+  };
   for (int64_t s = w * per; s < s1; s += AHEAD) {
     u32x4_t b[AHEAD], x[AHEAD][MB];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      if constexpr (WHOLE) {
-        if (s + j >= s1) break;
-        const int64_t k = 64 * (s + j) + 16 * q4;
-        b[j] = *reinterpret_cast<const u32x4_byte_t*>(wr + k);
+      if (s + j >= s1) break;
+      const int64_t k = 64 * (s + j) + 16 * q4;
+      b[j] = *reinterpret_cast<const u32x4_byte_t*>(wr + k);
 #pragma unroll
-        for (int i = 0; i < MB; ++i) x[j][i] = *reinterpret_cast<const u32x4_byte_t*>(xr[i] + k);
-      } else {
-        const int64_t k = s + j < s1 ? 64 * (s + j) + 16 * q4 : a.K;  // (behind the part: zeros)
-        b[j] = row_bytes(wr, k, a.K);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) x[j][i] = row_bytes(xr[i], k, a.K);
-      }
+      for (int i = 0; i < MB; ++i) x[j][i] = *reinterpret_cast<const u32x4_byte_t*>(xr[i] + k);
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      if (WHOLE && s + j >= s1) break;
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, x[j][i]), __builtin_bit_cast(i32x4_t, b[j]), acc[i], 0, 0, 0);
+      if (s + j >= s1) break;
+      product(b[j], x[j]);
     }
+  }
+  if (w == WAVES - 1 && a.K % 64 != 0) {
+    const int64_t k = 64 * steps + 16 * q4;
+    u32x4_t x[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) x[i] = row_bytes(xr[i], k, a.K);
+    product(row_bytes(wr, k, a.K), x);
   }
 #pragma unroll
   for (int i = 0; i < MB; ++i) part[w][i][lane] = acc[i];
@@ -289,10 +300,14 @@ void int8_big_kernel(Int8Args a) {
 template <typename T>
 __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
   __shared__ __attribute__((aligned(16))) char smem[2][2][64 * 128];
+  __shared__ float steps[64];
   int64_t m0, n0;
   if (!int8_origin(a, 64, 64, m0, n0)) return;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int wm = 32 * (w >> 1), wn = 32 * (w & 1), lr = lane & 31, half = lane >> 5;
+  const int64_t col = n0 + wn + lr < a.N ? n0 + wn + lr : a.N - 1;
+  const float ws = a.ws[col * a.ws_s], bias = a.bias ? Num<T>::load(static_cast<const T*>(a.bias) + col) : 0.f;
+  if (tid < 64) steps[tid] = a.xs[(m0 + tid < a.M ? m0 + tid : a.M - 1) * a.xs_s];
   // chunk tid % 8 of rows tid / 8 and 32 further, of both operands
   const int row = tid >> 3, chunk = tid & 7;
   const int8_t *xr[2], *wr[2];
@@ -302,59 +317,85 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
     xr[i] = a.x + m * a.ldx;
     wr[i] = a.w + n * a.ldw;
   }
-  constexpr int AHEAD = 4;  // steps whose loads are on their way
+  // Whole steps: AHEAD of them are on their way.  (Loads past the last one fetch it again: issued without a condition they
+  // leave the compiler a count to wait for, not all of them; 16.7 -> 14.7 us for 100 x 8000 x 2050.)
+  constexpr int AHEAD = 4;
   u32x4_t x[AHEAD][2], v[AHEAD][2];
-  auto fetch = [&](int s, int64_t k) {
+  const int64_t whole = a.K / 128;
+  auto fetch = [&](int s, int64_t h) {
+    const int64_t k = 128 * (h < whole ? h : whole - 1) + 16 * chunk;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x[s][i] = row_bytes(xr[i], k + 16 * chunk, a.K);
-      v[s][i] = row_bytes(wr[i], k + 16 * chunk, a.K);
+      x[s][i] = *reinterpret_cast<const u32x4_byte_t*>(xr[i] + k);
+      v[s][i] = *reinterpret_cast<const u32x4_byte_t*>(wr[i] + k);
     }
   };
   i32x16_t acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0;
+  auto step = [&](int s, int buffer) {
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s)
-    if (128 * s < a.K) fetch(s, 128 * s);
-  for (int64_t k0 = 0; k0 < a.K; k0 += 128 * AHEAD)
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) {
-      const int64_t k = k0 + 128 * s;
-      if (k >= a.K) break;
-      const int cur = s & 1;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        *reinterpret_cast<u32x4_t*>(smem[cur][0] + lds_off(row + 32 * i, chunk)) = x[s][i];
-        *reinterpret_cast<u32x4_t*>(smem[cur][1] + lds_off(row + 32 * i, chunk)) = v[s][i];
-      }
-      __syncthreads();  // (two buffers: what is written next was read before this barrier)
-      if (k + 128 * AHEAD < a.K) fetch(s, k + 128 * AHEAD);
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-        Mfma<i8_t>::step(acc, *reinterpret_cast<const u32x4_t*>(smem[cur][0] + lds_off(wm + lr, 2 * p + half)),
-                         *reinterpret_cast<const u32x4_t*>(smem[cur][1] + lds_off(wn + lr, 2 * p + half)));
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<u32x4_t*>(smem[buffer][0] + lds_off(row + 32 * i, chunk)) = x[s][i];
+      *reinterpret_cast<u32x4_t*>(smem[buffer][1] + lds_off(row + 32 * i, chunk)) = v[s][i];
     }
-  const int64_t col = n0 + wn + lr;
-  if (col >= a.N) return;
-  const float ws = a.ws[col * a.ws_s], bias = a.bias ? Num<T>::load(static_cast<const T*>(a.bias) + col) : 0.f;
+    __syncthreads();  // (two buffers: what is written next was read before this barrier)
+  };
+  auto product = [&](int buffer) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      Mfma<i8_t>::step(acc, *reinterpret_cast<const u32x4_t*>(smem[buffer][0] + lds_off(wm + lr, 2 * p + half)),
+                       *reinterpret_cast<const u32x4_t*>(smem[buffer][1] + lds_off(wn + lr, 2 * p + half)));
+  };
+  if (whole > 0) {
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) fetch(s, s);
+    for (int64_t h0 = 0; h0 < whole; h0 += AHEAD)
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) {
+        if (h0 + s >= whole) break;
+        step(s, s & 1);
+        fetch(s, h0 + s + AHEAD);
+        product(s & 1);
+      }
+  }
+  if (a.K % 128 != 0) {
+    const int64_t k = 128 * whole + 16 * chunk;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[0][i] = row_bytes(xr[i], k, a.K);
+      v[0][i] = row_bytes(wr[i], k, a.K);
+    }
+    step(0, (int)(whole & 1));
+    product((int)(whole & 1));
+  }
+  // The output goes through LDS for 16-byte stores: straight from the accumulators 3000 x 4001 x 136 took
+  // 38.5 us, and 30.5 so.
+  __syncthreads();
+  T* const tile = reinterpret_cast<T*>(smem);  // [64][64]
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int64_t m = m0 + wm + 8 * (r >> 2) + 4 * half + (r & 3);
-    if (m < a.M) Num<T>::store(static_cast<T*>(a.y) + m * a.N + col, finished<T>(acc[r], a.xs[m * a.xs_s], ws, bias));
+    const int m = wm + 8 * (r >> 2) + 4 * half + (r & 3);
+    Num<T>::store(tile + 64 * m + wn + lr, finished<T>(acc[r], steps[m], ws, bias));
+  }
+  __syncthreads();
+  constexpr int VEC = 16 / (int)sizeof(T), CHUNKS = 64 / VEC;
+#pragma unroll
+  for (int i = 0; i < 64 * CHUNKS / 256; ++i) {
+    const int u = tid + 256 * i, m = u / CHUNKS, c = VEC * (u % CHUNKS);
+    if (m0 + m >= a.M) continue;
+    T* const to = static_cast<T*>(a.y) + (m0 + m) * a.N + n0 + c;
+    if (n0 + c + VEC <= a.N) *reinterpret_cast<u32x4_any_t*>(to) = *reinterpret_cast<const u32x4_t*>(tile + 64 * m + c);
+    else
+      for (int e = 0; n0 + c + e < a.N; ++e) to[e] = tile[64 * m + c + e];
   }
 }
 
-template <typename T, int MB, int WAVES>
-static void int8_few_waves(const Int8Args& a, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv(a.N, 16)), threads(64 * WAVES);
-  if (a.K % 64 == 0) hipLaunchKernelGGL((int8_few_kernel<T, MB, WAVES, true>), grid, threads, 0, s, a);
-  else hipLaunchKernelGGL((int8_few_kernel<T, MB, WAVES, false>), grid, threads, 0, s, a);
-}
 template <typename T, int MB>
 static int int8_few(const Int8Args& a, hipStream_t s) {
-  if (a.K > 4096 && a.N <= 4096) int8_few_waves<T, MB, 16>(a, s);
-  else int8_few_waves<T, MB, 4>(a, s);
+  const dim3 grid((unsigned)cdiv(a.N, 16));
+  if (a.K > 4096 && a.N <= 4096) hipLaunchKernelGGL((int8_few_kernel<T, MB, 16>), grid, dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((int8_few_kernel<T, MB, 4>), grid, dim3(256), 0, s, a);
   return check_launch("int8_few_kernel");
 }
 static void int8_tiles(Int8Args& a, int BM, int BN) {
@@ -370,13 +411,13 @@ static int int8_big(Int8Args a, hipStream_t s) {
 }
 template <typename T>
 static int int8_launch(Int8Args a, hipStream_t s) {
-  if (a.M <= 64) {
-    if (a.M <= 16) return int8_few<T, 1>(a, s);
-    if (a.M <= 32) return int8_few<T, 2>(a, s);
-    return int8_few<T, 4>(a, s);
-  }
-  const bool whole = a.K % 128 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+  const bool aligned = a.ldx % 16 == 0 && a.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+  const bool whole = aligned && a.K % 128 == 0;
+  // Every workgroup of the kernel for few rows reads all of them, 64 bytes of a row at a time, which is slow off 16 bytes.  us (few /
+  // blocks), K -> N: 2048 -> 8192 at 32 rows 9.1 / 9.5, at 64 13.2 / 8.0; 8192 -> 2048 at 32 14.2 / 19.5, at 64 21.7 / 19.3; 1024 ->
+  // 1024 at 32 4.7 / 7.2; off 16 bytes 2050 -> 8000 at 16 15.9 / 11.4, 8190 -> 2040 at 16 27.9 / 28.3, at 32 40 / 28.
+  if (a.M <= 16 && (aligned || a.N <= 2048)) return int8_few<T, 1>(a, s);
+  if (a.M <= 32 && aligned) return int8_few<T, 2>(a, s);
   if (whole) {
     // the blocks with the least rounds x time of a block (relative: a round of 256 x 256 is 1)
     static const struct { int bm, bn; double cost; } blocks[] = {{256, 256, 1.0}, {256, 128, 0.55}, {128, 128, 0.31}, {64, 128, 0.19}, {64, 64, 0.13}};
