@@ -650,9 +650,8 @@ __device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* 
           atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sub[(kNoIndex - (uint32_t)sh.item[at]) / kSampleSub]), (unsigned long long)units[i]);
       }
     } else {
-      // f(rank, y, bin) of the border's tokens, summed
-      auto sum_of = [&](auto f) {
-        uint64_t s = 0;
+      // f(rank, y, bin) of this thread's share of the border's tokens, and its sum over all of them
+      auto each = [&](auto f) {
         for (int i = 8 * tid; i < a.vocab; i += 8 * kSampleThreads) {
           float x[8];
           eight_logits<T>(row, i, a.vocab, x);
@@ -660,14 +659,34 @@ __device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* 
           for (int j = 0; j < 8; ++j) {
             const uint64_t y = of.octaves(x[j]);
             const int bin = of.bin(y);
-            if (at_border(border, bin) && of.units(y) != 0) s += f(rank_of(x[j], i + j), y, bin);
+            if (at_border(border, bin) && of.units(y) != 0) f(rank_of(x[j], i + j), y, bin);
           }
         }
+      };
+      auto sum_of = [&](auto f) {
+        uint64_t s = 0;
+        each([&](uint64_t rank, uint64_t y, int bin) { s += f(rank, y, bin); });
         return block_sum64(s, waves);
       };
-      // the largest rank x with f(x), which holds at 0 and, where it holds, for everything smaller
+      unsigned long long* const ends = reinterpret_cast<unsigned long long*>(sh.item);  // the smallest and the largest rank
+      if (tid == 0) {
+        ends[0] = ~0ull;
+        ends[1] = 0;
+      }
+      __syncthreads();
+      uint64_t smallest = ~0ull, most = 0;
+      each([&](uint64_t rank, uint64_t, int) {
+        smallest = rank < smallest ? rank : smallest;
+        most = rank > most ? rank : most;
+      });
+      if (most > 0) {
+        atomicMin(&ends[0], (unsigned long long)smallest);
+        atomicMax(&ends[1], (unsigned long long)most);
+      }
+      __syncthreads();
+      // the largest rank x with f(x), which holds at the smallest and, where it holds, for everything smaller
       auto largest = [&](auto f) {
-        uint64_t lo = 0, hi = ~0ull;
+        uint64_t lo = ends[0], hi = ends[1];
         while (lo < hi) {
           const uint64_t mid = lo + (hi - lo) / 2 + 1;
           if (f(mid)) lo = mid;
