@@ -12,8 +12,7 @@ A cache in 4 bits is four ``uint8`` tensors: keys ``[pages, page_size, kv_heads,
 / 32]``, values and theirs.  A row is cut into blocks of 32 elements.  A block's scale byte ``x`` stands for the power of two
 ``2 ** (x - 127)``; an element is a sign, two exponent bits and a mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6) times that power,
 two to a byte, the first in the low half.  (The OCP microscaling format MXFP4.)  The power is the smallest of which no
-element of the block is more than 7, so an element is off by at most that power and an eighth of the block's largest
-magnitude by more than a quarter of it.  Powers lie in [2 ** -125, 2 ** 125] for bfloat16 rows and [2 ** -23, 2 ** 13] for
+element of the block is more than 7, so no element is off by more than that power.  Powers lie in [2 ** -125, 2 ** 125] for bfloat16 rows and [2 ** -23, 2 ** 13] for
 float16 ones, where every value is a number of the rows' type; larger elements become the largest value.  A block with an
 infinity or NaN has the scale byte 255 and stands for NaN as a whole.
 """
@@ -240,8 +239,8 @@ def paged_cache_write_fp4(
     head_dim]`` and values ``[..., kv_heads, value_dim]``, each block to its power of two and its elements to the nearest level
     (ties to the even code), in place.  Slots are as there; the rows must not lie in the memory of the caches."""
     module, watch = _direct_watch()
-    if module and key_scales is not None and module.rotary_write(None, key, value, key_cache, value_cache, slots, None, key_scales, value_scales, 0, 0, 0, 0, 0,
-                                      watch.flag_at):
+    if module and key_scales is not None and module.rotary_write(
+            None, key, value, key_cache, value_cache, slots, None, key_scales, value_scales, 0, 0, 0, 0, 0, watch.flag_at):
         watch.after_call()
         return
     _refuse_transforms("paged_cache_write_fp4", key, value, key_cache, key_scales, value_cache, value_scales)
@@ -370,7 +369,7 @@ def paged_attention_fp4_batch_invariant(
 
 
 # -------------------------------------------------------------------------------- sampling ----
-_MOST_TOKENS, _MOST_ROWS = 1 << 20, 65536
+_MOST_TOKENS, _MOST_ROWS, _MOST_LOGITS = 1 << 20, 65536, 1 << 35
 
 
 def _setting(name, value, lead, dtypes, default, check):
@@ -410,7 +409,7 @@ def sample_tokens_batch_invariant(
 
     Logits of NaN count as -inf, which are never chosen; a row without any other gives -1.  Where logits are +inf only those
     can be chosen.  Weights are multiples of 2**-43 (what is less than half of that is never chosen, and not counted) and their
-    sums are exact, so a token does not depend on the batch.  Up to 2**20 tokens and 65536 rows.
+    sums are exact, so a token does not depend on the batch.  Up to 2**20 tokens, 65536 rows and 2**35 logits in all.
     """
     module = decoder._tensor_module or _direct()
     if module:
@@ -418,7 +417,7 @@ def sample_tokens_batch_invariant(
         if out is not None:
             return out
     settings = [x for x in (temperature, top_k, top_p, min_p) if isinstance(x, torch.Tensor)]
-    _refuse_transforms("sample_tokens_batch_invariant", logits, uniforms)
+    _refuse_transforms("sample_tokens_batch_invariant", logits, uniforms, *settings)
     if logits.dim() < 1 or logits.dtype not in nat.DIRECT_DTYPES:
         raise ValueError(f"logits must be float32, float16 or bfloat16 of shape [..., vocab], got {logits.dtype} {tuple(logits.shape)}")
     lead, vocab = logits.shape[:-1], logits.shape[-1]
@@ -426,6 +425,8 @@ def sample_tokens_batch_invariant(
         raise ValueError(f"rows must have 1 to {_MOST_TOKENS} logits, got {vocab}")
     if lead.numel() > _MOST_ROWS:
         raise ValueError(f"at most {_MOST_ROWS} rows, got {lead.numel()}")
+    if lead.numel() * vocab > _MOST_LOGITS:
+        raise ValueError(f"at most 2**35 logits, got {lead.numel()} rows of {vocab}")
     if uniforms.dtype != torch.float32 or uniforms.shape != lead:
         raise ValueError(f"uniforms must be float32 of shape {tuple(lead)}")
     floats = (torch.float32,)

@@ -11,13 +11,18 @@
 // A row's tokens are shared among `segs` workgroups, in five launches (one where a workgroup has a whole row):
 //   top     a segment's largest and smallest logit;
 //   bins    tokens by log2 of their weight in 2048 bins, each with its count and the sum of the places inside of it, which
-//           bound its weight to 2^-11 (one 32-bit sum a token: 64-bit ones for the weights took three times as long);
+//           bound its weight to 2^-11 (one 32-bit sum a token);
 //   join    the bins over all segments, and those that a border can lie in;
 //   sums    the weights in front of those bins, for every 512 tokens, and a list of the tokens inside of them;
 //   finish  the list sorted, the borders in its running sums, the sums of 512 tokens completed, and the token.
-// (Joins by the last workgroup of a launch took longer than launches of their own: what makes one XCD's writes visible to
-// another inside of a kernel cost 70 us a launch with 512 workgroups.)  Calls without top-k and top-p go without bins and join.
-// Where the list is too long (thousands of tokens in a bin: equal logits, mostly) finish finds the borders by bisection over the row.
+// Calls without top-k and top-p go without bins and join.  Where the list is too long (thousands of tokens in a bin: equal
+// logits, mostly) finish finds the borders by bisection over the row.
+//
+// 64 rows of 131072 in float32, 33.6 MB that are read three times (the second and third time mostly from the caches): 8, 15, 9, 23 and
+// 22 us, bound by the arithmetic of 64-bit weights, in finish by the sort's steps that wait for one another.  (With 64-bit
+// sums a bin, joined with the borders' list by the last workgroup of a launch, bins took 78 us and sums 73: fences make
+// each of an XCD's writes visible to the others.)  One row of 32000: 3, 5, 7, 6 and 9 us, each bound by a launch and a few
+// reads that wait for one another.  64 rows of 131072 equal logits, by bisection, 1.1 ms.
 #include "biops_common.h"
 
 namespace biops {
@@ -25,6 +30,7 @@ namespace biops {
 constexpr int kSampleThreads = 512, kSampleWaves = kSampleThreads / 64;
 constexpr int kSampleBins = 2048, kSampleInside = 32, kSampleList = 2048, kSampleSub = 512;
 constexpr int kSampleMost = 1 << 20;           // tokens of a row: sums of that many weights fit 64 bits
+constexpr int64_t kSampleAll = INT64_C(1) << 35;  // tokens of a call: a launch has less than 2^32 threads
 constexpr int kSampleSubs = kSampleMost / kSampleSub;
 constexpr int kSampleTable = 1024;
 constexpr int kSampleSeg = 8192;               // most tokens of a segment: 14 bits of a bin's word count, 18 add up places
@@ -869,7 +875,7 @@ static int sample_launch(const SampleArgs& a, hipStream_t s) {
 using namespace biops;
 
 extern "C" int64_t biops_sample_workspace_size(int64_t rows, int64_t vocab) {
-  if (rows < 0 || vocab < 1 || vocab > kSampleMost || rows > 65536) return -1;
+  if (rows < 0 || vocab < 1 || vocab > kSampleMost || rows > 65536 || rows * vocab > kSampleAll) return -1;
   return rows == 0 ? 0 : sample_space(rows, vocab).bytes;
 }
 
@@ -878,8 +884,8 @@ extern "C" int biops_sample(int dtype, int64_t rows, int64_t vocab, const void* 
                             const float* top_p, int64_t p_s, double p0, const float* min_p, int64_t m_s, double m0, int64_t* out,
                             void* workspace, int64_t workspace_bytes, void* stream) {
   if (!is_float_dtype(dtype)) return fail(BIOPS_ERR_DTYPE, "biops_sample: unsupported dtype %d", dtype);
-  if (rows < 0 || rows > 65536 || vocab < 1 || vocab > kSampleMost)
-    return fail(BIOPS_ERR_ARG, "biops_sample: rows of 1 to %d tokens, at most 65536 rows", kSampleMost);
+  if (rows < 0 || rows > 65536 || vocab < 1 || vocab > kSampleMost || rows * vocab > kSampleAll)
+    return fail(BIOPS_ERR_ARG, "biops_sample: rows of 1 to %d tokens, at most 65536 rows and 2^35 tokens in all", kSampleMost);
   if (rows == 0) return BIOPS_OK;
   if (!logits || !u || !out) return fail(BIOPS_ERR_ARG, "biops_sample: null pointer");
   const SampleSpace x = sample_space(rows, vocab);

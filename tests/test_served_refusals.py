@@ -144,6 +144,7 @@ def sample(logits=None, u=None, **kw):
     (lambda: sample(logits=zeros(2, 0)), "1 to 1048576"),
     (lambda: sample(logits=torch.zeros(1).expand(2, (1 << 20) + 1)), "1 to 1048576"),
     (lambda: sample(logits=torch.zeros(1).expand(65537, 2)), "65536 rows"),
+    (lambda: sample(logits=torch.zeros(1).expand(32769, 1 << 20)), "2\\*\\*35 logits"),
     (lambda: sample(u=zeros(2)), "uniforms"),
     (lambda: sample(u=zeros(3, dtype=F32)), "uniforms"),
     (lambda: sample(temperature=-0.5), "temperature"),
@@ -273,6 +274,8 @@ def test_sampling_entry():
     refused(call(dtype=3), 3, "dtype")
     refused(call(rows=-1), 1, "rows")
     refused(call(vocab=0), 1, "rows")
+    refused(call(rows=32769, vocab=1 << 20), 1, "2^35 tokens in all")
+    assert size(32768, 1 << 20) > 0 and size(32769, 1 << 20) == -1
     refused(call(logits=None), 1, "null")
     refused(call(bytes_=8), 5, "workspace")
     refused(call(ws=None), 5, "workspace")
