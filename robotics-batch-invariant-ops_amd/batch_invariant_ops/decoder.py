@@ -68,9 +68,9 @@ class _CacheWatch(_IndexWatch):
 
 
 def check_cache_indices(device: torch.device | str | int | None = None) -> None:
-    """Raise ``RuntimeError`` if a call of this module on ``device`` (default: the current device) met an
-    index outside its tensor since the last report.  Waits for the work queued on that device's current
-    stream."""
+    """Raise ``RuntimeError`` if a call of this module, or of a served decoder's cache operators, on
+    ``device`` (default: the current device) met an index outside its tensor since the last report.  Waits for
+    the work queued on that device's current stream."""
     device = _CacheWatch.device(device)
     with torch.cuda.device(device):
         _CacheWatch.of(device).check()
