@@ -18,10 +18,10 @@
 // Calls without top-k and top-p go without bins and join.  Where the list is too long (thousands of tokens in a bin: equal
 // logits, mostly) finish finds the borders by bisection over the row.
 //
-// 64 rows of 131072 in float32, 33.6 MB that are read three times (the second and third time mostly from the caches): 8, 15, 9, 23 and
-// 22 us, bound by the arithmetic of 64-bit weights, in finish by the sort's steps that wait for one another.  (With 64-bit
+// 64 rows of 131072 in float32, 33.6 MB that are read three times (the second and third time mostly from the caches): 8, 15, 8, 19.5 and
+// 21 us, bound by the arithmetic of 64-bit weights, in finish by the sort's steps that wait for one another.  (With 64-bit
 // sums a bin, joined with the borders' list by the last workgroup of a launch, bins took 78 us and sums 73: fences make
-// each of an XCD's writes visible to the others.)  One row of 32000: 3, 5, 7, 6 and 9 us, each bound by a launch and a few
+// each of an XCD's writes visible to the others.)  One row of 32000: 3, 5, 6, 5.5 and 7.5 us, each bound by a launch and a few
 // reads that wait for one another.  64 rows of 131072 equal logits, by bisection, 1.1 ms.
 #include "biops_common.h"
 
@@ -155,20 +155,26 @@ __device__ __forceinline__ void fill_table(double* table) {
   reinterpret_cast<u32x4_t*>(table)[threadIdx.x] = reinterpret_cast<const u32x4_t*>(kTable.value)[threadIdx.x];
 }
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, o, 64);
-  return v;
+// v plus what the lanes that CTRL names have (row_shr or row_bcast; 0 where there is none, or the row of 16 is not in ROWS).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t plus_lane(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((uint64_t)hi << 32 | lo);
 }
-// Inclusive sums over the wavefront's lanes.
+// Inclusive sums over the wavefront's lanes (all of them active): in rows of 16, then over the rows.
 __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t x = (uint64_t)__shfl_up((unsigned long long)v, o, 64);
-    if (lane >= o) v += x;
-  }
-  return v;
+  v = plus_lane<0x111, 0xf>(v);  // row_shr:1
+  v = plus_lane<0x112, 0xf>(v);
+  v = plus_lane<0x114, 0xf>(v);
+  v = plus_lane<0x118, 0xf>(v);
+  v = plus_lane<0x142, 0xa>(v);  // row_bcast:15
+  return plus_lane<0x143, 0xc>(v);  // row_bcast:31
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+  v = wave_scan64(v);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
 }
 // The sum in front of this thread and the sum of all, over the workgroup.
 __device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t* waves, uint64_t& all) {
@@ -477,56 +483,62 @@ __device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* 
 }
 
 // ---------------------------------------------------------------------------- the border and the token ----
+// A row that all lanes have, in scalar registers.
+__device__ __forceinline__ SampleRow alike(const SampleRow& row) {
+  constexpr int kWords = sizeof(SampleRow) / 4;
+  struct Words {
+    uint32_t word[kWords];
+  };
+  Words words = __builtin_bit_cast(Words, row);
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) words.word[i] = __builtin_amdgcn_readfirstlane(words.word[i]);
+  return __builtin_bit_cast(SampleRow, words);
+}
 __device__ __forceinline__ bool at_border(const SampleRow& row, int bin) { return (bin >= row.plo && bin <= row.phi) || bin == row.bk; }
 __device__ __forceinline__ SampleWeight weights_of(const SampleRow& row, const double* table) {
   return SampleWeight{row.top, row.c, row.top == INFINITY, row.scale, table};
 }
 
-template <typename T>
+// FILTERS: there is a top-k or a top-p.
+template <typename T, bool FILTERS>
 __device__ __forceinline__ void sums_step(const SampleArgs& a, int seg, int r, double* table, uint64_t* waves, SampleSums& sh) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
   const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
-  float next[8];  // (on their way while the row's settings are)
-  eight_logits<T>(row, seg * a.seg + kSampleSub * w + 8 * lane, a.vocab, next);
+  float x[8];  // (on their way while the row's settings are)
+  eight_logits<T>(row, seg * a.seg + kSampleSub * w + 8 * lane, a.vocab, x);
   fill_table(table);
   if (tid == 0) sh.met = 0u;
-  const SampleRow border = a.filters ? a.row[r] : plain_row(a, r, over_segments<false, false>(a, r));
+  const SampleRow border = alike(FILTERS ? a.row[r] : plain_row(a, r, over_segments<false, false>(a, r)));
   if (border.token != -2) return;
   const SampleWeight of = weights_of(border, table);
   __syncthreads();
   uint64_t before = 0, weight = 0;
   for (int s0 = seg * a.seg + kSampleSub * w; s0 < end; s0 += kSampleWaves * kSampleSub) {
-    float x[8];
     const int i = s0 + 8 * lane;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = next[j];
-    if (s0 + kSampleWaves * kSampleSub < end) eight_logits<T>(row, i + kSampleWaves * kSampleSub, a.vocab, next);
     uint64_t sum = 0;
-    uint32_t near = 0u;  // of the eight, those at the border
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint64_t y = of.octaves(x[j]), units = of.units(y);
+      if (!FILTERS) {
+        sum += y <= border.lightest ? units : 0u;
+        continue;
+      }
       const int bin = of.bin(y);
       const uint64_t mine = bin < border.plo ? units : 0u;
       before += mine;
       sum += y <= border.lightest ? mine : 0u;
       if (border.bk >= 0) weight += bin < border.bk ? units : 0u;
-      near |= (uint32_t)(at_border(border, bin) && units != 0) << j;
-    }
-    if (near != 0u) {
-      uint32_t at = atomicAdd(&sh.met, (uint32_t)__builtin_popcount(near));
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (near >> j & 1u) {
-          if (at < kSampleList) sh.item[at] = rank_of(x[j], i + j);
-          ++at;
-        }
+      if (at_border(border, bin) && units != 0) {
+        const uint32_t at = atomicAdd(&sh.met, 1u);
+        if (at < kSampleList) sh.item[at] = rank_of(x[j], i + j);
+      }
     }
     sum = wave_sum64(sum);
     if (lane == 0) a.sub[(int64_t)r * a.subs + s0 / kSampleSub] = sum;
+    if (s0 + kSampleWaves * kSampleSub < end) eight_logits<T>(row, i + kSampleWaves * kSampleSub, a.vocab, x);
   }
-  if (!a.filters) return;
+  if (!FILTERS) return;
   __syncthreads();
   uint32_t ready = 0u;  // (the sums go on while it comes)
   if (tid == 0 && sh.met > 0) ready = __hip_atomic_fetch_add(&a.listed[r], sh.met, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -789,12 +801,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_join(SampleArgs a) {
   __shared__ SampleJoin sh;
   join_step(a, blockIdx.x, waves, sh);
 }
-template <typename T>
-__global__ __launch_bounds__(kSampleThreads) void sample_sums(SampleArgs a) {
+// (registers for four workgroups a compute unit: with the next tokens' loads ahead of time they allow two, 64 x 131072 in 23.4 us
+// instead of 19.5)
+template <typename T, bool FILTERS>
+__global__ __launch_bounds__(kSampleThreads, 8) void sample_sums(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) double table[kSampleTable];
   __shared__ uint64_t waves[kSampleWaves];
   __shared__ SampleSums sh;
-  sums_step<T>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
+  sums_step<T, FILTERS>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void sample_finish(SampleArgs a) {
@@ -816,7 +830,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_whole(SampleArgs a) {
     join_step(a, r, sh.waves, sh.join);
     __syncthreads();
   }
-  sums_step<T>(a, 0, r, sh.table, sh.waves, sh.sums);
+  if (a.filters) sums_step<T, true>(a, 0, r, sh.table, sh.waves, sh.sums);
+  else sums_step<T, false>(a, 0, r, sh.table, sh.waves, sh.sums);
   __syncthreads();
   finish_step<T>(a, r, sh.table, sh.waves, sh.finish);
 }
@@ -864,7 +879,8 @@ static int sample_launch(const SampleArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(sample_join, rows, threads, 0, s, a);
     if (const int rc = check_launch("sample_join")) return rc;
   }
-  hipLaunchKernelGGL((sample_sums<T>), all, threads, 0, s, a);
+  if (a.filters) hipLaunchKernelGGL((sample_sums<T, true>), all, threads, 0, s, a);
+  else hipLaunchKernelGGL((sample_sums<T, false>), all, threads, 0, s, a);
   if (const int rc = check_launch("sample_sums")) return rc;
   hipLaunchKernelGGL((sample_finish<T>), rows, threads, 0, s, a);
   return check_launch("sample_finish");
