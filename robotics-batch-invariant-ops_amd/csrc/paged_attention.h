@@ -85,11 +85,12 @@ __device__ __forceinline__ bool paged_find(const PagedArgs& a, int it, int lane,
   const int len1 = first + 1 < a.batch ? paged_length(a, first + 1) : 0;
   const int one = paged_span(a, len0).chunks, both = one + paged_span(a, len1).chunks;
   int upto = both;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += x;
-  }
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8: sums in rows of 16 lanes
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xa, 0xf, false);  // row_bcast:15, 31: over the rows
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xc, 0xf, false);
   const uint64_t hit = __ballot(upto > it);
   if (hit == 0) return false;
   const int f = __builtin_ctzll(hit);
