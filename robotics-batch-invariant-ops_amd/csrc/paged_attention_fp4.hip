@@ -11,10 +11,10 @@
 // exchanges them through LDS together with the rows' places.
 //
 // A key's 4.25 bits an element leave less to wait for than to compute: 64 sequences of 250 to 16384 keys (16/4 heads of 128,
-// bf16) take 56 us and 5 for the join, 2.3 TB/s of 137 MB, where the 16-bit pages take 114 us.  Vector instructions issue in
-// about 60 % of the cycles (a value element costs half a conversion, a byte permutation and its share of two MFMAs).
+// bf16) take 53.5 us and 5 for the join, 2.3 TB/s of 137 MB, where the 16-bit pages take 114 us.  Vector instructions issue in
+// about half of the cycles (a value element costs half a conversion, a byte permutation and its share of two MFMAs).
 // Registers for three wavefronts a SIMD are what 128-wide heads fit into; for four, they spill and it is slower.  Values are
-// converted four columns at a time for the same reason.  One sequence of 2047 keys: 6.6 us, and 3.8 for the join, bound by
+// converted four columns at a time for the same reason.  One sequence of 2047 keys: 6.4 us, and 3.8 for the join, bound by
 // three reads that wait for one another (length, pages, rows).
 #include "fp4.h"
 #include "paged_attention.h"

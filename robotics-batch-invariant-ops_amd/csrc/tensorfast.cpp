@@ -1,4 +1,4 @@
-// The decoder operators on torch tensors without Python's per-attribute costs (about 0.1 us each, and
+// The operators of a served decoder on torch tensors without Python's per-attribute costs (about 0.1 us each, and
 // some sixty of them in a call): a call whose tensors are as the kernels take them is checked, given its
 // output and workspace, and launched here.  Every function returns None where it does not take the call
 // as it is -- other layouts, empty tensors, what needs a gradient, and everything that is refused: the
