@@ -3,12 +3,15 @@ definition."""
 
 from __future__ import annotations
 
+import importlib
+
 import pytest
 import torch
 
 from batch_invariant_ops import (
     check_cache_indices,
     multi_axis_rotary,
+    paged_attention_fp4_batch_invariant,
     paged_cache_read_fp4,
     paged_cache_write,
     paged_cache_write_fp4,
@@ -317,3 +320,46 @@ def test_far_offsets():
         same(scales.flatten(0, 1)[slots], want[1])
     rk, rv = paged_cache_read_fp4(kc, ks, vc, vs, slots)
     assert torch.equal(rk.cpu().double(), from_fp4(*to_fp4(k))) and torch.equal(rv.cpu().double(), from_fp4(*to_fp4(v)))
+
+
+def far(t, step):
+    """A copy of t whose first dimension has a stride of `step` elements."""
+    inner = torch.empty(t.shape[1:]).stride()
+    size = (t.shape[0] - 1) * step + t[0].numel()
+    return torch.empty(size, dtype=t.dtype, device="cuda").as_strided(t.shape, (step, *inner)).copy_(t)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("without_module", [False, True])
+def test_far_rows_and_pages(four, without_module, request):
+    """Offsets past 32 bits of new rows and of pages; with and without the host module."""
+    if without_module:
+        served = importlib.import_module("batch_invariant_ops.served")
+        kept = served.decoder._tensor_module
+        request.addfinalizer(lambda: setattr(served.decoder, "_tensor_module", kept))
+        served.decoder._tensor_module = False
+    q, k, v = (randn(3, 2, 64, seed=90 + i) for i in range(3))
+    slots = torch.tensor([8, 1, 5], device="cuda")
+    p = torch.tensor([[4, 0, 9]], device="cuda")
+    if four:
+        near = empty4(3, 3, 2, 64, 64)
+    else:
+        near = [randn(3, 3, 2, 64, seed=95 + i) for i in range(2)]
+    away = [far(c, (5 << 30) // (2 * c.element_size())) for c in near]
+
+    def write(q, k, v, caches):
+        scales = dict(key_scales=caches[1], value_scales=caches[3]) if four else {}
+        kc, vc = (caches[0], caches[2]) if four else caches
+        return rotary_cache_write(q, k, v, kc, vc, slots, p, (32,), **scales)
+
+    want = write(q, k, v, near)
+    got = write(far(q, 5 << 29), far(k, 5 << 29), far(v, 5 << 29), away)
+    assert_bitwise(got, want)
+    for a, b in zip(away, near):
+        assert torch.equal(a, b)
+    if four:
+        for a, b in zip(paged_cache_read_fp4(*away, slots), paged_cache_read_fp4(*near, slots)):
+            assert_bitwise(a, b)
+        table = torch.tensor([[2, 0, 1]], device="cuda")
+        length = torch.tensor([9], device="cuda")
+        assert_bitwise(paged_attention_fp4_batch_invariant(q[:1], *away, table, length), paged_attention_fp4_batch_invariant(q[:1], *near, table, length))

@@ -166,3 +166,28 @@ def test_a_linear_layer(dtype):
     dx, dw = 0.501 * s.cpu().double().view(-1, 1), 0.501 * ws.cpu().double().view(1, -1)
     bound = dx * w.double().abs().sum(1) + dw * x.double().abs().sum(1, keepdim=True) + 512 * dx * dw
     assert bool(((out.cpu().double() - full).abs() <= bound + HALF[dtype] * full.abs() + HALF[dtype] * bound).all())
+
+
+@pytest.mark.parametrize("m, k, step", [(3, 200, 3 << 30), (40, 256, (1 << 27) + 16), (40, 200, (1 << 27) + 1)])
+def test_far_rows(m, k, step):
+    """Offsets past 32 bits, in each kernel."""
+    args = case(m, 48, k, torch.bfloat16)
+    x = torch.empty((m - 1) * step + k, dtype=I8, device="cuda").as_strided((m, k), (step, 1))
+    x.copy_(args[0])
+    want = linear_int8_batch_invariant(*args)
+    assert_bitwise(linear_int8_batch_invariant(x, *args[1:]), want)
+    q, steps = quantize_tokens_int8(args[0].to(torch.bfloat16))
+    del x
+    rows = torch.empty((m - 1) * (step // 2) + k, dtype=torch.bfloat16, device="cuda").as_strided((m, k), (step // 2, 1))
+    rows.copy_(args[0])
+    far = quantize_tokens_int8(rows)
+    assert torch.equal(far[0], q) and torch.equal(far[1], steps)
+
+
+@pytest.mark.parametrize("k", [128, 100])
+def test_outputs_past_32_bits(k):
+    m, n = 70000, 32768
+    x, xs, w, ws, b = case(m, n, k, torch.bfloat16)
+    out = linear_int8_batch_invariant(x, xs, w, ws, b)
+    for rows in (slice(0, 3), slice(65530, 65540), slice(m - 2, m)):
+        assert_bitwise(out[rows], linear_int8_batch_invariant(x[rows], xs[rows], w, ws, b))

@@ -218,6 +218,25 @@ def test_the_largest_vocabulary():
     check_row(torch.zeros(1 << 20), 1.0, 999999, least=5e-7)  # (sums of equal weights are exact)
 
 
+@pytest.mark.parametrize("top_p", [None, 0.8])
+@pytest.mark.parametrize("vocab", [1000, 10000])
+def test_far_rows(vocab, top_p):
+    """Offsets past 32 bits."""
+    x = logits_of(vocab, 16, BF16, rows=3).cuda()
+    u = torch.rand(3, generator=torch.Generator().manual_seed(17)).cuda()
+    far = torch.empty(2 * (1 << 31) + vocab, dtype=BF16, device="cuda").as_strided((3, vocab), (1 << 31, 1))
+    far.copy_(x)
+    assert torch.equal(sample_tokens_batch_invariant(far, u, top_p=top_p), sample_tokens_batch_invariant(x, u, top_p=top_p))
+
+
+def test_a_tangent_of_a_setting_is_refused():
+    x, u = torch.zeros(2, 5, device="cuda"), torch.zeros(2, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        t = torch.autograd.forward_ad.make_dual(torch.ones(2, device="cuda"), torch.ones(2, device="cuda"))
+        with pytest.raises(ValueError, match="forward-mode"):
+            sample_tokens_batch_invariant(x, u, temperature=t)
+
+
 def test_needs_no_gradient():
     x = torch.zeros(2, 5, device="cuda", requires_grad=True)
     with pytest.raises(ValueError, match="no gradient"):
