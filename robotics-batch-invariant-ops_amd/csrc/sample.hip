@@ -8,7 +8,8 @@
 // Sums decide between neighbours, so they are exact: a weight is formed in 64 bits and rounded once to a multiple of 2^-43,
 // and sums of those are integers, the same in any order.  A row's token depends on its own row only.
 //
-// A row's tokens are shared among `segs` workgroups, in five launches (one where a workgroup has a whole row):
+// A row's tokens are shared among `segs` workgroups, in five launches (few workgroups four, and one where a workgroup has a
+// whole row):
 //   top     a segment's largest and smallest logit;
 //   bins    tokens by log2 of their weight in 2048 bins, each with its count and the sum of the places inside of it, which
 //           bound its weight to 2^-11 (one 32-bit sum a token);
@@ -21,7 +22,7 @@
 // 64 rows of 131072 in float32, 33.6 MB that are read three times (the second and third time mostly from the caches): 8, 15, 8, 19.5 and
 // 21 us, bound by the arithmetic of 64-bit weights, in finish by the sort's steps that wait for one another.  (With 64-bit
 // sums a bin, joined with the borders' list by the last workgroup of a launch, bins took 78 us and sums 73: fences make
-// each of an XCD's writes visible to the others.)  One row of 32000: 3, 5, 6, 5.5 and 7.5 us, each bound by a launch and a few
+// each of an XCD's writes visible to the others.)  One row of 32000: 3, 5, 10 and 7.5 us, each bound by a launch and a few
 // reads that wait for one another.  64 rows of 131072 equal logits, by bisection, 1.1 ms.
 #include "biops_common.h"
 
@@ -399,7 +400,7 @@ __device__ __forceinline__ void bins_step(const SampleArgs& a, int seg, int r, d
   *reinterpret_cast<u32x4_t*>(a.bins + at * kSampleBins + 4 * tid) = *reinterpret_cast<const u32x4_t*>(sh.bins + 4 * tid);
 }
 
-__device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* waves, SampleJoin& sh) {
+__device__ __forceinline__ SampleRow join_step(const SampleArgs& a, int r, uint64_t* waves, SampleJoin& sh) {
   const int tid = threadIdx.x;
   const uint64_t k = (uint64_t)row_k(a, r);
   const double p = row_p(a, r);
@@ -416,10 +417,7 @@ __device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* 
   }
   const SampleWhole whole = over_segments<true, false>(a, r);
   SampleRow row = plain_row(a, r, whole);
-  if (row.token != -2 || (k == 0 && p == 1.0)) {  // (there are no bins)
-    if (tid == 0) a.row[r] = row;
-    return;
-  }
+  if (row.token != -2 || (k == 0 && p == 1.0)) return row;  // (there are no bins)
   // A token of place i has y in [i w, (i + 1) w + 2^-26), w = 2^6 / scale octaves.  2^-y is convex: the sum over tokens whose
   // places have the mean f is at most the chord's from place 0 to the last, and at least their number times the value at f + 1.
   const double width = 64.0 / (double)row.scale;
@@ -479,7 +477,7 @@ __device__ __forceinline__ void join_step(const SampleArgs& a, int r, uint64_t* 
   row.phi = phi;
   row.bk = bk;
   row.count = by_k ? sh.count : 0u;
-  if (tid == 0) a.row[r] = row;
+  return row;
 }
 
 // ---------------------------------------------------------------------------- the border and the token ----
@@ -499,9 +497,9 @@ __device__ __forceinline__ SampleWeight weights_of(const SampleRow& row, const d
   return SampleWeight{row.top, row.c, row.top == INFINITY, row.scale, table};
 }
 
-// FILTERS: there is a top-k or a top-p.
-template <typename T, bool FILTERS>
-__device__ __forceinline__ void sums_step(const SampleArgs& a, int seg, int r, double* table, uint64_t* waves, SampleSums& sh) {
+// FILTERS: there is a top-k or a top-p.  row_of() gives the row's borders.
+template <typename T, bool FILTERS, typename RowOf>
+__device__ __forceinline__ void sums_step(const SampleArgs& a, int seg, int r, RowOf row_of, double* table, uint64_t* waves, SampleSums& sh) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const T* row = reinterpret_cast<const T*>(a.logits + r * a.ld);
   const int end = (seg + 1) * a.seg < a.vocab ? (seg + 1) * a.seg : a.vocab;
@@ -509,7 +507,7 @@ __device__ __forceinline__ void sums_step(const SampleArgs& a, int seg, int r, d
   eight_logits<T>(row, seg * a.seg + kSampleSub * w + 8 * lane, a.vocab, x);
   fill_table(table);
   if (tid == 0) sh.met = 0u;
-  const SampleRow border = alike(FILTERS ? a.row[r] : plain_row(a, r, over_segments<false, false>(a, r)));
+  const SampleRow border = alike(row_of());
   if (border.token != -2) return;
   const SampleWeight of = weights_of(border, table);
   __syncthreads();
@@ -799,7 +797,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_bins(SampleArgs a) {
 __global__ __launch_bounds__(kSampleThreads) void sample_join(SampleArgs a) {
   __shared__ uint64_t waves[kSampleWaves];
   __shared__ SampleJoin sh;
-  join_step(a, blockIdx.x, waves, sh);
+  const SampleRow row = join_step(a, blockIdx.x, waves, sh);
+  if (threadIdx.x == 0) a.row[blockIdx.x] = row;
 }
 // (registers for four workgroups a compute unit: with the next tokens' loads ahead of time they allow two, 64 x 131072 in 23.4 us
 // instead of 19.5)
@@ -808,7 +807,24 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sums(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) double table[kSampleTable];
   __shared__ uint64_t waves[kSampleWaves];
   __shared__ SampleSums sh;
-  sums_step<T, FILTERS>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
+  const int r = blockIdx.x / a.segs;
+  auto row_of = [&] { return FILTERS ? a.row[r] : plain_row(a, r, over_segments<false, false>(a, r)); };
+  sums_step<T, FILTERS>(a, blockIdx.x % a.segs, r, row_of, table, waves, sh);
+}
+// join and sums in one launch: every workgroup joins its row's bins.
+template <typename T>
+__global__ __launch_bounds__(kSampleThreads) void sample_join_sums(SampleArgs a) {
+  __shared__ __attribute__((aligned(16))) double table[kSampleTable];
+  __shared__ uint64_t waves[kSampleWaves];
+  __shared__ SampleJoin join;
+  __shared__ SampleSums sh;
+  const int r = blockIdx.x / a.segs, seg = blockIdx.x % a.segs;
+  auto row_of = [&] {
+    const SampleRow row = join_step(a, r, waves, join);
+    if (seg == 0 && threadIdx.x == 0) a.row[r] = row;
+    return row;
+  };
+  sums_step<T, true>(a, seg, r, row_of, table, waves, sh);
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void sample_finish(SampleArgs a) {
@@ -827,11 +843,13 @@ __global__ __launch_bounds__(kSampleThreads) void sample_whole(SampleArgs a) {
   if (a.filters) {
     bins_step<T>(a, 0, r, sh.table, sh.waves, sh.bins);
     __syncthreads();
-    join_step(a, r, sh.waves, sh.join);
+    const SampleRow row = join_step(a, r, sh.waves, sh.join);
+    if (threadIdx.x == 0) a.row[r] = row;
     __syncthreads();
+    sums_step<T, true>(a, 0, r, [&] { return a.row[r]; }, sh.table, sh.waves, sh.sums);
+  } else {
+    sums_step<T, false>(a, 0, r, [&] { return plain_row(a, r, over_segments<false, false>(a, r)); }, sh.table, sh.waves, sh.sums);
   }
-  if (a.filters) sums_step<T, true>(a, 0, r, sh.table, sh.waves, sh.sums);
-  else sums_step<T, false>(a, 0, r, sh.table, sh.waves, sh.sums);
   __syncthreads();
   finish_step<T>(a, r, sh.table, sh.waves, sh.finish);
 }
@@ -864,6 +882,10 @@ static SampleSpace sample_space(int64_t rows, int64_t vocab) {
   return s;
 }
 
+// Workgroups up to which each joins its row's bins itself: one launch less for bins that each of them reads.  us (joined /
+// apart): one row of 32000 10.5 / 6.2 + 5.6, 8 of 131072 (256 workgroups) 15.2 / 9.5 + 7.3, 16 21.0 / 9.4 + 10.6, 64 38.8 / 7.6 + 18.7.
+constexpr int kSampleJoined = 256;
+
 template <typename T>
 static int sample_launch(const SampleArgs& a, hipStream_t s) {
   const dim3 rows((unsigned)a.rows), all((unsigned)(a.rows * a.segs)), threads(kSampleThreads);
@@ -876,12 +898,19 @@ static int sample_launch(const SampleArgs& a, hipStream_t s) {
   if (a.filters) {
     hipLaunchKernelGGL((sample_bins<T>), all, threads, 0, s, a);
     if (const int rc = check_launch("sample_bins")) return rc;
-    hipLaunchKernelGGL(sample_join, rows, threads, 0, s, a);
-    if (const int rc = check_launch("sample_join")) return rc;
+    if (a.rows * a.segs <= kSampleJoined) {
+      hipLaunchKernelGGL((sample_join_sums<T>), all, threads, 0, s, a);
+      if (const int rc = check_launch("sample_join_sums")) return rc;
+    } else {
+      hipLaunchKernelGGL(sample_join, rows, threads, 0, s, a);
+      if (const int rc = check_launch("sample_join")) return rc;
+      hipLaunchKernelGGL((sample_sums<T, true>), all, threads, 0, s, a);
+      if (const int rc = check_launch("sample_sums")) return rc;
+    }
+  } else {
+    hipLaunchKernelGGL((sample_sums<T, false>), all, threads, 0, s, a);
+    if (const int rc = check_launch("sample_sums")) return rc;
   }
-  if (a.filters) hipLaunchKernelGGL((sample_sums<T, true>), all, threads, 0, s, a);
-  else hipLaunchKernelGGL((sample_sums<T, false>), all, threads, 0, s, a);
-  if (const int rc = check_launch("sample_sums")) return rc;
   hipLaunchKernelGGL((sample_finish<T>), rows, threads, 0, s, a);
   return check_launch("sample_finish");
 }
