@@ -214,6 +214,7 @@ struct SampleBins {
   uint32_t bins[kSampleBins];
 };
 struct SampleJoin {
+  uint64_t waves[3][kSampleWaves];
   int found[3];
   uint64_t bounds[2];
   uint32_t count;
@@ -400,7 +401,7 @@ __device__ __forceinline__ void bins_step(const SampleArgs& a, int seg, int r, d
   *reinterpret_cast<u32x4_t*>(a.bins + at * kSampleBins + 4 * tid) = *reinterpret_cast<const u32x4_t*>(sh.bins + 4 * tid);
 }
 
-__device__ __forceinline__ SampleRow join_step(const SampleArgs& a, int r, uint64_t* waves, SampleJoin& sh) {
+__device__ __forceinline__ SampleRow join_step(const SampleArgs& a, int r, SampleJoin& sh) {
   const int tid = threadIdx.x;
   const uint64_t k = (uint64_t)row_k(a, r);
   const double p = row_p(a, r);
@@ -433,12 +434,24 @@ __device__ __forceinline__ SampleRow join_step(const SampleArgs& a, int r, uint6
     least[i] = low > 0.0 ? (uint64_t)low : 0u;
     most[i] = n[i] ? (uint64_t)high + 1u : 0u;
   }
-  uint64_t total_n, total_least, total_most;
-  const uint64_t nb = block_scan64((uint64_t)n[0] + n[1] + n[2] + n[3], waves, total_n);
-  const uint64_t lb = block_scan64(least[0] + least[1] + least[2] + least[3], waves, total_least);
-  const uint64_t mb = block_scan64(most[0] + most[1] + most[2] + most[3], waves, total_most);
+  // the sums of all three in front of this thread, and all tokens
+  const uint64_t own[3] = {(uint64_t)n[0] + n[1] + n[2] + n[3], least[0] + least[1] + least[2] + least[3], most[0] + most[1] + most[2] + most[3]};
+  uint64_t front[3], total_n = 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    front[i] = wave_scan64(own[i]);
+    if ((tid & 63) == 63) sh.waves[i][tid >> 6] = front[i];
+    front[i] -= own[i];
+  }
   if (tid < 3) sh.found[tid] = kSampleBins - 1;
   __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; ++w) {
+    total_n += sh.waves[0][w];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) front[i] += w < (tid >> 6) ? sh.waves[i][w] : 0u;
+  }
+  const uint64_t nb = front[0], lb = front[1], mb = front[2];
   const bool by_k = k > 0 && k < total_n;
   if (by_k) {  // the bin of the k-th token
     uint64_t x = nb, low = lb, high = mb;
@@ -795,9 +808,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_bins(SampleArgs a) {
   bins_step<T>(a, blockIdx.x % a.segs, blockIdx.x / a.segs, table, waves, sh);
 }
 __global__ __launch_bounds__(kSampleThreads) void sample_join(SampleArgs a) {
-  __shared__ uint64_t waves[kSampleWaves];
   __shared__ SampleJoin sh;
-  const SampleRow row = join_step(a, blockIdx.x, waves, sh);
+  const SampleRow row = join_step(a, blockIdx.x, sh);
   if (threadIdx.x == 0) a.row[blockIdx.x] = row;
 }
 // (registers for four workgroups a compute unit: with the next tokens' loads ahead of time they allow two, 64 x 131072 in 23.4 us
@@ -820,7 +832,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_join_sums(SampleArgs a)
   __shared__ SampleSums sh;
   const int r = blockIdx.x / a.segs, seg = blockIdx.x % a.segs;
   auto row_of = [&] {
-    const SampleRow row = join_step(a, r, waves, join);
+    const SampleRow row = join_step(a, r, join);
     if (seg == 0 && threadIdx.x == 0) a.row[r] = row;
     return row;
   };
@@ -843,7 +855,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_whole(SampleArgs a) {
   if (a.filters) {
     bins_step<T>(a, 0, r, sh.table, sh.waves, sh.bins);
     __syncthreads();
-    const SampleRow row = join_step(a, r, sh.waves, sh.join);
+    const SampleRow row = join_step(a, r, sh.join);
     if (threadIdx.x == 0) a.row[r] = row;
     __syncthreads();
     sums_step<T, true>(a, 0, r, [&] { return a.row[r]; }, sh.table, sh.waves, sh.sums);
