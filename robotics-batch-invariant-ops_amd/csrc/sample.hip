@@ -20,7 +20,7 @@
 // logits, mostly) finish finds the borders by bisection over the row.
 //
 // 64 rows of 131072 in float32, 33.6 MB that are read three times (the second and third time mostly from the caches): 8, 15, 8, 19.5 and
-// 21 us, bound by the arithmetic of 64-bit weights, in finish by the sort's steps that wait for one another.  (With 64-bit
+// 11 us, bound by the arithmetic of 64-bit weights, in finish by steps that wait for one another.  (With 64-bit
 // sums a bin, joined with the borders' list by the last workgroup of a launch, bins took 78 us and sums 73: fences make
 // each of an XCD's writes visible to the others.)  One row of 32000: 3, 5, 10 and 7.5 us, each bound by a launch and a few
 // reads that wait for one another.  64 rows of 131072 equal logits, by bisection, 1.1 ms.
@@ -36,6 +36,7 @@ constexpr int kSampleSubs = kSampleMost / kSampleSub;
 constexpr int kSampleTable = 1024;
 constexpr int kSampleSeg = 8192;               // most tokens of a segment: 14 bits of a bin's word count, 18 add up places
 constexpr int kSamplePlace = 18;
+constexpr uint32_t kSampleCounted = 128;       // tokens of a list that are compared with one another
 constexpr uint32_t kNoIndex = 0xffffffffu;
 
 struct SampleRow {    // what join finds, and what several workgroups would have to compute again
@@ -566,6 +567,60 @@ __device__ __forceinline__ void sums_step(const SampleArgs& a, int seg, int r, R
     a.list[(int64_t)r * kSampleList + sh.ready + i] = sh.item[i];
 }
 
+// The list in its order, by buckets of weights (a bucket a thread) and the ranks inside of them: up to 978 tokens, 64 rows of 131072,
+// 11.3 us for the whole step, 20.8 where pairs are exchanged.  False, and the list as it was, where a bucket has many tokens.
+__device__ __forceinline__ bool sort_by_weight(const SampleArgs& a, int r, uint32_t listed, uint64_t some, const SampleWeight& of,
+                                               const SampleRow& border, uint64_t* waves, SampleFinish& sh) {
+  constexpr int kPer = kSampleList / kSampleThreads;
+  constexpr uint32_t kMany = 64;
+  const int tid = threadIdx.x;
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(sh.other);
+  uint32_t* const starts = counts + kSampleThreads;
+  // eighths of places; bins plo to phi have the first buckets, bin bk behind them has one for each of its eighths
+  constexpr uint32_t kBin = 8 * kSampleInside;
+  const uint32_t first = border.bk > border.phi ? kSampleThreads - kBin : kSampleThreads;
+  const uint32_t lo = (uint32_t)border.plo * kBin, range = (uint32_t)(border.phi + 1 - border.plo) * kBin;
+  counts[tid] = 0u;
+  __syncthreads();
+  uint64_t item[kPer];
+  uint32_t bucket[kPer], at[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int x = tid + kSampleThreads * i;
+    if (x >= (int)listed) break;
+    item[i] = i == 0 ? some : a.list[(int64_t)r * kSampleList + x];
+    const uint64_t y = of.octaves(float_of((uint32_t)(item[i] >> 32)));
+    const uint32_t eighth = (uint32_t)((uint64_t)(uint32_t)(y >> 14) * of.scale >> 29);
+    const bool behind = of.bin(y) > border.phi;
+    const uint32_t to = behind ? first + eighth - (uint32_t)border.bk * kBin : (eighth - lo) * first / range, end = behind ? kSampleThreads : first;
+    bucket[i] = to < end ? to : end - 1;
+    at[i] = atomicAdd(&counts[bucket[i]], 1u);
+  }
+  __syncthreads();
+  const uint32_t mine = counts[tid];
+  if (__syncthreads_or(mine > kMany)) return false;
+  uint64_t all;
+  starts[tid] = (uint32_t)block_scan64(mine, waves, all);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (tid + kSampleThreads * i < (int)listed) sh.item[starts[bucket[i]] + at[i]] = item[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (tid + kSampleThreads * i >= (int)listed) break;
+    const uint32_t start = starts[bucket[i]], end = start + counts[bucket[i]];
+    at[i] = start;
+    for (uint32_t x = start; x < end; ++x) at[i] += sh.item[x] > item[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (tid + kSampleThreads * i < (int)listed) sh.item[at[i]] = item[i];
+  __syncthreads();
+  return true;
+}
+
 template <typename T>
 __device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* table, uint64_t* waves, SampleFinish& sh) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -595,7 +650,8 @@ __device__ __forceinline__ void finish_step(const SampleArgs& a, int r, double* 
     uint64_t total = bk >= 0 ? whole.weight : whole.all;
     if (fits) {
       // the list from the largest rank down
-      if (listed <= kSampleThreads) {  // a token a thread, to the place behind all larger ones
+      if (listed > kSampleCounted && sort_by_weight(a, r, listed, some, of, border, waves, sh)) {
+      } else if (listed <= kSampleThreads) {  // a token a thread, to the place behind all larger ones
         sh.other[tid] = tid < (int)listed ? some : 0u;
         __syncthreads();
         int at = 0;
