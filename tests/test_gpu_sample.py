@@ -106,6 +106,22 @@ def test_few_different_logits(levels, top_k, share):
     check_row(row, 1.0, top_k, p)
 
 
+@pytest.mark.parametrize("vocab", [150, 600, 1100, 2048, 9000])
+@pytest.mark.parametrize("levels", [1, 2, 400])
+@pytest.mark.parametrize("top_k, share", [(None, 0.7), (101, None), (149, 0.6)])
+def test_borders_of_many_tokens(vocab, levels, top_k, share):
+    """Borders' lists of a hundred to two thousand tokens, of few or of many different weights, alone and among far smaller ones."""
+    g = torch.Generator().manual_seed(vocab + levels)
+    row = torch.full((vocab,), -30.0)
+    some = torch.randperm(vocab, generator=g)[:min(vocab, 2000)]
+    row[some] = torch.randint(0, levels, (len(some),), generator=g).float() * 1e-3
+    p = None
+    if share is not None:
+        w, stay = staying(row, 1.0, top_k)
+        p = middle(w, stay, share)
+    check_row(row, 1.0, top_k, p)
+
+
 @pytest.mark.parametrize("spread", [1e-6, 1e-3, 30.0, 1e4])
 @pytest.mark.parametrize("temperature", [1e-30, 1e-3, 1.0, 1e6])
 def test_narrow_and_wide_distributions(spread, temperature):
