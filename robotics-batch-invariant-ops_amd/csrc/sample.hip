@@ -5,8 +5,9 @@
 // less than p of the weight of the first k has gone (top-p), those with w_i >= min-p.  The token is the first index whose
 // running sum of the weights that stay is past u times all of them.
 //
-// Sums decide between neighbours, so they are exact: a weight is formed in 64 bits and rounded once to a multiple of 2^-43,
-// and sums of those are integers, the same in any order.  A row's token depends on its own row only.
+// Sums decide between neighbours, so they are exact: a weight is formed to 2^-33 of itself, by its own logit, the row's largest and
+// T alone, and rounded once to a multiple of 2^-43; sums of those are integers, the same in any order.  A row's token depends on its
+// own row only.
 //
 // A row's tokens are shared among `segs` workgroups, in five launches (few workgroups four, and one where a workgroup has a
 // whole row):
@@ -107,8 +108,8 @@ __device__ __forceinline__ void eight_logits(const T* row, int i, int vocab, flo
 }
 
 // Weights.  y = (M - l) log2 e / T in units of 2^-40 (at most 50, which is a weight of 0: logits of -inf and NaN have that);
-// 2^-y from a table of 2^(-i / 1024) and 1 - 2^-r = t - t^2 / 2 + t^3 / 6, t = r ln 2 < 2^-10.5, which 32 bits hold to
-// 2^-33: relative error of a weight, and of a sum at most that.
+// 2^-y from a table of 2^(-i / 1024) in 64 bits and 1 - 2^-r = t - t^2 / 2 + t^3 / 6, t = r ln 2 < 2^-10.5, in 32.  A weight is off by
+// less than 2^-33 of itself (2^-33.23 at most, over all 2^30 remainders r), and a sum by at most that.
 struct SampleWeight {
   double top, c;
   bool infinite;            // M is infinite: only logits of that count, alike
@@ -129,7 +130,7 @@ struct SampleWeight {
   __device__ __forceinline__ uint64_t units(uint64_t y) const {
     const uint32_t hi = (uint32_t)(y >> 32), lo = (uint32_t)y;
     const double t = table[(hi & 255u) << 2 | lo >> 30];
-    const float r = (float)(lo & 0x3fffffffu) * 6.3041396e-13f;  // ln 2 / 2^40
+    const float r = (float)(lo & 0x3fffffffu) * (float)(0.6931471805599453 / 1099511627776.0);  // ln 2 / 2^40
     const float off = r * __builtin_fmaf(r, __builtin_fmaf(r, 1.f / 6.f, -0.5f), 1.f);
     const double w = fma(-t, (double)off, t);
     const double sized = __hiloint2double(__double2hiint(w) + ((43 - (int)(hi >> 8)) << 20), __double2loint(w));

@@ -6,6 +6,8 @@ least 1e-5 of the whole: a 32-bit random number is off by 2^-25, the sums of at 
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -259,3 +261,22 @@ def test_needs_no_gradient():
         sample_tokens_batch_invariant(x, torch.zeros(2, device="cuda"))
     with torch.no_grad():
         assert sample_tokens_batch_invariant(x, torch.zeros(2, device="cuda")).tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("step", [1, (1 << 29) + 1, (1 << 30) - 1])
+def test_a_weight_is_off_by_less_than_a_part_in_2_33(step):
+    """Two logits 1 apart at temperatures that put the second one's octaves y = log2(e) / T next to the borders of each of the 1024
+    parts of an octave (and into the middle).  Its weight w is within 2^-33 w of the definition, and then rounded to a multiple of
+    2^-43 (2^-41 w at most, w being above 2^-3), y to one of 2^-40 (2^-41 w).  So with a top-p of 1 / (1 + w (1 - d)), d = 2^-33 + 2^-39,
+    more than that has gone before it only if it were too small: it stays; with 1 / (1 + w (1 + d)) it goes.  (top-p as a number is
+    one of 64 bits: 2^-53 / w.)"""
+    x, u = torch.tensor([[0.0, -1.0]]).cuda(), torch.tensor([0.99999994]).cuda()
+    d, got = 2.0**-33 + 2.0**-39, []
+    for i in range(1024):
+        t = 1.4426950408889634 / ((i % 2) + (i + step * 2.0**-30) / 1024)
+        w = math.exp(-1.0 / t)
+        for off in (-d, d):
+            got.append(sample_tokens_batch_invariant(x, u, temperature=t, top_p=1.0 / (1.0 + w * (1.0 + off))))
+    got = torch.cat(got).view(-1, 2).cpu()
+    assert int((got[:, 0] != 1).sum()) == 0, "weights that are too small"
+    assert int((got[:, 1] != 0).sum()) == 0, "weights that are too large"
