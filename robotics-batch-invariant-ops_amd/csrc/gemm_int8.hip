@@ -152,8 +152,16 @@ struct Int8Args {
   int nt;                    // non-temporal stores (gemm_big.h)
 };
 
-template <typename T>
+// The first product, sums of up to 2^31 times a row's step, is past 32-bit floats from a step of 2^97 on, whatever the result is.
+__device__ __forceinline__ bool far_step(float xs) { return fabsf(xs) >= 0x1p96f && fabsf(xs) < INFINITY; }
+// FAR: there may be such steps.  2^64 of them go to the channel's scale, exactly: what was in range has the same bits.
+template <bool FAR>
 __device__ __forceinline__ float finished(int32_t acc, float xs, float ws, float bias) {
+  if constexpr (FAR) {
+    const bool far = acc != 0 && far_step(xs);
+    xs = far ? xs * 0x1p-64f : xs;
+    ws = far ? ws * 0x1p64f : ws;
+  }
   return __builtin_fmaf((float)acc * xs, ws, bias);
 }
 
@@ -244,7 +252,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(Int8Args a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t m = 16 * i + 4 * (l >> 4) + j;
-      if (m < a.M) Num<T>::store(static_cast<T*>(a.y) + m * a.N + col, finished<T>(sum[j], a.xs[m * a.xs_s], ws, bias));
+      if (m < a.M) Num<T>::store(static_cast<T*>(a.y) + m * a.N + col, finished<true>(sum[j], a.xs[m * a.xs_s], ws, bias));
     }
   }
 }
@@ -273,10 +281,12 @@ void int8_big_kernel(Int8Args a) {
   float* const xs = reinterpret_cast<float*>(smem);  // the ring is idle
   for (int i = threadIdx.x; i < BM; i += 256) xs[i] = a.xs[(m0 + (i < rows ? i : rows - 1)) * a.xs_s];
   __syncthreads();
+  bool far = false;  // a row of this wavefront has such a step: it has a store of its own
+  for (int i = threadIdx.x & 63; i < Tile::WM; i += 64) far |= far_step(xs[(threadIdx.x >> 7) * Tile::WM + i]);
   T* const y = static_cast<T*>(a.y) + m0 * a.N + n0;
   int ldc = (int)a.N;
   asm volatile("" : "+s"(ldc));  // (keeps the compiler from holding all row offsets)
-  auto store = [&](auto checked, auto nt) {
+  auto store = [&](auto checked, auto nt, auto with_far) {
 #pragma unroll
     for (int j = 0; j < Tile::FN; ++j) {
       const int col = Tile::acc_col(j);
@@ -290,14 +300,17 @@ void int8_big_kernel(Int8Args a) {
           const int row = Tile::acc_row(i, r);
           if (checked && (!in || row >= rows)) continue;
           T* const p = y + (uint32_t)(row * ldc + col);
-          const float v = finished<T>(acc[i][j][r], xs[row], ws, bias);
+          const float v = finished<decltype(with_far)::value>(acc[i][j][r], xs[row], ws, bias);
           put_value<T, decltype(nt)::value>(p, v);
         }
     }
   };
-  if (rows < BM || cols < BN) store(std::true_type(), std::false_type());
-  else if (a.nt) store(std::false_type(), std::true_type());
-  else store(std::false_type(), std::false_type());
+  const std::true_type yes;
+  const std::false_type no;
+  if (__any(far)) store(yes, no, yes);
+  else if (rows < BM || cols < BN) store(yes, no, no);
+  else if (a.nt) store(no, yes, no);
+  else store(no, no, no);
 }
 
 // 64 x 64 blocks, operands through registers: any K, any alignment.
@@ -380,7 +393,7 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int m = wm + 8 * (r >> 2) + 4 * half + (r & 3);
-    Num<T>::store(tile + 64 * m + wn + lr, finished<T>(acc[r], steps[m], ws, bias));
+    Num<T>::store(tile + 64 * m + wn + lr, finished<true>(acc[r], steps[m], ws, bias));
   }
   __syncthreads();
   constexpr int VEC = 16 / (int)sizeof(T), CHUNKS = 64 / VEC;

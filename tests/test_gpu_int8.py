@@ -191,3 +191,27 @@ def test_outputs_past_32_bits(k):
     out = linear_int8_batch_invariant(x, xs, w, ws, b)
     for rows in (slice(0, 3), slice(65530, 65540), slice(m - 2, m)):
         assert_bitwise(out[rows], linear_int8_batch_invariant(x[rows], xs[rows], w, ws, b))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, n, k", [(4, 40, 64), (24, 40, 128), (100, 130, 128), (100, 130, 130), (512, 2048, 256), (2100, 4100, 128)])
+def test_large_rows_and_small_channels(dtype, m, n, k):
+    """Products whose sum times the row's step is past 32-bit floats, and the result is not: steps as rows at the end of bfloat16 have."""
+    x, xs, w, ws, b = case(m, n, k, dtype, seed=11)
+    g = torch.Generator().manual_seed(12)
+    xs = xs * torch.tensor([2.0**124, 2.0**123, 1.0, -(2.0**124)])[torch.randint(0, 4, (m,), generator=g)].cuda()  # (0.01 to 0.03 of them)
+    ws = ws * torch.tensor([2.0**-118, 2.0**-117])[torch.randint(0, 2, (n,), generator=g)].cuda()
+    x[1] = 0
+    assert float(((x.double() @ w.double().t()).abs() * xs.double().abs().view(-1, 1)).max()) > 2.0**128
+    out = linear_int8_batch_invariant(x, xs, w, ws, b, dtype=dtype)
+    assert bool(torch.isfinite(out).all())
+    check(out, x, xs, w, ws, b)
+    assert_bitwise(linear_int8_batch_invariant(x[:3], xs[:3], w, ws, b, dtype=dtype), out[:3])
+    # sums of 0 times what two large factors make; infinite and undefined steps and channels as before
+    ws[0], ws[1], ws[2], xs[1] = 2.0**100, float("nan"), float("inf"), 2.0**126
+    out = linear_int8_batch_invariant(x, xs, w, ws, b, dtype=dtype)
+    assert bool((out[1, 0] == b[0]) & torch.isnan(out[1, 1]) & torch.isnan(out[1, 2]))
+    assert_bitwise(out[1, 3:], b[3:])
+    xs[1], xs[3] = float("inf"), float("nan")
+    out = linear_int8_batch_invariant(x, xs, w, ws, b, dtype=dtype)
+    assert bool(torch.isnan(out[1]).all() & torch.isnan(out[3]).all())
