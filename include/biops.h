@@ -555,8 +555,8 @@ int64_t biops_sample_workspace_size(int64_t rows, int64_t vocab);
  * w_i = exp((l_i - max) / T).  Of the tokens ranked by logit (equal ones by index) stay the first k, those before which less than
  * p of the weight of the first k has gone (the first always), and those with w_i >= min_p; the token is the first index at
  * which the running sum of what stays exceeds u times all of it.  T <= 0: the most likely token.  Each setting comes from an
- * array (by its stride, in elements) or, where that is null, for all rows from t0, k0 (0: all), p0 (1: all) and m0.  NaN
- * logits count as -inf; a row without any other gives -1.  Workspace 16-byte aligned. */
+ * array (by its stride, in elements) or, where that is null, for all rows from t0, k0 (0: all), p0 (1: all) and m0; NaN is a
+ * T of 0 and no filter elsewhere.  NaN logits count as -inf; a row without any other gives -1.  Workspace 16-byte aligned. */
 int biops_sample(int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, int64_t u_s,
                  const float* temperature, int64_t t_s, double t0, const void* top_k, int k64, int64_t k_s, int64_t k0,
                  const float* top_p, int64_t p_s, double p0, const float* min_p, int64_t m_s, double m0, int64_t* out,

@@ -405,7 +405,8 @@ def sample_tokens_batch_invariant(
 
     Each setting is a number for all rows, or a tensor with one for each (float32; ``top_k`` int32 or int64).  In a tensor a
     temperature that is not positive means 0, a ``top_k`` below 1 and a ``top_p`` of 1 or more mean no filter, a ``top_p`` of 0 or
-    less the most likely token, and a ``min_p`` above 1 means 1.  Random numbers outside of [0, 1) count as the nearest inside.
+    less the most likely token, and a ``min_p`` above 1 means 1.  NaN is a temperature of 0, and no filter elsewhere.  Random
+    numbers outside of [0, 1) count as the nearest inside (NaN as 0).
 
     Logits of NaN count as -inf, which are never chosen; a row without any other gives -1.  Where logits are +inf only those
     can be chosen.  Weights are within 2**-33 of themselves, then rounded to multiples of 2**-43 (what is less than half of that is

@@ -336,7 +336,7 @@ __device__ __forceinline__ bool row_weights(const SampleWhole& whole, double t, 
 __device__ __forceinline__ double row_t(const SampleArgs& a, int r) { return row_value(a.temperature, a.t_s, a.t0, r); }
 // A row without borders.
 __device__ __forceinline__ SampleRow plain_row(const SampleArgs& a, int r, const SampleWhole& whole) {
-  const double min_p = fmin(row_value(a.min_p, a.m_s, a.m0, r), 1.0);
+  const double given = row_value(a.min_p, a.m_s, a.m0, r), min_p = given >= 1.0 ? 1.0 : given;  // (NaN: no filter)
   SampleRow row{0.0, 0.0, 50ull << 40, -2, 0u, kSampleBins, -1, -1, 0u, 0};
   SampleWeight of;
   int64_t token;

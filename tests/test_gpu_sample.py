@@ -280,3 +280,17 @@ def test_a_weight_is_off_by_less_than_a_part_in_2_33(step):
     got = torch.cat(got).view(-1, 2).cpu()
     assert int((got[:, 0] != 1).sum()) == 0, "weights that are too small"
     assert int((got[:, 1] != 0).sum()) == 0, "weights that are too large"
+
+
+def test_settings_that_are_not_numbers():
+    """NaN in a tensor: a temperature of 0, and no filter elsewhere."""
+    x = logits_of(5000, 18, rows=40).cuda()
+    u = torch.rand(40, generator=torch.Generator().manual_seed(19)).cuda()
+    nan = torch.full((40,), float("nan")).cuda()
+    plain = sample_tokens_batch_invariant(x, u)
+    assert int((plain != x.argmax(1)).sum()) > 20
+    assert torch.equal(sample_tokens_batch_invariant(x, u, temperature=nan), x.argmax(1))
+    assert torch.equal(sample_tokens_batch_invariant(x, u, top_p=nan), plain)
+    assert torch.equal(sample_tokens_batch_invariant(x, u, min_p=nan), plain)
+    kept = sample_tokens_batch_invariant(x, u, top_k=30, top_p=0.9)
+    assert torch.equal(sample_tokens_batch_invariant(x, u, top_k=30, top_p=0.9, min_p=nan), kept)
