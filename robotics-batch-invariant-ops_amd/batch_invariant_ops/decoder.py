@@ -349,7 +349,7 @@ def multi_axis_rotary(
 
 
 # -------------------------------------------------------------------------- paged cache ----
-def _check_caches(key_cache, value_cache) -> None:
+def _check_caches(key_cache, value_cache, by_page=False) -> None:
     if key_cache.dim() != 4 or value_cache.dim() != 4:
         raise ValueError("caches must have shape [pages, page_size, kv_heads, head_dim]")
     if key_cache.shape[:3] != value_cache.shape[:3]:
@@ -359,8 +359,13 @@ def _check_caches(key_cache, value_cache) -> None:
     for cache in (key_cache, value_cache):
         if cache.stride(3) != 1 and cache.shape[3] > 1:
             raise ValueError("cache rows must have a unit stride in head_dim")
-    if key_cache.shape[0] * key_cache.shape[1] > 0x7FFFFFFF:
-        raise ValueError("caches of more than 2**31 - 1 slots are not supported")
+    _check_slots(key_cache, by_page)
+
+
+def _check_slots(cache, by_page: bool) -> None:
+    """Slots are counted in 31 bits: those of a whole cache for a write, those of a page (of any number) for attention."""
+    if (1 if by_page else cache.shape[0]) * cache.shape[1] > 0x7FFFFFFF:
+        raise ValueError(f"{'pages' if by_page else 'caches'} of more than 2**31 - 1 slots are not supported")
 
 
 def _overlaps(t: torch.Tensor) -> bool:
@@ -529,7 +534,7 @@ def paged_attention_batch_invariant(
             watch.after_call()
             return out
     _refuse_transforms("paged_attention_batch_invariant", query, key_cache, value_cache)
-    _check_caches(key_cache, value_cache)
+    _check_caches(key_cache, value_cache, by_page=True)
     if query.dim() != 3:
         raise ValueError(f"query must have shape [batch, heads, head_dim], got {tuple(query.shape)}")
     if query.dtype != key_cache.dtype:

@@ -32,6 +32,7 @@ from .decoder import (
     _call,
     _check_caches,
     _check_scale,
+    _check_slots,
     _check_tensors,
     _check_window,
     _direct,
@@ -60,7 +61,7 @@ _HALVES = (torch.bfloat16, torch.float16)
 
 
 # ---------------------------------------------------------------------------- 4-bit caches ----
-def _check_fp4(key_cache, key_scales, value_cache, value_scales) -> tuple[int, int]:
+def _check_fp4(key_cache, key_scales, value_cache, value_scales, by_page=False) -> tuple[int, int]:
     """Head dimensions of the keys and the values of a cache in 4 bits."""
     dims = []
     for data, scales in ((key_cache, key_scales), (value_cache, value_scales)):
@@ -77,8 +78,7 @@ def _check_fp4(key_cache, key_scales, value_cache, value_scales) -> tuple[int, i
             if t.stride(3) != 1 and t.shape[3] > 1:
                 raise ValueError("cache rows must have a unit stride")
         dims.append(d)
-    if key_cache.shape[0] * key_cache.shape[1] > 0x7FFFFFFF:
-        raise ValueError("caches of more than 2**31 - 1 slots are not supported")
+    _check_slots(key_cache, by_page)
     return dims[0], dims[1]
 
 
@@ -321,7 +321,7 @@ def paged_attention_fp4_batch_invariant(
             watch.after_call()
             return out
     _refuse_transforms("paged_attention_fp4_batch_invariant", query, key_cache, key_scales, value_cache, value_scales)
-    d, dv = _check_fp4(key_cache, key_scales, value_cache, value_scales)
+    d, dv = _check_fp4(key_cache, key_scales, value_cache, value_scales, by_page=True)
     if query.dim() != 3:
         raise ValueError(f"query must have shape [batch, heads, head_dim], got {tuple(query.shape)}")
     if query.dtype not in _HALVES:

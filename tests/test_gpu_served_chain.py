@@ -9,6 +9,7 @@ from batch_invariant_ops import (
     check_cache_indices,
     linear_int8_batch_invariant,
     multi_axis_rotary,
+    paged_attention_batch_invariant,
     paged_attention_fp4_batch_invariant,
     paged_cache_read_fp4,
     paged_cache_write_fp4,
@@ -254,3 +255,20 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("path", ["module", "python"])
+@pytest.mark.parametrize("bits", [4, 16])
+def test_attention_over_more_than_31_bits_of_slots(path, bits, request):
+    """Pages are counted in 64 bits, on both host paths (a page repeated by its stride)."""
+    if path == "python":
+        request.getfixturevalue("in_python")
+    g = torch.Generator().manual_seed(9)
+    rows = [torch.randn(1, PAGE, HKV, D, generator=g).to(torch.bfloat16) for _ in range(2)]
+    caches = [c.cuda() for x in rows for c in (to_fp4(x) if bits == 4 else (x,))]
+    many = [c.expand((1 << 31) // PAGE + 5, *c.shape[1:]) for c in caches]
+    q = torch.randn(2, HQ, D, generator=g).to(torch.bfloat16).cuda()
+    lens = torch.tensor([40, 9]).cuda()
+    table = torch.tensor([[(1 << 31) // PAGE + 4, 0, (1 << 31) // PAGE], [1 << 27, 0, 0]]).cuda()
+    attention = paged_attention_fp4_batch_invariant if bits == 4 else paged_attention_batch_invariant
+    assert_bitwise(attention(q, *many, table, lens), attention(q, *caches, table * 0, lens))

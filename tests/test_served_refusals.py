@@ -302,3 +302,19 @@ def test_the_module_without_its_library(monkeypatch):
     served = importlib.import_module("batch_invariant_ops.served")
     with pytest.raises(ValueError, match="int8"):
         served.linear_int8_batch_invariant(zeros(3, 4), zeros(3, dtype=F32), zeros(5, 4, dtype=I8), zeros(5, dtype=F32))
+
+
+def test_caches_of_many_slots():
+    """A write addresses slots, in 31 bits; attention addresses pages."""
+    fours = [c[:1].expand(1 << 27, 16, *c.shape[2:]) for c in four()]
+    plain = [zeros(1, 16, 2, 64).expand(1 << 27, 16, 2, 64)] * 2
+    for call in (lambda: write4(caches=fours), lambda: bio.paged_cache_read_fp4(*fours, torch.zeros(3, dtype=torch.int64)),
+                 lambda: bio.paged_cache_write(zeros(3, 2, 64), zeros(3, 2, 64), *plain, torch.zeros(3, dtype=torch.int64))):
+        with pytest.raises(ValueError, match="caches of more than 2"):
+            call()
+    for call in (lambda: attend4(caches=fours), lambda: bio.paged_attention_batch_invariant(
+            zeros(2, 4, 64), *plain, zeros(2, 3, dtype=torch.int32), zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="ROCm GPU"):
+            call()
+    with pytest.raises(ValueError, match="pages of more than 2"):
+        attend4(caches=[c[:1, :1].expand(4, 1 << 31, *c.shape[2:]) for c in four()])
