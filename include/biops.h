@@ -548,7 +548,8 @@ int biops_paged_attention_fp4(int dtype, int64_t batch, int64_t hq, int64_t hkv,
                               int64_t sinks, float scale, void* out, int* flag, void* workspace, int64_t workspace_bytes,
                               void* stream);
 
-/* Workspace bytes of biops_sample, -1 for bad sizes (more than 2^20 tokens or 65536 rows). */
+/* Workspace bytes of biops_sample, -1 for bad sizes (more than 2^20 tokens or 65536 rows).  At most 2^29 and what alignment adds:
+ * of many rows some go after others through the same memory. */
 int64_t biops_sample_workspace_size(int64_t rows, int64_t vocab);
 
 /* The next token of each row of logits [rows, vocab] (rows `ld` elements apart) from u[row] in [0, 1).  Weights are

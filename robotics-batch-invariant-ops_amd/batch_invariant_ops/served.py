@@ -410,7 +410,8 @@ def sample_tokens_batch_invariant(
 
     Logits of NaN count as -inf, which are never chosen; a row without any other gives -1.  Where logits are +inf only those
     can be chosen.  Weights are within 2**-33 of themselves, then rounded to multiples of 2**-43 (what is less than half of that is
-    never chosen, and not counted), and their sums are exact, so a token does not depend on the batch.  Up to 2**20 tokens, 65536 rows and 2**35 logits in all.
+    never chosen, and not counted), and their sums are exact, so a token does not depend on the batch.  Up to 2**20 tokens, 65536 rows and 2**35 logits in all; the
+    workspace of a call is at most half a gigabyte.
     """
     module = decoder._tensor_module or _direct()
     if module:

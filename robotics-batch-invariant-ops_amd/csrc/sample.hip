@@ -932,8 +932,8 @@ static int sample_seg(int64_t rows, int64_t vocab) {
 struct SampleSpace {
   int64_t row, part, sub, list, bins, listed, bytes;
 };
-static SampleSpace sample_space(int64_t rows, int64_t vocab) {
-  const int64_t segs = cdiv(vocab, sample_seg(rows, vocab)), subs = cdiv(vocab, kSampleSub);
+static SampleSpace sample_space(int64_t rows, int64_t vocab, int64_t seg) {
+  const int64_t segs = cdiv(vocab, seg), subs = cdiv(vocab, kSampleSub);
   SampleSpace s;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -949,6 +949,13 @@ static SampleSpace sample_space(int64_t rows, int64_t vocab) {
   s.listed = take(rows * 4);
   s.bytes = at;
   return s;
+}
+// Rows that go through the launches together: a row has 16 KB of list and 8 KB of bins for each segment, which would be gigabytes for
+// many rows.  Half a gigabyte is 3600 rows of 131072 tokens or 21800 short ones: many rounds of workgroups in every launch.
+constexpr int64_t kSampleSpace = INT64_C(1) << 29;
+static int64_t sample_rows(int64_t rows, int64_t vocab) {
+  const int64_t most = kSampleSpace / sample_space(1, vocab, sample_seg(rows, vocab)).bytes;
+  return cdiv(rows, cdiv(rows, most));
 }
 
 // Workgroups up to which each joins its row's bins itself: one launch less for bins that each of them reads.  us (joined /
@@ -990,7 +997,7 @@ using namespace biops;
 
 extern "C" int64_t biops_sample_workspace_size(int64_t rows, int64_t vocab) {
   if (rows < 0 || vocab < 1 || vocab > kSampleMost || rows > 65536 || rows * vocab > kSampleAll) return -1;
-  return rows == 0 ? 0 : sample_space(rows, vocab).bytes;
+  return rows == 0 ? 0 : sample_space(sample_rows(rows, vocab), vocab, sample_seg(rows, vocab)).bytes;
 }
 
 extern "C" int biops_sample(int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, int64_t u_s,
@@ -1002,7 +1009,8 @@ extern "C" int biops_sample(int dtype, int64_t rows, int64_t vocab, const void* 
     return fail(BIOPS_ERR_ARG, "biops_sample: rows of 1 to %d tokens, at most 65536 rows and 2^35 tokens in all", kSampleMost);
   if (rows == 0) return BIOPS_OK;
   if (!logits || !u || !out) return fail(BIOPS_ERR_ARG, "biops_sample: null pointer");
-  const SampleSpace x = sample_space(rows, vocab);
+  const int64_t some = sample_rows(rows, vocab);
+  const SampleSpace x = sample_space(some, vocab, sample_seg(rows, vocab));
   if (!workspace || workspace_bytes < x.bytes)
     return fail(BIOPS_ERR_SIZE, "biops_sample: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)x.bytes);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BIOPS_ERR_LAYOUT, "biops_sample: workspace not 16-byte aligned");
@@ -1012,13 +1020,24 @@ extern "C" int biops_sample(int dtype, int64_t rows, int64_t vocab, const void* 
   a.u_s = u_s, a.t_s = t_s, a.k_s = k_s, a.p_s = p_s, a.m_s = m_s;
   a.t0 = t0, a.p0 = p0, a.m0 = m0, a.k0 = k0, a.k64 = k64 != 0;
   a.filters = top_k || top_p || (k0 > 0 && k0 < vocab) || p0 < 1.0;
-  a.out = out, a.rows = (int)rows, a.vocab = (int)vocab;
+  a.vocab = (int)vocab;
   a.seg = sample_seg(rows, vocab), a.segs = (int)cdiv(vocab, a.seg), a.subs = (int)cdiv(vocab, kSampleSub);
   char* const base = static_cast<char*>(workspace);
   a.row = reinterpret_cast<SampleRow*>(base + x.row), a.part = reinterpret_cast<SampleSeg*>(base + x.part);
   a.sub = reinterpret_cast<uint64_t*>(base + x.sub), a.list = reinterpret_cast<uint64_t*>(base + x.list);
   a.bins = reinterpret_cast<uint32_t*>(base + x.bins), a.listed = reinterpret_cast<uint32_t*>(base + x.listed);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  BIOPS_DISPATCH_FLOAT(dtype, return sample_launch<T>(a, s));
+  for (int64_t r = 0; r < rows; r += some) {  // one after another in the same workspace
+    a.rows = (int)(rows - r < some ? rows - r : some);
+    a.logits = static_cast<const char*>(logits) + r * a.ld, a.out = out + r;
+    a.u = u + r * u_s;
+    if (temperature) a.temperature = temperature + r * t_s;
+    if (top_p) a.top_p = top_p + r * p_s;
+    if (min_p) a.min_p = min_p + r * m_s;
+    if (top_k) a.top_k = static_cast<const char*>(top_k) + r * k_s * (k64 ? 8 : 4);
+    int rc = BIOPS_OK;
+    BIOPS_DISPATCH_FLOAT(dtype, rc = sample_launch<T>(a, s));
+    if (rc != BIOPS_OK) return rc;
+  }
   return BIOPS_OK;
 }

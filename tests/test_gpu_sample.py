@@ -294,3 +294,21 @@ def test_settings_that_are_not_numbers():
     assert torch.equal(sample_tokens_batch_invariant(x, u, min_p=nan), plain)
     kept = sample_tokens_batch_invariant(x, u, top_k=30, top_p=0.9)
     assert torch.equal(sample_tokens_batch_invariant(x, u, top_k=30, top_p=0.9, min_p=nan), kept)
+
+
+@pytest.mark.parametrize("rows, vocab, each", [(50000, 100, True), (50000, 30, False), (9000, 40001, True)])
+def test_more_rows_than_a_workspace_holds(rows, vocab, each):
+    """The same tokens as in calls of few rows, with settings by strides."""
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    x = (torch.randn(rows, vocab, generator=g, device="cuda") * 2).to(BF16)
+    wide = torch.rand(rows, 8, generator=g, device="cuda")
+    kw = dict(top_k=11, top_p=0.9)
+    if each:
+        kw = dict(temperature=wide[:, 1] + 0.2, top_k=(wide[:, 2:4] * vocab).long()[:, 1], top_p=wide[:, 4], min_p=wide[:, 5] * 0.1)
+    got = sample_tokens_batch_invariant(x, wide[:, 0], **kw)
+    for at in range(0, rows, 3000):
+        part = slice(at, at + 3000)
+        few = {k: t[part] if isinstance(t, torch.Tensor) else t for k, t in kw.items()}
+        assert torch.equal(sample_tokens_batch_invariant(x[part], wide[part, 0], **few), got[part])
+    last = {k: t[-1:] if isinstance(t, torch.Tensor) else t for k, t in kw.items()}
+    assert torch.equal(sample_tokens_batch_invariant(x[-1:], wide[-1:, 0], **last), got[-1:])

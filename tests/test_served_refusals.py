@@ -318,3 +318,9 @@ def test_caches_of_many_slots():
             call()
     with pytest.raises(ValueError, match="pages of more than 2"):
         attend4(caches=[c[:1, :1].expand(4, 1 << 31, *c.shape[2:]) for c in four()])
+
+
+@pytest.mark.parametrize("rows, vocab", [(65536, 100), (65536, 4096), (65536, 8192), (65536, 1 << 19), (32768, 1 << 20), (4000, 131072), (500, 1 << 20)])
+def test_the_workspace_of_sampling_is_bounded(rows, vocab):
+    size = entry("biops_sample_workspace_size")
+    assert 0 < size(rows, vocab) < (1 << 29) + 256 and size(1, vocab) <= size(rows, vocab)
