@@ -219,3 +219,30 @@ def test_far_offsets():
     q = torch.randn(1, 4, d, generator=g).to(BF16).cuda()
     out = paged_attention_fp4_batch_invariant(q, *caches, torch.tensor([[pages - 1, 0]], device="cuda"), torch.tensor([100], device="cuda"))
     check_token(out[0], q[0], from_fp4(*small[:2]), from_fp4(*small[2:]), torch.tensor([0, 1]), 100)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("hq, hkv", [(16, 1), (17, 1), (32, 2), (33, 1)])
+@pytest.mark.parametrize("d, dv", [(32, 256), (256, 160), (256, 256), (96, 192)])
+def test_many_query_heads_and_wide_values(dtype, hq, hkv, d, dv):
+    """Workgroups with 16 query heads of the widest outputs, alone and in chunks that are joined."""
+    batch = Batch([1, 0, 130, 700], hq, hkv, d, dv, 16, dtype, seed=15)
+    batch.check(batch.run())
+    only = Batch([40], hq, hkv, d, dv, 16, dtype, seed=16)
+    only.check(only.run())
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n, far", [(3000, 4.0), (40000, 9.0), (40000, 15.0), (200000, 16.0)])
+def test_one_key_far_above_many(dtype, n, far):
+    """The others' small weights are most of what its small value leaves."""
+    page, d = 64, 64
+    pages = -(-n // page)
+    k, v = torch.zeros(pages, page, 1, d), torch.full((pages, page, 1, d), 2.0)
+    k[0, 3, 0, 0], v[0, 3, 0] = 4.0, 0.5
+    caches = [*to_fp4(k.to(dtype)), *to_fp4(v.to(dtype))]
+    q = torch.zeros(1, 2, d, dtype=dtype)
+    q[0, :, 0] = torch.tensor([far / 4, far / 8])
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    out = paged_attention_fp4_batch_invariant(q.cuda(), *(c.cuda() for c in caches), table.cuda(), torch.tensor([n]).cuda(), scale=1.0)
+    check_token(out[0], q[0], from_fp4(*caches[:2]), from_fp4(*caches[2:]), table[0], n, scale=1.0)
