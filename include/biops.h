@@ -516,9 +516,9 @@ int64_t biops_window_attention_workspace_size(int64_t nseq, int64_t hq, int64_t 
 int64_t biops_rotary_write_workspace_size(int64_t rows);
 
 /* biops_rotary of q [rows, hq, d] (-> oq) and k [rows, hk, d], and biops_paged_write of the rotated keys and of v [rows, hk, dv],
- * with their bits, in one launch (more than 1024 rows: two for each 65536).  ks and vs null: caches of dtype; otherwise caches in 4 bits (fp16 or
- * bf16 rows, d and dv multiples of 32), of rotated keys rounded to dtype.  hq may be 0, and pairs 0 (positions, turns and axis
- * then null).  Rows and caches must not share memory. */
+ * with their bits, in one launch (more than 1024 rows: two for each 65536).  ks and vs null: caches of dtype; otherwise caches in 4
+ * bits (fp16 or bf16 rows, d and dv multiples of 32), of rotated keys rounded to dtype.  hq may be 0, and pairs 0 (positions,
+ * turns and axis then null).  Rows and caches must not share memory. */
 int biops_rotary_write(int dtype, int64_t rows, int64_t hq, int64_t hk, int64_t d, int64_t dv,
                        const void* q, int64_t sqT, int64_t sqH, void* oq, int64_t soqT, int64_t soqH,
                        const void* k, int64_t skT, int64_t skH, const void* v, int64_t svT, int64_t svH,

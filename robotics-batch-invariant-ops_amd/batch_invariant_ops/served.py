@@ -12,9 +12,9 @@ A cache in 4 bits is four ``uint8`` tensors: keys ``[pages, page_size, kv_heads,
 / 32]``, values and theirs.  A row is cut into blocks of 32 elements.  A block's scale byte ``x`` stands for the power of two
 ``2 ** (x - 127)``; an element is a sign, two exponent bits and a mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6) times that power,
 two to a byte, the first in the low half.  (The OCP microscaling format MXFP4.)  The power is the smallest of which no
-element of the block is more than 7, so no element is off by more than that power.  Powers lie in [2 ** -125, 2 ** 125] for bfloat16 rows and [2 ** -23, 2 ** 13] for
-float16 ones, where every value is a number of the rows' type; larger elements become the largest value.  A block with an
-infinity or NaN has the scale byte 255 and stands for NaN as a whole.
+element of the block is more than 7, so no element is off by more than that power.  Powers lie in [2 ** -125, 2 ** 125] for
+bfloat16 rows and [2 ** -23, 2 ** 13] for float16 ones, where every value is a number of the rows' type; larger elements
+become the largest value.  A block with an infinity or NaN has the scale byte 255 and stands for NaN as a whole.
 """
 
 from __future__ import annotations
@@ -186,7 +186,7 @@ def rotary_cache_write(
 
     With ``key_scales`` and ``value_scales`` the caches are in 4 bits (see the module): rows are bfloat16 or float16, and a
     rotated key is rounded to its type first.  The new rows must not lie in the memory of the caches, and the caches and their
-    scales share none with one another.
+    scales share none with one another.  A row has at most 2**22 elements.
     """
     plan = _rotary_plan(tuple(sections), float(base), None if inv_freq is None else tuple(map(float, inv_freq)),
                         bool(interleaved_axes), bool(interleaved_pairs))
@@ -264,7 +264,7 @@ def paged_cache_read_fp4(
     """Keys ``[..., kv_heads, head_dim]`` and values ``[..., kv_heads, value_dim]`` of the slots ``[...]`` (int32 or int64) of a
     cache in 4 bits (see the module), as attention sees them: for the prefix of a longer prompt, for example.  Exact in the
     type of the rows that were written.  A negative slot gives zeros; one past the cache too, and is reported as an error
-    later."""
+    later.  At most 2**36 elements."""
     module, watch = _direct_watch()
     if module and dtype in _HALVES:
         out = module.paged_read4(key_cache, key_scales, value_cache, value_scales, slots, nat.DIRECT_DTYPES[dtype], watch.flag_at)
@@ -311,7 +311,7 @@ def paged_attention_fp4_batch_invariant(
 
     The cache's values become numbers of the query's type exactly (for rows that were written in that type); scores, softmax
     and sums are in 32 bits, with one rounding to the output's type, and products take the weights as two 16-bit parts.
-    Returns ``[batch, heads, value_dim]``.
+    Returns ``[batch, heads, value_dim]``, at most 2**24 rows.
     """
     module, watch = _direct_watch()
     if module and window != 0 and (max_length is None or max_length >= 0):
@@ -400,8 +400,8 @@ def sample_tokens_batch_invariant(
     Weights are ``w_i = exp((l_i - max l) / temperature)``.  Tokens are ranked by their logits, equal ones by their index, and of
     this order stay those that every filter allows: the first ``top_k``; those before which less than ``top_p`` of the weight of
     the first ``top_k`` has gone (the most likely one always stays); those with ``w_i >= min_p``.  The token is the first index
-    at which the running sum of the weights that stay, in the order of the vocabulary, exceeds ``uniforms`` times all of them.  A temperature of 0
-    is the most likely token (the first of equal ones).
+    at which the running sum of the weights that stay, in the order of the vocabulary, exceeds ``uniforms`` times all of them.  A
+    temperature of 0 is the most likely token (the first of equal ones).
 
     Each setting is a number for all rows, or a tensor with one for each (float32; ``top_k`` int32 or int64).  In a tensor a
     temperature that is not positive means 0, a ``top_k`` below 1 and a ``top_p`` of 1 or more mean no filter, a ``top_p`` of 0 or
@@ -409,9 +409,9 @@ def sample_tokens_batch_invariant(
     numbers outside of [0, 1) count as the nearest inside (NaN as 0).
 
     Logits of NaN count as -inf, which are never chosen; a row without any other gives -1.  Where logits are +inf only those
-    can be chosen.  Weights are within 2**-33 of themselves, then rounded to multiples of 2**-43 (what is less than half of that is
-    never chosen, and not counted), and their sums are exact, so a token does not depend on the batch.  Up to 2**20 tokens, 65536 rows and 2**35 logits in all; the
-    workspace of a call is at most half a gigabyte.
+    can be chosen.  Weights are formed with a relative error below 2**-33 and rounded to multiples of 2**-43 (what is less than half
+    of that is never chosen, and not counted); their sums are exact, so a token does not depend on the batch.  Up to 2**20 tokens,
+    65536 rows and 2**35 logits in all; the workspace of a call is at most half a gigabyte.
     """
     module = decoder._tensor_module or _direct()
     if module:
@@ -464,7 +464,7 @@ def quantize_tokens_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows ``[..., features]`` (bfloat16, float16 or float32) as 8-bit integers of the same shape with a step for each row
     (float32, ``[...]``): with ``m`` the row's largest magnitude, ``step = m / 127`` and ``q = round(x * (127 / m))``, in 32-bit
     arithmetic, ties to even.  (``m`` counts as at least 2**-100.)  A row with an infinity or NaN has a step of NaN and
-    zeros.  At most 131071 features."""
+    zeros.  At most 131071 features and 2**23 rows."""
     module = decoder._tensor_module or _direct()
     if module:
         out = module.quantize8(x)
@@ -501,7 +501,8 @@ def linear_int8_batch_invariant(
     ``[out_features]`` is of ``dtype`` (bfloat16, float16 or float32), the output's type.
 
     The integer sums are exact (32 bits; at most 131071 terms), what follows is in 32-bit floats with one rounding, so the
-    bits depend neither on the other rows nor on how the work is split."""
+    bits depend neither on the other rows nor on how the work is split.  At most 2**23 rows, 2**22 output channels and 2**35 outputs
+    (in blocks of 64 x 64)."""
     module = decoder._tensor_module or _direct()
     if module:
         out = module.linear8(x, x_scale, weight, weight_scale, bias, nat.DIRECT_DTYPES.get(dtype, -1))

@@ -11,8 +11,8 @@
 // are those of the 16-bit products (gemm_big.h) with twice the elements to a byte; K off the 128-byte step, or rows off 16
 // bytes, go through registers in 64 x 64 blocks instead.
 //
-// 16 x 2048 -> 8192 takes 7.1 us, 2.4 TB/s of the weight (from the caches where they hold it); 4096 x 8192 -> 2048 70 us, 1.97 Pop/s,
-// where the library's product of 8192^3 reaches 2.1; 777 x 2050 -> 1031 12.9 us.  Quantising reads a row once (its elements stay in
+// 16 x 2048 -> 8192 takes 7.1 us, 2.4 TB/s of the weight (from the caches where they hold it); 4096 x 8192 -> 2048 65 to 70 us, 2.0 to
+// 2.1 Pop/s, where the library's product of 8192^3 reaches 2.1; 777 x 2050 -> 1031 11.9 to 15.7 us by machine.  Quantising reads a row once (its elements stay in
 // registers up to 8192 of them): 4096 x 8192 in bf16 20 to 23 us, 4.4 to 5 TB/s.
 #include "gemm_big.h"
 
@@ -433,6 +433,8 @@ static int int8_launch(Int8Args a, hipStream_t s) {
   // Every workgroup of the kernel for few rows reads all of them, 64 bytes of a row at a time, which is slow off 16 bytes.  us (few /
   // blocks), K -> N: 2048 -> 8192 at 32 rows 9.1 / 9.5, at 64 13.2 / 8.0; 8192 -> 2048 at 32 14.2 / 19.5, at 64 21.7 / 19.3; 1024 ->
   // 1024 at 32 4.7 / 7.2; off 16 bytes 2050 -> 8000 at 16 15.9 / 11.4, 8190 -> 2040 at 16 27.9 / 28.3, at 32 40 / 28.
+  // (Few columns leave few workgroups, each with all of K: the 16-bit layer of narrow blocks is then faster, 8192 -> 2048 in bf16 at
+  // 32, 64 and 128 rows 11 to 15, 12 to 16 and 16 to 20 us, here 14, 19 and 19.)
   if (a.M <= 16 && (aligned || a.N <= 2048)) return int8_few<T, 1>(a, s);
   if (a.M <= 32 && aligned) return int8_few<T, 2>(a, s);
   if (whole) {
