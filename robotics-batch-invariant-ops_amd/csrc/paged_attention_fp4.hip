@@ -11,7 +11,7 @@
 // exchanges them through LDS together with the rows' places.
 //
 // A key's 4.25 bits an element leave less to wait for than to compute: 64 sequences of 250 to 16384 keys (16/4 heads of 128,
-// bf16) take 53.5 us and 5 for the join, 2.3 TB/s of 137 MB, where the 16-bit pages take 114 us.  Vector instructions issue in
+// bf16) take 54 us and 5 for the join, 2.3 TB/s of 137 MB, where the 16-bit pages take 114 us.  Vector instructions issue in
 // about half of the cycles (a value element costs half a conversion, a byte permutation and its share of two MFMAs).
 // Registers for three wavefronts a SIMD are what 128-wide heads fit into; for four, they spill and it is slower.  Values are
 // converted four columns at a time for the same reason.  One sequence of 2047 keys: 6.4 us, and 3.8 for the join, bound by
@@ -33,6 +33,9 @@ typedef uint32_t u32_byte_t __attribute__((aligned(1)));
 typedef uint16_t u16_byte_t __attribute__((aligned(1)));
 
 constexpr float kSlack = 8.f;  // powers of two that a weight may be larger than 1
+// fp16 weights are 2^7 times their size, with the slack up to half of the type's range: those down to 2^-32 of the largest count
+// (2^-25 without it: of 128 keys beside one of weight 1 whose value is 0, 31 of weight e^-15 were off by 2.6 %, and at e^-18 gone).
+template <typename T> constexpr float kUp = std::is_same<T, f16_t>::value ? 7.f : 0.f;
 
 // Wavefronts per SIMD that registers are given out for.
 template <int DP, int DVP>
@@ -189,7 +192,7 @@ void paged4_chunk_kernel(Paged4Args a) {
   // of query m16: largest product so far, the same or 0 where that is -inf, sum (of this lane's keys)
   float m, from, l;
   f32x4_t acc[NT];
-  float down = 0.f;  // powers of two that are off the weights
+  float down = -kUp<T>;  // powers of two that are off the weights
   for (;;) {
     m = -INFINITY, from = 0.f, l = 0.f;
 #pragma unroll

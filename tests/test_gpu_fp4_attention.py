@@ -8,7 +8,7 @@ import torch
 import batch_invariant_ops as bio
 from batch_invariant_ops import check_cache_indices, paged_attention_fp4_batch_invariant
 
-from _decoder import check_token
+from _decoder import assert_within, attend64, attention_bound, check_token
 from _served import from_fp4, to_fp4
 from _tol import assert_bitwise
 
@@ -246,3 +246,23 @@ def test_one_key_far_above_many(dtype, n, far):
     table = torch.arange(pages, dtype=torch.int32).view(1, -1)
     out = paged_attention_fp4_batch_invariant(q.cuda(), *(c.cuda() for c in caches), table.cuda(), torch.tensor([n]).cuda(), scale=1.0)
     check_token(out[0], q[0], from_fp4(*caches[:2]), from_fp4(*caches[2:]), table[0], n, scale=1.0)
+
+
+@pytest.mark.parametrize("n", [40, 128, 900, 5000])
+@pytest.mark.parametrize("far", [11.0, 14.0, 15.0, 16.5, 18.0])
+def test_small_weights_of_fp16_count(n, far):
+    """One key far above many, with values of 0: the output is what the others' weights of e^-far say.  They are held times 2^7 in
+    two parts of fp16: to 2^-22 of themselves, or to half of its smallest step over 2^7, 2^-32 of the largest."""
+    page, d = 16, 64
+    pages = -(-n // page)
+    k, v = torch.zeros(pages, page, 1, d), torch.full((pages, page, 1, d), 1536.0)
+    k[0, 3, 0, 0], v[0, 3, 0] = 4.0, 0.0
+    caches = [*to_fp4(k.to(F16)), *to_fp4(v.to(F16))]
+    q = torch.zeros(1, 2, d, dtype=F16)
+    q[0, :, 0] = torch.tensor([far / 4, far / 4 - 0.0625])
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    out = paged_attention_fp4_batch_invariant(q.cuda(), *(c.cuda() for c in caches), table.cuda(), torch.tensor([n]).cuda(), scale=1.0)
+    keys, values = (from_fp4(*caches[i:i + 2]).flatten(0, 1)[:n, 0] for i in (0, 2))
+    for h in range(2):
+        parts = attend64(q[:, h], keys, values, torch.ones(1, n, dtype=torch.bool), 1.0)
+        assert_within(out[:, h], parts[0], attention_bound(F16, *parts, n, 2.0**-22, 2.0**-32), f"head {h}")
