@@ -126,7 +126,7 @@ void paged_chunk_kernel(PagedArgs a) {
   // of query m16: largest product so far, the same or 0 where that is -inf, sum (of this lane's keys)
   float m, from, l;
   f32x4_t acc[NT];
-  float down = 0.f;  // powers of two that are off the weights
+  float down = -kPagedUp<T>;  // powers of two that are off the weights
   for (;;) {
     m = -INFINITY, from = 0.f, l = 0.f;
 #pragma unroll

@@ -33,9 +33,6 @@ typedef uint32_t u32_byte_t __attribute__((aligned(1)));
 typedef uint16_t u16_byte_t __attribute__((aligned(1)));
 
 constexpr float kSlack = 8.f;  // powers of two that a weight may be larger than 1
-// fp16 weights are 2^7 times their size, with the slack up to half of the type's range: those down to 2^-32 of the largest count
-// (2^-25 without it: of 128 keys beside one of weight 1 whose value is 0, 31 of weight e^-15 were off by 2.6 %, and at e^-18 gone).
-template <typename T> constexpr float kUp = std::is_same<T, f16_t>::value ? 7.f : 0.f;
 
 // Wavefronts per SIMD that registers are given out for.
 template <int DP, int DVP>
@@ -192,7 +189,7 @@ void paged4_chunk_kernel(Paged4Args a) {
   // of query m16: largest product so far, the same or 0 where that is -inf, sum (of this lane's keys)
   float m, from, l;
   f32x4_t acc[NT];
-  float down = -kUp<T>;  // powers of two that are off the weights
+  float down = -kPagedUp<T>;  // powers of two that are off the weights
   for (;;) {
     m = -INFINITY, from = 0.f, l = 0.f;
 #pragma unroll

@@ -8,12 +8,12 @@ import torch
 import batch_invariant_ops as bio
 from batch_invariant_ops import check_cache_indices, paged_attention_batch_invariant, paged_cache_write
 
-from _decoder import check_token
+from _decoder import assert_within, attend64, attention_bound, check_token
 from _tol import assert_bitwise
 
 pytestmark = pytest.mark.gpu
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
-BF16 = torch.bfloat16
+BF16, F16 = torch.bfloat16, torch.float16
 
 
 @pytest.fixture(autouse=True)
@@ -463,3 +463,21 @@ def test_many_sequences():
     for b in (0, 1, 2, 17, 1499, 2998, 2999):
         check_token(out[b], q[b], kc, vc, table[b], lengths[b], what=f"sequence {b}")
     assert bio.paged_attention_batch_invariant is paged_attention_batch_invariant
+
+
+@pytest.mark.parametrize("n", [40, 128, 900, 5000])
+@pytest.mark.parametrize("far", [11.0, 14.0, 15.0, 16.5, 18.0])
+def test_small_weights_of_fp16_count(n, far):
+    """One key far above many, with values of 0: the output is what the others' weights of e^-far say.  They are held times 2^7 in
+    two parts of fp16: to 2^-22 of themselves, or to half of its smallest step over 2^7, 2^-32 of the largest."""
+    page, d = 16, 64
+    pages = -(-n // page)
+    k, v = torch.zeros(pages, page, 1, d, dtype=F16), torch.full((pages, page, 1, d), 1536.0, dtype=F16)
+    k[0, 3, 0, 0], v[0, 3, 0] = 4.0, 0.0
+    q = torch.zeros(1, 2, d, dtype=F16)
+    q[0, :, 0] = torch.tensor([far / 4, far / 4 - 0.0625])
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    out = paged_attention_batch_invariant(q.cuda(), k.cuda(), v.cuda(), table.cuda(), torch.tensor([n]).cuda(), scale=1.0)
+    for h in range(2):
+        parts = attend64(q[:, h], k.flatten(0, 1)[:n, 0], v.flatten(0, 1)[:n, 0], torch.ones(1, n, dtype=torch.bool), 1.0)
+        assert_within(out[:, h], parts[0], attention_bound(F16, *parts, n, 2.0**-22, 2.0**-32), f"head {h}")
